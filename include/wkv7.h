@@ -578,6 +578,55 @@ size_t wkv7_proj_workspace_bytes(int64_t m, const wkv7_proj_group *groups, int32
 int wkv7_proj_grouped_noalloc(int64_t m, const wkv7_proj_group *groups, int32_t ngroups,
                               void *stream);
 
+/*
+ * The next token of every row of a batch of logits, by the row's own settings and
+ * from given random numbers, and the token's log-probability.
+ *
+ * With M = max x, w_i = exp((x_i - M) / temperature) and the tokens ordered by
+ * logit, larger first, ties by lower index, the kept tokens are
+ *     top_k  the first top_k of the order (0: all)
+ *     top_p  of those, the shortest prefix whose weight reaches top_p times theirs,
+ *            at least one token (1: all)
+ *     min_p  of those, the ones with w_i >= min_p (0: all)
+ * and one of them is drawn with probability w_i / (sum of the kept w): in groups
+ * of WKV7_SAMPLE_GROUP consecutive tokens, with W_j the kept weight of group j,
+ *     j = argmin noise[GROUP + j] / W_j,   token = argmin noise[i - GROUP j] / w_i
+ * over the kept i of that group (ties: lower index). temperature <= 0 takes the
+ * largest logit (lowest index). NaN logits count as -inf, +inf as the largest
+ * finite number. A row with nothing above -inf gets token -1 and logprob -inf.
+ *     logprob = x_token - log sum_i exp(x_i)   (over all tokens, untempered)
+ *
+ * Replaces the per-request host sampling of the reference (sample_token,
+ * wkvm/runner/sampling.py:40) and the batched argmax of a decode step
+ * (wkvm/engine.py:163).
+ *
+ *   logits       [rows, vocab] bf16 (WKV7_Y_BF16) or fp32 (WKV7_Y_F32), rows
+ *                row_stride elements apart
+ *   noise        [rows, GROUP + ceil(vocab / GROUP)] fp32, rows noise_stride elements
+ *                apart: independent exponential variates, > 0 (others give some
+ *                token of the vocabulary)
+ *   params       host struct; each setting is a device array [rows] or, where its
+ *                pointer is NULL, the value beside it for every row. NaN turns
+ *                a filter off and a temperature to greedy; min_p is held to <= 1
+ *   tokens       [rows] int32;  logprobs [rows] fp32, or NULL
+ * vocab is at most WKV7_SAMPLE_MAX_VOCAB (else WKV7_ERR_SHAPE).
+ */
+#define WKV7_SAMPLE_GROUP 256
+#define WKV7_SAMPLE_MAX_VOCAB (1 << 21)
+
+struct wkv7_sample_params {
+    const float *temperature;
+    const int32_t *top_k;
+    const float *top_p, *min_p;
+    float temperature1;
+    int32_t top_k1;
+    float top_p1, min_p1;
+};
+int wkv7_sample_tokens(const void *logits, int32_t logits_dtype, int32_t rows, int32_t vocab,
+                       int64_t row_stride, const float *noise, int64_t noise_stride,
+                       const struct wkv7_sample_params *params, int32_t *tokens,
+                       float *logprobs, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

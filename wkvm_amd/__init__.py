@@ -14,6 +14,8 @@ reference's slot-tensor layout and op signatures:
   reference's model layer calls
 * ``DecodeGraph`` -- a decode step's WKV launches captured as one HIP graph
   (the role of experiments/m2_engine_bench.py GraphedDecode)
+* ``sample_tokens`` -- a batch's next tokens by per-request settings
+  (wkvm/runner/sampling.py)
 * ``StateStore`` -- HOT/WARM/COLD state handles, wkvm/store.py, with the
   HOT <-> WARM copies as strided DMA transfers
 """
@@ -29,6 +31,7 @@ from .ops import (
 )
 from .graph import DecodeGraph
 from .runner import WKV7Runner
+from .sampling import sample_noise_size, sample_tokens
 from .state import RWKV7StateBank, SlotCache
 from .store import FingerprintMismatch, StateRecord, StateStore
 
@@ -38,4 +41,5 @@ __all__ = [
     "StateStore", "StateRecord", "FingerprintMismatch",
     "wkv7_decode_slots", "wkv7_prefill_varlen", "slot_copy", "slot_zero",
     "chunk_rwkv7", "fused_recurrent_rwkv7",
+    "sample_tokens", "sample_noise_size",
 ]

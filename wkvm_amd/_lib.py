@@ -40,6 +40,8 @@ WKV7_PROJ_FEW_ROWS = 16
 WKV7_ACT_NONE = 0
 WKV7_ACT_TANH = 1
 WKV7_ACT_SIGMOID = 2
+WKV7_SAMPLE_GROUP = 256
+WKV7_SAMPLE_MAX_VOCAB = 1 << 21
 
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
@@ -60,6 +62,12 @@ class SlotFamily(ctypes.Structure):
     """struct wkv7_slot_family of include/wkv7.h."""
     _fields_ = [("base", _vp), ("outer_stride", _i64), ("slot_stride", _i64), ("rows", _i64),
                 ("outer", _i64), ("row_bytes", _i64), ("dst_ids", _vp), ("src_ids", _vp)]
+
+
+class SampleParams(ctypes.Structure):
+    """struct wkv7_sample_params of include/wkv7.h."""
+    _fields_ = [("temperature", _vp), ("top_k", _vp), ("top_p", _vp), ("min_p", _vp),
+                ("temperature1", _f32), ("top_k1", _i32), ("top_p1", _f32), ("min_p1", _f32)]
 
 
 # name -> (restype, argtypes); must match include/wkv7.h.
@@ -107,6 +115,8 @@ SIGNATURES = {
     "wkv7_proj_grouped_noalloc": (ctypes.c_int, [_i64, ctypes.POINTER(ProjGroup), _i32, _vp]),
     "wkv7_decode_block": (ctypes.c_int, [
         _vp, _i64, _i32, _vp, _vp, _i32] + [_vp] * 13 + [_f32, _f32, _vp, _vp, _vp]),
+    "wkv7_sample_tokens": (ctypes.c_int, [
+        _vp, _i32, _i32, _i32, _i64, _vp, _i64, ctypes.POINTER(SampleParams), _vp, _vp, _vp]),
 }
 
 _lib = None

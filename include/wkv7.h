@@ -609,6 +609,8 @@ int wkv7_proj_grouped_noalloc(int64_t m, const wkv7_proj_group *groups, int32_t 
  *                pointer is NULL, the value beside it for every row. NaN turns
  *                a filter off and a temperature to greedy; min_p is held to <= 1
  *   tokens       [rows] int32;  logprobs [rows] fp32, or NULL
+ *   workspace    device, 16-byte aligned, at least wkv7_sample_workspace_bytes(rows,
+ *                vocab) (else WKV7_ERR_WORKSPACE); holds nothing between calls
  * vocab is at most WKV7_SAMPLE_MAX_VOCAB (else WKV7_ERR_SHAPE).
  */
 #define WKV7_SAMPLE_GROUP 256
@@ -625,7 +627,8 @@ struct wkv7_sample_params {
 int wkv7_sample_tokens(const void *logits, int32_t logits_dtype, int32_t rows, int32_t vocab,
                        int64_t row_stride, const float *noise, int64_t noise_stride,
                        const struct wkv7_sample_params *params, int32_t *tokens,
-                       float *logprobs, void *stream);
+                       float *logprobs, void *workspace, size_t workspace_bytes, void *stream);
+size_t wkv7_sample_workspace_bytes(int32_t rows, int32_t vocab);
 
 #ifdef __cplusplus
 }

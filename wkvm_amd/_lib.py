@@ -116,7 +116,9 @@ SIGNATURES = {
     "wkv7_decode_block": (ctypes.c_int, [
         _vp, _i64, _i32, _vp, _vp, _i32] + [_vp] * 13 + [_f32, _f32, _vp, _vp, _vp]),
     "wkv7_sample_tokens": (ctypes.c_int, [
-        _vp, _i32, _i32, _i32, _i64, _vp, _i64, ctypes.POINTER(SampleParams), _vp, _vp, _vp]),
+        _vp, _i32, _i32, _i32, _i64, _vp, _i64, ctypes.POINTER(SampleParams), _vp, _vp, _vp,
+        _sz, _vp]),
+    "wkv7_sample_workspace_bytes": (_sz, [_i32, _i32]),
 }
 
 _lib = None

@@ -19,8 +19,6 @@
 // Weights that are added in an order that varies (LDS atomics) are fixed-point
 // numbers of 42 fraction bits (w <= 1), so every sum is exact and the token does
 // not depend on the order; plain sums are fp32 per thread, joined in a fixed order.
-#include <algorithm>
-
 #include "wkv7_common.h"
 
 namespace wkv7 {
@@ -28,11 +26,20 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kThreads = 1024;
+constexpr int kGroup = WKV7_SAMPLE_GROUP;
+constexpr int kChunk = 2048;              // tokens of one wave of the scan
+constexpr int kSub = 32;                  // tokens whose maximum the scan keeps
+constexpr int kChunkSubs = kChunk / kSub;
+constexpr int kChunkGroups = kChunk / kGroup;
+constexpr int kScanThreads = 256;
+
+constexpr int kThreads = 1024;            // of the finish
 constexpr int kWaves = kThreads / kWave;
 constexpr int kBins = 2048;
-constexpr int kGroup = WKV7_SAMPLE_GROUP;
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kList = 6144;               // candidates held in LDS
+constexpr int kSubs = 4096;               // runs of kSub tokens that may hold candidates
+// The candidate list's group weights take the place of the histogram.
+constexpr int kListGroups = kBins + kBins / 2;
 
 struct SampleArgs {
   const void* logits;
@@ -43,35 +50,56 @@ struct SampleArgs {
   const int32_t* top_k;
   float temperature1, top_p1, min_p1;
   int32_t top_k1;
-  int32_t V;
+  int32_t V, rows, chunks;
   int32_t* tokens;
   float* logprobs;
+  // what the scan leaves for the finish, per row
+  float* sub_max;   // [chunks * kChunkSubs]
+  float* mass;      // [chunks * kChunkGroups]: group weights relative to the chunk's maximum
+  float2* chunk;    // [chunks]: maximum, sum of exp(x - maximum)
 };
 
-struct Found {
-  uint32_t bin, before_cnt, cnt;
-  u64 before_wgt, wgt;
+struct Settings {
+  float c;        // log2(e) / temperature
+  float top_p;
+  float floor_z;  // min-p: the least (x - M) c
+  int32_t top_k;
+  bool greedy, by_k, by_p;
 };
 
-struct Shared {
-  uint32_t cnt[kBins];
-  u64 wgt[kBins];
-  Found found;
-  u64 red[kWaves];
-  uint32_t wave_cnt[kWaves];
-  u64 wave_wgt[kWaves];
-};
+__device__ __forceinline__ Settings settings(const SampleArgs& a, int64_t b) {
+  const float temp = a.temperature ? a.temperature[b] : a.temperature1;
+  const float min_p = a.min_p ? a.min_p[b] : a.min_p1;
+  Settings s;
+  s.top_p = a.top_p ? a.top_p[b] : a.top_p1;
+  s.top_k = a.top_k ? a.top_k[b] : a.top_k1;
+  // the clamp keeps c and every product a number
+  s.c = 1.44269504088896340736f / fminf(fmaxf(temp, 0x1p-60f), 0x1p60f);
+  s.floor_z = min_p > 0.f ? log2f(fminf(min_p, 1.f)) : -INFINITY;
+  s.greedy = !(temp > 0.f);
+  s.by_k = s.top_k > 0 && s.top_k < a.V;
+  s.by_p = s.top_p < 1.f;
+  return s;
+}
 
 // Ascending in the order of the tokens: the largest logit has the smallest key.
 __device__ __forceinline__ uint32_t order_key(float x) {
   const uint32_t u = __float_as_uint(x + 0.f);  // (-0 and +0 are equal)
   return (u >> 31) ? u : ~u & 0x7fffffffu;
 }
+__device__ __forceinline__ float key_logit(uint32_t k) {
+  return __uint_as_float((k >> 31) ? k : ~k & 0x7fffffffu);
+}
 
 // NaN counts as -inf, +inf as the largest finite number.
 __device__ __forceinline__ float clean(float x) {
   return fminf(fmaxf(x, -INFINITY), 3.402823466e38f);
 }
+
+__device__ __forceinline__ float load_one(const float* p) { return clean(*p); }
+__device__ __forceinline__ float load_one(const uint16_t* p) { return clean(bf16_to_f32(*p)); }
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // 42 fraction bits of w in [0, 1].
 __device__ __forceinline__ u64 fixed(float w) {
@@ -80,19 +108,184 @@ __device__ __forceinline__ u64 fixed(float w) {
   return (u64(uint32_t(hi)) << 21) + uint32_t(lo);
 }
 
-template <typename V, typename Op>
-__device__ __forceinline__ V wave_all(V v, Op op) {
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) v = op(v, __shfl_xor(v, o));
+// Lane exchanges inside 16 lanes; after the smaller steps the mirrors act as xor 4 and xor 8.
+constexpr int kXor1 = 0xb1, kXor2 = 0x4e, kXor4 = 0x141, kXor8 = 0x140;
+template <int kCtrl>
+__device__ __forceinline__ float dpp(float v) {
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(v), kCtrl, 0xf, 0xf, true));
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+  v = fmaxf(v, dpp<kXor1>(v));
+  v = fmaxf(v, dpp<kXor2>(v));
+  v = fmaxf(v, dpp<kXor4>(v));
+  v = fmaxf(v, dpp<kXor8>(v));
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+// The sum over the 2^kLog lanes around a lane.
+template <int kLog>
+__device__ __forceinline__ float lanes_sum(float v) {
+  v += dpp<kXor1>(v);
+  v += dpp<kXor2>(v);
+  v += dpp<kXor4>(v);
+  if constexpr (kLog > 3) v += dpp<kXor8>(v);
+  if constexpr (kLog > 4) v += __shfl_xor(v, 16);
+  if constexpr (kLog > 5) v += __shfl_xor(v, 32);
   return v;
 }
+
+// Elements of one 16-byte load, as they lie in memory.
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+  static constexpr int N = 4;
+  typedef float Raw __attribute__((ext_vector_type(4), aligned(4)));
+  Raw x;
+  __device__ __forceinline__ float get(int e) const { return clean(x[e]); }
+};
+template <> struct Vec<uint16_t> {
+  static constexpr int N = 8;
+  typedef uint32_t Raw __attribute__((ext_vector_type(4), aligned(2)));
+  Raw x;
+  __device__ __forceinline__ float get(int e) const {
+    return clean((e & 1) ? bf16_hi(x[e / 2]) : bf16_lo(x[e / 2]));
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ Vec<T> load_full(const T* p) {
+  return {*reinterpret_cast<const typename Vec<T>::Raw*>(p)};
+}
+// The vector at element i of a row of n; elements past the end are -inf.
+template <typename T>
+__device__ __forceinline__ Vec<T> load_part(const T* row, int i, int n) {
+  if (i + Vec<T>::N <= n) return load_full(row + i);
+  Vec<T> v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (sizeof(T) == 4) {
+      v.x[e] = i + e < n ? row[i + e] : -INFINITY;
+    } else {
+      const uint32_t lo = i + 2 * e < n ? row[i + 2 * e] : 0xff80u;
+      const uint32_t hi = i + 2 * e + 1 < n ? row[i + 2 * e + 1] : 0xff80u;
+      v.x[e] = lo | hi << 16;
+    }
+  }
+  return v;
+}
+
+// -- the scan: one wave per chunk of 2,048 tokens, one pass over the logits -----------------------
+
+// Of every chunk: its maximum and sum of exponentials; of every 32 tokens the maximum, for the
+// finish to know where the largest logits are; and, where nothing but min-p is asked for or top-p
+// needs the row's weight, the weight of every group. Everything is relative to the chunk's own
+// maximum, so the chunks need nothing of each other.
+template <typename T>
+__global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(const SampleArgs args) {
+  constexpr int N = Vec<T>::N;
+  constexpr int kSteps = kChunk / (kWave * N);
+  constexpr int kSubLanes = kSub / N;      // 8 or 4 lanes hold 32 tokens
+  constexpr int kGroupLanes = kGroup / N;  // 64 or 32 lanes hold a group
+  const int64_t id = int64_t(blockIdx.x) * (kScanThreads / kWave) +
+                     __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  if (id >= int64_t(args.rows) * args.chunks) return;
+  const int64_t b = id / args.chunks;
+  const int first = int(id - b * args.chunks) * kChunk;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int V = args.V;
+  const T* row = static_cast<const T*>(args.logits) + b * args.stride;
+  Vec<T> v[kSteps];
+  if (first + kChunk <= V) {
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) v[j] = load_full(row + first + (j * kWave + lane) * N);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) v[j] = load_part(row, first + (j * kWave + lane) * N, V);
+  }
+  const Settings set = settings(args, b);
+  float x[kSteps][N];
+  float top = -INFINITY;
+  float* sub = args.sub_max + id * kChunkSubs;
+#pragma unroll
+  for (int j = 0; j < kSteps; ++j) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      x[j][e] = v[j].get(e);
+      m = fmaxf(m, x[j][e]);
+    }
+    top = fmaxf(top, m);
+    m = fmaxf(m, dpp<kXor1>(m));
+    m = fmaxf(m, dpp<kXor2>(m));
+    if constexpr (kSubLanes == 8) m = fmaxf(m, dpp<kXor4>(m));
+    if (lane % kSubLanes == 0) sub[(j * kWave + lane) / kSubLanes] = m;
+  }
+  top = wave_max(top);
+  float raw = 0.f;
+  // (a chunk of nothing but -inf: its sums stay zero)
+  const float base = top == -INFINITY ? 0.f : top;
+  if (args.logprobs) {
+    const float c = 1.44269504088896340736f;
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+      for (int e = 0; e < N; ++e) raw += exp2_hw((x[j][e] - base) * c);
+    raw = lanes_sum<6>(raw);
+  }
+  if (lane == 0) args.chunk[id] = make_float2(top, raw);
+  // group weights: for the race where no filter applies, and for top-p's total
+  if (set.greedy || set.by_k || (!set.by_p && set.floor_z > -INFINITY)) return;
+  float w[kSteps];
+#pragma unroll
+  for (int j = 0; j < kSteps; ++j) {
+    w[j] = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) w[j] += exp2_hw((x[j][e] - base) * set.c);
+  }
+  float* mass = args.mass + id * kChunkGroups;
+#pragma unroll
+  for (int j = 0; j < kSteps; ++j) {
+    const float s = kGroupLanes == 64 ? lanes_sum<6>(w[j]) : lanes_sum<5>(w[j]);
+    if (lane % kGroupLanes == 0) mass[(j * kWave + lane) / kGroupLanes] = s;
+  }
+}
+
+// -- the finish: one workgroup per row ----------------------------------------------------------------
+
+struct Found {
+  uint32_t bin, before_cnt, cnt;
+  u64 before_wgt, wgt;
+};
+
+struct Shared {
+  union {
+    struct {
+      u64 wgt[kBins];
+      uint32_t cnt[kBins];
+      uint2 list[kList];  // logit bits, index
+      uint32_t subs[kSubs];
+    };
+    u64 mass[kListGroups];  // takes the place of the histogram
+  };
+  uint32_t n_list, n_subs;
+  Found found;
+  u64 red[kWaves];
+  uint32_t wave_cnt[kWaves];
+  u64 wave_wgt[kWaves];
+};
+
+struct MaxF { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+struct AddD { __device__ double operator()(double a, double b) const { return a + b; } };
+struct AddU { __device__ u64 operator()(u64 a, u64 b) const { return a + b; } };
+struct MinU { __device__ u64 operator()(u64 a, u64 b) const { return a < b ? a : b; } };
 
 // Reduction over the block; every thread gets the result.
 template <typename V, typename Op>
 __device__ __forceinline__ V block_all(V v, Op op, Shared& sm) {
   static_assert(sizeof(V) <= sizeof(u64), "fits a slot");
   V* slot = reinterpret_cast<V*>(sm.red);
-  v = wave_all(v, op);
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) v = op(v, __shfl_xor(v, o));
   __syncthreads();
   if ((threadIdx.x & (kWave - 1)) == 0) slot[threadIdx.x / kWave] = v;
   __syncthreads();
@@ -102,93 +295,34 @@ __device__ __forceinline__ V block_all(V v, Op op, Shared& sm) {
   return r;
 }
 
-struct MaxF { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
-struct AddD { __device__ double operator()(double a, double b) const { return a + b; } };
-struct MinU { __device__ u64 operator()(u64 a, u64 b) const { return a < b ? a : b; } };
-
 // An arrival time (not negative) with its index: the smaller time wins, then the lower index.
 __device__ __forceinline__ u64 arrival(float t, uint32_t i) {
   return (u64(__float_as_uint(t)) << 32) | i;
 }
 
-// Elements of one 16-byte load.
-template <typename T> struct Vec;
-template <> struct Vec<float> {
-  static constexpr int N = 4;
-  float x[4];
-  __device__ float get(int e) const { return clean(x[e]); }
-};
-template <> struct Vec<uint16_t> {
-  static constexpr int N = 8;
-  uint32_t x[4];
-  __device__ float get(int e) const {
-    return clean((e & 1) ? bf16_hi(x[e / 2]) : bf16_lo(x[e / 2]));
-  }
-};
-
-template <typename T> struct Unaligned;
-template <> struct Unaligned<float> {
-  typedef float type __attribute__((ext_vector_type(4), aligned(4)));
-};
-template <> struct Unaligned<uint16_t> {
-  typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2)));
-};
-
-// The vector at element i of a row of n; elements past the end are -inf.
+// A row that every pass reads again: f(logit, index) for the tokens of this thread.
 template <typename T>
-__device__ __forceinline__ Vec<T> load_vec(const T* row, int i, int n) {
-  Vec<T> v;
-  if (i + Vec<T>::N <= n) {
-    const auto r = *reinterpret_cast<const typename Unaligned<T>::type*>(row + i);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v.x[e] = r[e];
-  } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v.x[e] = i + e < n ? row[i + e] : -INFINITY;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t lo = i + 2 * e < n ? row[i + 2 * e] : 0xff80u;
-      const uint32_t hi = i + 2 * e + 1 < n ? row[i + 2 * e + 1] : 0xff80u;
-      v.x[e] = lo | hi << 16;
-    }
-  }
-  return v;
-}
-
-// A row: R > 0 vectors per thread held in registers, or R = 0, read again by every pass.
-template <typename T, int R>
 struct Row {
   static constexpr int N = Vec<T>::N;
   static constexpr int kStep = kThreads * N;
   const T* p;
   int n;
-  Vec<T> v[R > 0 ? R : 1];
 
-  __device__ void load(const T* row, int len) {
-    p = row;
-    n = len;
-    if constexpr (R > 0) {
-#pragma unroll
-      for (int j = 0; j < R; ++j)
-        if (j * kStep < n) v[j] = load_vec(p, j * kStep + int(threadIdx.x) * N, n);
-    }
-  }
   // f(vector, index of its first element); every thread makes the same calls.
   template <typename F>
   __device__ __forceinline__ void vectors(F f) const {
-    if constexpr (R > 0) {
+    constexpr int U = 4;
+    int i = int(threadIdx.x) * N;
+    int done = 0;
+    for (; done + U * kStep <= n; done += U * kStep) {
+      Vec<T> v[U];
 #pragma unroll
-      for (int j = 0; j < R; ++j)
-        if (j * kStep < n) f(v[j], j * kStep + int(threadIdx.x) * N);
-    } else {
-      for (int j = 0; j * kStep < n; ++j) {
-        const int i = j * kStep + int(threadIdx.x) * N;
-        f(load_vec(p, i, n), i);
-      }
+      for (int u = 0; u < U; ++u) v[u] = load_full(p + done + u * kStep + i);
+#pragma unroll
+      for (int u = 0; u < U; ++u) f(v[u], done + u * kStep + i);
     }
+    for (; done < n; done += kStep) f(load_part(p, done + i, n), done + i);
   }
-  // f(logit, index) for the tokens of this thread
   template <typename F>
   __device__ __forceinline__ void operator()(F f) const {
     vectors([&](const Vec<T>& x, int i) {
@@ -196,6 +330,18 @@ struct Row {
       for (int e = 0; e < N; ++e)
         if (i + e < n) f(x.get(e), uint32_t(i + e));
     });
+  }
+};
+
+struct ListRow {
+  const Shared& sm;
+  uint32_t n;
+  template <typename F>
+  __device__ __forceinline__ void operator()(F f) const {
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+      const uint2 c = sm.list[i];
+      f(__uint_as_float(c.x), c.y);
+    }
   }
 };
 
@@ -208,15 +354,10 @@ __device__ __forceinline__ void clear_bins(Shared& sm) {
   __syncthreads();
 }
 
-// The bin in which the cumulated count (or weight) reaches target >= 1; the last bin that
-// holds anything where it never does.
-__device__ __forceinline__ Found find_bin(Shared& sm, bool by_weight, u64 target) {
-  const int t = threadIdx.x, lane = t & (kWave - 1), wave = t / kWave;
-  __syncthreads();
-  const uint32_t c0 = sm.cnt[2 * t], c1 = sm.cnt[2 * t + 1];
-  const u64 w0 = sm.wgt[2 * t], w1 = sm.wgt[2 * t + 1];
-  uint32_t c = c0 + c1;
-  u64 w = w0 + w1;
+// Inclusive sums over the block, in thread order.
+__device__ __forceinline__ void block_scan(uint32_t& c, u64& w, uint32_t& all_c, u64& all_w,
+                                           Shared& sm) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
 #pragma unroll
   for (int o = 1; o < kWave; o <<= 1) {
     const uint32_t cu = __shfl_up(c, o);
@@ -226,25 +367,38 @@ __device__ __forceinline__ Found find_bin(Shared& sm, bool by_weight, u64 target
       w += wu;
     }
   }
+  __syncthreads();
   if (lane == kWave - 1) {
     sm.wave_cnt[wave] = c;
     sm.wave_wgt[wave] = w;
   }
   __syncthreads();
-  uint32_t cb = 0, ct = 0;
-  u64 wb = 0, wt = 0;
+  all_c = 0;
+  all_w = 0;
 #pragma unroll
   for (int i = 0; i < kWaves; ++i) {
     if (i < wave) {
-      cb += sm.wave_cnt[i];
-      wb += sm.wave_wgt[i];
+      c += sm.wave_cnt[i];
+      w += sm.wave_wgt[i];
     }
-    ct += sm.wave_cnt[i];
-    wt += sm.wave_wgt[i];
+    all_c += sm.wave_cnt[i];
+    all_w += sm.wave_wgt[i];
   }
-  const u64 goal = min(target, by_weight ? wt : u64(ct));
-  cb += c - c0 - c1;  // before bin 2 t
-  wb += w - w0 - w1;
+}
+
+// The bin in which the cumulated count (or weight) reaches target >= 1; the last bin that
+// holds anything where it never does.
+__device__ __forceinline__ Found find_bin(Shared& sm, bool by_weight, u64 target) {
+  const int t = threadIdx.x;
+  __syncthreads();
+  const uint32_t c0 = sm.cnt[2 * t], c1 = sm.cnt[2 * t + 1];
+  const u64 w0 = sm.wgt[2 * t], w1 = sm.wgt[2 * t + 1];
+  uint32_t cb = c0 + c1, all_c;
+  u64 wb = w0 + w1, all_w;
+  block_scan(cb, wb, all_c, all_w, sm);
+  cb -= c0 + c1;  // before bin 2 t
+  wb -= w0 + w1;
+  const u64 goal = min(target, by_weight ? all_w : u64(all_c));
   const u64 b0 = by_weight ? wb : cb, v0 = by_weight ? w0 : c0, v1 = by_weight ? w1 : c1;
   if (b0 < goal && b0 + v0 >= goal) sm.found = {uint32_t(2 * t), cb, c0, wb, w0};
   if (b0 + v0 < goal && b0 + v0 + v1 >= goal)
@@ -265,9 +419,8 @@ struct Cut {
 // The cut after the tokens whose count (or weight) reaches target, among those of `rows`
 // that pred takes; `upto` gets the weight up to it (where weights are wanted).
 template <typename Rows, typename Pred, typename Weight>
-__device__ __forceinline__ Cut descend(const Rows& rows, Pred pred, Weight weight,
-                                       bool want_weight, bool by_weight, u64 target, u64* upto,
-                                       Shared& sm) {
+__device__ __forceinline__ Cut descend(const Rows& rows, Pred pred, Weight weight, bool want_weight,
+                                    bool by_weight, u64 target, u64* upto, Shared& sm) {
   uint32_t prefix = 0, before_cnt = 0;
   u64 before_wgt = 0;
   Found f{};
@@ -316,10 +469,68 @@ __device__ __forceinline__ Cut descend(const Rows& rows, Pred pred, Weight weigh
   return cut;
 }
 
-// The race over the tokens that `kept` takes. A group is the vectors of 256 / N neighbouring
-// lanes.
-template <typename T, int R, typename Kept, typename Weight>
-__device__ __forceinline__ uint32_t race_row(const Row<T, R>& row, Kept kept, Weight weight,
+// Top-k's and top-p's cut among the tokens of `rows`. `total`: the weight that top-p's share is
+// of, where top-k does not give it.
+template <typename Rows, typename Weight>
+__device__ __forceinline__ Cut cut_rows(const Rows& rows, const Settings& set, double total,
+                                        Weight weight, Shared& sm) {
+  Cut cut{0xffffffffu, 0xffffffffu};
+  if (set.by_k) {
+    u64 upto = 0;
+    cut = descend(rows, [](float, uint32_t) { return true; }, weight, set.by_p, false,
+                  u64(set.top_k), &upto, sm);
+    total = double(upto) * 0x1p-42;
+  }
+  if (set.by_p) {
+    const Cut outer = cut;
+    const u64 target = max(u64(1), u64(ceil(fmax(double(set.top_p), 0.) * total * 0x1p42)));
+    cut = descend(rows, [outer](float x, uint32_t i) { return outer.keeps(x, i); }, weight, true,
+                  true, target, static_cast<u64*>(nullptr), sm);
+    // (all of a key's tokens: all that top-k left of them)
+    if (cut.key == outer.key) cut.index = min(cut.index, outer.index);
+  }
+  return cut;
+}
+
+// The race over the candidates that `kept` takes.
+template <typename Kept, typename Weight>
+__device__ __forceinline__ uint32_t race_list(const ListRow& rows, Kept kept, Weight weight,
+                                              const float* noise, int groups, Shared& sm) {
+  __syncthreads();
+  for (int g = threadIdx.x; g < groups; g += kThreads) sm.mass[g] = 0;
+  __syncthreads();
+  rows([&](float x, uint32_t i) {
+    if (kept(x, i)) atomicAdd(&sm.mass[i / kGroup], fixed(weight(x)));
+  });
+  __syncthreads();
+  u64 best = ~0ull;
+  for (int g = threadIdx.x; g < groups; g += kThreads)
+    if (sm.mass[g]) best = min(best, arrival(noise[kGroup + g] / float(sm.mass[g]), uint32_t(g)));
+  const uint32_t group = uint32_t(block_all(best, MinU(), sm));
+  best = ~0ull;
+  rows([&](float x, uint32_t i) {
+    if (i / kGroup == group && kept(x, i))
+      best = min(best, arrival(noise[i % kGroup] / weight(x), i));
+  });
+  return uint32_t(block_all(best, MinU(), sm));
+}
+
+// The race inside a group, over the tokens that `kept` takes.
+template <typename T, typename Kept, typename Weight>
+__device__ __forceinline__ uint32_t race_group(const Row<T>& row, uint32_t group, Kept kept,
+                                               Weight weight, const float* noise, Shared& sm) {
+  u64 best = ~0ull;
+  const int i = int(group) * kGroup + int(threadIdx.x);
+  if (threadIdx.x < kGroup && i < row.n) {
+    const float x = load_one(row.p + i);
+    if (kept(x, uint32_t(i))) best = arrival(noise[threadIdx.x] / weight(x), uint32_t(i));
+  }
+  return uint32_t(block_all(best, MinU(), sm));
+}
+
+// The race over the whole row. A group is the vectors of 256 / N neighbouring lanes.
+template <typename T, typename Kept, typename Weight>
+__device__ __forceinline__ uint32_t race_row(const Row<T>& row, Kept kept, Weight weight,
                                              const float* noise, Shared& sm) {
   constexpr int kLanes = kGroup / Vec<T>::N;
   u64 best = ~0ull;
@@ -328,113 +539,239 @@ __device__ __forceinline__ uint32_t race_row(const Row<T, R>& row, Kept kept, We
 #pragma unroll
     for (int e = 0; e < Vec<T>::N; ++e) {
       const float v = x.get(e);
-      if (i + e < row.n && kept(v, uint32_t(i + e))) w += weight(v);
+      if (kept(v, uint32_t(i + e))) w += weight(v);
     }
-#pragma unroll
-    for (int o = 1; o < kLanes; o <<= 1) w += __shfl_xor(w, o);
+    w = kLanes == 64 ? lanes_sum<6>(w) : lanes_sum<5>(w);
     if (w > 0.f && (threadIdx.x & (kLanes - 1)) == 0) {
       const int g = i / kGroup;
       best = min(best, arrival(noise[kGroup + g] / w, uint32_t(g)));
     }
   });
   const uint32_t group = uint32_t(block_all(best, MinU(), sm));
-  best = ~0ull;
-  const int i = int(group) * kGroup + int(threadIdx.x);
-  if (threadIdx.x < kGroup && i < row.n) {
-    float v;
-    if constexpr (sizeof(T) == 4) v = clean(row.p[i]);
-    else v = clean(bf16_to_f32(row.p[i]));
-    if (kept(v, uint32_t(i))) best = arrival(noise[threadIdx.x] / weight(v), uint32_t(i));
-  }
-  return uint32_t(block_all(best, MinU(), sm));
+  return race_group(row, group, kept, weight, noise, sm);
 }
 
-template <typename T, int R>
-__global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs args) {
+// Sorts one key per thread, ascending over the block; `n` of them matter, the others are ~0.
+__device__ __forceinline__ u64 block_sort(u64 v, uint32_t n, Shared& sm) {
+  u64* swap = sm.wgt;
+  const uint32_t t = threadIdx.x;
+#pragma unroll 1
+  for (uint32_t k = 2; k < 2 * n; k <<= 1) {
+#pragma unroll 1
+    for (uint32_t j = k / 2; j > 0; j >>= 1) {
+      u64 o;
+      if (j >= kWave) {
+        __syncthreads();
+        swap[t] = v;
+        __syncthreads();
+        o = swap[t ^ j];
+      } else {
+        o = __shfl_xor(v, int(j));
+      }
+      const bool up = (t & k) == 0, low = (t & j) == 0;
+      v = (up == low) ? min(v, o) : max(v, o);
+    }
+  }
+  return v;
+}
+
+// Candidates: every token whose logit `takes` accepts (a condition that holds for every larger
+// logit too), found through the maxima of the runs of 32 tokens. False where they are too many.
+template <typename T, typename Takes>
+__device__ __forceinline__ bool gather(const Row<T>& row, const float* sub_max, int n_sub,
+                                       Takes takes, Shared& sm) {
+  constexpr int N = Vec<T>::N, kLanes = kSub / N;
+  __syncthreads();
+  if (threadIdx.x == 0) sm.n_list = sm.n_subs = 0;
+  __syncthreads();
+  for (int s = threadIdx.x; s < n_sub; s += kThreads) {
+    if (takes(sub_max[s])) {
+      const uint32_t at = atomicAdd(&sm.n_subs, 1u);
+      if (at < kSubs) sm.subs[at] = uint32_t(s);
+    }
+  }
+  __syncthreads();
+  const uint32_t n = sm.n_subs;
+  if (n > kSubs) return false;
+  for (uint32_t at = threadIdx.x / kLanes; at < n; at += kThreads / kLanes) {
+    const int i = int(sm.subs[at]) * kSub + int(threadIdx.x % kLanes) * N;
+    const Vec<T> v = load_part(row.p, i, row.n);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float x = v.get(e);
+      if (i + e < row.n && takes(x)) {
+        const uint32_t to = atomicAdd(&sm.n_list, 1u);
+        if (to < kList) sm.list[to] = make_uint2(__float_as_uint(x), uint32_t(i + e));
+      }
+    }
+  }
+  __syncthreads();
+  return sm.n_list <= kList;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_finish_kernel(const SampleArgs args) {
   __shared__ Shared sm;
   const int64_t b = blockIdx.x;
-  const int V = args.V;
-  Row<T, R> row;
-  row.load(static_cast<const T*>(args.logits) + b * args.stride, V);
+  const int t = threadIdx.x, V = args.V, chunks = args.chunks;
+  const Row<T> row{static_cast<const T*>(args.logits) + b * args.stride, V};
   const float* noise = args.noise + b * args.noise_stride;
-  const float temp = args.temperature ? args.temperature[b] : args.temperature1;
-  const float top_p = args.top_p ? args.top_p[b] : args.top_p1;
-  const float min_p = args.min_p ? args.min_p[b] : args.min_p1;
-  const int32_t top_k = args.top_k ? args.top_k[b] : args.top_k1;
-  const bool greedy = !(temp > 0.f);
-  const bool by_k = top_k > 0 && top_k < V;
-  const bool by_p = top_p < 1.f;
+  const Settings set = settings(args, b);
+  const float2* chunk = args.chunk + b * chunks;
+  const float* sub_max = args.sub_max + b * chunks * kChunkSubs;
+  const float* mass = args.mass + b * chunks * kChunkGroups;
+  const int groups = (V + kGroup - 1) / kGroup, n_sub = (V + kSub - 1) / kSub;
 
-  float tmax = -INFINITY;
-  row([&](float x, uint32_t) { tmax = fmaxf(tmax, x); });
-  const float top = block_all(tmax, MaxF(), sm);
+  float m = -INFINITY;
+  for (int i = t; i < chunks; i += kThreads) m = fmaxf(m, chunk[i].x);
+  const float top = block_all(m, MaxF(), sm);
   if (top == -INFINITY) {  // nothing to choose from
-    if (threadIdx.x == 0) {
+    if (t == 0) {
       args.tokens[b] = -1;
       if (args.logprobs) args.logprobs[b] = -INFINITY;
     }
     return;
   }
-  // w = 2^((x - top) c); the clamp keeps c and every product a number
-  const float c = kLog2e / fminf(fmaxf(temp, 0x1p-60f), 0x1p60f);
-  auto weight = [&](float x) { return __builtin_amdgcn_exp2f((x - top) * c); };
-  const float floor_z = min_p > 0.f ? log2f(fminf(min_p, 1.f)) : -INFINITY;
-  auto over_floor = [&](float x) { return (x - top) * c >= floor_z; };
-
-  double total = 0., raw = 0.;
+  auto weight = [top, c = set.c](float x) { return exp2_hw((x - top) * c); };
+  auto over_floor = [top, c = set.c, z = set.floor_z](float x) { return (x - top) * c >= z; };
+  double raw = 0.;
   if (args.logprobs) {
-    float s = 0.f;
-    row([&](float x, uint32_t) { s += __builtin_amdgcn_exp2f((x - top) * kLog2e); });
-    raw = block_all(double(s), AddD(), sm);
+    for (int i = t; i < chunks; i += kThreads) {
+      const float2 h = chunk[i];
+      raw += double(h.y) * double(exp2_hw((h.x - top) * 1.44269504088896340736f));
+    }
+    raw = block_all(raw, AddD(), sm);
   }
+  // a group's weight relative to the row's maximum
+  auto group_weight = [&](int g) {
+    return mass[g] * exp2_hw((chunk[g / kChunkGroups].x - top) * set.c);
+  };
+
   uint32_t token;
-  if (greedy) {
-    u64 best = ~0ull;
-    row([&](float x, uint32_t i) { best = min(best, u64(order_key(x)) << 32 | i); });
+  if (set.greedy) {
+    u64 best = ~0ull;  // the first run that holds the maximum, and the first such token in it
+    for (int s = t; s < n_sub; s += kThreads)
+      if (sub_max[s] == top) best = min(best, u64(s));
+    const int i = int(block_all(best, MinU(), sm)) * kSub + t;
+    best = t < kSub && i < V && load_one(row.p + i) == top ? u64(i) : ~0ull;
     token = uint32_t(block_all(best, MinU(), sm));
-  } else if (!by_k && !by_p) {
-    token = race_row(row, [&](float x, uint32_t) { return over_floor(x); }, weight, noise, sm);
+  } else if (!set.by_k && !set.by_p && set.floor_z == -INFINITY) {
+    u64 best = ~0ull;
+    for (int g = t; g < groups; g += kThreads) {
+      const float w = group_weight(g);
+      if (w > 0.f) best = min(best, arrival(noise[kGroup + g] / w, uint32_t(g)));
+    }
+    const uint32_t group = uint32_t(block_all(best, MinU(), sm));
+    token = race_group(row, group, [](float, uint32_t) { return true; }, weight, noise, sm);
   } else {
-    if (by_p && !by_k) {
-      float s = 0.f;
-      row([&](float x, uint32_t) { s += weight(x); });
-      total = block_all(double(s), AddD(), sm);
+    double total = 0.;
+    if (set.by_p && !set.by_k) {
+      for (int g = t; g < groups; g += kThreads) total += double(group_weight(g));
+      total = block_all(total, AddD(), sm);
     }
-    auto all = [](float, uint32_t) { return true; };
-    Cut cut{0xffffffffu, 0xffffffffu};
-    if (by_k) {
-      u64 upto = 0;
-      cut = descend(row, all, weight, by_p, false, u64(top_k), &upto, sm);
-      total = double(upto) * 0x1p-42;
+    const u64 share = max(u64(1), u64(ceil(fmax(double(set.top_p), 0.) * total * 0x1p42)));
+    bool done = false, listed = groups <= kListGroups;
+    if (listed && (set.by_k || set.by_p)) {
+      // Distance from the maximum in 2,048 steps: the run maxima's histogram says from which
+      // step on there are at least top_k tokens (the runs' maxima alone are that many), or, for
+      // top-p alone, a first guess at how far down its tokens reach.
+      const float scale = 128.f * fminf(set.c, 1.f);
+      auto step = [top, scale](float x) {
+        return uint32_t(fminf((top - x) * scale, float(kBins - 1)));
+      };
+      clear_bins(sm);
+      for (int s = t; s < n_sub; s += kThreads) atomicAdd(&sm.cnt[step(sub_max[s])], 1u);
+      const int want = set.by_k ? set.top_k : V <= kThreads ? V : min(512, (n_sub + 1) / 2);
+      const uint32_t last = want > n_sub ? kBins - 1 : find_bin(sm, false, u64(want)).bin;
+      // (min-p may thin the candidates only where top-p's share does not count them)
+      const bool thin = !set.by_p;
+      listed = gather(row, sub_max, n_sub, [=](float x) {
+        return step(x) <= last && (!thin || over_floor(x)); }, sm);
+    } else if (listed) {
+      listed = gather(row, sub_max, n_sub, over_floor, sm);
     }
-    if (by_p) {
-      const Cut outer = cut;
-      const u64 target = max(u64(1), u64(ceil(fmax(double(top_p), 0.) * total * 0x1p42)));
-      cut = descend(row, [&](float x, uint32_t i) { return outer.keeps(x, i); }, weight, true,
-                    true, target, static_cast<u64*>(nullptr), sm);
-      // (all of a key's tokens: all that top-k left of them)
-      if (cut.key == outer.key) cut.index = min(cut.index, outer.index);
+    if (listed) {
+      const uint32_t n = sm.n_list;
+      const ListRow rows{sm, n};
+      if (!set.by_k && !set.by_p) {
+        token = race_list(rows, [](float, uint32_t) { return true; }, weight, noise, groups, sm);
+        done = true;
+      } else if (n <= kThreads) {
+        u64 v = ~0ull;
+        if (uint32_t(t) < n)
+          v = u64(order_key(__uint_as_float(sm.list[t].x))) << 32 | sm.list[t].y;
+        v = block_sort(v, n, sm);
+        const float x = key_logit(uint32_t(v >> 32));
+        const bool mine = uint32_t(t) < n && (!set.by_k || t < set.top_k);
+        const u64 w = mine ? fixed(weight(x)) : 0;
+        u64 upto = w, all;
+        uint32_t one = 0, none;
+        block_scan(one, upto, none, all, sm);
+        const u64 target =
+            set.by_k ? max(u64(1), u64(ceil(fmax(double(set.top_p), 0.) * double(all)))) : share;
+        if (set.by_k || all >= share) {
+          const bool kept = mine && (t == 0 || !set.by_p || upto - w < target);
+          if (kept) sm.list[t] = make_uint2(__float_as_uint(x), uint32_t(v));
+          const ListRow first{sm, uint32_t(__syncthreads_count(kept))};
+          token = race_list(first, [=](float x, uint32_t) { return over_floor(x); }, weight,
+                            noise, groups, sm);
+          done = true;
+        }
+      } else {
+        u64 in_list = 0;
+        bool enough = set.by_k;
+        if (!enough) {
+          rows([&](float x, uint32_t) { in_list += fixed(weight(x)); });
+          enough = block_all(in_list, AddU(), sm) >= share;
+        }
+        if (enough) {
+          const Cut cut = cut_rows(rows, set, total, weight, sm);
+          token = race_list(rows, [=](float x, uint32_t i) {
+            return cut.keeps(x, i) && over_floor(x); }, weight, noise, groups, sm);
+          done = true;
+        }
+      }
     }
-    token = race_row(row, [&](float x, uint32_t i) { return cut.keeps(x, i) && over_floor(x); },
-                     weight, noise, sm);
+    if (!done) {
+      const Cut cut = cut_rows(row, set, total, weight, sm);
+      token = race_row(row, [=](float x, uint32_t i) {
+        return cut.keeps(x, i) && over_floor(x); }, weight, noise, sm);
+    }
   }
-  if (threadIdx.x == 0) {
+  if (t == 0) {
     args.tokens[b] = int32_t(token);
-    if (args.logprobs) {
-      const T* p = static_cast<const T*>(args.logits) + b * args.stride;
-      float x;
-      if constexpr (sizeof(T) == 4) x = clean(p[token]);
-      else x = clean(bf16_to_f32(p[token]));
-      args.logprobs[b] = float(double(x - top) - log(raw));
-    }
+    if (args.logprobs)
+      args.logprobs[b] = float(double(load_one(row.p + token) - top) - log(raw));
   }
 }
 
+size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
+
+struct Layout {
+  size_t sub_max, mass, chunk, bytes;
+  int32_t chunks;
+};
+
+Layout layout(int64_t rows, int32_t vocab) {
+  Layout l;
+  l.chunks = (vocab + kChunk - 1) / kChunk;
+  const size_t n = size_t(rows) * l.chunks;
+  l.sub_max = 0;
+  l.mass = align256(n * kChunkSubs * sizeof(float));
+  l.chunk = l.mass + align256(n * kChunkGroups * sizeof(float));
+  l.bytes = l.chunk + align256(n * sizeof(float2));
+  return l;
+}
+
 template <typename T>
-int launch(const SampleArgs& args, int32_t rows, hipStream_t s) {
-  constexpr int kStep = Row<T, 0>::kStep;
-  if (args.V <= 16 * kStep) sample_kernel<T, 16><<<rows, kThreads, 0, s>>>(args);
-  else sample_kernel<T, 0><<<rows, kThreads, 0, s>>>(args);
+int launch(const SampleArgs& args, hipStream_t s) {
+  const int64_t waves = int64_t(args.rows) * args.chunks;
+  const int64_t blocks = (waves * kWave + kScanThreads - 1) / kScanThreads;
+  if (blocks > 0x7fffffff) return WKV7_ERR_ARG;
+  sample_scan_kernel<T><<<unsigned(blocks), kScanThreads, 0, s>>>(args);
+  const int rc = launch_status();
+  if (rc != WKV7_OK) return rc;
+  sample_finish_kernel<T><<<unsigned(args.rows), kThreads, 0, s>>>(args);
   return launch_status();
 }
 
@@ -443,10 +780,16 @@ int launch(const SampleArgs& args, int32_t rows, hipStream_t s) {
 
 using namespace wkv7;
 
+extern "C" size_t wkv7_sample_workspace_bytes(int32_t rows, int32_t vocab) {
+  if (rows < 1 || vocab < 1 || vocab > WKV7_SAMPLE_MAX_VOCAB) return 0;
+  return layout(rows, vocab).bytes;
+}
+
 extern "C" int wkv7_sample_tokens(const void* logits, int32_t logits_dtype, int32_t rows,
                                   int32_t vocab, int64_t row_stride, const float* noise,
                                   int64_t noise_stride, const struct wkv7_sample_params* params,
-                                  int32_t* tokens, float* logprobs, void* stream) {
+                                  int32_t* tokens, float* logprobs, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
   if (rows < 0 || vocab < 1 || !params) return WKV7_ERR_ARG;
   if (logits_dtype != WKV7_Y_BF16 && logits_dtype != WKV7_Y_F32) return WKV7_ERR_ARG;
   if (rows == 0) return WKV7_OK;
@@ -457,6 +800,10 @@ extern "C" int wkv7_sample_tokens(const void* logits, int32_t logits_dtype, int3
   const size_t width = logits_dtype == WKV7_Y_F32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(logits) % width || reinterpret_cast<uintptr_t>(noise) % 4)
     return WKV7_ERR_SHAPE;
+  const Layout l = layout(rows, vocab);
+  if (!workspace || workspace_bytes < l.bytes || reinterpret_cast<uintptr_t>(workspace) % 16)
+    return WKV7_ERR_WORKSPACE;
+  char* ws = static_cast<char*>(workspace);
   const SampleArgs args{logits,
                         row_stride,
                         noise,
@@ -470,8 +817,13 @@ extern "C" int wkv7_sample_tokens(const void* logits, int32_t logits_dtype, int3
                         params->min_p1,
                         params->top_k1,
                         vocab,
+                        rows,
+                        l.chunks,
                         tokens,
-                        logprobs};
-  return logits_dtype == WKV7_Y_F32 ? launch<float>(args, rows, as_stream(stream))
-                                    : launch<uint16_t>(args, rows, as_stream(stream));
+                        logprobs,
+                        reinterpret_cast<float*>(ws + l.sub_max),
+                        reinterpret_cast<float*>(ws + l.mass),
+                        reinterpret_cast<float2*>(ws + l.chunk)};
+  return logits_dtype == WKV7_Y_F32 ? launch<float>(args, as_stream(stream))
+                                    : launch<uint16_t>(args, as_stream(stream));
 }

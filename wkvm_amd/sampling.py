@@ -101,9 +101,11 @@ def sample_tokens(logits: torch.Tensor, noise: torch.Tensor, *, temperature=1.0,
         return tokens, logp
     params = _lib.SampleParams(*(ops._ptr(t) for t, _ in got.values()),
                                *(v for _, v in got.values()))
-    rc = _lib.load().wkv7_sample_tokens(
+    lib = _lib.load()
+    ws = torch.empty(lib.wkv7_sample_workspace_bytes(B, V), dtype=torch.uint8, device=dev)
+    rc = lib.wkv7_sample_tokens(
         logits.data_ptr(), code, B, V, logits.stride(0) if B > 1 else V, noise.data_ptr(),
         noise.stride(0) if B > 1 else noise.shape[1], params, tokens.data_ptr(), ops._ptr(logp),
-        ops._stream_ptr(dev))
+        ws.data_ptr(), ws.numel(), ops._stream_ptr(dev))
     _lib.check(rc, "wkv7_sample_tokens")
     return tokens, logp

@@ -579,6 +579,56 @@ int wkv7_proj_grouped_noalloc(int64_t m, const wkv7_proj_group *groups, int32_t 
                               void *stream);
 
 /*
+ * wkv7_proj_grouped with a low-rank adapter of each row's own request beside the
+ * shared weights: for row m with adapter a = ids[m] (-1: none) and every product g,
+ *     y[m] = act( x[m] w^T + bias + scale_a (x[m] A_a^T) B_a^T )
+ * bf16 operands, fp32 sums (x A^T enters the second product with all of its 24
+ * bits), and y is rounded once. Any number of rows (one token of each
+ * request, or the tokens of many prompts), any mix of adapters.
+ *
+ * No counterpart in the reference, whose model layers are nn.Linear calls without
+ * adapters (external; reached through the model forward,
+ * wkvm/runner/runner.py:80-88). It serves fine-tuned requests from one base model.
+ *
+ * A set holds the adapters of one product's weight, all of them loaded once:
+ *   a      [count][16 slabs][k] bf16, 16-byte aligned: A_a's rows, then zeros
+ *   b      [count][slabs][n][16] bf16, 16-byte aligned: B_a's columns in slabs of 16,
+ *          zeros past its rank
+ *   scale  [count] fp32;  rank [count] int32 (0: this product has no such adapter)
+ * a == NULL: a product without adapters. All pointers are device memory.
+ *
+ * wkv7_adapter_plan writes the order in which the rows are visited (by adapter) to
+ * host memory: wkv7_adapter_plan_ints(m, count) int32, from ids [m] on the host; an id
+ * outside [-1, count) is WKV7_ERR_ARG. wkv7_proj_adapters reads a device copy of it
+ * (16-byte aligned); count there is the plan's, at most every set's.
+ *
+ *   groups, ngroups   as wkv7_proj_grouped (same alignment rules)
+ *   workspace         device, 16-byte aligned, at least
+ *                     wkv7_proj_adapters_workspace_bytes(..) (else
+ *                     WKV7_ERR_WORKSPACE); holds nothing between calls
+ */
+#define WKV7_ADAPTER_SLAB 16
+#define WKV7_ADAPTER_MAX_RANK 256
+
+typedef struct wkv7_adapter_set {
+  const uint16_t *a;
+  const uint16_t *b;
+  const float *scale;
+  const int32_t *rank;
+  int32_t count;
+  int32_t slabs;
+} wkv7_adapter_set;
+
+int64_t wkv7_adapter_plan_ints(int64_t m, int32_t count);
+int wkv7_adapter_plan(const int32_t *ids, int64_t m, int32_t count, int32_t *plan,
+                      int64_t plan_ints);
+int wkv7_proj_adapters(int64_t m, const wkv7_proj_group *groups, const wkv7_adapter_set *sets,
+                       int32_t ngroups, const int32_t *plan, int32_t count, void *workspace,
+                       size_t workspace_bytes, void *stream);
+size_t wkv7_proj_adapters_workspace_bytes(int64_t m, const wkv7_proj_group *groups,
+                                          const wkv7_adapter_set *sets, int32_t ngroups);
+
+/*
  * The next token of every row of a batch of logits, by the row's own settings and
  * from given random numbers, and the token's log-probability.
  *

@@ -1,0 +1,309 @@
+"""proj_adapters against the formula in 64 bits.
+
+The kernel's sums are fp32, x A^T enters the second product with all of its 24 bits, and y
+is rounded once to bf16 (half an ulp). An output is therefore within one bf16 ulp of the
+exact value, where an output much smaller than its terms is measured by the ulp of 1/256 of
+the outputs' scale: cancellation leaves the sums' absolute error, which random sums of
+k <= 4096 terms keep below a third of that ulp (2^-24 sqrt(k) of the scale against 2^-16 of it).
+"""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from wkvm_amd import AdapterBank, adapter_plan, ops, proj_adapters
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    return torch.device("cuda", 0)
+
+
+def _rand(shape, gen, dev, std=1.0):
+    return (torch.randn(shape, generator=gen) * std).to(torch.bfloat16).to(dev)
+
+
+def _bank(gen, dev, ranks, k, n, max_rank=None):
+    """A bank of adapters (rank 0: an empty place) and its pairs."""
+    bank = AdapterBank(len(ranks), k, n, max_rank or max(max(ranks), 1), dev)
+    pairs = []
+    for i, r in enumerate(ranks):
+        if r == 0:
+            pairs.append(None)
+            continue
+        a = _rand((r, k), gen, dev, 1 / math.sqrt(k))
+        b = _rand((n, r), gen, dev, 0.5 / math.sqrt(r))
+        s = 1.0 + 0.25 * i
+        bank.load(i, a, b, s)
+        pairs.append((a, b, s))
+    return bank, pairs
+
+
+def _exact(x, w, bias, act, pairs, ids):
+    x = x.double().cpu()
+    y = x @ w.double().cpu().T
+    for a, pair in enumerate(pairs or []):
+        rows = np.flatnonzero(np.asarray(ids) == a)
+        if pair is None or rows.size == 0:
+            continue
+        A, B, s = pair
+        y[rows] += s * (x[rows] @ A.double().cpu().T) @ B.double().cpu().T
+    if bias is not None:
+        y = y + bias.double().cpu()
+    return torch.tanh(y) if act == "tanh" else torch.sigmoid(y) if act == "sigmoid" else y
+
+
+def _assert_close(got, exact):
+    got = got.double().cpu()
+    mag = exact.abs().clamp_min(exact.pow(2).mean().sqrt().item() / 256 + 1e-30)
+    ulp = torch.exp2(torch.floor(torch.log2(mag)) - 7)
+    worst = ((got - exact).abs() / ulp).max().item()
+    assert worst <= 1.0, f"max error {worst:.3f} bf16 ulp"
+
+
+def _ids(kind, m, count, rng):
+    if kind == "none":
+        return np.full(m, -1)
+    if kind == "one":
+        return np.zeros(m, int)
+    if kind == "each":
+        return np.arange(m) % count
+    if kind == "runs":
+        return np.sort(rng.integers(-1, count, m))
+    return rng.integers(-1, count, m)  # any order, some without
+
+
+@pytest.mark.parametrize("kind", ["none", "one", "each", "runs", "any"])
+@pytest.mark.parametrize("m", [1, 2, 15, 16, 17, 33, 64, 129, 300, 512, 513, 1111])
+def test_rows_and_mixes(dev, m, kind):
+    gen = torch.Generator().manual_seed(m)
+    k, n, ranks = 256, 208, [16, 8, 1, 33, 5, 0, 64, 17, 16]
+    x, w = _rand((m, k), gen, dev), _rand((n, k), gen, dev, 1 / math.sqrt(k))
+    bank, pairs = _bank(gen, dev, ranks, k, n)
+    ids = _ids(kind, m, len(ranks), np.random.default_rng(m))
+    (y,) = proj_adapters([(x, w, None, None, bank)], adapter_plan(ids.tolist(), len(ranks), dev))
+    _assert_close(y, _exact(x, w, None, None, pairs, ids))
+
+
+@pytest.mark.parametrize("k,n", [(32, 1), (64, 16), (96, 17), (768, 768), (1056, 65), (2048, 2048),
+                                 (2080, 529), (4096, 300)])
+@pytest.mark.parametrize("m", [1, 5, 16, 40, 200, 700])
+def test_widths(dev, m, k, n):
+    gen = torch.Generator().manual_seed(k + n)
+    ranks = [16, 40, 3]
+    x, w = _rand((m, k), gen, dev), _rand((n, k), gen, dev, 1 / math.sqrt(k))
+    bias = _rand((n,), gen, dev)
+    bank, pairs = _bank(gen, dev, ranks, k, n)
+    ids = np.random.default_rng(k).integers(-1, 3, m)
+    (y,) = proj_adapters([(x, w, bias, "tanh", bank)], adapter_plan(ids, 3, dev))
+    _assert_close(y, _exact(x, w, bias, "tanh", pairs, ids))
+
+
+@pytest.mark.parametrize("rank", [1, 4, 15, 16, 31, 32, 64, 100, 128, 255, 256])
+@pytest.mark.parametrize("m", [3, 48, 600])
+def test_ranks(dev, m, rank):
+    gen = torch.Generator().manual_seed(rank)
+    k, n = 512, 320
+    x, w = _rand((m, k), gen, dev), _rand((n, k), gen, dev, 1 / math.sqrt(k))
+    bank, pairs = _bank(gen, dev, [rank, max(1, rank // 3), rank], k, n)
+    ids = np.random.default_rng(rank).integers(-1, 3, m)
+    (y,) = proj_adapters([(x, w, None, None, bank)], adapter_plan(ids, 3, dev))
+    _assert_close(y, _exact(x, w, None, None, pairs, ids))
+
+
+@pytest.mark.parametrize("m", [1, 9, 64, 256, 1500])
+def test_a_group_of_products(dev, m):
+    """Different inputs, widths, activations and banks in one call; one product has none."""
+    gen = torch.Generator().manual_seed(m)
+    count = 6
+    ids = np.random.default_rng(m).integers(-1, count, m)
+    prods, exact = [], []
+    for i, (k, n, act) in enumerate([(768, 768, None), (768, 96, "tanh"), (2048, 64, "sigmoid"),
+                                     (128, 1024, None)]):
+        x, w = _rand((m, k), gen, dev), _rand((n, k), gen, dev, 1 / math.sqrt(k))
+        bias = _rand((n,), gen, dev) if i % 2 else None
+        bank, pairs = (None, None) if i == 2 else _bank(gen, dev, [16, 8, 32, 16, 0, 4], k, n, 48)
+        prods.append((x, w, bias, act, bank))
+        exact.append(_exact(x, w, bias, act, pairs, ids))
+    for y, e in zip(proj_adapters(prods, adapter_plan(ids, count, dev)), exact):
+        _assert_close(y, e)
+
+
+def test_many_rows_and_adapters(dev):
+    """A prefill's row count over the 1.5B width."""
+    gen = torch.Generator().manual_seed(7)
+    m, k, n = 4100, 2048, 2048
+    x, w = _rand((m, k), gen, dev), _rand((n, k), gen, dev, 1 / math.sqrt(k))
+    bank, pairs = _bank(gen, dev, [16, 32, 8, 16], k, n)
+    ids = np.repeat([2, -1, 0, 3, 1, 0], [1000, 37, 900, 1163, 1, 999])
+    (y,) = proj_adapters([(x, w, None, None, bank)], adapter_plan(ids, 4, dev))
+    _assert_close(y, _exact(x, w, None, None, pairs, ids))
+
+
+def test_without_adapters_it_is_the_grouped_projection(dev):
+    """Rows without an adapter get proj_grouped's own bits, in batches of either kernel."""
+    gen = torch.Generator().manual_seed(11)
+    for m in (4, 100, 400):
+        x, w = _rand((m, 2048), gen, dev), _rand((2048, 2048), gen, dev, 1 / math.sqrt(2048))
+        bank, _ = _bank(gen, dev, [16, 16], 2048, 2048)
+        (want,) = ops.proj_grouped([(x, w)])
+        (none,) = proj_adapters([(x, w, None, None, bank)], adapter_plan([-1] * m, 2, dev))
+        assert torch.equal(none, want)
+        ids = [0 if i % 3 else -1 for i in range(m)]
+        (some,) = proj_adapters([(x, w, None, None, bank)], adapter_plan(ids, 2, dev))
+        base = [i for i in range(m) if i % 3 == 0]
+        assert torch.equal(some[base], want[base])
+
+
+def test_strided_inputs_and_outputs(dev):
+    gen = torch.Generator().manual_seed(13)
+    m, k, n = 70, 256, 130
+    wide = _rand((m, 3 * k + 8), gen, dev)
+    x = wide[:, k:2 * k]
+    w = _rand((n, k), gen, dev, 1 / math.sqrt(k))
+    bank, pairs = _bank(gen, dev, [16, 8], k, n)
+    ids = np.arange(m) % 3 - 1
+    out = torch.zeros((m, n + 11), dtype=torch.bfloat16, device=dev)
+    plan = adapter_plan(ids, 2, dev)
+    proj_adapters([(x, w, None, None, bank)], plan, outs=[out[:, 3:3 + n]])
+    _assert_close(out[:, 3:3 + n], _exact(x, w, None, None, pairs, ids))
+    assert not out[:, :3].any() and not out[:, 3 + n:].any()
+    odd = wide[:, 1:1 + k]  # not 16-byte aligned: copied
+    (y,) = proj_adapters([(odd, w, None, None, bank)], plan)
+    _assert_close(y, _exact(odd, w, None, None, pairs, ids))
+    none = proj_adapters([(x[:0], w, None, None, bank)], adapter_plan([], 2, dev))
+    assert none[0].shape == (0, n)
+
+
+@pytest.mark.parametrize("m", [8, 48, 640])
+def test_a_broken_adapter_stays_with_its_rows(dev, m):
+    """Infinities and NaN in one adapter, or in one row, reach no other row."""
+    gen = torch.Generator().manual_seed(17)
+    k, n = 256, 96
+    x, w = _rand((m, k), gen, dev), _rand((n, k), gen, dev, 1 / math.sqrt(k))
+    bank, pairs = _bank(gen, dev, [8, 8, 8], k, n)
+    ids = np.arange(m) % 4 - 1
+    plan = adapter_plan(ids, 3, dev)
+    (want,) = proj_adapters([(x, w, None, None, bank)], plan)
+    a, b, s = pairs[1]
+    b = b.clone()
+    b[::5] = math.nan
+    b[1::5] = math.inf
+    bank.load(1, a, b, s)
+    (got,) = proj_adapters([(x, w, None, None, bank)], plan)
+    others = np.flatnonzero(ids != 1)
+    assert torch.equal(got[others], want[others])
+    assert not got[np.flatnonzero(ids == 1)][:, ::5].isfinite().any()
+    bank.load(1, a, pairs[1][1], s)
+    bad = x.clone()
+    bad[5] = math.inf
+    (got,) = proj_adapters([(bad, w, None, None, bank)], plan)
+    rest = [i for i in range(m) if i != 5]
+    assert torch.equal(got[rest], want[rest])
+
+
+def test_an_infinite_term_is_infinite_as_in_the_formula(dev):
+    """h = inf in one rank: its column of B gives inf, not NaN from a rounding part or a
+    padding rank."""
+    k, n = 32, 16
+    x = torch.zeros((1, k), dtype=torch.bfloat16, device=dev)
+    x[0, 0] = math.inf
+    w = torch.full((n, k), 0.0, dtype=torch.bfloat16, device=dev)
+    w[:, 0] = 1.0  # (and zeros times x's zeros elsewhere)
+    bank = AdapterBank(1, k, n, 16, dev)
+    a = torch.zeros((1, k), dtype=torch.bfloat16, device=dev)
+    a[0, 0] = 1.0
+    bank.load(0, a, torch.ones((n, 1), dtype=torch.bfloat16, device=dev))
+    (y,) = proj_adapters([(x, w, None, None, bank)], adapter_plan([0], 1, dev))
+    assert bool((y == math.inf).all())
+
+
+def test_places_are_loaded_replaced_and_cleared(dev):
+    gen = torch.Generator().manual_seed(19)
+    m, k, n = 20, 128, 64
+    x, w = _rand((m, k), gen, dev), _rand((n, k), gen, dev, 1 / math.sqrt(k))
+    bank, pairs = _bank(gen, dev, [40, 40], k, n)
+    ids = np.arange(m) % 2
+    plan = adapter_plan(ids, 2, dev)
+    a, b = _rand((7, k), gen, dev, 0.1), _rand((n, 7), gen, dev)  # fewer ranks than before
+    bank.load(1, a, b, 0.5)
+    (y,) = proj_adapters([(x, w, None, None, bank)], plan)
+    _assert_close(y, _exact(x, w, None, None, [pairs[0], (a, b, 0.5)], ids))
+    bank.clear(0)
+    (y,) = proj_adapters([(x, w, None, None, bank)], plan)
+    _assert_close(y, _exact(x, w, None, None, [None, (a, b, 0.5)], ids))
+
+
+def test_calls_repeat_and_run_on_other_streams(dev):
+    gen = torch.Generator().manual_seed(23)
+    m, k, n = 90, 1024, 512
+    x, w = _rand((m, k), gen, dev), _rand((n, k), gen, dev, 1 / math.sqrt(k))
+    bank, _ = _bank(gen, dev, [16] * 12, k, n)
+    plan = adapter_plan(np.arange(m) % 13 - 1, 12, dev)
+    (want,) = proj_adapters([(x, w, None, None, bank)], plan)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        (got,) = proj_adapters([(x, w, None, None, bank)], plan)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("m", [6, 60])
+def test_under_graph_capture(dev, m):
+    gen = torch.Generator().manual_seed(29)
+    k, n = 2048, 256
+    x, w = _rand((m, k), gen, dev), _rand((n, k), gen, dev, 1 / math.sqrt(k))
+    bank, pairs = _bank(gen, dev, [16, 8, 32], k, n)
+    ids = np.arange(m) % 4 - 1
+    plan = adapter_plan(ids, 3, dev)
+    proj_adapters([(x, w, None, None, bank)], plan)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (out,) = proj_adapters([(x, w, None, None, bank)], plan)
+    for i in range(3):
+        x.copy_(_rand((m, k), gen, dev))
+        graph.replay()
+        torch.cuda.synchronize()
+        (eager,) = proj_adapters([(x, w, None, None, bank)], plan)
+        assert torch.equal(out, eager)
+        _assert_close(out, _exact(x, w, None, None, pairs, ids))
+
+
+def test_refusals(dev):
+    gen = torch.Generator().manual_seed(31)
+    k, n = 64, 48
+    x, w = _rand((4, k), gen, dev), _rand((n, k), gen, dev)
+    bank, _ = _bank(gen, dev, [8, 8], k, n)
+    plan = adapter_plan([0, 1, -1, 0], 2, dev)
+    for ids in ([2], [-2], [0, 5]):
+        with pytest.raises(ValueError, match="out of range"):
+            adapter_plan(ids, 2, dev)
+    for prods, p in [([(x[:3], w, None, None, bank)], plan),              # rows of the plan
+                     ([(x, w[:, :32], None, None, bank)], plan),           # k of x and w
+                     ([(x, w[:40], None, None, bank)], plan),              # n of the bank
+                     ([(x, w, None, None, bank)], adapter_plan([0] * 4, 3, dev)),
+                     ([(x.float(), w, None, None, bank)], plan),
+                     ([(x.cpu(), w, None, None, bank)], plan),
+                     ([(x, w, None, "relu", bank)], plan), ([], plan),
+                     ([(x, w, None, None, bank)] * 9, plan),
+                     ([(x, w, None, None, bank)], adapter_plan([0] * 4, 2, "cpu"))]:
+        with pytest.raises(ValueError):
+            proj_adapters(prods, p)
+    a, b = _rand((8, k), gen, dev), _rand((n, 8), gen, dev)
+    for args in [(2, a, b), (-1, a, b), (0, a.float(), b), (0, a, b[:, :4]), (0, a[:, :32], b),
+                 (0, _rand((9, k), gen, dev), _rand((n, 9), gen, dev)), (0, a, b, math.nan)]:
+        with pytest.raises(ValueError):
+            bank.load(*args)
+    with pytest.raises(ValueError):
+        bank.clear(7)
+    for args in [(0, k, n, 8), (1, 40, n, 8), (1, k, 0, 8), (1, k, n, 0), (1, k, n, 257)]:
+        with pytest.raises(ValueError):
+            AdapterBank(*args, dev)

@@ -14,12 +14,15 @@ reference's slot-tensor layout and op signatures:
   reference's model layer calls
 * ``DecodeGraph`` -- a decode step's WKV launches captured as one HIP graph
   (the role of experiments/m2_engine_bench.py GraphedDecode)
+* ``AdapterBank`` / ``proj_adapters`` -- projections with low-rank adapters of
+  each request's own
 * ``sample_tokens`` -- a batch's next tokens by per-request settings
   (wkvm/runner/sampling.py)
 * ``StateStore`` -- HOT/WARM/COLD state handles, wkvm/store.py, with the
   HOT <-> WARM copies as strided DMA transfers
 """
 
+from .adapters import AdapterBank, AdapterPlan, adapter_plan, proj_adapters
 from .layout import HEAD_SIZE, WKV_DTYPE, ModelStateSpec, RWKV7StateLayout, StateFamilySpec
 from .ops import (
     chunk_rwkv7,
@@ -41,5 +44,5 @@ __all__ = [
     "StateStore", "StateRecord", "FingerprintMismatch",
     "wkv7_decode_slots", "wkv7_prefill_varlen", "slot_copy", "slot_zero",
     "chunk_rwkv7", "fused_recurrent_rwkv7",
-    "sample_tokens", "sample_noise_size",
+    "AdapterBank", "AdapterPlan", "adapter_plan", "proj_adapters", "sample_tokens", "sample_noise_size",
 ]

@@ -40,6 +40,8 @@ WKV7_PROJ_FEW_ROWS = 16
 WKV7_ACT_NONE = 0
 WKV7_ACT_TANH = 1
 WKV7_ACT_SIGMOID = 2
+WKV7_ADAPTER_SLAB = 16
+WKV7_ADAPTER_MAX_RANK = 256
 WKV7_SAMPLE_GROUP = 256
 WKV7_SAMPLE_MAX_VOCAB = 1 << 21
 
@@ -62,6 +64,12 @@ class SlotFamily(ctypes.Structure):
     """struct wkv7_slot_family of include/wkv7.h."""
     _fields_ = [("base", _vp), ("outer_stride", _i64), ("slot_stride", _i64), ("rows", _i64),
                 ("outer", _i64), ("row_bytes", _i64), ("dst_ids", _vp), ("src_ids", _vp)]
+
+
+class AdapterSet(ctypes.Structure):
+    """struct wkv7_adapter_set of include/wkv7.h."""
+    _fields_ = [("a", _vp), ("b", _vp), ("scale", _vp), ("rank", _vp), ("count", _i32),
+                ("slabs", _i32)]
 
 
 class SampleParams(ctypes.Structure):
@@ -115,6 +123,13 @@ SIGNATURES = {
     "wkv7_proj_grouped_noalloc": (ctypes.c_int, [_i64, ctypes.POINTER(ProjGroup), _i32, _vp]),
     "wkv7_decode_block": (ctypes.c_int, [
         _vp, _i64, _i32, _vp, _vp, _i32] + [_vp] * 13 + [_f32, _f32, _vp, _vp, _vp]),
+    "wkv7_adapter_plan_ints": (_i64, [_i64, _i32]),
+    "wkv7_adapter_plan": (ctypes.c_int, [_vp, _i64, _i32, _vp, _i64]),
+    "wkv7_proj_adapters": (ctypes.c_int, [
+        _i64, ctypes.POINTER(ProjGroup), ctypes.POINTER(AdapterSet), _i32, _vp, _i32, _vp, _sz,
+        _vp]),
+    "wkv7_proj_adapters_workspace_bytes": (_sz, [
+        _i64, ctypes.POINTER(ProjGroup), ctypes.POINTER(AdapterSet), _i32]),
     "wkv7_sample_tokens": (ctypes.c_int, [
         _vp, _i32, _i32, _i32, _i64, _vp, _i64, ctypes.POINTER(SampleParams), _vp, _vp, _vp,
         _sz, _vp]),

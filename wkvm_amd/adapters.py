@@ -1,0 +1,158 @@
+"""Low-rank adapters of many requests at once, beside the projections they share.
+
+A batch whose requests run on different fine-tunings of one base model shares
+every weight but the low-rank pairs (A, B): row m of a product with adapter a is
+``act(x w^T + bias + scale_a (x A_a^T) B_a^T)``. ``AdapterBank`` holds the pairs of one
+weight in the kernels' layout, ``adapter_plan`` the batch's adapter ids, and
+``proj_adapters`` runs up to 8 products of a batch (a decode step's rows or
+the tokens of packed prompts) in two launches whatever the mix.
+
+The reference has no counterpart (its projections are plain nn.Linear calls of
+the external model, wkvm/runner/runner.py:80-88).
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Sequence
+
+import numpy as np
+import torch
+
+from . import _lib, ops
+
+_SLAB = _lib.WKV7_ADAPTER_SLAB
+
+
+class AdapterBank:
+    """The adapters of one ``[n, k]`` weight: ``num_adapters`` places of up to ``max_rank``
+    ranks. ``a`` ``[N, R, k]`` and ``b`` ``[N, R/16, n, 16]`` bf16 hold the pairs with zeros
+    past each one's rank (R is ``max_rank`` rounded up to 16), ``scale`` fp32 and ``rank``
+    int32 ``[N]`` the rest. An empty place has rank 0 and adds nothing."""
+
+    def __init__(self, num_adapters: int, k: int, n: int, max_rank: int,
+                 device: torch.device | str = "cuda") -> None:
+        if num_adapters < 1:
+            raise ValueError("num_adapters must be >= 1")
+        if not 1 <= max_rank <= _lib.WKV7_ADAPTER_MAX_RANK:
+            raise ValueError(f"max_rank must be in [1, {_lib.WKV7_ADAPTER_MAX_RANK}], "
+                             f"got {max_rank}")
+        if k < 32 or k % 32:
+            raise ValueError(f"k must be a positive multiple of 32, got {k}")
+        if n < 1:
+            raise ValueError("n must be >= 1")
+        self.num_adapters, self.k, self.n = int(num_adapters), int(k), int(n)
+        self.max_rank = int(max_rank)
+        self.device = torch.device(device)
+        self.slabs = (self.max_rank + _SLAB - 1) // _SLAB
+        bf16, dev = torch.bfloat16, self.device
+        self.a = torch.zeros((num_adapters, self.slabs * _SLAB, k), dtype=bf16, device=dev)
+        self.b = torch.zeros((num_adapters, self.slabs, n, _SLAB), dtype=bf16, device=dev)
+        self.scale = torch.zeros(num_adapters, dtype=torch.float32, device=dev)
+        self.rank = torch.zeros(num_adapters, dtype=torch.int32, device=dev)
+
+    def _check_place(self, index: int) -> int:
+        if not 0 <= index < self.num_adapters:
+            raise ValueError(f"adapter {index} out of range [0, {self.num_adapters})")
+        return int(index)
+
+    def load(self, index: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0) -> None:
+        """Put the pair ``a [r, k]``, ``b [n, r]`` (bf16) with its factor (alpha / r) into a
+        place, on the current stream."""
+        index = self._check_place(index)
+        for t, name in ((a, "a"), (b, "b")):
+            if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or t.dim() != 2:
+                raise ValueError(f"{name} must be a 2-D bfloat16 tensor")
+        r = int(a.shape[0])
+        if not 1 <= r <= self.max_rank:
+            raise ValueError(f"rank must be in [1, {self.max_rank}], got {r}")
+        if tuple(a.shape) != (r, self.k) or tuple(b.shape) != (self.n, r):
+            raise ValueError(f"a must be [{r}, {self.k}] and b [{self.n}, {r}], got "
+                             f"{tuple(a.shape)} and {tuple(b.shape)}")
+        if not math.isfinite(scale):
+            raise ValueError(f"scale must be finite, got {scale}")
+        whole = r // _SLAB
+        self.a[index, :r] = a
+        self.a[index, r:] = 0
+        place = self.b[index]
+        if whole:
+            place[:whole] = b[:, :whole * _SLAB].reshape(self.n, whole, _SLAB).transpose(0, 1)
+        place[whole:] = 0
+        if r % _SLAB:
+            place[whole, :, :r % _SLAB] = b[:, whole * _SLAB:]
+        self.scale[index] = float(scale)
+        self.rank[index] = r
+
+    def clear(self, index: int) -> None:
+        """Empty a place: rows that name it get the shared product alone."""
+        self.rank[self._check_place(index)] = 0
+
+
+class AdapterPlan:
+    """A batch's adapter ids on the device: its rows in the order of their adapters."""
+
+    def __init__(self, rows: int, num_adapters: int, buf: torch.Tensor) -> None:
+        self.rows, self.num_adapters, self.buf = rows, num_adapters, buf
+
+
+def plan_ints(ids, num_adapters: int) -> np.ndarray:
+    """The plan of ``ids`` (host integers, -1: no adapter) in host memory."""
+    if isinstance(ids, torch.Tensor):
+        ids = ids.tolist() if ids.is_cuda else ids.numpy()
+    wide = np.asarray(ids, dtype=np.int64).reshape(-1)
+    bad = wide[(wide < -1) | (wide >= num_adapters)]
+    if bad.size:
+        raise ValueError(f"adapter id {bad[0]} out of range [-1, {num_adapters})")
+    flat = np.ascontiguousarray(wide, dtype=np.int32)
+    lib = _lib.load()
+    out = np.empty(lib.wkv7_adapter_plan_ints(flat.size, num_adapters), dtype=np.int32)
+    rc = lib.wkv7_adapter_plan(flat.ctypes.data, flat.size, num_adapters, out.ctypes.data, out.size)
+    _lib.check(rc, "wkv7_adapter_plan")
+    return out
+
+
+def adapter_plan(ids, num_adapters: int, device: torch.device | str = "cuda") -> AdapterPlan:
+    """Device plan of a batch whose row m runs on adapter ``ids[m]`` (host integers; -1: the
+    base model alone). It is complete when returned, serves every product of the batch
+    and stays right for as long as the rows keep their adapters."""
+    host = plan_ints(ids, num_adapters)
+    rows = int(np.asarray(ids).size) if not isinstance(ids, torch.Tensor) else ids.numel()
+    return AdapterPlan(rows, int(num_adapters), torch.from_numpy(host).to(torch.device(device)))
+
+
+def proj_adapters(products: Sequence[tuple], plan: AdapterPlan,
+                  outs: Sequence[torch.Tensor | None] | None = None) -> list[torch.Tensor]:
+    """``ops.proj_grouped`` with the rows' adapters beside the shared weights
+    (``wkv7_proj_adapters``): ``products`` holds up to 8 tuples ``(x, w, bias, act, bank)``, all but
+    the first two optional; ``bank`` is the ``AdapterBank`` of ``w`` or None. Every ``x`` has the
+    plan's row count, which is not bounded. Returns the ``[M, n]`` bf16 outputs."""
+    groups, ys, keep, M = ops.proj_groups(products, outs)
+    if M != plan.rows:
+        raise ValueError(f"products of {M} rows for a plan of {plan.rows}")
+    n = len(products)
+    dev = ys[0].device
+    if plan.buf.device != dev:
+        raise ValueError(f"plan on {plan.buf.device}, products on {dev}")
+    sets = (_lib.AdapterSet * n)()
+    for i, prod in enumerate(products):
+        bank = prod[4] if len(prod) > 4 else None
+        if bank is None:
+            continue
+        if (bank.k, bank.n) != (groups[i].k, groups[i].n):
+            raise ValueError(f"adapters of a [{bank.n}, {bank.k}] weight beside a "
+                             f"[{groups[i].n}, {groups[i].k}] one")
+        if bank.num_adapters < plan.num_adapters:
+            raise ValueError(f"a bank of {bank.num_adapters} adapters for a plan of "
+                             f"{plan.num_adapters}")
+        if bank.a.device != dev:
+            raise ValueError(f"adapters on {bank.a.device}, products on {dev}")
+        sets[i] = _lib.AdapterSet(bank.a.data_ptr(), bank.b.data_ptr(), bank.scale.data_ptr(),
+                                  bank.rank.data_ptr(), bank.num_adapters, bank.slabs)
+    if M:
+        lib = _lib.load()
+        ws_bytes = int(lib.wkv7_proj_adapters_workspace_bytes(M, groups, sets, n))
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+        rc = lib.wkv7_proj_adapters(M, groups, sets, n, plan.buf.data_ptr(), plan.num_adapters,
+                                    ops._ptr(ws), ws_bytes, ops._stream_ptr(dev))
+        _lib.check(rc, "wkv7_proj_adapters")
+    return ys

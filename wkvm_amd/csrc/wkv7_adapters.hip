@@ -1,0 +1,344 @@
+// Projections shared by all rows with a low-rank adapter of each row's own beside them:
+//   y[m] = act( x[m] W^T + bias + s_a (x[m] A_a^T) B_a^T ),   a = id[m]
+//
+// Two launches for any mix of adapters. The first computes h = s_a x A_a^T, tiles of at most 16
+// rows of one adapter by 16 ranks; the rows are visited in the order of their adapters, so every
+// A is read about once. The second is the shared product itself (wkv7_proj_core.h) over the rows
+// in that order, which adds h B_a^T to its accumulators before bias, activation and the one
+// rounding. h is summed in fp32 and kept whole as three bf16 parts, which the matrix cores
+// multiply with B in two instructions per slab of 16 ranks.
+#include <algorithm>
+
+#include "wkv7_proj_plan.h"
+
+namespace wkv7 {
+namespace {
+
+constexpr int kSlab = WKV7_ADAPTER_SLAB;  // ranks of a slab, rows of a tile
+constexpr int kParts = 3;                 // bf16 parts of a value of h
+
+struct ShrinkGroup {
+  const uint16_t* x;
+  const uint16_t* a;    // [count][16 slabs][k]
+  const float* scale;   // [count]
+  const int32_t* rank;  // [count]
+  uint16_t* h;          // [m][slabs][kParts][16]
+  int64_t ldx;
+  int32_t k, count, slabs;
+};
+
+struct ShrinkArgs {
+  ShrinkGroup g[WKV7_PROJ_MAX_GROUPS];
+  const int32_t* order;
+  const int32_t* tiles;  // [ntiles][3]: first position, rows, adapter
+  int32_t ntiles;
+  int64_t m;
+};
+
+// A tile of the plan, held to what the call has; false where there is nothing to do.
+struct Tile {
+  int64_t first;
+  int rows, id, rank, slabs;
+};
+__device__ __forceinline__ bool get_tile(const ShrinkArgs& args, const ShrinkGroup& G, int t,
+                                         Tile* out) {
+  const int32_t* e = args.tiles + 3 * int64_t(t);
+  out->first = e[0];
+  out->rows = e[1];
+  out->id = e[2];
+  if (out->rows < 1 || out->rows > kSlab || out->id < 0 || out->id >= G.count || out->first < 0 ||
+      out->first + out->rows > args.m)
+    return false;
+  out->rank = min(G.rank[out->id], G.slabs * kSlab);
+  out->slabs = (out->rank + kSlab - 1) / kSlab;
+  return true;
+}
+
+// s times four of a row's sums, `left` of them ranks that the adapter has (a padding rank is 0
+// also where x is not finite), as bf16 parts; an infinite part has no parts after it.
+__device__ __forceinline__ void store_h(uint16_t* h, const f32x4& v, float s, int left) {
+  float x[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = e < left ? s * v[e] : 0.f;
+#pragma unroll
+  for (int p = 0; p < kParts; ++p) {
+    const uint2 part = {pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+    *reinterpret_cast<uint2*>(h + p * kSlab) = part;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t pair = e < 2 ? part.x : part.y;
+      const float top = (e & 1) ? bf16_hi(pair) : bf16_lo(pair);
+      x[e] = __builtin_isinf(top) ? 0.f : x[e] - top;
+    }
+  }
+}
+
+// Few tiles: a workgroup per tile and slab, k dealt to NW waves in 64-wide chunks whose sums
+// are joined through LDS in wave order.
+template <int NW>
+__global__ __launch_bounds__(64 * NW) void shrink_thin_kernel(const ShrinkArgs args) {
+  __shared__ f32x4 red[NW][64];
+  const ShrinkGroup& G = args.g[blockIdx.z];
+  Tile tile;
+  const int slab = blockIdx.y;
+  if (!G.a || !get_tile(args, G, blockIdx.x, &tile) || slab >= tile.slabs) return;
+  const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int K = G.k;
+  const int64_t row = min(max(int64_t(args.order[tile.first + min(li, tile.rows - 1)]), int64_t(0)),
+                          args.m - 1);
+  const uint16_t* xp = G.x + row * G.ldx + 8 * lg;
+  const uint16_t* ap = G.a + ((int64_t(tile.id) * G.slabs + slab) * kSlab + li) * K + 8 * lg;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  auto chunks = [&](int c, auto u_c) {
+    constexpr int U = decltype(u_c)::value;
+    uint4 af[U][2], xf[U][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k0 = 64 * (c + u * NW), k1 = k0 + 32 < K ? k0 + 32 : k0;
+      af[u][0] = *reinterpret_cast<const uint4*>(ap + k0);
+      af[u][1] = *reinterpret_cast<const uint4*>(ap + k1);
+      xf[u][0] = *reinterpret_cast<const uint4*>(xp + k0);
+      xf[u][1] = *reinterpret_cast<const uint4*>(xp + k1);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      acc = mma(af[u][0], xf[u][0], acc);
+      if (64 * (c + u * NW) + 32 < K) acc = mma(af[u][1], xf[u][1], acc);
+    }
+  };
+  const int nc = (K + 63) / 64;
+  int c = wave;
+  for (; c + 3 * NW < nc; c += 4 * NW) chunks(c, std::integral_constant<int, 4>{});
+  if (c + 2 * NW < nc) chunks(c, std::integral_constant<int, 3>{});
+  else if (c + NW < nc) chunks(c, std::integral_constant<int, 2>{});
+  else if (c < nc) chunks(c, std::integral_constant<int, 1>{});
+  red[wave][lane] = acc;
+  __syncthreads();
+  if (wave != 0) return;
+#pragma unroll
+  for (int w = 1; w < NW; ++w) acc += red[w][lane];
+  // lane: ranks 4 lg .. 4 lg + 3 of row li
+  if (li < tile.rows)
+    store_h(G.h + ((tile.first + li) * G.slabs + slab) * kParts * kSlab + 4 * lg, acc, G.scale[tile.id],
+            tile.rank - slab * kSlab - 4 * lg);
+}
+
+// Many tiles: a wave per tile, all of k, up to four slabs at once.
+__global__ __launch_bounds__(256) void shrink_wide_kernel(const ShrinkArgs args) {
+  const ShrinkGroup& G = args.g[blockIdx.y];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t index = int64_t(blockIdx.x) * 4 + wave;
+  Tile tile;
+  if (!G.a || index >= args.ntiles || !get_tile(args, G, int(index), &tile)) return;
+  const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+  const int K = G.k;
+  const int64_t row = min(max(int64_t(args.order[tile.first + min(li, tile.rows - 1)]), int64_t(0)),
+                          args.m - 1);
+  const uint16_t* xp = G.x + row * G.ldx + 8 * lg;
+  const float scale = G.scale[tile.id];
+  auto slabs = [&](int s0, auto n_c) {
+    constexpr int NS = decltype(n_c)::value;
+    constexpr int U = 4;
+    const uint16_t* ap = G.a + ((int64_t(tile.id) * G.slabs + s0) * kSlab + li) * K + 8 * lg;
+    f32x4 acc[NS];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) acc[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+    int k = 0;
+    for (; k + 32 * U <= K; k += 32 * U) {
+      uint4 xf[U], af[U][NS];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        xf[u] = *reinterpret_cast<const uint4*>(xp + k + 32 * u);
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+          af[u][s] = *reinterpret_cast<const uint4*>(ap + int64_t(s) * kSlab * K + k + 32 * u);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int s = 0; s < NS; ++s) acc[s] = mma(af[u][s], xf[u], acc[s]);
+    }
+    for (; k < K; k += 32) {
+      const uint4 xf = *reinterpret_cast<const uint4*>(xp + k);
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+        acc[s] = mma(*reinterpret_cast<const uint4*>(ap + int64_t(s) * kSlab * K + k), xf, acc[s]);
+    }
+    if (li < tile.rows) {
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+        store_h(G.h + ((tile.first + li) * G.slabs + s0 + s) * kParts * kSlab + 4 * lg, acc[s], scale,
+                tile.rank - (s0 + s) * kSlab - 4 * lg);
+    }
+  };
+  int s = 0;
+  for (; s + 4 <= tile.slabs; s += 4) slabs(s, std::integral_constant<int, 4>{});
+  if (tile.slabs - s == 3) slabs(s, std::integral_constant<int, 3>{});
+  else if (tile.slabs - s == 2) slabs(s, std::integral_constant<int, 2>{});
+  else if (tile.slabs - s == 1) slabs(s, std::integral_constant<int, 1>{});
+}
+
+int64_t max_tiles(int64_t m, int32_t count) { return m / kSlab + std::min<int64_t>(m, count) + 1; }
+
+// Where the plan's parts start, in ints.
+int64_t plan_part(int64_t m, int part) { return part * ((m + 3) / 4 * 4); }
+
+size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
+
+int check_sets(const wkv7_adapter_set* sets, int32_t ngroups, int32_t count) {
+  for (int i = 0; i < ngroups; ++i) {
+    const wkv7_adapter_set& s = sets[i];
+    if (!s.a) continue;
+    if (!s.b || !s.scale || !s.rank || s.count < count || s.slabs < 1 ||
+        s.slabs > WKV7_ADAPTER_MAX_RANK / kSlab)
+      return WKV7_ERR_ARG;
+    if (!aligned16(s.a) || !aligned16(s.b)) return WKV7_ERR_SHAPE;
+  }
+  return WKV7_OK;
+}
+
+struct Work {
+  Plan plan;
+  int waves;  // of the thin kernel, 0: the tiled one
+  size_t h[WKV7_PROJ_MAX_GROUPS];
+  size_t partials, bytes;
+};
+
+Work make_work(int64_t m, const wkv7_proj_group* groups, const wkv7_adapter_set* sets, int ng,
+               int cus) {
+  Work w{};
+  w.waves = thin_waves(m, groups, ng, cus);
+  w.plan = make_plan(m, groups, ng, cus);
+  for (int i = 0; i < ng; ++i) {
+    w.h[i] = w.bytes;
+    if (sets[i].a) w.bytes += align256(size_t(m) * sets[i].slabs * kParts * kSlab * sizeof(uint16_t));
+  }
+  w.partials = w.bytes;
+  if (!w.waves) w.bytes += w.plan.ws_bytes;
+  return w;
+}
+
+}  // namespace
+}  // namespace wkv7
+
+using namespace wkv7;
+
+extern "C" int64_t wkv7_adapter_plan_ints(int64_t m, int32_t count) {
+  if (m < 0 || m > 0x7fffffff || count < 0) return 0;
+  return plan_part(m, 3) + 3 * max_tiles(m, count);
+}
+
+extern "C" int wkv7_adapter_plan(const int32_t* ids, int64_t m, int32_t count, int32_t* plan,
+                                 int64_t plan_ints) {
+  if (m < 0 || m > 0x7fffffff || count < 0 || !plan || (m > 0 && !ids)) return WKV7_ERR_ARG;
+  if (plan_ints < wkv7_adapter_plan_ints(m, count)) return WKV7_ERR_WORKSPACE;
+  for (int64_t i = 0; i < m; ++i)
+    if (ids[i] < -1 || ids[i] >= count) return WKV7_ERR_ARG;
+  int32_t* order = plan;
+  int32_t* id = plan + plan_part(m, 1);
+  int32_t* end = plan + plan_part(m, 2);
+  int32_t* tile = plan + plan_part(m, 3);
+  int32_t* const last = tile + 3 * max_tiles(m, count);
+  // rows by adapter, in their own order within it, those without one last (a stable sort of the
+  // rows that have an adapter, which needs no memory of its own)
+  int64_t n = 0;
+  for (int64_t i = 0; i < m; ++i)
+    if (ids[i] >= 0) order[n++] = int32_t(i);
+  std::sort(order, order + n, [ids](int32_t x, int32_t y) {
+    return ids[x] != ids[y] ? ids[x] < ids[y] : x < y;
+  });
+  for (int64_t i = 0, p = n; i < m; ++i)
+    if (ids[i] < 0) order[p++] = int32_t(i);
+  for (int64_t p = 0; p < m;) {
+    const int32_t a = ids[order[p]];
+    int64_t e = p;
+    while (e < m && ids[order[e]] == a) ++e;
+    for (int64_t i = p; i < e; ++i) {
+      id[i] = a;
+      end[i] = int32_t(e);
+    }
+    for (int64_t i = p; a >= 0 && i < e; i += kSlab, tile += 3) {
+      tile[0] = int32_t(i);
+      tile[1] = int32_t(std::min<int64_t>(kSlab, e - i));
+      tile[2] = a;
+    }
+    p = e;
+  }
+  std::fill(tile, last, 0);
+  return WKV7_OK;
+}
+
+extern "C" size_t wkv7_proj_adapters_workspace_bytes(int64_t m, const wkv7_proj_group* groups,
+                                                     const wkv7_adapter_set* sets,
+                                                     int32_t ngroups) {
+  if (validate(m, groups, ngroups) != WKV7_OK || !sets || m == 0 ||
+      check_sets(sets, ngroups, 0) != WKV7_OK)
+    return 0;
+  int cus = 0;
+  if (device_cus(&cus) != WKV7_OK) return 0;
+  return make_work(m, groups, sets, ngroups, cus).bytes;
+}
+
+extern "C" int wkv7_proj_adapters(int64_t m, const wkv7_proj_group* groups,
+                                  const wkv7_adapter_set* sets, int32_t ngroups,
+                                  const int32_t* plan, int32_t count, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  int rc = validate(m, groups, ngroups);
+  if (rc != WKV7_OK) return rc;
+  if (!sets || count < 0 || (m > 0 && !plan)) return WKV7_ERR_ARG;
+  rc = check_sets(sets, ngroups, count);
+  if (rc != WKV7_OK) return rc;
+  if (m == 0) return WKV7_OK;
+  if (!aligned16(plan)) return WKV7_ERR_SHAPE;
+  int cus = 0;
+  rc = device_cus(&cus);
+  if (rc != WKV7_OK) return rc;
+  const Work work = make_work(m, groups, sets, ngroups, cus);
+  if (work.bytes && (!workspace || workspace_bytes < work.bytes || !aligned16(workspace)))
+    return WKV7_ERR_WORKSPACE;
+  char* ws = static_cast<char*>(workspace);
+  hipStream_t s = as_stream(stream);
+
+  Adapters ad{};
+  ad.order = plan;
+  ad.id = plan + plan_part(m, 1);
+  ad.end = plan + plan_part(m, 2);
+  ShrinkArgs sh{};
+  sh.order = plan;
+  sh.tiles = plan + plan_part(m, 3);
+  sh.ntiles = int32_t(max_tiles(m, count));
+  sh.m = m;
+  int slabs = 0, kmax = 0;
+  for (int i = 0; i < ngroups; ++i) {
+    const wkv7_adapter_set& set = sets[i];
+    if (!set.a) continue;
+    uint16_t* h = reinterpret_cast<uint16_t*>(ws + work.h[i]);
+    // (only the plan's own ids: a set may hold more adapters than the plan knows)
+    sh.g[i] = {groups[i].x, set.a,          set.scale, set.rank, h,
+               groups[i].ldx, groups[i].k, count,     set.slabs};
+    ad.h[i] = h;
+    ad.b[i] = set.b;
+    ad.rank[i] = set.rank;
+    ad.count[i] = count;
+    ad.slabs[i] = set.slabs;
+    slabs = std::max(slabs, set.slabs);
+    kmax = std::max(kmax, groups[i].k);
+  }
+  if (slabs && count) {
+    if (int64_t(sh.ntiles) * slabs * ngroups <= 8 * int64_t(cus)) {
+      const dim3 grid(unsigned(sh.ntiles), unsigned(slabs), unsigned(ngroups));
+      if (kmax <= 1024) shrink_thin_kernel<4><<<grid, 256, 0, s>>>(sh);
+      else shrink_thin_kernel<8><<<grid, 512, 0, s>>>(sh);
+    } else {
+      const dim3 grid(unsigned((sh.ntiles + 3) / 4), unsigned(ngroups));
+      shrink_wide_kernel<<<grid, 256, 0, s>>>(sh);
+    }
+    rc = launch_status();
+    if (rc != WKV7_OK) return rc;
+  }
+  if (work.waves == 4) return launch_thin<4>(m, groups, ngroups, ad, s);
+  if (work.waves == 8) return launch_thin<8>(m, groups, ngroups, ad, s);
+  return launch_plan(m, groups, ngroups, work.plan, reinterpret_cast<float*>(ws + work.partials), ad,
+                     s);
+}

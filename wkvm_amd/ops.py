@@ -1194,16 +1194,9 @@ ACTIVATIONS = {None: _lib.WKV7_ACT_NONE, "tanh": _lib.WKV7_ACT_TANH,
                "sigmoid": _lib.WKV7_ACT_SIGMOID}
 
 
-def proj_grouped(products: Sequence[tuple], outs: Sequence[torch.Tensor | None] | None = None,
-                 ) -> list[torch.Tensor]:
-    """Independent projections ``act(x @ w.T + bias)`` in one launch
-    (``wkv7_proj_grouped``): ``products`` holds up to 8 tuples ``(x, w)``,
-    ``(x, w, bias)`` or ``(x, w, bias, act)`` with ``x [M, k]`` (row stride
-    a multiple of 8, unit column stride), ``w [n, k]`` bf16 (nn.Linear's
-    [out, in]), ``bias [n]`` or None and ``act`` None, ``"tanh"`` or
-    ``"sigmoid"``; every ``x`` has the same M. Returns the ``[M, n]`` bf16
-    outputs (written into ``outs[i]`` where given, which may be strided
-    row views)."""
+def proj_groups(products: Sequence[tuple], outs: Sequence[torch.Tensor | None] | None = None):
+    """The checked products of a grouped launch: ``(ProjGroup array, outputs, tensors that the
+    launch reads, row count)``."""
     if not 1 <= len(products) <= _lib.WKV7_PROJ_MAX_GROUPS:
         raise ValueError(f"1..{_lib.WKV7_PROJ_MAX_GROUPS} products per launch, got {len(products)}")
     groups = (_lib.ProjGroup * len(products))()
@@ -1249,6 +1242,20 @@ def proj_grouped(products: Sequence[tuple], outs: Sequence[torch.Tensor | None] 
                                    ACTIVATIONS[act], 0)
         keep += [x, w, bias]
         ys.append(y)
+    return groups, ys, keep, M
+
+
+def proj_grouped(products: Sequence[tuple], outs: Sequence[torch.Tensor | None] | None = None,
+                 ) -> list[torch.Tensor]:
+    """Independent projections ``act(x @ w.T + bias)`` in one launch
+    (``wkv7_proj_grouped``): ``products`` holds up to 8 tuples ``(x, w)``,
+    ``(x, w, bias)`` or ``(x, w, bias, act)`` with ``x [M, k]`` (row stride
+    a multiple of 8, unit column stride), ``w [n, k]`` bf16 (nn.Linear's
+    [out, in]), ``bias [n]`` or None and ``act`` None, ``"tanh"`` or
+    ``"sigmoid"``; every ``x`` has the same M. Returns the ``[M, n]`` bf16
+    outputs (written into ``outs[i]`` where given, which may be strided
+    row views)."""
+    groups, ys, keep, M = proj_groups(products, outs)
     if M:
         lib = _lib.load()
         n = len(products)

@@ -583,8 +583,8 @@ int wkv7_proj_grouped_noalloc(int64_t m, const wkv7_proj_group *groups, int32_t 
  * shared weights: for row m with adapter a = ids[m] (-1: none) and every product g,
  *     y[m] = act( x[m] w^T + bias + scale_a (x[m] A_a^T) B_a^T )
  * bf16 operands, fp32 sums (x A^T enters the second product with all of its 24
- * bits), and y is rounded once. Any number of rows (one token of each
- * request, or the tokens of many prompts), any mix of adapters.
+ * bits), and y is rounded once. Up to WKV7_ADAPTER_MAX_ROWS rows (one token of
+ * each request, or the tokens of many prompts), any mix of adapters.
  *
  * No counterpart in the reference, whose model layers are nn.Linear calls without
  * adapters (external; reached through the model forward,
@@ -609,6 +609,10 @@ int wkv7_proj_grouped_noalloc(int64_t m, const wkv7_proj_group *groups, int32_t 
  */
 #define WKV7_ADAPTER_SLAB 16
 #define WKV7_ADAPTER_MAX_RANK 256
+#define WKV7_ADAPTER_MAX_ROWS (1 << 28)
+/* Up to this many rows a plan's runs of an adapter follow one another; in plans of more
+ * rows each starts at a multiple of 32 positions. */
+#define WKV7_ADAPTER_PACKED_ROWS 512
 
 typedef struct wkv7_adapter_set {
   const uint16_t *a;
@@ -626,7 +630,8 @@ int wkv7_proj_adapters(int64_t m, const wkv7_proj_group *groups, const wkv7_adap
                        int32_t ngroups, const int32_t *plan, int32_t count, void *workspace,
                        size_t workspace_bytes, void *stream);
 size_t wkv7_proj_adapters_workspace_bytes(int64_t m, const wkv7_proj_group *groups,
-                                          const wkv7_adapter_set *sets, int32_t ngroups);
+                                          const wkv7_adapter_set *sets, int32_t ngroups,
+                                          int32_t count);
 
 /*
  * The next token of every row of a batch of logits, by the row's own settings and

@@ -129,7 +129,7 @@ SIGNATURES = {
         _i64, ctypes.POINTER(ProjGroup), ctypes.POINTER(AdapterSet), _i32, _vp, _i32, _vp, _sz,
         _vp]),
     "wkv7_proj_adapters_workspace_bytes": (_sz, [
-        _i64, ctypes.POINTER(ProjGroup), ctypes.POINTER(AdapterSet), _i32]),
+        _i64, ctypes.POINTER(ProjGroup), ctypes.POINTER(AdapterSet), _i32, _i32]),
     "wkv7_sample_tokens": (ctypes.c_int, [
         _vp, _i32, _i32, _i32, _i64, _vp, _i64, ctypes.POINTER(SampleParams), _vp, _vp, _vp,
         _sz, _vp]),

@@ -150,7 +150,8 @@ def proj_adapters(products: Sequence[tuple], plan: AdapterPlan,
                                   bank.rank.data_ptr(), bank.num_adapters, bank.slabs)
     if M:
         lib = _lib.load()
-        ws_bytes = int(lib.wkv7_proj_adapters_workspace_bytes(M, groups, sets, n))
+        ws_bytes = int(lib.wkv7_proj_adapters_workspace_bytes(M, groups, sets, n,
+                                                              plan.num_adapters))
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
         rc = lib.wkv7_proj_adapters(M, groups, sets, n, plan.buf.data_ptr(), plan.num_adapters,
                                     ops._ptr(ws), ws_bytes, ops._stream_ptr(dev))

@@ -10,12 +10,14 @@
 #include <algorithm>
 
 #include "wkv7_proj_plan.h"
+#include "wkv7_proj_wide.h"
 
 namespace wkv7 {
 namespace {
 
 constexpr int kSlab = WKV7_ADAPTER_SLAB;  // ranks of a slab, rows of a tile
 constexpr int kParts = 3;                 // bf16 parts of a value of h
+constexpr int kAlign = 32;                // positions that a run starts at a multiple of (many rows)
 
 struct ShrinkGroup {
   const uint16_t* x;
@@ -32,7 +34,7 @@ struct ShrinkArgs {
   const int32_t* order;
   const int32_t* tiles;  // [ntiles][3]: first position, rows, adapter
   int32_t ntiles;
-  int64_t m;
+  int64_t m, positions;
 };
 
 // A tile of the plan, held to what the call has; false where there is nothing to do.
@@ -47,7 +49,7 @@ __device__ __forceinline__ bool get_tile(const ShrinkArgs& args, const ShrinkGro
   out->rows = e[1];
   out->id = e[2];
   if (out->rows < 1 || out->rows > kSlab || out->id < 0 || out->id >= G.count || out->first < 0 ||
-      out->first + out->rows > args.m)
+      out->first + out->rows > args.positions)
     return false;
   out->rank = min(G.rank[out->id], G.slabs * kSlab);
   out->slabs = (out->rank + kSlab - 1) / kSlab;
@@ -139,7 +141,7 @@ __global__ __launch_bounds__(256) void shrink_wide_kernel(const ShrinkArgs args)
   const float scale = G.scale[tile.id];
   auto slabs = [&](int s0, auto n_c) {
     constexpr int NS = decltype(n_c)::value;
-    constexpr int U = 4;
+    constexpr int U = NS <= 2 ? 8 : 4;
     const uint16_t* ap = G.a + ((int64_t(tile.id) * G.slabs + s0) * kSlab + li) * K + 8 * lg;
     f32x4 acc[NS];
 #pragma unroll
@@ -181,8 +183,15 @@ __global__ __launch_bounds__(256) void shrink_wide_kernel(const ShrinkArgs args)
 
 int64_t max_tiles(int64_t m, int32_t count) { return m / kSlab + std::min<int64_t>(m, count) + 1; }
 
+// Positions of a plan: the rows, and where the runs of an adapter are aligned the gaps too.
+int64_t positions(int64_t m, int32_t count) {
+  if (m <= WKV7_ADAPTER_PACKED_ROWS) return m;
+  const int64_t runs = std::min<int64_t>(m, int64_t(count) + 1);
+  return (m + (kAlign - 1) * runs + kAlign - 1) / kAlign * kAlign;
+}
+
 // Where the plan's parts start, in ints.
-int64_t plan_part(int64_t m, int part) { return part * ((m + 3) / 4 * 4); }
+int64_t plan_part(int64_t positions, int part) { return part * ((positions + 3) / 4 * 4); }
 
 size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 
@@ -198,24 +207,60 @@ int check_sets(const wkv7_adapter_set* sets, int32_t ngroups, int32_t count) {
   return WKV7_OK;
 }
 
+// Whether the wide kernel's 32-bit row offsets reach every row.
+bool offsets_fit(int64_t m, const wkv7_proj_group* groups, int ng) {
+  for (int i = 0; i < ng; ++i) {
+    const int64_t k = groups[i].k;
+    if (((m - 1) * groups[i].ldx + k) * 2 > int64_t(0xffffffff) ||
+        ((int64_t(groups[i].n) - 1) * groups[i].ldw + k) * 2 > int64_t(0xffffffff))
+      return false;
+  }
+  return true;
+}
+
+// The row tile of the wide kernel (in units of 64 rows), 0 for the others: whichever takes the
+// least time by its rounds over the units. Microseconds per round of one tile per unit, measured
+// at k = 2048 (they scale together with k): 256 x 256 tiles 79, 128 x 256 47, the other kernel's
+// 128 x 64 tiles 16.5. Three products of 2048 columns and 2048 k: 3001 rows 118 in 128 x 256 (127
+// in 256 x 256, 165 in 128 x 64), 32,768 rows 973 in 256 x 256 (1187, about 2200). A plan of few
+// rows does not align its runs as the wide kernel needs.
+int wide_tile(int64_t m, int64_t positions, const wkv7_proj_group* groups, int ng, int cus) {
+  if (m <= WKV7_ADAPTER_PACKED_ROWS || !offsets_fit(m, groups, ng)) return 0;
+  const struct { TileShape shape; int tm; double us; } kinds[] = {
+      {{128, 64}, 0, 16.5}, {{128, 256}, 2, 47.}, {{256, 256}, 4, 79.}};
+  double best = 0.;
+  int tm = 0;
+  for (const auto& k : kinds) {
+    const int64_t tiles = count_tiles(positions, groups, ng, k.shape);
+    const double us = k.us * double((tiles + cus - 1) / cus);
+    if (best == 0. || us < best) {
+      best = us;
+      tm = k.tm;
+    }
+  }
+  return tm;
+}
+
 struct Work {
   Plan plan;
   int waves;  // of the thin kernel, 0: the tiled one
+  int wide;   // row tile of the wide kernel, 0: another one
   size_t h[WKV7_PROJ_MAX_GROUPS];
   size_t partials, bytes;
 };
 
-Work make_work(int64_t m, const wkv7_proj_group* groups, const wkv7_adapter_set* sets, int ng,
-               int cus) {
+Work make_work(int64_t rows, int64_t m, const wkv7_proj_group* groups, const wkv7_adapter_set* sets,
+               int ng, int cus) {
   Work w{};
   w.waves = thin_waves(m, groups, ng, cus);
+  w.wide = wide_tile(rows, m, groups, ng, cus);
   w.plan = make_plan(m, groups, ng, cus);
   for (int i = 0; i < ng; ++i) {
     w.h[i] = w.bytes;
     if (sets[i].a) w.bytes += align256(size_t(m) * sets[i].slabs * kParts * kSlab * sizeof(uint16_t));
   }
   w.partials = w.bytes;
-  if (!w.waves) w.bytes += w.plan.ws_bytes;
+  if (!w.waves && !w.wide) w.bytes += w.plan.ws_bytes;
   return w;
 }
 
@@ -225,59 +270,68 @@ Work make_work(int64_t m, const wkv7_proj_group* groups, const wkv7_adapter_set*
 using namespace wkv7;
 
 extern "C" int64_t wkv7_adapter_plan_ints(int64_t m, int32_t count) {
-  if (m < 0 || m > 0x7fffffff || count < 0) return 0;
-  return plan_part(m, 3) + 3 * max_tiles(m, count);
+  if (m < 0 || m > WKV7_ADAPTER_MAX_ROWS || count < 0) return 0;
+  return plan_part(positions(m, count), 3) + 3 * max_tiles(m, count);
 }
 
 extern "C" int wkv7_adapter_plan(const int32_t* ids, int64_t m, int32_t count, int32_t* plan,
                                  int64_t plan_ints) {
-  if (m < 0 || m > 0x7fffffff || count < 0 || !plan || (m > 0 && !ids)) return WKV7_ERR_ARG;
+  if (m < 0 || m > WKV7_ADAPTER_MAX_ROWS || count < 0 || !plan || (m > 0 && !ids)) return WKV7_ERR_ARG;
   if (plan_ints < wkv7_adapter_plan_ints(m, count)) return WKV7_ERR_WORKSPACE;
   for (int64_t i = 0; i < m; ++i)
     if (ids[i] < -1 || ids[i] >= count) return WKV7_ERR_ARG;
+  const int64_t all = positions(m, count);
+  const int64_t align = m <= WKV7_ADAPTER_PACKED_ROWS ? 1 : kAlign;
   int32_t* order = plan;
-  int32_t* id = plan + plan_part(m, 1);
-  int32_t* end = plan + plan_part(m, 2);
-  int32_t* tile = plan + plan_part(m, 3);
+  int32_t* id = plan + plan_part(all, 1);
+  int32_t* end = plan + plan_part(all, 2);
+  int32_t* tile = plan + plan_part(all, 3);
   int32_t* const last = tile + 3 * max_tiles(m, count);
-  // rows by adapter, in their own order within it, those without one last (a stable sort of the
-  // rows that have an adapter, which needs no memory of its own)
+  // rows by adapter, in their own order within it, those without one last: sorted in the place
+  // of `id`, which is written behind them
   int64_t n = 0;
   for (int64_t i = 0; i < m; ++i)
-    if (ids[i] >= 0) order[n++] = int32_t(i);
-  std::sort(order, order + n, [ids](int32_t x, int32_t y) {
+    if (ids[i] >= 0) id[n++] = int32_t(i);
+  std::sort(id, id + n, [ids](int32_t x, int32_t y) {
     return ids[x] != ids[y] ? ids[x] < ids[y] : x < y;
   });
   for (int64_t i = 0, p = n; i < m; ++i)
-    if (ids[i] < 0) order[p++] = int32_t(i);
-  for (int64_t p = 0; p < m;) {
-    const int32_t a = ids[order[p]];
-    int64_t e = p;
-    while (e < m && ids[order[e]] == a) ++e;
-    for (int64_t i = p; i < e; ++i) {
-      id[i] = a;
-      end[i] = int32_t(e);
-    }
-    for (int64_t i = p; a >= 0 && i < e; i += kSlab, tile += 3) {
-      tile[0] = int32_t(i);
-      tile[1] = int32_t(std::min<int64_t>(kSlab, e - i));
+    if (ids[i] < 0) id[p++] = int32_t(i);
+  int64_t p = 0;
+  for (int64_t i = 0; i < m;) {
+    const int32_t a = ids[id[i]];
+    for (; p % align; ++p) order[p] = -1;
+    const int64_t start = p;
+    for (; i < m && ids[id[i]] == a; ++i) order[p++] = id[i];
+    for (int64_t f = start; a >= 0 && f < p; f += kSlab, tile += 3) {
+      tile[0] = int32_t(f);
+      tile[1] = int32_t(std::min<int64_t>(kSlab, p - f));
       tile[2] = a;
     }
-    p = e;
   }
+  std::fill(order + p, order + all, -1);
   std::fill(tile, last, 0);
+  for (int64_t f = 0; f < all;) {
+    const int32_t a = order[f] < 0 ? -1 : ids[order[f]];
+    int64_t e = f;
+    while (e < all && (order[e] < 0 ? -1 : ids[order[e]]) == a) ++e;
+    for (; f < e; ++f) {
+      id[f] = a;
+      end[f] = int32_t(e);
+    }
+  }
   return WKV7_OK;
 }
 
 extern "C" size_t wkv7_proj_adapters_workspace_bytes(int64_t m, const wkv7_proj_group* groups,
                                                      const wkv7_adapter_set* sets,
-                                                     int32_t ngroups) {
-  if (validate(m, groups, ngroups) != WKV7_OK || !sets || m == 0 ||
-      check_sets(sets, ngroups, 0) != WKV7_OK)
+                                                     int32_t ngroups, int32_t count) {
+  if (validate(m, groups, ngroups) != WKV7_OK || !sets || m == 0 || m > WKV7_ADAPTER_MAX_ROWS ||
+      count < 0 || check_sets(sets, ngroups, count) != WKV7_OK)
     return 0;
   int cus = 0;
   if (device_cus(&cus) != WKV7_OK) return 0;
-  return make_work(m, groups, sets, ngroups, cus).bytes;
+  return make_work(m, positions(m, count), groups, sets, ngroups, cus).bytes;
 }
 
 extern "C" int wkv7_proj_adapters(int64_t m, const wkv7_proj_group* groups,
@@ -286,7 +340,7 @@ extern "C" int wkv7_proj_adapters(int64_t m, const wkv7_proj_group* groups,
                                   size_t workspace_bytes, void* stream) {
   int rc = validate(m, groups, ngroups);
   if (rc != WKV7_OK) return rc;
-  if (!sets || count < 0 || (m > 0 && !plan)) return WKV7_ERR_ARG;
+  if (!sets || count < 0 || m > WKV7_ADAPTER_MAX_ROWS || (m > 0 && !plan)) return WKV7_ERR_ARG;
   rc = check_sets(sets, ngroups, count);
   if (rc != WKV7_OK) return rc;
   if (m == 0) return WKV7_OK;
@@ -294,7 +348,8 @@ extern "C" int wkv7_proj_adapters(int64_t m, const wkv7_proj_group* groups,
   int cus = 0;
   rc = device_cus(&cus);
   if (rc != WKV7_OK) return rc;
-  const Work work = make_work(m, groups, sets, ngroups, cus);
+  const int64_t all = positions(m, count);
+  const Work work = make_work(m, all, groups, sets, ngroups, cus);
   if (work.bytes && (!workspace || workspace_bytes < work.bytes || !aligned16(workspace)))
     return WKV7_ERR_WORKSPACE;
   char* ws = static_cast<char*>(workspace);
@@ -302,13 +357,15 @@ extern "C" int wkv7_proj_adapters(int64_t m, const wkv7_proj_group* groups,
 
   Adapters ad{};
   ad.order = plan;
-  ad.id = plan + plan_part(m, 1);
-  ad.end = plan + plan_part(m, 2);
+  ad.id = plan + plan_part(all, 1);
+  ad.end = plan + plan_part(all, 2);
+  ad.rows = m;
   ShrinkArgs sh{};
   sh.order = plan;
-  sh.tiles = plan + plan_part(m, 3);
+  sh.tiles = plan + plan_part(all, 3);
   sh.ntiles = int32_t(max_tiles(m, count));
   sh.m = m;
+  sh.positions = all;
   int slabs = 0, kmax = 0;
   for (int i = 0; i < ngroups; ++i) {
     const wkv7_adapter_set& set = sets[i];
@@ -337,8 +394,10 @@ extern "C" int wkv7_proj_adapters(int64_t m, const wkv7_proj_group* groups,
     rc = launch_status();
     if (rc != WKV7_OK) return rc;
   }
-  if (work.waves == 4) return launch_thin<4>(m, groups, ngroups, ad, s);
-  if (work.waves == 8) return launch_thin<8>(m, groups, ngroups, ad, s);
-  return launch_plan(m, groups, ngroups, work.plan, reinterpret_cast<float*>(ws + work.partials), ad,
-                     s);
+  if (work.wide == 4) return launch_wide<4>(all, groups, ngroups, ad, s);
+  if (work.wide == 2) return launch_wide<2>(all, groups, ngroups, ad, s);
+  if (work.waves == 4) return launch_thin<4>(all, groups, ngroups, ad, s);
+  if (work.waves == 8) return launch_thin<8>(all, groups, ngroups, ad, s);
+  return launch_plan(all, groups, ngroups, work.plan, reinterpret_cast<float*>(ws + work.partials),
+                     ad, s);
 }

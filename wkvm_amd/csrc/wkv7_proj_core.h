@@ -95,7 +95,9 @@ __device__ __forceinline__ void wait_pending(int pending) {
 // Every row's own low-rank term, or none of it.
 struct NoAdapters {
   static constexpr bool kOn = false;
-  __device__ __forceinline__ int64_t row(int64_t m, int64_t) const { return m; }
+  __device__ __forceinline__ int64_t row(int64_t m) const { return m; }
+  __device__ __forceinline__ int64_t out_row(int64_t m) const { return m; }
+  __device__ __forceinline__ bool empty(int64_t) const { return false; }
 };
 
 // The rows are taken in the order of their adapters ("positions"), so that a tile holds few of
@@ -105,16 +107,61 @@ struct NoAdapters {
 // values multiply a slab's parts with the same 16 columns of B.
 struct Adapters {
   static constexpr bool kOn = true;
-  const int32_t* order;  // [m] row of every position
-  const int32_t* id;     // [m] its adapter, or a negative number
-  const int32_t* end;    // [m] one past the last position of its adapter
+  const int32_t* order;  // [positions] row of every position, or a negative number: none
+  const int32_t* id;     // [positions] its adapter, or a negative number
+  const int32_t* end;    // [positions] one past the last position of its adapter
+  int64_t rows;
   const uint16_t* h[WKV7_PROJ_MAX_GROUPS];
   const uint16_t* b[WKV7_PROJ_MAX_GROUPS];  // NULL: a product without adapters
   const int32_t* rank[WKV7_PROJ_MAX_GROUPS];
   int32_t count[WKV7_PROJ_MAX_GROUPS];
   int32_t slabs[WKV7_PROJ_MAX_GROUPS];
-  __device__ __forceinline__ int64_t row(int64_t m, int64_t M) const {
-    return min(max(int64_t(order[m]), int64_t(0)), M - 1);
+  // the row that a position reads (one that has none reads some row)
+  __device__ __forceinline__ int64_t row(int64_t p) const {
+    return min(max(int64_t(order[p]), int64_t(0)), rows - 1);
+  }
+  // the row that it writes, or a negative number
+  __device__ __forceinline__ int64_t out_row(int64_t p) const {
+    const int64_t r = order[p];
+    return r < rows ? r : -1;
+  }
+  // in a plan of many rows: no row at the first position of a tile, none in all of it
+  __device__ __forceinline__ bool empty(int64_t p) const { return order[p] < 0; }
+};
+
+// Walks the (run, slab) pairs of up to 64 positions from p0: runs of positions that share an
+// adapter, and the slabs of 16 ranks that it has. Uniform over the wave; a lane looks at one
+// position, so that the walk itself waits for nothing.
+struct Pairs {
+  int lo = 0, hi = 0, a = 0, s = 0;  // positions [lo, hi), adapter, slab
+  int sn = 0;
+  int id = -1, end = 0, ns = 0;      // of the lane's position
+  uint64_t starts;
+  __device__ __forceinline__ Pairs(const Adapters& ad, int g, int64_t p0, int rows) {
+    const int lane = threadIdx.x & 63;
+    if (lane < rows) {
+      id = ad.id[p0 + lane];
+      end = int(min(int64_t(ad.end[p0 + lane]) - p0, int64_t(rows)));
+      if (id >= 0 && id < ad.count[g]) ns = min((ad.rank[g][id] + 15) >> 4, ad.slabs[g]);
+    }
+    const int before = __shfl_up(end, 1);
+    starts = __ballot(ns > 0 && (lane == 0 || before != end));
+  }
+  __device__ __forceinline__ bool next() {
+    if (++s < sn) return true;
+    if (!starts) return false;
+    lo = __builtin_ctzll(starts);
+    starts &= starts - 1;
+    hi = __builtin_amdgcn_readlane(end, lo);
+    a = __builtin_amdgcn_readlane(id, lo);
+    sn = __builtin_amdgcn_readlane(ns, lo);
+    s = 0;
+    return true;
+  }
+  __device__ __forceinline__ bool next(int n) {
+    bool more = true;
+    for (int i = 0; i < n && more; ++i) more = next();
+    return more;
   }
 };
 
@@ -133,33 +180,8 @@ __device__ __forceinline__ void expand(const Adapters& ad, int g, int64_t p0, in
   const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
   const int rows = int(min(int64_t(16 * TM), M - p0));
   const int slabs = ad.slabs[g];
-  int id = -1, end = 0, ns = 0;
-  if (lane < rows) {
-    id = ad.id[p0 + lane];
-    end = int(min(int64_t(ad.end[p0 + lane]) - p0, int64_t(rows)));
-    if (id >= 0 && id < ad.count[g]) ns = min((ad.rank[g][id] + 15) >> 4, slabs);
-  }
-  const int before = __shfl_up(end, 1);
-  uint64_t starts = __ballot(ns > 0 && (lane == 0 || before != end));
-  // the pair to come: positions [lo, hi), slab s of sn
-  int lo = 0, hi = 0, a = 0, s = 0, sn = 0;
-  auto next = [&]() {
-    if (++s < sn) return true;
-    if (!starts) return false;
-    lo = __builtin_ctzll(starts);
-    starts &= starts - 1;
-    hi = __builtin_amdgcn_readlane(end, lo);
-    a = __builtin_amdgcn_readlane(id, lo);
-    sn = __builtin_amdgcn_readlane(ns, lo);
-    s = 0;
-    return true;
-  };
-  auto skip = [&](int n) {
-    bool more = true;
-    for (int i = 0; i < n && more; ++i) more = next();
-    return more;
-  };
-  bool more = skip(mine + 1);
+  Pairs pairs(ad, g, p0, rows);
+  bool more = pairs.next(mine + 1);
   const uint16_t* hp = ad.h[g] + (p0 * slabs) * 48 + 8 * lg;
   while (more) {
     uint4 hf[U][TM][2], bf[U][TN];
@@ -168,21 +190,21 @@ __device__ __forceinline__ void expand(const Adapters& ad, int g, int64_t p0, in
     for (int u = 0; u < U; ++u) {
       from[u] = to[u] = 0;
       if (!more) continue;
-      from[u] = lo;
-      to[u] = hi;
-      const uint16_t* bp = ad.b[g] + ((int64_t(a) * slabs + s) * N) * 16 + 8 * (lg & 1);
+      from[u] = pairs.lo;
+      to[u] = pairs.hi;
+      const uint16_t* bp = ad.b[g] + ((int64_t(pairs.a) * slabs + pairs.s) * N) * 16 + 8 * (lg & 1);
 #pragma unroll
       for (int j = 0; j < TN; ++j)
         bf[u][j] = *reinterpret_cast<const uint4*>(bp + int64_t(min(n0 + 16 * j + li, N - 1)) * 16);
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
-        const int r = min(max(16 * i + li, lo), hi - 1);
-        const uint16_t* p = hp + (int64_t(r) * slabs + s) * 48;
+        const int r = min(max(16 * i + li, pairs.lo), pairs.hi - 1);
+        const uint16_t* p = hp + (int64_t(r) * slabs + pairs.s) * 48;
         hf[u][i][0] = *reinterpret_cast<const uint4*>(p);
         hf[u][i][1] = uint4{0, 0, 0, 0};
         if (lg < 2) hf[u][i][1] = *reinterpret_cast<const uint4*>(p + 32);
       }
-      more = skip(step);
+      more = pairs.next(step);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -265,7 +287,7 @@ __global__ __launch_bounds__(64 * GM * GN) void proj_kernel(const ProjArgs args,
     const int c = (lane % KC) ^ (row & (KC - 1));
     chunk_k[i] = 8 * c;
     if (row < BM) {
-      const int64_t m = ex.row(min(m0 + row, M - 1), M);
+      const int64_t m = ex.row(min(m0 + row, M - 1));
       src[i] = G.x + m * G.ldx + 8 * c;
     } else {
       const int64_t n = min(int64_t(n0 + row - BM), int64_t(N - 1));
@@ -416,8 +438,9 @@ __global__ __launch_bounds__(64 * GM * GN) void proj_kernel(const ProjArgs args,
     for (int a = 0; a < TM; ++a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int64_t row = m0 + wm * WM + a * 16 + 4 * lg + e;
-        if (row < M) G.y[ex.row(row, M) * G.ldy + col] = f32_to_bf16(activate(acc[a][b][e] + bias, act));
+        const int64_t p = m0 + wm * WM + a * 16 + 4 * lg + e;
+        const int64_t row = p < M ? ex.out_row(p) : -1;
+        if (row >= 0) G.y[row * G.ldy + col] = f32_to_bf16(activate(acc[a][b][e] + bias, act));
       }
     }
   }
@@ -440,7 +463,8 @@ __global__ __launch_bounds__(256) void proj_reduce_kernel(const ProjArgs args, c
   float sum = 0.f;
   for (int p = 0; p < args.parts; ++p) sum += src[p * plane];
   const float bias = G.bias ? bf16_to_f32(G.bias[col]) : 0.f;
-  G.y[ex.row(row, args.m) * G.ldy + col] = f32_to_bf16(activate(sum + bias, G.act));
+  const int64_t to = ex.out_row(row);
+  if (to >= 0) G.y[to * G.ldy + col] = f32_to_bf16(activate(sum + bias, G.act));
 }
 
 // One row tile (m <= 16): a 16-column tile of a product by one workgroup, its
@@ -469,7 +493,7 @@ __global__ __launch_bounds__(64 * NW) void proj_thin_kernel(const ProjArgs args,
   // A: 16 rows of w, B: 16 rows of x (rows past the end repeat the last one and
   // are not stored); the accumulator holds columns n0 + 4 lg .. + 3 of row li.
   const uint16_t* wp = G.w + int64_t(min(n0 + li, N - 1)) * G.ldw + 8 * lg;
-  const uint16_t* xp = G.x + ex.row(min(li, M - 1), M) * G.ldx + 8 * lg;
+  const uint16_t* xp = G.x + ex.row(min(li, M - 1)) * G.ldx + 8 * lg;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   // U chunks of this wave from chunk c on. Only the last chunk of all can be
   // half a chunk wide: its second half re-reads the first and is left out.
@@ -511,7 +535,8 @@ __global__ __launch_bounds__(64 * NW) void proj_thin_kernel(const ProjArgs args,
 #pragma unroll
   for (int w = 0; w < NW; ++w) sum += part[w * 64 * 4];
   const float bias = G.bias ? bf16_to_f32(G.bias[n0 + col]) : 0.f;
-  G.y[ex.row(row, M) * G.ldy + n0 + col] = f32_to_bf16(activate(sum + bias, G.act));
+  const int64_t to = ex.out_row(row);
+  if (to >= 0) G.y[to * G.ldy + n0 + col] = f32_to_bf16(activate(sum + bias, G.act));
 }
 
 }  // namespace

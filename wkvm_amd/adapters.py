@@ -22,6 +22,7 @@ import torch
 from . import _lib, ops
 
 _SLAB = _lib.WKV7_ADAPTER_SLAB
+_SET_ARRAYS = [_lib.AdapterSet * n for n in range(_lib.WKV7_PROJ_MAX_GROUPS + 1)]
 
 
 class AdapterBank:
@@ -50,6 +51,8 @@ class AdapterBank:
         self.b = torch.zeros((num_adapters, self.slabs, n, _SLAB), dtype=bf16, device=dev)
         self.scale = torch.zeros(num_adapters, dtype=torch.float32, device=dev)
         self.rank = torch.zeros(num_adapters, dtype=torch.int32, device=dev)
+        self.set = _lib.AdapterSet(self.a.data_ptr(), self.b.data_ptr(), self.scale.data_ptr(),
+                                   self.rank.data_ptr(), self.num_adapters, self.slabs)
 
     def _check_place(self, index: int) -> int:
         if not 0 <= index < self.num_adapters:
@@ -133,21 +136,21 @@ def proj_adapters(products: Sequence[tuple], plan: AdapterPlan,
     dev = ys[0].device
     if plan.buf.device != dev:
         raise ValueError(f"plan on {plan.buf.device}, products on {dev}")
-    sets = (_lib.AdapterSet * n)()
+    sets = _SET_ARRAYS[n]()
     for i, prod in enumerate(products):
         bank = prod[4] if len(prod) > 4 else None
         if bank is None:
             continue
-        if (bank.k, bank.n) != (groups[i].k, groups[i].n):
+        group = groups[i]
+        if bank.k != group.k or bank.n != group.n:
             raise ValueError(f"adapters of a [{bank.n}, {bank.k}] weight beside a "
-                             f"[{groups[i].n}, {groups[i].k}] one")
+                             f"[{group.n}, {group.k}] one")
         if bank.num_adapters < plan.num_adapters:
             raise ValueError(f"a bank of {bank.num_adapters} adapters for a plan of "
                              f"{plan.num_adapters}")
         if bank.a.device != dev:
             raise ValueError(f"adapters on {bank.a.device}, products on {dev}")
-        sets[i] = _lib.AdapterSet(bank.a.data_ptr(), bank.b.data_ptr(), bank.scale.data_ptr(),
-                                  bank.rank.data_ptr(), bank.num_adapters, bank.slabs)
+        sets[i] = bank.set
     if M:
         lib = _lib.load()
         ws_bytes = int(lib.wkv7_proj_adapters_workspace_bytes(M, groups, sets, n,

@@ -29,31 +29,31 @@ struct ShrinkGroup {
   int32_t k, count, slabs;
 };
 
+constexpr int kTileInts = 20;  // first position, rows, adapter, 0, the 16 rows
+
 struct ShrinkArgs {
   ShrinkGroup g[WKV7_PROJ_MAX_GROUPS];
-  const int32_t* order;
-  const int32_t* tiles;  // [ntiles][3]: first position, rows, adapter
+  const int32_t* tiles;  // [ntiles][kTileInts]
   int32_t ntiles;
   int64_t m, positions;
 };
 
-// A tile of the plan, held to what the call has; false where there is nothing to do.
+// A tile of the plan, held to what the call has: rows is 0 where there is nothing to do. `row` is
+// the row of the lane's position (of the last one, past the end).
 struct Tile {
-  int64_t first;
-  int rows, id, rank, slabs;
+  int64_t first, row;
+  int rows, id;
 };
-__device__ __forceinline__ bool get_tile(const ShrinkArgs& args, const ShrinkGroup& G, int t,
-                                         Tile* out) {
-  const int32_t* e = args.tiles + 3 * int64_t(t);
-  out->first = e[0];
-  out->rows = e[1];
-  out->id = e[2];
-  if (out->rows < 1 || out->rows > kSlab || out->id < 0 || out->id >= G.count || out->first < 0 ||
-      out->first + out->rows > args.positions)
-    return false;
-  out->rank = min(G.rank[out->id], G.slabs * kSlab);
-  out->slabs = (out->rank + kSlab - 1) / kSlab;
-  return true;
+__device__ __forceinline__ Tile get_tile(const ShrinkArgs& args, const ShrinkGroup& G, int64_t t,
+                                         int li) {
+  const int32_t* e = args.tiles + kTileInts * t;
+  const int4 head = *reinterpret_cast<const int4*>(e);
+  Tile tile{head.x, e[4 + li], head.y, head.z};
+  if (tile.rows < 1 || tile.rows > kSlab || tile.id < 0 || tile.id >= G.count || tile.first < 0 ||
+      tile.first + tile.rows > args.positions)
+    tile.rows = 0;
+  tile.row = min(max(tile.row, int64_t(0)), args.m - 1);
+  return tile;
 }
 
 // s times four of a row's sums, `left` of them ranks that the adapter has (a padding rank is 0
@@ -81,15 +81,18 @@ template <int NW>
 __global__ __launch_bounds__(64 * NW) void shrink_thin_kernel(const ShrinkArgs args) {
   __shared__ f32x4 red[NW][64];
   const ShrinkGroup& G = args.g[blockIdx.z];
-  Tile tile;
   const int slab = blockIdx.y;
-  if (!G.a || !get_tile(args, G, blockIdx.x, &tile) || slab >= tile.slabs) return;
+  if (!G.a || slab >= G.slabs) return;
   const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const Tile tile = get_tile(args, G, blockIdx.x, li);
+  if (tile.rows == 0) return;
   const int K = G.k;
-  const int64_t row = min(max(int64_t(args.order[tile.first + min(li, tile.rows - 1)]), int64_t(0)),
-                          args.m - 1);
-  const uint16_t* xp = G.x + row * G.ldx + 8 * lg;
+  // (the first slab is read before its adapter's rank is known: it nearly always has one)
+  const int left = G.rank[tile.id] - slab * kSlab;
+  if (slab > 0 && left <= 0) return;
+  const float scale = G.scale[tile.id];
+  const uint16_t* xp = G.x + tile.row * G.ldx + 8 * lg;
   const uint16_t* ap = G.a + ((int64_t(tile.id) * G.slabs + slab) * kSlab + li) * K + 8 * lg;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   auto chunks = [&](int c, auto u_c) {
@@ -122,8 +125,8 @@ __global__ __launch_bounds__(64 * NW) void shrink_thin_kernel(const ShrinkArgs a
   for (int w = 1; w < NW; ++w) acc += red[w][lane];
   // lane: ranks 4 lg .. 4 lg + 3 of row li
   if (li < tile.rows)
-    store_h(G.h + ((tile.first + li) * G.slabs + slab) * kParts * kSlab + 4 * lg, acc, G.scale[tile.id],
-            tile.rank - slab * kSlab - 4 * lg);
+    store_h(G.h + ((tile.first + li) * G.slabs + slab) * kParts * kSlab + 4 * lg, acc, scale,
+            left - 4 * lg);
 }
 
 // Many tiles: a wave per tile, all of k, up to four slabs at once.
@@ -131,13 +134,13 @@ __global__ __launch_bounds__(256) void shrink_wide_kernel(const ShrinkArgs args)
   const ShrinkGroup& G = args.g[blockIdx.y];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t index = int64_t(blockIdx.x) * 4 + wave;
-  Tile tile;
-  if (!G.a || index >= args.ntiles || !get_tile(args, G, int(index), &tile)) return;
   const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+  if (!G.a || index >= args.ntiles) return;
+  const Tile tile = get_tile(args, G, index, li);
+  if (tile.rows == 0) return;
   const int K = G.k;
-  const int64_t row = min(max(int64_t(args.order[tile.first + min(li, tile.rows - 1)]), int64_t(0)),
-                          args.m - 1);
-  const uint16_t* xp = G.x + row * G.ldx + 8 * lg;
+  const int rank = min(G.rank[tile.id], G.slabs * kSlab), all = (rank + kSlab - 1) / kSlab;
+  const uint16_t* xp = G.x + tile.row * G.ldx + 8 * lg;
   const float scale = G.scale[tile.id];
   auto slabs = [&](int s0, auto n_c) {
     constexpr int NS = decltype(n_c)::value;
@@ -171,14 +174,14 @@ __global__ __launch_bounds__(256) void shrink_wide_kernel(const ShrinkArgs args)
 #pragma unroll
       for (int s = 0; s < NS; ++s)
         store_h(G.h + ((tile.first + li) * G.slabs + s0 + s) * kParts * kSlab + 4 * lg, acc[s], scale,
-                tile.rank - (s0 + s) * kSlab - 4 * lg);
+                rank - (s0 + s) * kSlab - 4 * lg);
     }
   };
   int s = 0;
-  for (; s + 4 <= tile.slabs; s += 4) slabs(s, std::integral_constant<int, 4>{});
-  if (tile.slabs - s == 3) slabs(s, std::integral_constant<int, 3>{});
-  else if (tile.slabs - s == 2) slabs(s, std::integral_constant<int, 2>{});
-  else if (tile.slabs - s == 1) slabs(s, std::integral_constant<int, 1>{});
+  for (; s + 4 <= all; s += 4) slabs(s, std::integral_constant<int, 4>{});
+  if (all - s == 3) slabs(s, std::integral_constant<int, 3>{});
+  else if (all - s == 2) slabs(s, std::integral_constant<int, 2>{});
+  else if (all - s == 1) slabs(s, std::integral_constant<int, 1>{});
 }
 
 int64_t max_tiles(int64_t m, int32_t count) { return m / kSlab + std::min<int64_t>(m, count) + 1; }
@@ -271,7 +274,7 @@ using namespace wkv7;
 
 extern "C" int64_t wkv7_adapter_plan_ints(int64_t m, int32_t count) {
   if (m < 0 || m > WKV7_ADAPTER_MAX_ROWS || count < 0) return 0;
-  return plan_part(positions(m, count), 3) + 3 * max_tiles(m, count);
+  return plan_part(positions(m, count), 3) + kTileInts * max_tiles(m, count);
 }
 
 extern "C" int wkv7_adapter_plan(const int32_t* ids, int64_t m, int32_t count, int32_t* plan,
@@ -286,7 +289,7 @@ extern "C" int wkv7_adapter_plan(const int32_t* ids, int64_t m, int32_t count, i
   int32_t* id = plan + plan_part(all, 1);
   int32_t* end = plan + plan_part(all, 2);
   int32_t* tile = plan + plan_part(all, 3);
-  int32_t* const last = tile + 3 * max_tiles(m, count);
+  int32_t* const last = tile + kTileInts * max_tiles(m, count);
   // rows by adapter, in their own order within it, those without one last: sorted in the place
   // of `id`, which is written behind them
   int64_t n = 0;
@@ -303,10 +306,12 @@ extern "C" int wkv7_adapter_plan(const int32_t* ids, int64_t m, int32_t count, i
     for (; p % align; ++p) order[p] = -1;
     const int64_t start = p;
     for (; i < m && ids[id[i]] == a; ++i) order[p++] = id[i];
-    for (int64_t f = start; a >= 0 && f < p; f += kSlab, tile += 3) {
+    for (int64_t f = start; a >= 0 && f < p; f += kSlab, tile += kTileInts) {
       tile[0] = int32_t(f);
       tile[1] = int32_t(std::min<int64_t>(kSlab, p - f));
       tile[2] = a;
+      tile[3] = 0;
+      for (int r = 0; r < kSlab; ++r) tile[4 + r] = order[std::min<int64_t>(f + r, p - 1)];
     }
   }
   std::fill(order + p, order + all, -1);
@@ -361,7 +366,6 @@ extern "C" int wkv7_proj_adapters(int64_t m, const wkv7_proj_group* groups,
   ad.end = plan + plan_part(all, 2);
   ad.rows = m;
   ShrinkArgs sh{};
-  sh.order = plan;
   sh.tiles = plan + plan_part(all, 3);
   sh.ntiles = int32_t(max_tiles(m, count));
   sh.m = m;

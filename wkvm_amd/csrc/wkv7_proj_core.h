@@ -165,37 +165,51 @@ struct Pairs {
   }
 };
 
-// Adds the low-rank terms of 16 TM positions from p0 (at most 64) and 16 TN columns from n0 to
-// acc: for every run of positions that share an adapter and every slab of it, one MFMA per tile,
-// of which the run's own positions are taken (not the others times zero: an adapter with an inf
-// or NaN in it must not reach other requests). The operands come straight to registers, U (run,
-// slab) pairs in flight at once: a tile of a decode batch may meet an adapter per row, and each
-// of them is one pass from memory. kSwap: acc holds the transposed tile. Pairs are dealt to
-// `step` waves.
+// The low-rank terms of 16 TM positions from p0 (at most 64) and 16 TN columns from n0: for every
+// run of positions that share an adapter and every slab of it, two MFMAs per tile, of which the
+// run's own positions are taken (not the others times zero: an adapter with an inf or NaN in it
+// must not reach other requests). The operands come straight to registers, U (run, slab) pairs
+// in flight at once: a tile of a decode batch may meet an adapter per row, and each of them is
+// one pass from memory. The first U are under way from the constructor on, so they arrive while
+// the shared product is computed; add() multiplies them and fetches the others. kSwap: acc holds
+// the transposed tile. Pairs are dealt to `step` waves.
 template <int TM, int TN, int U, bool kSwap>
-__device__ __forceinline__ void expand(const Adapters& ad, int g, int64_t p0, int64_t M, int n0,
-                                       int N, f32x4 (&acc)[TM][TN], int mine = 0, int step = 1) {
+struct Expand {
   static_assert(TM <= 4, "a lane per position");
-  if (!ad.b[g]) return;
-  const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
-  const int rows = int(min(int64_t(16 * TM), M - p0));
-  const int slabs = ad.slabs[g];
-  Pairs pairs(ad, g, p0, rows);
-  bool more = pairs.next(mine + 1);
-  const uint16_t* hp = ad.h[g] + (p0 * slabs) * 48 + 8 * lg;
-  while (more) {
-    uint4 hf[U][TM][2], bf[U][TN];
-    int from[U], to[U];
+  const uint16_t *hp, *bp;
+  int n0, N, rows, slabs, step;
+  Pairs pairs;
+  bool more;
+  uint4 hf[U][TM][2], bf[U][TN];
+  int from[U], to[U];
+
+  __device__ __forceinline__ Expand(const Adapters& ad, int g, int64_t p0, int64_t M, int n0_,
+                                    int N_, bool any, int mine, int step_)
+      : n0(n0_),
+        N(N_),
+        rows(any && ad.b[g] ? int(min(int64_t(16 * TM), M - p0)) : 0),
+        slabs(ad.slabs[g]),
+        step(step_),
+        pairs(ad, g, p0, rows) {
+    const int lg = (threadIdx.x & 63) >> 4;
+    hp = ad.h[g] + (p0 * slabs) * 48 + 8 * lg;
+    bp = ad.b[g] + 8 * (lg & 1);
+    more = pairs.next(mine + 1);
+    fetch();
+  }
+
+  __device__ __forceinline__ void fetch() {
+    const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       from[u] = to[u] = 0;
       if (!more) continue;
       from[u] = pairs.lo;
       to[u] = pairs.hi;
-      const uint16_t* bp = ad.b[g] + ((int64_t(pairs.a) * slabs + pairs.s) * N) * 16 + 8 * (lg & 1);
+      const uint16_t* b = bp + ((int64_t(pairs.a) * slabs + pairs.s) * N) * 16;
 #pragma unroll
       for (int j = 0; j < TN; ++j)
-        bf[u][j] = *reinterpret_cast<const uint4*>(bp + int64_t(min(n0 + 16 * j + li, N - 1)) * 16);
+        bf[u][j] = *reinterpret_cast<const uint4*>(b + int64_t(min(n0 + 16 * j + li, N - 1)) * 16);
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
         const int r = min(max(16 * i + li, pairs.lo), pairs.hi - 1);
@@ -206,34 +220,47 @@ __device__ __forceinline__ void expand(const Adapters& ad, int g, int64_t p0, in
       }
       more = pairs.next(step);
     }
+  }
+
+  __device__ __forceinline__ void add(f32x4 (&acc)[TM][TN]) {
+    const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+    for (;;) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        if (to[u] <= 16 * i || from[u] >= 16 * i + 16) continue;
-        const bool whole = from[u] <= 16 * i && to[u] >= min(rows, 16 * i + 16);
+        for (int i = 0; i < TM; ++i) {
+          if (to[u] <= 16 * i || from[u] >= 16 * i + 16) continue;
+          const bool whole = from[u] <= 16 * i && to[u] >= min(rows, 16 * i + 16);
 #pragma unroll
-        for (int j = 0; j < TN; ++j) {
-          auto term = [&](f32x4 c) {  // the small parts first
+          for (int j = 0; j < TN; ++j) {
+            auto term = [&](f32x4 c) {  // the small parts first
 #pragma unroll
-            for (int q = 1; q >= 0; --q)
-              c = kSwap ? mma(bf[u][j], hf[u][i][q], c) : mma(hf[u][i][q], bf[u][j], c);
-            return c;
-          };
-          if (whole) {
-            acc[i][j] = term(acc[i][j]);
-            continue;
-          }
-          const f32x4 d = term(f32x4{0.f, 0.f, 0.f, 0.f});
+              for (int q = 1; q >= 0; --q)
+                c = kSwap ? mma(bf[u][j], hf[u][i][q], c) : mma(hf[u][i][q], bf[u][j], c);
+              return c;
+            };
+            if (whole) {
+              acc[i][j] = term(acc[i][j]);
+              continue;
+            }
+            const f32x4 d = term(f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = 16 * i + (kSwap ? li : 4 * lg + e);
-            acc[i][j][e] += r >= from[u] && r < to[u] ? d[e] : 0.f;
+            for (int e = 0; e < 4; ++e) {
+              const int r = 16 * i + (kSwap ? li : 4 * lg + e);
+              acc[i][j][e] += r >= from[u] && r < to[u] ? d[e] : 0.f;
+            }
           }
         }
-      }
+      if (!more) return;
+      fetch();
+    }
   }
-}
+};
+
+struct NoExpand {
+  template <class... T>
+  __device__ __forceinline__ explicit NoExpand(T...) {}
+};
 
 template <int BM, int BN, int S, int GM, int GN, int BK, bool kSplit, class Extra>
 __global__ __launch_bounds__(64 * GM * GN) void proj_kernel(const ProjArgs args, const Extra ex) {
@@ -324,6 +351,11 @@ __global__ __launch_bounds__(64 * GM * GN) void proj_kernel(const ProjArgs args,
 #pragma unroll
     for (int b = 0; b < TN; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+  // (16 waves have 128 registers each)
+  constexpr int kPairs = NW >= 16 ? 2 : TM > 1 ? 4 : 8;
+  std::conditional_t<Extra::kOn, Expand<TM, TN, kPairs, false>, NoExpand> extra(
+      ex, g, m0 + wm * WM, M, n0 + wn * WN, N, part == 0, 0, 1);
+
   // A stage: all fragment reads first, then its MFMAs with the next stage's
   // loads (when kIssue) spread between them, so the matrix core works while
   // a load waits for the load pipe. Inline-assembly loads are scheduling
@@ -408,9 +440,7 @@ __global__ __launch_bounds__(64 * GM * GN) void proj_kernel(const ProjArgs args,
     }
   }
 
-  if constexpr (Extra::kOn) {
-    if (part == 0) expand<TM, TN, 4, false>(ex, g, m0 + wm * WM, M, n0 + wn * WN, N, acc);
-  }
+  if constexpr (Extra::kOn) extra.add(acc);
 
   if constexpr (kSplit) {  // fp32 partial tile; proj_reduce_kernel finishes the sum
     float* wsp = args.ws + args.ws_off[g] + int64_t(part) * M * N;
@@ -495,6 +525,9 @@ __global__ __launch_bounds__(64 * NW) void proj_thin_kernel(const ProjArgs args,
   const uint16_t* wp = G.w + int64_t(min(n0 + li, N - 1)) * G.ldw + 8 * lg;
   const uint16_t* xp = G.x + ex.row(min(li, M - 1)) * G.ldx + 8 * lg;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  std::conditional_t<Extra::kOn, Expand<1, 1, 4, true>, NoExpand> extra(ex, g, int64_t(0),
+                                                                         int64_t(M), n0, N, true,
+                                                                         wave, NW);
   // U chunks of this wave from chunk c on. Only the last chunk of all can be
   // half a chunk wide: its second half re-reads the first and is left out.
   auto chunks = [&](int c, auto u_c) {
@@ -521,9 +554,9 @@ __global__ __launch_bounds__(64 * NW) void proj_thin_kernel(const ProjArgs args,
   else if (c + NW < nc) chunks(c, std::integral_constant<int, 2>{});
   else if (c < nc) chunks(c, std::integral_constant<int, 1>{});
   if constexpr (Extra::kOn) {
-    f32x4 more[1][1] = {{acc}};
-    expand<1, 1, 4, true>(ex, g, 0, M, n0, N, more, wave, NW);
-    acc = more[0][0];
+    f32x4 sum[1][1] = {{acc}};
+    extra.add(sum);
+    acc = sum[0][0];
   }
   red[wave][lane] = acc;
   __syncthreads();

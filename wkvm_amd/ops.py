@@ -24,6 +24,7 @@ Error behaviour mirrors the reference: invalid arguments raise ``ValueError``
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from collections import OrderedDict
 from typing import Iterable, Sequence
@@ -1194,55 +1195,72 @@ ACTIVATIONS = {None: _lib.WKV7_ACT_NONE, "tanh": _lib.WKV7_ACT_TANH,
                "sigmoid": _lib.WKV7_ACT_SIGMOID}
 
 
+_GROUP_ARRAYS = [_lib.ProjGroup * n for n in range(_lib.WKV7_PROJ_MAX_GROUPS + 1)]
+_GROUP_PACK = struct.Struct("@QQQQqqqiiii")  # the fields of ProjGroup
+assert _GROUP_PACK.size == ctypes.sizeof(_lib.ProjGroup)
+
+
 def proj_groups(products: Sequence[tuple], outs: Sequence[torch.Tensor | None] | None = None):
     """The checked products of a grouped launch: ``(ProjGroup array, outputs, tensors that the
-    launch reads, row count)``."""
-    if not 1 <= len(products) <= _lib.WKV7_PROJ_MAX_GROUPS:
-        raise ValueError(f"1..{_lib.WKV7_PROJ_MAX_GROUPS} products per launch, got {len(products)}")
-    groups = (_lib.ProjGroup * len(products))()
+    launch reads, row count)``. (A decode step makes several such calls and its host time is
+    mostly this: attributes are read once, and the structs packed rather than constructed.)"""
+    n_products = len(products)
+    if not 1 <= n_products <= _lib.WKV7_PROJ_MAX_GROUPS:
+        raise ValueError(f"1..{_lib.WKV7_PROJ_MAX_GROUPS} products per launch, got {n_products}")
+    packed = bytearray(_GROUP_PACK.size * n_products)
     ys, keep = [], []
-    M = None
+    M = dev = None
+    bf16 = torch.bfloat16
     for i, prod in enumerate(products):
         x, w = prod[0], prod[1]
         bias = prod[2] if len(prod) > 2 else None
         act = prod[3] if len(prod) > 3 else None
         if act not in ACTIVATIONS:
             raise ValueError(f"act must be one of {list(ACTIVATIONS)}, got {act!r}")
-        for t, n in ((x, "x"), (w, "w")):
-            _require_cuda(t, n)
-            if t.dtype != torch.bfloat16 or t.dim() != 2:
-                raise ValueError(f"{n} must be a 2-D bfloat16 tensor")
-        if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
+        for t, name in ((x, "x"), (w, "w")):
+            if not (isinstance(t, torch.Tensor) and t.is_cuda):
+                _require_cuda(t, name)
+            if t.dtype is not bf16 or t.dim() != 2:
+                raise ValueError(f"{name} must be a 2-D bfloat16 tensor")
+        ldx, step = x.stride()
+        if step != 1 or ldx % 8 or x.data_ptr() % 16:
             x = x.clone(memory_format=torch.contiguous_format)
-        w = _bf16_2d(w, "w")
-        m, k = int(x.shape[0]), int(x.shape[1])
-        n = int(w.shape[0])
+            ldx = x.stride(0)
+        if not w.is_contiguous() or w.data_ptr() % 16:
+            w = _bf16_2d(w, "w")
+        m, k = x.shape
+        n, wk = w.shape
         if M is None:
-            M = m
+            M, dev = m, x.device
         if m != M:
             raise ValueError("every product needs the same row count")
-        if int(w.shape[1]) != k:
+        if wk != k:
             raise ValueError(f"w must be [n, {k}], got {tuple(w.shape)}")
         if k < 32 or k % 32:
             raise ValueError(f"k must be a positive multiple of 32, got {k}")
         if bias is not None:
             bias = _bf16_2d(bias.reshape(-1), "bias", (n,))
+            if bias.device != dev:
+                raise ValueError("projection tensors must share a device")
         y = outs[i] if outs is not None and i < len(outs) else None
         if y is None:
-            y = torch.empty((M, n), dtype=torch.bfloat16, device=x.device)
+            y = torch.empty((M, n), dtype=bf16, device=dev)
+            ldy = n
         else:
             _require_cuda(y, "out")
-            if y.dtype != torch.bfloat16 or tuple(y.shape) != (M, n) or y.stride(1) != 1:
+            if y.dtype != bf16 or tuple(y.shape) != (M, n) or y.stride(1) != 1:
                 raise ValueError(f"out must be a bf16 [{M}, {n}] tensor with unit column stride")
-        for t in (w, y) + ((bias,) if bias is not None else ()):
-            if t.device != x.device:
+            ldy = y.stride(0)
+            if y.device != dev:
                 raise ValueError("projection tensors must share a device")
-        groups[i] = _lib.ProjGroup(x.data_ptr(), w.data_ptr(), _ptr(bias), y.data_ptr(),
-                                   x.stride(0), w.stride(0), y.stride(0), n, k,
-                                   ACTIVATIONS[act], 0)
+        if x.device != dev or w.device != dev:
+            raise ValueError("projection tensors must share a device")
+        _GROUP_PACK.pack_into(packed, _GROUP_PACK.size * i, x.data_ptr(), w.data_ptr(),
+                              0 if bias is None else bias.data_ptr(), y.data_ptr(), ldx, k, ldy,
+                              n, k, ACTIVATIONS[act], 0)
         keep += [x, w, bias]
         ys.append(y)
-    return groups, ys, keep, M
+    return _GROUP_ARRAYS[n_products].from_buffer(packed), ys, keep, M
 
 
 def proj_grouped(products: Sequence[tuple], outs: Sequence[torch.Tensor | None] | None = None,

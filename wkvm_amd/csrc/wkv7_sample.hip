@@ -33,10 +33,10 @@ constexpr int kChunkSubs = kChunk / kSub;
 constexpr int kChunkGroups = kChunk / kGroup;
 constexpr int kScanThreads = 256;
 
-constexpr int kThreads = 1024;            // of the finish
+constexpr int kThreads = 512;             // of the finish: two workgroups share a unit
 constexpr int kWaves = kThreads / kWave;
 constexpr int kBins = 2048;
-constexpr int kList = 6144;               // candidates held in LDS
+constexpr int kList = 4096;               // candidates held in LDS
 constexpr int kSubs = 4096;               // runs of kSub tokens that may hold candidates
 // The candidate list's group weights take the place of the histogram.
 constexpr int kListGroups = kBins + kBins / 2;
@@ -263,9 +263,10 @@ struct Shared {
       u64 wgt[kBins];
       uint32_t cnt[kBins];
       uint2 list[kList];  // logit bits, index
-      uint32_t subs[kSubs];
+      uint16_t subs[kSubs];
     };
-    u64 mass[kListGroups];  // takes the place of the histogram
+    u64 mass[kListGroups];           // takes the place of the histogram
+    float row_mass[WKV7_SAMPLE_MAX_VOCAB / kGroup];
   };
   uint32_t n_list, n_subs;
   Found found;
@@ -289,9 +290,9 @@ __device__ __forceinline__ V block_all(V v, Op op, Shared& sm) {
   __syncthreads();
   if ((threadIdx.x & (kWave - 1)) == 0) slot[threadIdx.x / kWave] = v;
   __syncthreads();
-  V r = slot[0];
+  V r = slot[threadIdx.x & (kWaves - 1)];
 #pragma unroll
-  for (int i = 1; i < kWaves; ++i) r = op(r, slot[i]);
+  for (int o = 1; o < kWaves; o <<= 1) r = op(r, __shfl_xor(r, o));
   return r;
 }
 
@@ -308,20 +309,30 @@ struct Row {
   const T* p;
   int n;
 
-  // f(vector, index of its first element); every thread makes the same calls.
+  // f(vector, index of its first element); every thread makes the same calls. The next U vectors
+  // are under way while f works on U.
   template <typename F>
   __device__ __forceinline__ void vectors(F f) const {
     constexpr int U = 4;
-    int i = int(threadIdx.x) * N;
-    int done = 0;
-    for (; done + U * kStep <= n; done += U * kStep) {
-      Vec<T> v[U];
+    const int i = int(threadIdx.x) * N;
+    Vec<T> v[U], w[U];
+    auto fetch = [&](Vec<T>(&to)[U], int at) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = load_full(p + done + u * kStep + i);
+      for (int u = 0; u < U; ++u) {
+        const int first = at + u * kStep;
+        if (first + kStep <= n) to[u] = load_full(p + first + i);
+        else if (first < n) to[u] = load_part(p, first + i, n);
+      }
+    };
+    fetch(v, 0);
+    for (int at = 0; at < n; at += U * kStep) {
+      fetch(w, at + U * kStep);
 #pragma unroll
-      for (int u = 0; u < U; ++u) f(v[u], done + u * kStep + i);
+      for (int u = 0; u < U; ++u)
+        if (at + u * kStep < n) f(v[u], at + u * kStep + i);
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = w[u];
     }
-    for (; done < n; done += kStep) f(load_part(p, done + i, n), done + i);
   }
   template <typename F>
   __device__ __forceinline__ void operator()(F f) const {
@@ -329,6 +340,14 @@ struct Row {
 #pragma unroll
       for (int e = 0; e < N; ++e)
         if (i + e < n) f(x.get(e), uint32_t(i + e));
+    });
+  }
+  // the same with -inf for the tokens past the end
+  template <typename F>
+  __device__ __forceinline__ void padded(F f) const {
+    vectors([&](const Vec<T>& x, int i) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) f(x.get(e), uint32_t(i + e));
     });
   }
 };
@@ -389,20 +408,32 @@ __device__ __forceinline__ void block_scan(uint32_t& c, u64& w, uint32_t& all_c,
 // The bin in which the cumulated count (or weight) reaches target >= 1; the last bin that
 // holds anything where it never does.
 __device__ __forceinline__ Found find_bin(Shared& sm, bool by_weight, u64 target) {
+  constexpr int kEach = kBins / kThreads;
   const int t = threadIdx.x;
   __syncthreads();
-  const uint32_t c0 = sm.cnt[2 * t], c1 = sm.cnt[2 * t + 1];
-  const u64 w0 = sm.wgt[2 * t], w1 = sm.wgt[2 * t + 1];
-  uint32_t cb = c0 + c1, all_c;
-  u64 wb = w0 + w1, all_w;
+  uint32_t c[kEach], cb = 0, all_c;
+  u64 w[kEach], wb = 0, all_w;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    c[i] = sm.cnt[kEach * t + i];
+    w[i] = sm.wgt[kEach * t + i];
+    cb += c[i];
+    wb += w[i];
+  }
+  const uint32_t mine_c = cb;
+  const u64 mine_w = wb;
   block_scan(cb, wb, all_c, all_w, sm);
-  cb -= c0 + c1;  // before bin 2 t
-  wb -= w0 + w1;
+  cb -= mine_c;  // before this thread's bins
+  wb -= mine_w;
   const u64 goal = min(target, by_weight ? all_w : u64(all_c));
-  const u64 b0 = by_weight ? wb : cb, v0 = by_weight ? w0 : c0, v1 = by_weight ? w1 : c1;
-  if (b0 < goal && b0 + v0 >= goal) sm.found = {uint32_t(2 * t), cb, c0, wb, w0};
-  if (b0 + v0 < goal && b0 + v0 + v1 >= goal)
-    sm.found = {uint32_t(2 * t + 1), cb + c0, c1, wb + w0, w1};
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const u64 before = by_weight ? wb : u64(cb), here = by_weight ? w[i] : u64(c[i]);
+    if (before < goal && before + here >= goal)
+      sm.found = {uint32_t(kEach * t + i), cb, c[i], wb, w[i]};
+    cb += c[i];
+    wb += w[i];
+  }
   __syncthreads();
   return sm.found;
 }
@@ -410,9 +441,10 @@ __device__ __forceinline__ Found find_bin(Shared& sm, bool by_weight, u64 target
 // A cut in the order: what lies before it or on it is kept.
 struct Cut {
   uint32_t key, index;
-  __device__ __forceinline__ bool keeps(float x, uint32_t i) const {
-    const uint32_t k = order_key(x);
-    return k < key || (k == key && i <= index);
+  float x;  // the key's logit
+  __device__ __forceinline__ Cut(uint32_t k, uint32_t i) : key(k), index(i), x(key_logit(k)) {}
+  __device__ __forceinline__ bool keeps(float v, uint32_t i) const {
+    return v > x || (v == x && i <= index);
   }
 };
 
@@ -449,7 +481,7 @@ __device__ __forceinline__ Cut descend(const Rows& rows, Pred pred, Weight weigh
   u64 ties = by_weight ? (each ? (rest + each - 1) / each : 1) : rest;
   ties = max(u64(1), min(ties, u64(f.cnt)));
   if (upto) *upto = before_wgt + ties * each;
-  Cut cut{prefix, 0xffffffffu};
+  Cut cut(prefix, 0xffffffffu);
   if (ties >= f.cnt) return cut;
   // the lowest `ties` indices among them
   uint32_t before = 0, high = 0;
@@ -474,7 +506,7 @@ __device__ __forceinline__ Cut descend(const Rows& rows, Pred pred, Weight weigh
 template <typename Rows, typename Weight>
 __device__ __forceinline__ Cut cut_rows(const Rows& rows, const Settings& set, double total,
                                         Weight weight, Shared& sm) {
-  Cut cut{0xffffffffu, 0xffffffffu};
+  Cut cut(order_key(-INFINITY), 0xffffffffu);
   if (set.by_k) {
     u64 upto = 0;
     cut = descend(rows, [](float, uint32_t) { return true; }, weight, set.by_p, false,
@@ -528,44 +560,53 @@ __device__ __forceinline__ uint32_t race_group(const Row<T>& row, uint32_t group
   return uint32_t(block_all(best, MinU(), sm));
 }
 
-// The race over the whole row. A group is the vectors of 256 / N neighbouring lanes.
+// The race over the whole row. A group is the vectors of 256 / N neighbouring lanes; its weight
+// goes through LDS, so that the variates are read in one go.
 template <typename T, typename Kept, typename Weight>
 __device__ __forceinline__ uint32_t race_row(const Row<T>& row, Kept kept, Weight weight,
                                              const float* noise, Shared& sm) {
   constexpr int kLanes = kGroup / Vec<T>::N;
-  u64 best = ~0ull;
+  const int groups = (row.n + kGroup - 1) / kGroup;
+  __syncthreads();
   row.vectors([&](const Vec<T>& x, int i) {
     float w = 0.f;
 #pragma unroll
     for (int e = 0; e < Vec<T>::N; ++e) {
       const float v = x.get(e);
-      if (kept(v, uint32_t(i + e))) w += weight(v);
+      w += kept(v, uint32_t(i + e)) ? weight(v) : 0.f;
     }
     w = kLanes == 64 ? lanes_sum<6>(w) : lanes_sum<5>(w);
-    if (w > 0.f && (threadIdx.x & (kLanes - 1)) == 0) {
-      const int g = i / kGroup;
-      best = min(best, arrival(noise[kGroup + g] / w, uint32_t(g)));
-    }
+    if ((threadIdx.x & (kLanes - 1)) == 0 && i < row.n) sm.row_mass[i / kGroup] = w;
   });
+  __syncthreads();
+  u64 best = ~0ull;
+  for (int g = threadIdx.x; g < groups; g += kThreads) {
+    const float w = sm.row_mass[g];
+    if (w > 0.f) best = min(best, arrival(noise[kGroup + g] / w, uint32_t(g)));
+  }
   const uint32_t group = uint32_t(block_all(best, MinU(), sm));
   return race_group(row, group, kept, weight, noise, sm);
 }
 
-// Sorts one key per thread, ascending over the block; `n` of them matter, the others are ~0.
+// Sorts one key per thread, ascending over the block; `n` of them matter, the others are ~0. Waves
+// past the power of two that holds n have nothing to do.
 __device__ __forceinline__ u64 block_sort(u64 v, uint32_t n, Shared& sm) {
   u64* swap = sm.wgt;
   const uint32_t t = threadIdx.x;
+  const bool idle = __builtin_amdgcn_readfirstlane(t) >= 2 * n;
 #pragma unroll 1
   for (uint32_t k = 2; k < 2 * n; k <<= 1) {
 #pragma unroll 1
     for (uint32_t j = k / 2; j > 0; j >>= 1) {
-      u64 o;
+      u64 o = v;
       if (j >= kWave) {
         __syncthreads();
-        swap[t] = v;
+        if (!idle) swap[t] = v;
         __syncthreads();
+        if (idle) continue;
         o = swap[t ^ j];
       } else {
+        if (idle) break;
         o = __shfl_xor(v, int(j));
       }
       const bool up = (t & k) == 0, low = (t & j) == 0;
@@ -573,6 +614,14 @@ __device__ __forceinline__ u64 block_sort(u64 v, uint32_t n, Shared& sm) {
     }
   }
   return v;
+}
+
+// The candidates of the list in order, one per thread (its key, then its index), ~0 past the end.
+__device__ __forceinline__ u64 sorted_candidate(uint32_t n, Shared& sm) {
+  u64 v = ~0ull;
+  if (threadIdx.x < n)
+    v = u64(order_key(__uint_as_float(sm.list[threadIdx.x].x))) << 32 | sm.list[threadIdx.x].y;
+  return block_sort(v, n, sm);
 }
 
 // Candidates: every token whose logit `takes` accepts (a condition that holds for every larger
@@ -587,7 +636,7 @@ __device__ __forceinline__ bool gather(const Row<T>& row, const float* sub_max, 
   for (int s = threadIdx.x; s < n_sub; s += kThreads) {
     if (takes(sub_max[s])) {
       const uint32_t at = atomicAdd(&sm.n_subs, 1u);
-      if (at < kSubs) sm.subs[at] = uint32_t(s);
+      if (at < kSubs) sm.subs[at] = uint16_t(s);
     }
   }
   __syncthreads();
@@ -610,7 +659,7 @@ __device__ __forceinline__ bool gather(const Row<T>& row, const float* sub_max, 
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_finish_kernel(const SampleArgs args) {
+__global__ __launch_bounds__(kThreads, 4) void sample_finish_kernel(const SampleArgs args) {
   __shared__ Shared sm;
   const int64_t b = blockIdx.x;
   const int t = threadIdx.x, V = args.V, chunks = args.chunks;
@@ -670,66 +719,128 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(const SampleArg
       total = block_all(total, AddD(), sm);
     }
     const u64 share = max(u64(1), u64(ceil(fmax(double(set.top_p), 0.) * total * 0x1p42)));
-    bool done = false, listed = groups <= kListGroups;
-    if (listed && (set.by_k || set.by_p)) {
-      // Distance from the maximum in 2,048 steps: the run maxima's histogram says from which
-      // step on there are at least top_k tokens (the runs' maxima alone are that many), or, for
-      // top-p alone, a first guess at how far down its tokens reach.
-      const float scale = 128.f * fminf(set.c, 1.f);
-      auto step = [top, scale](float x) {
-        return uint32_t(fminf((top - x) * scale, float(kBins - 1)));
-      };
-      clear_bins(sm);
-      for (int s = t; s < n_sub; s += kThreads) atomicAdd(&sm.cnt[step(sub_max[s])], 1u);
-      const int want = set.by_k ? set.top_k : V <= kThreads ? V : min(512, (n_sub + 1) / 2);
-      const uint32_t last = want > n_sub ? kBins - 1 : find_bin(sm, false, u64(want)).bin;
-      // (min-p may thin the candidates only where top-p's share does not count them)
-      const bool thin = !set.by_p;
-      listed = gather(row, sub_max, n_sub, [=](float x) {
-        return step(x) <= last && (!thin || over_floor(x)); }, sm);
-    } else if (listed) {
-      listed = gather(row, sub_max, n_sub, over_floor, sm);
-    }
-    if (listed) {
-      const uint32_t n = sm.n_list;
-      const ListRow rows{sm, n};
-      if (!set.by_k && !set.by_p) {
-        token = race_list(rows, [](float, uint32_t) { return true; }, weight, noise, groups, sm);
+    // Every token that top-p keeps of all weighs more than (1 - p) / V of the row: those that weigh
+    // less add up to less than 1 - p. In log2 of the weight:
+    const float rest_of = (1.f - fmaxf(set.top_p, 0.f)) * float(total) / float(V);
+    const float low = fminf(log2f(fmaxf(rest_of, 0x1p-80f)), 0.f) - 0.01f;
+    bool done = false;
+    if (groups > kListGroups) {
+      // (no room for the candidates' group weights)
+    } else if (!set.by_k && !set.by_p) {
+      if (gather(row, sub_max, n_sub, over_floor, sm)) {
+        token = race_list(ListRow{sm, sm.n_list}, [](float, uint32_t) { return true; }, weight,
+                          noise, groups, sm);
         done = true;
-      } else if (n <= kThreads) {
-        u64 v = ~0ull;
-        if (uint32_t(t) < n)
-          v = u64(order_key(__uint_as_float(sm.list[t].x))) << 32 | sm.list[t].y;
-        v = block_sort(v, n, sm);
-        const float x = key_logit(uint32_t(v >> 32));
-        const bool mine = uint32_t(t) < n && (!set.by_k || t < set.top_k);
-        const u64 w = mine ? fixed(weight(x)) : 0;
-        u64 upto = w, all;
-        uint32_t one = 0, none;
-        block_scan(one, upto, none, all, sm);
-        const u64 target =
-            set.by_k ? max(u64(1), u64(ceil(fmax(double(set.top_p), 0.) * double(all)))) : share;
-        if (set.by_k || all >= share) {
+      }
+    } else {
+      // Distance from the maximum in 2,048 steps: the histogram of the run maxima says from which
+      // step on there are enough tokens, for the maxima alone are that many, or weigh that much.
+      // For top-k the steps are 1/128 of a logit or, where the last one would hold its end,
+      // coarser; for top-p alone they end where its tokens end. min-p may thin the candidates
+      // only where top-p's share does not count them.
+      const bool thin = !set.by_p;
+      float scale = set.by_k ? 128.f * fminf(set.c, 1.f) : float(kBins - 1) / -low * set.c;
+      uint32_t last = kBins - 1;
+      bool enough = set.by_k && set.top_k > n_sub;  // (more tokens than runs: all of them)
+      for (int j = 0; !enough && j < 5; ++j, scale *= 0.0625f) {
+        clear_bins(sm);
+        for (int s = t; s < n_sub; s += kThreads) {
+          const float x = sub_max[s];
+          const int bin = int(fminf((top - x) * scale, float(kBins - 1)));
+          atomicAdd(&sm.cnt[bin], 1u);
+          if (!set.by_k) atomicAdd(&sm.wgt[bin], fixed(weight(x)));
+        }
+        const Found f = find_bin(sm, !set.by_k, set.by_k ? u64(set.top_k) : share);
+        last = f.bin;
+        if (!set.by_k) {
+          enough = f.before_wgt + f.wgt >= share && last < kBins - 1;
+          break;
+        }
+        enough = last < kBins - 1;
+        if (enough) break;
+      }
+      // (top-k among tokens of the last step of the coarsest scale: every token is a candidate)
+      if (set.by_k) enough = true;
+      if (V <= kList && !enough) {
+        enough = true;
+        last = kBins - 1;
+      }
+      if (enough && gather(row, sub_max, n_sub, [=](float x) {
+            return uint32_t(fminf((top - x) * scale, float(kBins - 1))) <= last &&
+                   (!thin || over_floor(x));
+          }, sm)) {
+        const uint32_t n = sm.n_list;
+        done = true;
+        if (n <= kThreads) {
+          const uint64_t limit = set.by_k ? uint64_t(set.top_k) : ~0ull;
+          const u64 v = sorted_candidate(n, sm);
+          const float x = key_logit(uint32_t(v >> 32));
+          const bool mine = uint32_t(t) < n && uint64_t(t) < limit;
+          const u64 w = mine ? fixed(weight(x)) : 0;
+          u64 upto = w, all;
+          uint32_t one = 0, none;
+          block_scan(one, upto, none, all, sm);
+          const u64 target =
+              set.by_k ? max(u64(1), u64(ceil(fmax(double(set.top_p), 0.) * double(all)))) : share;
           const bool kept = mine && (t == 0 || !set.by_p || upto - w < target);
           if (kept) sm.list[t] = make_uint2(__float_as_uint(x), uint32_t(v));
           const ListRow first{sm, uint32_t(__syncthreads_count(kept))};
           token = race_list(first, [=](float x, uint32_t) { return over_floor(x); }, weight,
                             noise, groups, sm);
-          done = true;
-        }
-      } else {
-        u64 in_list = 0;
-        bool enough = set.by_k;
-        if (!enough) {
-          rows([&](float x, uint32_t) { in_list += fixed(weight(x)); });
-          enough = block_all(in_list, AddU(), sm) >= share;
-        }
-        if (enough) {
+        } else {
+          const ListRow rows{sm, n};
           const Cut cut = cut_rows(rows, set, total, weight, sm);
           token = race_list(rows, [=](float x, uint32_t i) {
             return cut.keeps(x, i) && over_floor(x); }, weight, noise, groups, sm);
-          done = true;
         }
+      }
+    }
+    if (!done && set.by_p && !set.by_k) {
+      // Top-p's share reaches far down: a pass over 2,048 bins of its tokens' range in log weight
+      // leaves one short run of the order to look at closely.
+      const float steps = float(kBins) / fmaxf(-low, 1.f);
+      auto bin_of = [top, c = set.c, steps](float x) { return (top - x) * c * steps; };
+      clear_bins(sm);
+      row.padded([&](float x, uint32_t) {
+        const float d = bin_of(x);
+        // (32 fraction bits: what a row's tokens lose to them is 10^-6 of its weight)
+        if (d < float(kBins)) atomicAdd(&sm.wgt[int(d)], u64(uint32_t(weight(x) * 0x1p32f)));
+      });
+      const Found f = find_bin(sm, true, (share + 1023) >> 10);
+      __syncthreads();
+      if (t == 0) sm.n_list = 0;
+      __syncthreads();
+      row.padded([&](float x, uint32_t i) {
+        const float d = bin_of(x);
+        if (d >= float(kBins) || uint32_t(d) != f.bin) return;
+        const uint32_t to = atomicAdd(&sm.n_list, 1u);
+        if (to < kList) sm.list[to] = make_uint2(__float_as_uint(x), i);
+      });
+      __syncthreads();
+      const uint32_t n = sm.n_list;
+      if (n > 0 && n <= kList) {
+        const u64 before = f.before_wgt << 10, rest = share > before ? share - before : 1;
+        Cut cut(0u, 0u);
+        if (n <= kThreads) {
+          const u64 v = sorted_candidate(n, sm);
+          const u64 w = uint32_t(t) < n ? fixed(weight(key_logit(uint32_t(v >> 32)))) : 0;
+          u64 upto = w, all;
+          uint32_t one = 0, none;
+          block_scan(one, upto, none, all, sm);
+          // the last token that still begins before the share is reached
+          const bool kept = uint32_t(t) < n && (t == 0 || upto - w < rest);
+          const int last = __syncthreads_count(kept) - 1;
+          if (t == last) sm.red[0] = v;
+          __syncthreads();
+          cut = Cut(uint32_t(sm.red[0] >> 32), uint32_t(sm.red[0]));
+          __syncthreads();
+        } else {
+          cut = descend(ListRow{sm, n}, [](float, uint32_t) { return true; }, weight, true, true,
+                        rest, static_cast<u64*>(nullptr), sm);
+        }
+        token = race_row(row, [=](float x, uint32_t i) {
+          return cut.keeps(x, i) && over_floor(x); }, weight, noise, sm);
+        done = true;
       }
     }
     if (!done) {

@@ -23,6 +23,10 @@ place, and every element-wise stage is one of this library's kernels:
     -> time_mix_output      per-head GroupNorm, bonus, gate
     -> o_proj
 
+A block may hold low-rank adapters of its r, k, v and o projections
+(``add_adapters``); a batch that names its requests' adapters then runs those
+products on ``proj_adapters``, at any token count.
+
 Weights are stored [out, in] as nn.Linear holds them (each projection is
 ``linear(x, W)``), the layout both the grouped kernel and the vendor BLAS
 read best. At decode sizes each library GEMM is a separate 4-13 us launch;
@@ -44,6 +48,7 @@ import torch
 import torch.nn.functional as F
 
 from . import ops
+from .adapters import AdapterBank, AdapterPlan, adapter_plan, plan_ints, proj_adapters
 from .layout import HEAD_SIZE, RWKV7StateLayout
 from .state import RWKV7StateBank
 
@@ -64,7 +69,8 @@ class TokenBatch:
     """Device plan of one token batch: slot ids, ragged offsets, visiting order.
 
     ``decode``: one token per slot (``cu_seqlens`` = 0..B); otherwise ragged
-    prefill rows, sequence s owning tokens cu_seqlens[s]:cu_seqlens[s+1]."""
+    prefill rows, sequence s owning tokens cu_seqlens[s]:cu_seqlens[s+1].
+    ``adapters`` is the plan of every token's adapter (None: the base model)."""
 
     slot_ids: torch.Tensor
     cu_seqlens: torch.Tensor
@@ -72,20 +78,35 @@ class TokenBatch:
     nseq: int
     tokens: int
     decode: bool
+    adapters: AdapterPlan | None = None
 
     @classmethod
-    def plan(cls, bank: RWKV7StateBank, slot_ids, cu_seqlens=None) -> TokenBatch:
+    def plan(cls, bank: RWKV7StateBank, slot_ids, cu_seqlens=None, adapter_ids=None,
+             num_adapters: int = 0) -> TokenBatch:
+        """``adapter_ids``: every sequence's adapter (host integers below ``num_adapters``, -1:
+        none), for blocks that hold adapters."""
         rows, dev = bank.num_slots + 1, bank.device
+
+        def adapters(lengths: list[int]) -> AdapterPlan | None:
+            if adapter_ids is None:
+                return None
+            ids = [int(a) for a in adapter_ids]
+            if len(ids) != len(lengths):
+                raise ValueError(f"{len(ids)} adapter ids for {len(lengths)} sequences")
+            return adapter_plan([a for a, n in zip(ids, lengths) for _ in range(n)],
+                                num_adapters, dev)
         if cu_seqlens is None:
             ids, order = ops.decode_plan(slot_ids, rows, dev)
             n = int(ids.shape[0])
-            return cls(ids, torch.arange(n + 1, dtype=torch.int32, device=dev), order, n, n, True)
+            return cls(ids, torch.arange(n + 1, dtype=torch.int32, device=dev), order, n, n, True,
+                       adapters([1] * n))
         cu = cu_seqlens.tolist() if isinstance(cu_seqlens, torch.Tensor) else list(cu_seqlens)
         T = int(cu[-1]) if cu else 0
         ids, cu_t, n = ops.seq_plan(slot_ids, cu, rows, T, dev)
         order = torch.tensor(ops.longest_first([int(c) for c in cu]), dtype=torch.int32,
                              device=dev)
-        return cls(ids, cu_t, order, n, T, False)
+        return cls(ids, cu_t, order, n, T, False,
+                   adapters([int(cu[i + 1]) - int(cu[i]) for i in range(n)]))
 
 
 class RWKV7TimeMix:
@@ -104,6 +125,18 @@ class RWKV7TimeMix:
         self.layer_idx = layer_idx
         self.w = weights
         self.eps = HEAD_SIZE * 1e-5
+        self.adapters: dict[str, AdapterBank] = {}
+
+    def add_adapters(self, num_adapters: int, max_rank: int, names=("r", "k", "v", "o"),
+                     ) -> dict[str, AdapterBank]:
+        """Empty banks of ``num_adapters`` places for the named projections; ``load`` fills
+        them. A batch planned with ``adapter_ids`` uses them."""
+        for name in names:
+            if name not in ("r", "k", "v", "o"):
+                raise ValueError(f"adapters are held by r, k, v and o, not {name!r}")
+            n, k = self.w[name].shape
+            self.adapters[name] = AdapterBank(num_adapters, k, n, max_rank, self.w[name].device)
+        return self.adapters
 
     @classmethod
     def random(cls, layout: RWKV7StateLayout, layer_idx: int, device, seed: int = 0,
@@ -160,7 +193,7 @@ class RWKV7TimeMix:
         xr, xw, xk, xv, xa, xg = ops.token_shift_mix(
             x, bank.shift[l, 0], batch.slot_ids, W["mix"],
             None if batch.decode else batch.cu_seqlens)
-        if batch.tokens <= self.PROJ_MAX_ROWS:
+        if batch.tokens <= self.PROJ_MAX_ROWS or batch.adapters is not None:
             return self._forward_grouped(bank, batch, v_first, zero_init,
                                          (xr, xw, xk, xv, xa, xg))
 
@@ -209,14 +242,26 @@ class RWKV7TimeMix:
                  (xa, W["a1"]), (xg, W["g1"], None, "sigmoid")]
         if l > 0:
             first.append((xv, W["v1"]))
-        r, k, v, hw, ha, hg, *hv = ops.proj_grouped(first)
+        r, k, v, hw, ha, hg, *hv = self._project(batch, first, ("r", "k", "v"))
         second = [(hw, W["w2"], W["w0"]), (ha, W["a2"], W["a0"]), (hg, W["g2"])]
         if l > 0:
             second.append((hv[0], W["v2"], W["v0"]))
-        w_l, a_l, g, *v_l = ops.proj_grouped(second)
+        if batch.tokens <= self.PROJ_MAX_ROWS:
+            w_l, a_l, g, *v_l = ops.proj_grouped(second)
+        else:
+            w_l, a_l, g, *v_l = (F.linear(*product) for product in second)
         o_in, v_first = self._wkv_stage(bank, batch, v_first, zero_init, r, k, v, w_l, a_l,
                                         v_l[0] if v_l else None, g)
-        return ops.proj_grouped([(o_in, W["o"])])[0], v_first
+        return self._project(batch, [(o_in, W["o"])], ("o",))[0], v_first
+
+    def _project(self, batch, products, names):
+        """The products in one grouped launch, the first ones (``names``) with their adapters
+        where the batch has any."""
+        if batch.adapters is None:
+            return ops.proj_grouped(products)
+        padded = [p + (None,) * (4 - len(p)) for p in products]
+        banks = [self.adapters.get(n) for n in names] + [None] * (len(products) - len(names))
+        return proj_adapters([p + (b,) for p, b in zip(padded, banks)], batch.adapters)
 
     def _wkv_stage(self, bank, batch, v_first, zero_init, r, k, v, w_l, a_l, v_l, g):
         """time_mix_inputs -> in-place WKV7 -> time_mix_output (one fused
@@ -256,10 +301,11 @@ class TimeMixDecodeGraph:
     their slot-sorted visiting order and the one-token-per-slot offsets live
     in one device buffer refreshed by ``set_slots``. A graph is bound to a
     batch size and to the bank's tensors (the reference's per-bucket graphs,
-    experiments/m2_engine_bench.py:44-131)."""
+    experiments/m2_engine_bench.py:44-131). With ``num_adapters`` the blocks' adapters take part:
+    ``set_adapters`` names every row's (none until then)."""
 
     def __init__(self, bank: RWKV7StateBank, layers: list[RWKV7TimeMix], batch_size: int,
-                 side_streams: int | None = None):
+                 side_streams: int | None = None, num_adapters: int = 0):
         if batch_size < 1:
             raise ValueError("batch_size must be >= 1")
         if len(layers) < 1 or any(l.layer_idx != i for i, l in enumerate(layers)):
@@ -273,7 +319,10 @@ class TimeMixDecodeGraph:
         self._order = ops.ReplayOrder()
         self.x = torch.zeros((len(layers), B, D), dtype=torch.bfloat16, device=dev)
         self.o: list[torch.Tensor] = []
-        batch = TokenBatch(self.plan[:B], self.plan[2 * B:], self.plan[B:2 * B], B, B, True)
+        self.num_adapters = int(num_adapters)
+        self.adapter_plan = adapter_plan([-1] * B, num_adapters, dev) if num_adapters else None
+        batch = TokenBatch(self.plan[:B], self.plan[2 * B:], self.plan[B:2 * B], B, B, True,
+                           self.adapter_plan)
         # side streams (default priority) for the block's independent GEMM
         # chains when they run on the vendor BLAS (batches above
         # PROJ_MAX_ROWS; default 2 there, none below); the graph keeps their
@@ -309,6 +358,16 @@ class TimeMixDecodeGraph:
                              f"{self.batch_size}")
         order = sorted(range(len(lst)), key=lst.__getitem__)
         self._order.refresh(self.plan[:2 * self.batch_size], lst + order)
+
+    def set_adapters(self, adapter_ids) -> None:
+        """The rows' adapters (host integers, -1: none), uploaded as ``set_slots`` uploads the
+        slots."""
+        if self.adapter_plan is None:
+            raise ValueError("a graph captured without adapters (num_adapters = 0)")
+        ids = [int(a) for a in adapter_ids]
+        if len(ids) != self.batch_size:
+            raise ValueError(f"{len(ids)} adapter ids for a graph of batch size {self.batch_size}")
+        self._order.refresh(self.adapter_plan.buf, plan_ints(ids, self.num_adapters).tolist())
 
     def replay(self) -> list[torch.Tensor]:
         """Run the captured step; returns the static outputs ``o`` (L x [B, D])."""

@@ -623,6 +623,11 @@ typedef struct wkv7_adapter_set {
   int32_t slabs;
 } wkv7_adapter_set;
 
+/* Puts the pair a [r, k], b [n, r] (device, rows lda and ldb elements apart) with its scale into
+ * place `index` of a set, whose memory is written; 1 <= r <= 16 slabs. */
+int wkv7_adapter_load(const wkv7_adapter_set *set, int32_t index, int32_t n, int32_t k,
+                      const uint16_t *a, int64_t lda, const uint16_t *b, int64_t ldb, int32_t r,
+                      float scale, void *stream);
 int64_t wkv7_adapter_plan_ints(int64_t m, int32_t count);
 int wkv7_adapter_plan(const int32_t *ids, int64_t m, int32_t count, int32_t *plan,
                       int64_t plan_ints);

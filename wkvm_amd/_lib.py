@@ -123,6 +123,8 @@ SIGNATURES = {
     "wkv7_proj_grouped_noalloc": (ctypes.c_int, [_i64, ctypes.POINTER(ProjGroup), _i32, _vp]),
     "wkv7_decode_block": (ctypes.c_int, [
         _vp, _i64, _i32, _vp, _vp, _i32] + [_vp] * 13 + [_f32, _f32, _vp, _vp, _vp]),
+    "wkv7_adapter_load": (ctypes.c_int, [
+        ctypes.POINTER(AdapterSet), _i32, _i32, _i32, _vp, _i64, _vp, _i64, _i32, _f32, _vp]),
     "wkv7_adapter_plan_ints": (_i64, [_i64, _i32]),
     "wkv7_adapter_plan": (ctypes.c_int, [_vp, _i64, _i32, _vp, _i64]),
     "wkv7_proj_adapters": (ctypes.c_int, [

@@ -74,17 +74,19 @@ class AdapterBank:
                              f"{tuple(a.shape)} and {tuple(b.shape)}")
         if not math.isfinite(scale):
             raise ValueError(f"scale must be finite, got {scale}")
-        whole = r // _SLAB
-        self.a[index, :r] = a
-        self.a[index, r:] = 0
-        place = self.b[index]
-        if whole:
-            place[:whole] = b[:, :whole * _SLAB].reshape(self.n, whole, _SLAB).transpose(0, 1)
-        place[whole:] = 0
-        if r % _SLAB:
-            place[whole, :, :r % _SLAB] = b[:, whole * _SLAB:]
-        self.scale[index] = float(scale)
-        self.rank[index] = r
+        for t, name in ((a, "a"), (b, "b")):
+            ops._require_cuda(t, name)
+            if t.device != self.a.device:
+                raise ValueError(f"{name} on {t.device}, the bank on {self.a.device}")
+        if a.stride(1) != 1 or r > 1 and a.stride(0) < self.k:
+            a = a.contiguous()
+        if b.stride(1) != 1 or self.n > 1 and b.stride(0) < r:
+            b = b.contiguous()
+        rc = _lib.load().wkv7_adapter_load(self.set, index, self.n, self.k, a.data_ptr(),
+                                           max(a.stride(0), self.k), b.data_ptr(),
+                                           max(b.stride(0), r), r, float(scale),
+                                           ops._stream_ptr(self.a.device))
+        _lib.check(rc, "wkv7_adapter_load")
 
     def clear(self, index: int) -> None:
         """Empty a place: rows that name it get the shared product alone."""

@@ -184,6 +184,47 @@ __global__ __launch_bounds__(256) void shrink_wide_kernel(const ShrinkArgs args)
   else if (all - s == 1) slabs(s, std::integral_constant<int, 1>{});
 }
 
+// Puts one adapter into its place: A's rows and then zeros (blocks [0, a_blocks)), B's columns in
+// slabs of 16 with zeros past the rank, scale and rank. A thread moves 16 bytes of the place.
+struct LoadArgs {
+  const uint16_t *a, *b;
+  uint16_t *to_a, *to_b;
+  float* to_scale;
+  int32_t* to_rank;
+  int64_t lda, ldb;
+  float scale;
+  int32_t r, k, n, slabs, a_blocks;
+};
+
+__global__ __launch_bounds__(256) void adapter_load_kernel(const LoadArgs args) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    *args.to_scale = args.scale;
+    *args.to_rank = args.r;
+  }
+  uint16_t v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (int(blockIdx.x) < args.a_blocks) {
+    const int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 8;  // in [16 slabs][k]
+    const int64_t row = i / args.k;
+    if (row >= int64_t(kSlab) * args.slabs) return;
+    if (row < args.r) {
+      const uint16_t* p = args.a + row * args.lda + (i - row * args.k);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = p[e];
+    }
+    *reinterpret_cast<uint4*>(args.to_a + i) = *reinterpret_cast<const uint4*>(v);
+    return;
+  }
+  const int64_t i = (int64_t(blockIdx.x - args.a_blocks) * 256 + threadIdx.x) * 8;  // [slabs][n][16]
+  const int64_t row = i / kSlab % args.n, slab = i / kSlab / args.n;
+  if (slab >= args.slabs) return;
+  const int64_t col = slab * kSlab + i % kSlab;
+  const uint16_t* p = args.b + row * args.ldb + col;
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (col + e < args.r) v[e] = p[e];
+  *reinterpret_cast<uint4*>(args.to_b + i) = *reinterpret_cast<const uint4*>(v);
+}
+
 int64_t max_tiles(int64_t m, int32_t count) { return m / kSlab + std::min<int64_t>(m, count) + 1; }
 
 // Positions of a plan: the rows, and where the runs of an adapter are aligned the gaps too.
@@ -258,6 +299,20 @@ Work make_work(int64_t rows, int64_t m, const wkv7_proj_group* groups, const wkv
   w.waves = thin_waves(m, groups, ng, cus);
   w.wide = wide_tile(rows, m, groups, ng, cus);
   w.plan = make_plan(m, groups, ng, cus);
+  // 128 x 64 tiles for at most half of the units and k of 4096 or more: k split over two
+  // workgroups per tile, which also share its adapters. 203 rows of a 4096 x 4096 product, 24
+  // adapters of 64 ranks: XX us in place of 49. (At half that k the second launch takes what the
+  // split gains, and without adapters the bits are wkv7_proj_grouped's.)
+  const int64_t tiles = count_tiles(m, groups, ng, kShapes[2]);
+  int kmin = groups[0].k;
+  for (int i = 1; i < ng; ++i) kmin = std::min(kmin, groups[i].k);
+  if (!w.waves && !w.wide && w.plan.shape == 2 && w.plan.parts == 1 && 2 * tiles <= cus &&
+      kmin >= 4096) {
+    int64_t cols = 0;
+    for (int i = 0; i < ng; ++i) cols += groups[i].n;
+    w.plan.parts = 2;
+    w.plan.ws_bytes = 2 * size_t(m) * size_t(cols) * sizeof(float);
+  }
   for (int i = 0; i < ng; ++i) {
     w.h[i] = w.bytes;
     if (sets[i].a) w.bytes += align256(size_t(m) * sets[i].slabs * kParts * kSlab * sizeof(uint16_t));
@@ -326,6 +381,37 @@ extern "C" int wkv7_adapter_plan(const int32_t* ids, int64_t m, int32_t count, i
     }
   }
   return WKV7_OK;
+}
+
+extern "C" int wkv7_adapter_load(const wkv7_adapter_set* set, int32_t index, int32_t n, int32_t k,
+                                 const uint16_t* a, int64_t lda, const uint16_t* b, int64_t ldb,
+                                 int32_t r, float scale, void* stream) {
+  if (!set || !set->a || !set->b || !set->scale || !set->rank || !a || !b) return WKV7_ERR_ARG;
+  if (index < 0 || index >= set->count || set->slabs < 1 ||
+      set->slabs > WKV7_ADAPTER_MAX_RANK / kSlab || n < 1 || k < 32 || k % 32 || r < 1 ||
+      r > set->slabs * kSlab)
+    return WKV7_ERR_ARG;
+  if (lda < k || ldb < r || !aligned16(set->a) || !aligned16(set->b)) return WKV7_ERR_SHAPE;
+  const int64_t size_a = int64_t(kSlab) * set->slabs * k, size_b = int64_t(kSlab) * set->slabs * n;
+  const int64_t a_blocks = (size_a + 2047) / 2048, b_blocks = (size_b + 2047) / 2048;
+  if (a_blocks + b_blocks > 0x7fffffff) return WKV7_ERR_ARG;
+  // (the set's pointers are the bank's own memory, which a launch of this kind may write)
+  const LoadArgs args{a,
+                      b,
+                      const_cast<uint16_t*>(set->a) + index * size_a,
+                      const_cast<uint16_t*>(set->b) + index * size_b,
+                      const_cast<float*>(set->scale) + index,
+                      const_cast<int32_t*>(set->rank) + index,
+                      lda,
+                      ldb,
+                      scale,
+                      r,
+                      k,
+                      n,
+                      set->slabs,
+                      int32_t(a_blocks)};
+  adapter_load_kernel<<<unsigned(a_blocks + b_blocks), 256, 0, as_stream(stream)>>>(args);
+  return launch_status();
 }
 
 extern "C" size_t wkv7_proj_adapters_workspace_bytes(int64_t m, const wkv7_proj_group* groups,

@@ -172,7 +172,7 @@ struct Pairs {
 // in flight at once: a tile of a decode batch may meet an adapter per row, and each of them is
 // one pass from memory. The first U are under way from the constructor on, so they arrive while
 // the shared product is computed; add() multiplies them and fetches the others. kSwap: acc holds
-// the transposed tile. Pairs are dealt to `step` waves.
+// the transposed tile. Pairs are dealt to `step` waves, or workgroups that share a tile.
 template <int TM, int TN, int U, bool kSwap>
 struct Expand {
   static_assert(TM <= 4, "a lane per position");
@@ -184,10 +184,10 @@ struct Expand {
   int from[U], to[U];
 
   __device__ __forceinline__ Expand(const Adapters& ad, int g, int64_t p0, int64_t M, int n0_,
-                                    int N_, bool any, int mine, int step_)
+                                    int N_, int mine, int step_)
       : n0(n0_),
         N(N_),
-        rows(any && ad.b[g] ? int(min(int64_t(16 * TM), M - p0)) : 0),
+        rows(ad.b[g] ? int(min(int64_t(16 * TM), M - p0)) : 0),
         slabs(ad.slabs[g]),
         step(step_),
         pairs(ad, g, p0, rows) {
@@ -354,7 +354,7 @@ __global__ __launch_bounds__(64 * GM * GN) void proj_kernel(const ProjArgs args,
   // (16 waves have 128 registers each)
   constexpr int kPairs = NW >= 16 ? 2 : TM > 1 ? 4 : 8;
   std::conditional_t<Extra::kOn, Expand<TM, TN, kPairs, false>, NoExpand> extra(
-      ex, g, m0 + wm * WM, M, n0 + wn * WN, N, part == 0, 0, 1);
+      ex, g, m0 + wm * WM, M, n0 + wn * WN, N, part, kSplit ? args.parts : 1);
 
   // A stage: all fragment reads first, then its MFMAs with the next stage's
   // loads (when kIssue) spread between them, so the matrix core works while
@@ -526,8 +526,8 @@ __global__ __launch_bounds__(64 * NW) void proj_thin_kernel(const ProjArgs args,
   const uint16_t* xp = G.x + ex.row(min(li, M - 1)) * G.ldx + 8 * lg;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   std::conditional_t<Extra::kOn, Expand<1, 1, 4, true>, NoExpand> extra(ex, g, int64_t(0),
-                                                                         int64_t(M), n0, N, true,
-                                                                         wave, NW);
+                                                                         int64_t(M), n0, N, wave,
+                                                                         NW);
   // U chunks of this wave from chunk c on. Only the last chunk of all can be
   // half a chunk wide: its second half re-reads the first and is left out.
   auto chunks = [&](int c, auto u_c) {

@@ -251,11 +251,12 @@ int check_sets(const wkv7_adapter_set* sets, int32_t ngroups, int32_t count) {
   return WKV7_OK;
 }
 
-// Whether the wide kernel's 32-bit row offsets reach every row.
-bool offsets_fit(int64_t m, const wkv7_proj_group* groups, int ng) {
+// What the wide kernel needs of the products: whole stages of k, and rows that its 32-bit offsets
+// reach.
+bool wide_fits(int64_t m, const wkv7_proj_group* groups, int ng) {
   for (int i = 0; i < ng; ++i) {
     const int64_t k = groups[i].k;
-    if (((m - 1) * groups[i].ldx + k) * 2 > int64_t(0xffffffff) ||
+    if (k % 64 || ((m - 1) * groups[i].ldx + k) * 2 > int64_t(0xffffffff) ||
         ((int64_t(groups[i].n) - 1) * groups[i].ldw + k) * 2 > int64_t(0xffffffff))
       return false;
   }
@@ -269,7 +270,7 @@ bool offsets_fit(int64_t m, const wkv7_proj_group* groups, int ng) {
 // in 256 x 256, 165 in 128 x 64), 32,768 rows 973 in 256 x 256 (1187, about 2200). A plan of few
 // rows does not align its runs as the wide kernel needs.
 int wide_tile(int64_t m, int64_t positions, const wkv7_proj_group* groups, int ng, int cus) {
-  if (m <= WKV7_ADAPTER_PACKED_ROWS || !offsets_fit(m, groups, ng)) return 0;
+  if (m <= WKV7_ADAPTER_PACKED_ROWS || !wide_fits(m, groups, ng)) return 0;
   const struct { TileShape shape; int tm; double us; } kinds[] = {
       {{128, 64}, 0, 16.5}, {{128, 256}, 2, 47.}, {{256, 256}, 4, 79.}};
   double best = 0.;

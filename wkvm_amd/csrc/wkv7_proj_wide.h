@@ -147,47 +147,45 @@ __global__ __launch_bounds__(64 * kWideWaves) void proj_wide_kernel(const ProjAr
                              : int64_t(min(n0 + row - BM, N - 1)) * G.ldw;
     off[i] = uint32_t((r + 8 * chunk) * 2);
   }
-  const int nk = (K + 63) / 64;
-  const bool half = K % 64 != 0;  // the last stage is 32 wide
-  // (its chunks past k are the ones before them once more; nothing multiplies them)
-  const uint32_t back = half && chunk >= 4 ? 64 : 0;
+  const int nk = K / 64;
   const char* const xb = reinterpret_cast<const char*>(G.x);
   const char* const wb = reinterpret_cast<const char*>(G.w);
   const uint32_t ring_base = lds_addr(ring);
-  // Load i of stage kt into the slot at byte `slot`; past the last stage it is the last one that
-  // is read again (and not used).
-  auto load = [&](int kt, uint32_t slot, int i) {
-    load_lds16_from((i < LX ? xb : wb) + int64_t(min(kt, nk - 1)) * 128,
-                    off[i] - (kt >= nk - 1 ? back : 0),
-                    ring_base + slot + 1024u * (kWideWaves * i + wave));
+  // Load i of the stage at byte k of the rows, into the slot at `to` (this wave's part of it).
+  auto load = [&](uint32_t k, uint32_t to, int i) {
+    load_lds16_from((i < LX ? xb : wb) + k, off[i], to + 1024u * kWideWaves * i);
   };
+  // (what is loaded ahead of the end, and not used, is the last stage again)
+  auto stage_k = [&](int kt) { return uint32_t(min(kt, nk - 1)) * 128; };
 
   f32x16 acc[TM][TN] = {};
   // Operands of a step: two sets of w tiles; of the x tiles one set, which the next step's reads
   // refill as its tiles are done with, and a second of the last one, so that no read is the last
   // thing before a barrier.
   uint4 wf[2][TN], xf[TM - 1], xl[2];
-  uint32_t x_at[4], w_at[4];
+  uint32_t x_at[4], w_at[4];  // of the four steps, in the slot that is read
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
     const uint32_t in_tile = 128 * li + 16 * ((2 * s + lh) ^ (li & 7));
     x_at[s] = ring_base + 128 * (wm * WM) + in_tile;
     w_at[s] = ring_base + 128 * (BM + wn * WN) + in_tile;
   }
-  auto read_w = [&](uint32_t slot, auto s_c, int i) {
+  auto read_w = [&](auto s_c, int i) {
     constexpr int s = decltype(s_c)::value;
-    wf[s & 1][i] = lds_read(w_at[s] + slot, 4096 * i);
+    wf[s & 1][i] = lds_read(w_at[s], 4096 * i);
   };
-  auto read_x = [&](uint32_t slot, auto s_c, int i) {
+  auto read_x = [&](auto s_c, int i) {
     constexpr int s = decltype(s_c)::value;
-    const uint4 v = lds_read(x_at[s] + slot, 4096 * i);
+    const uint4 v = lds_read(x_at[s], 4096 * i);
     if (i < TM - 1) xf[i] = v;
     else xl[s & 1] = v;
   };
-  // Multiplies step s of a stage with the reads of step r (kRead, from slot rs) and the loads
-  // [l0, l1) of stage kl, to slot ls, placed between the MFMAs.
-  auto multiply = [&](auto s_c, auto r_c, uint32_t rs, auto l0, auto l1, int kl, uint32_t ls) {
-    constexpr int s = decltype(s_c)::value & 1, r = decltype(r_c)::value;
+  // Multiplies step s of a stage with the reads of step r and the loads [l0, l1) of the stage at
+  // byte k, to the slot at `to`, placed between the MFMAs. Between two MFMAs a wave issues
+  // only a handful of instructions, so addresses are kept ready: the operands' are advanced once
+  // per stage (through an asm, lest the compiler add the slot to each of them at every read).
+  auto multiply = [&](auto s_c, auto r_c, auto l0, auto l1, uint32_t k, uint32_t to) {
+    constexpr int s = decltype(s_c)::value & 1;
     constexpr int kFrom = decltype(l0)::value, kLoads = decltype(l1)::value - kFrom;
     constexpr int kAll = TM * TN;
     int done = 0;
@@ -195,16 +193,13 @@ __global__ __launch_bounds__(64 * kWideWaves) void proj_wide_kernel(const ProjAr
     for (int m = 0; m < kAll; ++m) {
       const int a = m / TN, b = m % TN;
       acc[a][b] = mma16(wf[s][b], a < TM - 1 ? xf[a] : xl[s], acc[a][b]);
-      if constexpr (r >= 0) {
-        if (m < TN) read_w(rs, r_c, m);
-        else if (b == 0) read_x(rs, r_c, a - 1);
-        else if (m == TN + 1) read_x(rs, r_c, TM - 1);
-      }
-      if (done < kLoads && (m + 1) * kLoads >= (done + 1) * kAll) load(kl, ls, kFrom + done++);
+      if (m < TN) read_w(r_c, m);
+      else if (b == 0) read_x(r_c, a - 1);
+      else if (m == TN + 1) read_x(r_c, TM - 1);
+      if (done < kLoads && (m + 1) * kLoads >= (done + 1) * kAll) load(k, to, kFrom + done++);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  const std::integral_constant<int, -1> none{};
   const std::integral_constant<int, 0> c0{};
   const std::integral_constant<int, 1> c1{};
   const std::integral_constant<int, 2> c2{};
@@ -212,28 +207,34 @@ __global__ __launch_bounds__(64 * kWideWaves) void proj_wide_kernel(const ProjAr
   const std::integral_constant<int, LE> le{};
   const std::integral_constant<int, LR> lr{};
 
+  uint32_t to = ring_base + 1024u * wave;  // the slot of the stage at hand
+  uint32_t flip = kSlot;                   // from it to the other one
 #pragma unroll
-  for (int i = 0; i < LR; ++i) load(0, 0, i);
+  for (int i = 0; i < LR; ++i) load(0, to, i);
 #pragma unroll
-  for (int i = 0; i < LE; ++i) load(1, kSlot, i);
+  for (int i = 0; i < LE; ++i) load(stage_k(1), to + flip, i);
   stage_barrier<LE>();
 #pragma unroll
-  for (int i = 0; i < TN; ++i) read_w(0, c0, i);
+  for (int i = 0; i < TN; ++i) read_w(c0, i);
 #pragma unroll
-  for (int i = 0; i < TM; ++i) read_x(0, c0, i);
-  // Stage kt is in slot; the early loads of stage kt + 1 are under way. At the barrier before its
-  // last step, stage kt + 1 has arrived and every wave has read stage kt, whose slot then takes
-  // the early loads of stage kt + 2.
-  uint32_t slot = 0;
+  for (int i = 0; i < TM; ++i) read_x(c0, i);
+  // The early loads of stage kt + 1 are under way. At the barrier before its last step, stage kt + 1
+  // has arrived and every wave has read stage kt, whose slot then takes the early loads of
+  // stage kt + 2.
   for (int kt = 0; kt < nk; ++kt) {
-    const uint32_t other = kSlot - slot;
-    multiply(c0, c1, slot, le, lr, kt + 1, other);
-    multiply(c1, c2, slot, c0, c0, 0, 0);
-    if (half && kt + 1 == nk) break;
-    multiply(c2, c3, slot, c0, c0, 0, 0);
+    multiply(c0, c1, le, lr, stage_k(kt + 1), to + flip);
+    multiply(c1, c2, c0, c0, 0, 0);
+    multiply(c2, c3, c0, c0, 0, 0);
     stage_barrier<0>();
-    multiply(c3, c0, other, c0, le, kt + 2, slot);
-    slot = other;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      x_at[s] += flip;
+      w_at[s] += flip;
+      asm volatile("" : "+v"(x_at[s]), "+v"(w_at[s]));
+    }
+    multiply(c3, c0, c0, le, stage_k(kt + 2), to);
+    to += flip;
+    flip = -flip;
   }
   // (the loads past the last stage: none may be under way when the workgroup ends)
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");

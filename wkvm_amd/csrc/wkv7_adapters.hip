@@ -129,59 +129,101 @@ __global__ __launch_bounds__(64 * NW) void shrink_thin_kernel(const ShrinkArgs a
             left - 4 * lg);
 }
 
-// Many tiles: a wave per tile, all of k, up to four slabs at once.
-__global__ __launch_bounds__(256) void shrink_wide_kernel(const ShrinkArgs args) {
+// Many tiles: a workgroup for two of them, k dealt to its waves as above and up to four slabs at
+// once. Two tiles of one adapter, as nearly all of a prompt's are, share the reads of A, which
+// are otherwise twice x's. (32,768 rows of 2048 in three products of rank 32, x alone 400 MB: with
+// a wave per tile, which walks 16 rows in steps of 64 bytes, 165 us; a workgroup per tile 148;
+// two tiles 109, and 116 with four chunks of k in flight in place of two.)
+constexpr int kWideShrink = 4;
+
+__global__ __launch_bounds__(64 * kWideShrink) void shrink_wide_kernel(const ShrinkArgs args) {
+  constexpr int NW = kWideShrink;
+  __shared__ f32x4 red[NW][4][64];
   const ShrinkGroup& G = args.g[blockIdx.y];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t index = int64_t(blockIdx.x) * 4 + wave;
-  const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
-  if (!G.a || index >= args.ntiles) return;
-  const Tile tile = get_tile(args, G, index, li);
-  if (tile.rows == 0) return;
-  const int K = G.k;
-  const int rank = min(G.rank[tile.id], G.slabs * kSlab), all = (rank + kSlab - 1) / kSlab;
-  const uint16_t* xp = G.x + tile.row * G.ldx + 8 * lg;
-  const float scale = G.scale[tile.id];
-  auto slabs = [&](int s0, auto n_c) {
-    constexpr int NS = decltype(n_c)::value;
-    constexpr int U = NS <= 2 ? 8 : 4;
-    const uint16_t* ap = G.a + ((int64_t(tile.id) * G.slabs + s0) * kSlab + li) * K + 8 * lg;
-    f32x4 acc[NS];
+  if (!G.a) return;
+  const int t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int K = G.k, nc = (K + 63) / 64;
+  // NT tiles of one adapter, NS of its slabs from s0 on
+  auto slabs = [&](const Tile* tiles, int rank, int s0, auto nt_c, auto n_c) {
+    constexpr int NT = decltype(nt_c)::value, NS = decltype(n_c)::value;
+    constexpr int U = NS * NT <= 2 ? 4 : 2;
+    const int id = __builtin_amdgcn_readfirstlane(tiles[0].id);
+    const uint16_t* ap = G.a + ((int64_t(id) * G.slabs + s0) * kSlab + li) * K + 8 * lg;
+    const uint16_t* xp[NT];
+    f32x4 acc[NT][NS];
 #pragma unroll
-    for (int s = 0; s < NS; ++s) acc[s] = f32x4{0.f, 0.f, 0.f, 0.f};
-    int k = 0;
-    for (; k + 32 * U <= K; k += 32 * U) {
-      uint4 xf[U], af[U][NS];
+    for (int i = 0; i < NT; ++i) {
+      xp[i] = G.x + tiles[i].row * G.ldx + 8 * lg;
+#pragma unroll
+      for (int s = 0; s < NS; ++s) acc[i][s] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int c = wave; c < nc; c += U * NW) {
+      uint4 xf[U][2][NT], af[U][2][NS];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        xf[u] = *reinterpret_cast<const uint4*>(xp + k + 32 * u);
+        // (past the end: the last chunk once more, left out below)
+        const int k0 = 64 * min(c + u * NW, nc - 1), k1 = k0 + 32 < K ? k0 + 32 : k0;
 #pragma unroll
-        for (int s = 0; s < NS; ++s)
-          af[u][s] = *reinterpret_cast<const uint4*>(ap + int64_t(s) * kSlab * K + k + 32 * u);
+        for (int i = 0; i < NT; ++i) {
+          xf[u][0][i] = *reinterpret_cast<const uint4*>(xp[i] + k0);
+          xf[u][1][i] = *reinterpret_cast<const uint4*>(xp[i] + k1);
+        }
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          af[u][0][s] = *reinterpret_cast<const uint4*>(ap + int64_t(s) * kSlab * K + k0);
+          af[u][1][s] = *reinterpret_cast<const uint4*>(ap + int64_t(s) * kSlab * K + k1);
+        }
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) {
+        if (c + u * NW >= nc) break;
 #pragma unroll
-        for (int s = 0; s < NS; ++s) acc[s] = mma(af[u][s], xf[u], acc[s]);
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int s = 0; s < NS; ++s) {
+            acc[i][s] = mma(af[u][0][s], xf[u][0][i], acc[i][s]);
+            if (64 * (c + u * NW) + 32 < K) acc[i][s] = mma(af[u][1][s], xf[u][1][i], acc[i][s]);
+          }
+      }
     }
-    for (; k < K; k += 32) {
-      const uint4 xf = *reinterpret_cast<const uint4*>(xp + k);
+    const float scale = G.scale[id];
 #pragma unroll
-      for (int s = 0; s < NS; ++s)
-        acc[s] = mma(*reinterpret_cast<const uint4*>(ap + int64_t(s) * kSlab * K + k), xf, acc[s]);
-    }
-    if (li < tile.rows) {
+    for (int i = 0; i < NT; ++i) {
+      __syncthreads();
 #pragma unroll
-      for (int s = 0; s < NS; ++s)
-        store_h(G.h + ((tile.first + li) * G.slabs + s0 + s) * kParts * kSlab + 4 * lg, acc[s], scale,
-                rank - (s0 + s) * kSlab - 4 * lg);
+      for (int s = 0; s < NS; ++s) red[wave][s][lane] = acc[i][s];
+      __syncthreads();
+      for (int s = wave; s < NS; s += NW) {  // a slab per wave
+        f32x4 sum = red[0][s][lane];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) sum += red[w][s][lane];
+        if (li < tiles[i].rows)
+          store_h(G.h + ((tiles[i].first + li) * G.slabs + s0 + s) * kParts * kSlab + 4 * lg, sum,
+                  scale, rank - (s0 + s) * kSlab - 4 * lg);
+      }
     }
   };
-  int s = 0;
-  for (; s + 4 <= all; s += 4) slabs(s, std::integral_constant<int, 4>{});
-  if (all - s == 3) slabs(s, std::integral_constant<int, 3>{});
-  else if (all - s == 2) slabs(s, std::integral_constant<int, 2>{});
-  else if (all - s == 1) slabs(s, std::integral_constant<int, 1>{});
+  auto run = [&](const Tile* tiles, auto nt_c) {
+    const int rank = min(G.rank[tiles[0].id], G.slabs * kSlab), all = (rank + kSlab - 1) / kSlab;
+    int s = 0;
+    for (; s + 4 <= all; s += 4) slabs(tiles, rank, s, nt_c, std::integral_constant<int, 4>{});
+    if (all - s == 3) slabs(tiles, rank, s, nt_c, std::integral_constant<int, 3>{});
+    else if (all - s == 2) slabs(tiles, rank, s, nt_c, std::integral_constant<int, 2>{});
+    else if (all - s == 1) slabs(tiles, rank, s, nt_c, std::integral_constant<int, 1>{});
+  };
+  const int64_t first = 2 * int64_t(blockIdx.x);
+  Tile tiles[2] = {get_tile(args, G, first, li), {}};
+  if (first + 1 < args.ntiles) tiles[1] = get_tile(args, G, first + 1, li);
+  if (tiles[0].rows > 0 && tiles[1].rows > 0 && tiles[0].id == tiles[1].id) {
+    run(tiles, std::integral_constant<int, 2>{});
+    return;
+  }
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) {
+    const Tile one = i == 0 ? tiles[0] : tiles[1];
+    if (one.rows > 0) run(&one, std::integral_constant<int, 1>{});
+  }
 }
 
 // Puts one adapter into its place: A's rows and then zeros (blocks [0, a_blocks)), B's columns in
@@ -302,7 +344,7 @@ Work make_work(int64_t rows, int64_t m, const wkv7_proj_group* groups, const wkv
   w.plan = make_plan(m, groups, ng, cus);
   // 128 x 64 tiles for at most half of the units and k of 4096 or more: k split over two
   // workgroups per tile, which also share its adapters. 203 rows of a 4096 x 4096 product, 24
-  // adapters of 64 ranks: XX us in place of 49. (At half that k the second launch takes what the
+  // adapters of 64 ranks: 45 us in place of 49. (At half that k the second launch takes what the
   // split gains, and without adapters the bits are wkv7_proj_grouped's.)
   const int64_t tiles = count_tiles(m, groups, ng, kShapes[2]);
   int kmin = groups[0].k;
@@ -479,8 +521,8 @@ extern "C" int wkv7_proj_adapters(int64_t m, const wkv7_proj_group* groups,
       if (kmax <= 1024) shrink_thin_kernel<4><<<grid, 256, 0, s>>>(sh);
       else shrink_thin_kernel<8><<<grid, 512, 0, s>>>(sh);
     } else {
-      const dim3 grid(unsigned((sh.ntiles + 3) / 4), unsigned(ngroups));
-      shrink_wide_kernel<<<grid, 256, 0, s>>>(sh);
+      const dim3 grid(unsigned((sh.ntiles + 1) / 2), unsigned(ngroups));
+      shrink_wide_kernel<<<grid, 64 * kWideShrink, 0, s>>>(sh);
     }
     rc = launch_status();
     if (rc != WKV7_OK) return rc;

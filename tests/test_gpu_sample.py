@@ -126,6 +126,17 @@ def test_mixed_settings(vocab, dtype):
     _check(logits, noise, temp, k, p, m, got)
 
 
+@pytest.mark.parametrize("vocab", [800003, 1048579, 1 << 21])
+def test_large_vocabularies(vocab):
+    """More groups than the candidates' group weights have room for."""
+    rows = 8
+    logits, noise = _inputs(rows, vocab, torch.bfloat16, 7)
+    temp, k, p, m = _settings(rows, 9)
+    got = sample_tokens(logits, noise, temperature=temp.cuda(), top_k=k.cuda(), top_p=p.cuda(),
+                        min_p=m.cuda())
+    _check(logits, noise, temp, k, p, m, got, ambiguous=0.5)
+
+
 @pytest.mark.parametrize("top_k,top_p,min_p", [(0, 1.0, 0.0), (40, 1.0, 0.0), (0, 0.95, 0.0),
                                                (0, 1.0, 0.05), (50, 0.9, 0.02), (5000, 1.0, 0.0),
                                                (20000, 0.99, 0.0), (0, 0.0, 0.0), (1, 1.0, 0.0),

@@ -388,16 +388,27 @@ extern "C" int wkv7_adapter_plan(const int32_t* ids, int64_t m, int32_t count, i
   int32_t* end = plan + plan_part(all, 2);
   int32_t* tile = plan + plan_part(all, 3);
   int32_t* const last = tile + kTileInts * max_tiles(m, count);
-  // rows by adapter, in their own order within it, those without one last: sorted in the place
-  // of `id`, which is written behind them
-  int64_t n = 0;
-  for (int64_t i = 0; i < m; ++i)
-    if (ids[i] >= 0) id[n++] = int32_t(i);
-  std::sort(id, id + n, [ids](int32_t x, int32_t y) {
-    return ids[x] != ids[y] ? ids[x] < ids[y] : x < y;
-  });
-  for (int64_t i = 0, p = n; i < m; ++i)
-    if (ids[i] < 0) id[p++] = int32_t(i);
+  // Rows by adapter, in their own order within it, those without one last, in the place of `id`
+  // (which is written behind them): counted in the place of `end`, or sorted where there are more
+  // adapters than places.
+  if (count < all) {
+    std::fill(end, end + count + 1, 0);
+    auto slot = [&](int64_t i) { return ids[i] < 0 ? count : ids[i]; };
+    for (int64_t i = 0; i < m; ++i) ++end[slot(i)];
+    int32_t at = 0;
+    for (int32_t a = 0; a <= count; ++a) {
+      const int32_t n = end[a];
+      end[a] = at;
+      at += n;
+    }
+    for (int64_t i = 0; i < m; ++i) id[end[slot(i)]++] = int32_t(i);
+  } else {
+    for (int64_t i = 0; i < m; ++i) id[i] = int32_t(i);
+    std::sort(id, id + m, [ids](int32_t x, int32_t y) {
+      const uint32_t a = uint32_t(ids[x]), b = uint32_t(ids[y]);  // (-1 is the largest)
+      return a != b ? a < b : x < y;
+    });
+  }
   int64_t p = 0;
   for (int64_t i = 0; i < m;) {
     const int32_t a = ids[id[i]];

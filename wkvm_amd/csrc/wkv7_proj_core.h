@@ -170,9 +170,12 @@ struct Pairs {
 // run's own positions are taken (not the others times zero: an adapter with an inf or NaN in it
 // must not reach other requests). The operands come straight to registers, U (run, slab) pairs
 // in flight at once: a tile of a decode batch may meet an adapter per row, and each of them is
-// one pass from memory. The first U are under way from the constructor on, so they arrive while
-// the shared product is computed; add() multiplies them and fetches the others. kSwap: acc holds
-// the transposed tile. Pairs are dealt to `step` waves, or workgroups that share a tile.
+// one pass from memory. This comes after the shared product: with the first U fetched ahead of it
+// they would be held in registers all through the loop, and the compiler waits for them before the
+// first of the loop's own loads (three products of 256 rows of 2048, 32 adapters of 32 ranks: 34.6
+// us so, 34.1 now; one of 203 rows of 4096, 24 adapters of 64 ranks: 45 and 42).
+// kSwap: acc holds the transposed tile. Pairs are dealt to `step` waves, or workgroups that share
+// a tile.
 template <int TM, int TN, int U, bool kSwap>
 struct Expand {
   static_assert(TM <= 4, "a lane per position");
@@ -195,7 +198,6 @@ struct Expand {
     hp = ad.h[g] + (p0 * slabs) * 48 + 8 * lg;
     bp = ad.b[g] + 8 * (lg & 1);
     more = pairs.next(mine + 1);
-    fetch();
   }
 
   __device__ __forceinline__ void fetch() {
@@ -224,7 +226,8 @@ struct Expand {
 
   __device__ __forceinline__ void add(f32x4 (&acc)[TM][TN]) {
     const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
-    for (;;) {
+    while (more) {
+      fetch();
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -251,15 +254,8 @@ struct Expand {
             }
           }
         }
-      if (!more) return;
-      fetch();
     }
   }
-};
-
-struct NoExpand {
-  template <class... T>
-  __device__ __forceinline__ explicit NoExpand(T...) {}
 };
 
 template <int BM, int BN, int S, int GM, int GN, int BK, bool kSplit, class Extra>
@@ -351,11 +347,6 @@ __global__ __launch_bounds__(64 * GM * GN) void proj_kernel(const ProjArgs args,
 #pragma unroll
     for (int b = 0; b < TN; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // (16 waves have 128 registers each)
-  constexpr int kPairs = NW >= 16 ? 2 : TM > 1 ? 4 : 8;
-  std::conditional_t<Extra::kOn, Expand<TM, TN, kPairs, false>, NoExpand> extra(
-      ex, g, m0 + wm * WM, M, n0 + wn * WN, N, part, kSplit ? args.parts : 1);
-
   // A stage: all fragment reads first, then its MFMAs with the next stage's
   // loads (when kIssue) spread between them, so the matrix core works while
   // a load waits for the load pipe. Inline-assembly loads are scheduling
@@ -440,7 +431,13 @@ __global__ __launch_bounds__(64 * GM * GN) void proj_kernel(const ProjArgs args,
     }
   }
 
-  if constexpr (Extra::kOn) extra.add(acc);
+  if constexpr (Extra::kOn) {
+    // (16 waves have 128 registers each)
+    constexpr int kPairs = NW >= 16 ? 2 : TM > 1 ? 4 : 8;
+    Expand<TM, TN, kPairs, false>(ex, g, m0 + wm * WM, M, n0 + wn * WN, N, part,
+                                  kSplit ? args.parts : 1)
+        .add(acc);
+  }
 
   if constexpr (kSplit) {  // fp32 partial tile; proj_reduce_kernel finishes the sum
     float* wsp = args.ws + args.ws_off[g] + int64_t(part) * M * N;
@@ -525,9 +522,6 @@ __global__ __launch_bounds__(64 * NW) void proj_thin_kernel(const ProjArgs args,
   const uint16_t* wp = G.w + int64_t(min(n0 + li, N - 1)) * G.ldw + 8 * lg;
   const uint16_t* xp = G.x + ex.row(min(li, M - 1)) * G.ldx + 8 * lg;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  std::conditional_t<Extra::kOn, Expand<1, 1, 4, true>, NoExpand> extra(ex, g, int64_t(0),
-                                                                         int64_t(M), n0, N, wave,
-                                                                         NW);
   // U chunks of this wave from chunk c on. Only the last chunk of all can be
   // half a chunk wide: its second half re-reads the first and is left out.
   auto chunks = [&](int c, auto u_c) {
@@ -555,7 +549,7 @@ __global__ __launch_bounds__(64 * NW) void proj_thin_kernel(const ProjArgs args,
   else if (c < nc) chunks(c, std::integral_constant<int, 1>{});
   if constexpr (Extra::kOn) {
     f32x4 sum[1][1] = {{acc}};
-    extra.add(sum);
+    Expand<1, 1, 4, true>(ex, g, 0, M, n0, N, wave, NW).add(sum);
     acc = sum[0][0];
   }
   red[wave][lane] = acc;

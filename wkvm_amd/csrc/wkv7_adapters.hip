@@ -344,7 +344,7 @@ Work make_work(int64_t rows, int64_t m, const wkv7_proj_group* groups, const wkv
   w.plan = make_plan(m, groups, ng, cus);
   // 128 x 64 tiles for at most half of the units and k of 4096 or more: k split over two
   // workgroups per tile, which also share its adapters. 203 rows of a 4096 x 4096 product, 24
-  // adapters of 64 ranks: 45 us in place of 49. (At half that k the second launch takes what the
+  // adapters of 64 ranks: 42 us in place of 49. (At half that k the second launch takes what the
   // split gains, and without adapters the bits are wkv7_proj_grouped's.)
   const int64_t tiles = count_tiles(m, groups, ng, kShapes[2]);
   int kmin = groups[0].k;

@@ -270,6 +270,7 @@ struct Shared {
   };
   uint32_t n_list, n_subs;
   Found found;
+  u64 first;
   u64 red[kWaves];
   uint32_t wave_cnt[kWaves];
   u64 wave_wgt[kWaves];
@@ -588,6 +589,49 @@ __device__ __forceinline__ uint32_t race_row(const Row<T>& row, Kept kept, Weigh
   return race_group(row, group, kept, weight, noise, sm);
 }
 
+// The same where the scan has left the groups' whole weights: a group's first arrival is no earlier
+// than its whole weight says, so only groups that could still be first are looked at, in place of
+// the whole row: about as many as the row weighs more than what is kept. Every wave has its own
+// share of the groups; what one of them has found ends the others.
+template <typename T, typename Kept, typename Weight, typename Whole>
+__device__ __forceinline__ uint32_t race_bounded(const Row<T>& row, Kept kept, Weight weight,
+                                                 Whole whole, const float* noise, Shared& sm) {
+  const int groups = (row.n + kGroup - 1) / kGroup;
+  const int lane = threadIdx.x & (kWave - 1);
+  u64 best = ~0ull, seen = 0;
+  __syncthreads();
+  if (threadIdx.x == 0) sm.first = ~0ull;
+  __syncthreads();
+#pragma unroll 1
+  for (;;) {
+    u64 next = ~0ull;  // the earliest possible arrival that has not been looked at
+    for (int g = threadIdx.x; g < groups; g += kThreads) {
+      const float w = whole(g) * (1.f + 0x1p-12f);  // (more than the two sums' rounding)
+      if (!(w > 0.f)) continue;
+      const u64 a = arrival(noise[kGroup + g] / w, uint32_t(g)) + 1;
+      if (a > seen) next = min(next, a);
+    }
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) next = min(next, __shfl_xor(next, o));
+    if (next >= __hip_atomic_load(&sm.first, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)) break;
+    seen = next;
+    const uint32_t g = uint32_t(next - 1);
+    float w = 0.f;
+#pragma unroll
+    for (int e = 0; e < kGroup / kWave; ++e) {
+      const int i = int(g) * kGroup + e * kWave + lane;
+      const float x = i < row.n ? load_one(row.p + i) : -INFINITY;
+      w += kept(x, uint32_t(i)) ? weight(x) : 0.f;
+    }
+    w = lanes_sum<6>(w);
+    if (!(w > 0.f)) continue;
+    best = min(best, arrival(noise[kGroup + g] / w, g));
+    if (lane == 0) atomicMin(&sm.first, best);
+  }
+  const uint32_t group = uint32_t(block_all(best, MinU(), sm));
+  return race_group(row, group, kept, weight, noise, sm);
+}
+
 // Sorts one key per thread, ascending over the block; `n` of them matter, the others are ~0. Waves
 // past the power of two that holds n have nothing to do.
 __device__ __forceinline__ u64 block_sort(u64 v, uint32_t n, Shared& sm) {
@@ -804,7 +848,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_finish_kernel(const Sample
       row.padded([&](float x, uint32_t) {
         const float d = bin_of(x);
         // (32 fraction bits: what a row's tokens lose to them is 10^-6 of its weight)
-        if (d < float(kBins)) atomicAdd(&sm.wgt[int(d)], u64(uint32_t(weight(x) * 0x1p32f)));
+        if (d < float(kBins)) atomicAdd(&sm.wgt[int(d)], u64(uint32_t(fminf(weight(x) * 0x1p32f, 0x1.fffffep31f))));
       });
       const Found f = find_bin(sm, true, (share + 1023) >> 10);
       __syncthreads();
@@ -838,8 +882,10 @@ __global__ __launch_bounds__(kThreads, 4) void sample_finish_kernel(const Sample
           cut = descend(ListRow{sm, n}, [](float, uint32_t) { return true; }, weight, true, true,
                         rest, static_cast<u64*>(nullptr), sm);
         }
-        token = race_row(row, [=](float x, uint32_t i) {
-          return cut.keeps(x, i) && over_floor(x); }, weight, noise, sm);
+        auto kept = [=](float x, uint32_t i) { return cut.keeps(x, i) && over_floor(x); };
+        token = set.floor_z > -INFINITY  // (which may leave little of what the groups weigh)
+                    ? race_row(row, kept, weight, noise, sm)
+                    : race_bounded(row, kept, weight, group_weight, noise, sm);
         done = true;
       }
     }

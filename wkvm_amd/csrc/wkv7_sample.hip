@@ -38,6 +38,7 @@ constexpr int kWaves = kThreads / kWave;
 constexpr int kBins = 2048;
 constexpr int kList = 4096;               // candidates held in LDS
 constexpr int kSubs = 4096;               // runs of kSub tokens that may hold candidates
+constexpr int kFarBins = 8192;            // of a whole row's weights
 // The candidate list's group weights take the place of the histogram.
 constexpr int kListGroups = kBins + kBins / 2;
 
@@ -141,15 +142,17 @@ template <> struct Vec<float> {
   static constexpr int N = 4;
   typedef float Raw __attribute__((ext_vector_type(4), aligned(4)));
   Raw x;
-  __device__ __forceinline__ float get(int e) const { return clean(x[e]); }
+  __device__ __forceinline__ float raw(int e) const { return x[e]; }
+  __device__ __forceinline__ float get(int e) const { return clean(raw(e)); }
 };
 template <> struct Vec<uint16_t> {
   static constexpr int N = 8;
   typedef uint32_t Raw __attribute__((ext_vector_type(4), aligned(2)));
   Raw x;
-  __device__ __forceinline__ float get(int e) const {
-    return clean((e & 1) ? bf16_hi(x[e / 2]) : bf16_lo(x[e / 2]));
+  __device__ __forceinline__ float raw(int e) const {
+    return (e & 1) ? bf16_hi(x[e / 2]) : bf16_lo(x[e / 2]);
   }
+  __device__ __forceinline__ float get(int e) const { return clean(raw(e)); }
 };
 
 template <typename T>
@@ -266,6 +269,7 @@ struct Shared {
       uint16_t subs[kSubs];
     };
     u64 mass[kListGroups];           // takes the place of the histogram
+    u64 far[kFarBins];
     float row_mass[WKV7_SAMPLE_MAX_VOCAB / kGroup];
   };
   uint32_t n_list, n_subs;
@@ -341,14 +345,6 @@ struct Row {
 #pragma unroll
       for (int e = 0; e < N; ++e)
         if (i + e < n) f(x.get(e), uint32_t(i + e));
-    });
-  }
-  // the same with -inf for the tokens past the end
-  template <typename F>
-  __device__ __forceinline__ void padded(F f) const {
-    vectors([&](const Vec<T>& x, int i) {
-#pragma unroll
-      for (int e = 0; e < N; ++e) f(x.get(e), uint32_t(i + e));
     });
   }
 };
@@ -434,6 +430,30 @@ __device__ __forceinline__ Found find_bin(Shared& sm, bool by_weight, u64 target
       sm.found = {uint32_t(kEach * t + i), cb, c[i], wb, w[i]};
     cb += c[i];
     wb += w[i];
+  }
+  __syncthreads();
+  return sm.found;
+}
+
+// The same over the far bins, which hold weights alone.
+__device__ __forceinline__ Found find_far(Shared& sm, u64 target) {
+  constexpr int kEach = kFarBins / kThreads;
+  const int t = threadIdx.x;
+  __syncthreads();
+  uint32_t none = 0, all_c;
+  u64 before = 0, all_w;
+  // (each lane starts at another bin of its own, lest they all read the same banks)
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) before += sm.far[kEach * t + (i + t) % kEach];
+  const u64 mine = before;
+  block_scan(none, before, all_c, all_w, sm);
+  before -= mine;
+  const u64 goal = min(target, all_w);
+  if (before < goal && before + mine >= goal) {
+    uint32_t bin = kEach * t;
+    u64 here = sm.far[bin];
+    for (; before + here < goal; here = sm.far[++bin]) before += here;
+    sm.found = {bin, 0, 0, before, here};
   }
   __syncthreads();
   return sm.found;
@@ -840,30 +860,56 @@ __global__ __launch_bounds__(kThreads, 4) void sample_finish_kernel(const Sample
       }
     }
     if (!done && set.by_p && !set.by_k) {
-      // Top-p's share reaches far down: a pass over 2,048 bins of its tokens' range in log weight
-      // leaves one short run of the order to look at closely.
-      const float steps = float(kBins) / fmaxf(-low, 1.f);
-      auto bin_of = [top, c = set.c, steps](float x) { return (top - x) * c * steps; };
-      clear_bins(sm);
-      row.padded([&](float x, uint32_t) {
-        const float d = bin_of(x);
-        // (32 fraction bits: what a row's tokens lose to them is 10^-6 of its weight)
-        if (d < float(kBins)) atomicAdd(&sm.wgt[int(d)], u64(uint32_t(fminf(weight(x) * 0x1p32f, 0x1.fffffep31f))));
-      });
-      const Found f = find_bin(sm, true, (share + 1023) >> 10);
+      // Top-p's share reaches far down: a pass over 8,192 bins of its tokens' range in log weight
+      // leaves one short run of the order to look at closely. What bounds the pass is the work per
+      // token, half instructions and half LDS atomics; the bins are many lest the run be long.
+      const float steps = float(kFarBins) / fmaxf(-low, 1.f);
       __syncthreads();
+      for (int i = t; i < kFarBins; i += kThreads) sm.far[i] = 0;
+      __syncthreads();
+      row.vectors([&](const Vec<T>& v, int) {
+#pragma unroll
+        for (int e = 0; e < Vec<T>::N; ++e) {
+          const float z = (top - v.raw(e)) * set.c, d = z * steps;
+          if (!(d < float(kFarBins))) continue;  // (and NaN, and -inf past the row's end)
+          // 31 fraction bits, rounded: over a row their errors cancel to 10^-7 of its weight
+          const uint32_t w = uint32_t(fmaf(exp2_hw(-fmaxf(z, 0.f)), 0x1p31f, 0.5f));
+          atomicAdd(&sm.far[uint32_t(fmaxf(d, 0.f))], u64(w));
+        }
+      });
+      const Found f = find_far(sm, (share + 2047) >> 11);
       if (t == 0) sm.n_list = 0;
       __syncthreads();
-      row.padded([&](float x, uint32_t i) {
-        const float d = bin_of(x);
-        if (d >= float(kBins) || uint32_t(d) != f.bin) return;
-        const uint32_t to = atomicAdd(&sm.n_list, 1u);
-        if (to < kList) sm.list[to] = make_uint2(__float_as_uint(x), i);
+      // The bin's tokens: first those in a range of logits that surely holds the bin (d is within
+      // 0.01 of the exact quotient, the range's ends within 2^-21 of top's and their own size); of
+      // them the others become -inf.
+      const float width = 1.f / (set.c * steps);
+      const float down = top - (float(f.bin) + 1.02f) * width;
+      const float up = top - (float(f.bin) - 0.02f) * width;
+      const float slack = (fabsf(top) + fabsf(down)) * 0x1p-21f;
+      const float least = down - slack, most = up + slack;
+      row.vectors([&](const Vec<T>& v, int i) {
+        uint32_t in = 0;
+#pragma unroll
+        for (int e = 0; e < Vec<T>::N; ++e)
+          in |= (v.raw(e) >= least) & (v.raw(e) <= most) ? 1u << e : 0u;
+        for (; in; in &= in - 1) {
+          const uint32_t to = atomicAdd(&sm.n_list, 1u);
+          if (to < kList) sm.list[to].y = uint32_t(i + __builtin_ctz(in));
+        }
       });
+      __syncthreads();
+      for (uint32_t i = t; i < min(sm.n_list, uint32_t(kList)); i += kThreads) {
+        const uint32_t token = sm.list[i].y;
+        const float x = token < uint32_t(V) ? load_one(row.p + token) : -INFINITY;
+        const float d = (top - x) * set.c * steps;
+        const bool in = d < float(kFarBins) && uint32_t(d) == f.bin;
+        sm.list[i].x = __float_as_uint(in ? x : -INFINITY);
+      }
       __syncthreads();
       const uint32_t n = sm.n_list;
       if (n > 0 && n <= kList) {
-        const u64 before = f.before_wgt << 10, rest = share > before ? share - before : 1;
+        const u64 before = f.before_wgt << 11, rest = share > before ? share - before : 1;
         Cut cut(0u, 0u);
         if (n <= kThreads) {
           const u64 v = sorted_candidate(n, sm);
@@ -872,15 +918,16 @@ __global__ __launch_bounds__(kThreads, 4) void sample_finish_kernel(const Sample
           uint32_t one = 0, none;
           block_scan(one, upto, none, all, sm);
           // the last token that still begins before the share is reached
-          const bool kept = uint32_t(t) < n && (t == 0 || upto - w < rest);
+          const bool kept = uint32_t(t) < n && v >> 32 != order_key(-INFINITY) &&
+                            (t == 0 || upto - w < rest);
           const int last = __syncthreads_count(kept) - 1;
-          if (t == last) sm.red[0] = v;
+          if (t == max(last, 0)) sm.red[0] = v;
           __syncthreads();
           cut = Cut(uint32_t(sm.red[0] >> 32), uint32_t(sm.red[0]));
           __syncthreads();
         } else {
-          cut = descend(ListRow{sm, n}, [](float, uint32_t) { return true; }, weight, true, true,
-                        rest, static_cast<u64*>(nullptr), sm);
+          cut = descend(ListRow{sm, n}, [](float x, uint32_t) { return x > -INFINITY; }, weight,
+                        true, true, rest, static_cast<u64*>(nullptr), sm);
         }
         auto kept = [=](float x, uint32_t i) { return cut.keeps(x, i) && over_floor(x); };
         token = set.floor_z > -INFINITY  // (which may leave little of what the groups weigh)

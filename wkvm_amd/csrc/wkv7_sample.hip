@@ -269,7 +269,7 @@ struct Shared {
       uint16_t subs[kSubs];
     };
     u64 mass[kListGroups];           // takes the place of the histogram
-    u64 far[kFarBins];
+    u64 far[kFarBins + kWave];       // the last 64 take what is in no bin, each from one lane
     float row_mass[WKV7_SAMPLE_MAX_VOCAB / kGroup];
   };
   uint32_t n_list, n_subs;
@@ -315,29 +315,29 @@ struct Row {
   int n;
 
   // f(vector, index of its first element); every thread makes the same calls. The next U vectors
-  // are under way while f works on U.
+  // are under way while f works on U. The one that the row may end in is read apart: the code of
+  // its guarded loads is long, and a workgroup runs through most of the kernel's code once.
   template <typename F>
   __device__ __forceinline__ void vectors(F f) const {
     constexpr int U = 4;
-    const int i = int(threadIdx.x) * N;
-    Vec<T> v[U], w[U];
+    const int i = int(threadIdx.x) * N, whole = n / kStep * kStep;
+    Vec<T> v[U], w[U], last;
     auto fetch = [&](Vec<T>(&to)[U], int at) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int first = at + u * kStep;
-        if (first + kStep <= n) to[u] = load_full(p + first + i);
-        else if (first < n) to[u] = load_part(p, first + i, n);
-      }
+      for (int u = 0; u < U; ++u)
+        if (at + u * kStep < whole) to[u] = load_full(p + at + u * kStep + i);
     };
+    if (whole < n) last = load_part(p, whole + i, n);
     fetch(v, 0);
-    for (int at = 0; at < n; at += U * kStep) {
+    for (int at = 0; at < whole; at += U * kStep) {
       fetch(w, at + U * kStep);
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (at + u * kStep < n) f(v[u], at + u * kStep + i);
+        if (at + u * kStep < whole) f(v[u], at + u * kStep + i);
 #pragma unroll
       for (int u = 0; u < U; ++u) v[u] = w[u];
     }
+    if (whole < n) f(last, whole + i);
   }
   template <typename F>
   __device__ __forceinline__ void operator()(F f) const {
@@ -868,14 +868,22 @@ __global__ __launch_bounds__(kThreads, 4) void sample_finish_kernel(const Sample
       for (int i = t; i < kFarBins; i += kThreads) sm.far[i] = 0;
       __syncthreads();
       row.vectors([&](const Vec<T>& v, int) {
+        constexpr int N = Vec<T>::N;
+        uint32_t bin[N], w[N];
 #pragma unroll
-        for (int e = 0; e < Vec<T>::N; ++e) {
-          const float z = (top - v.raw(e)) * set.c, d = z * steps;
-          if (!(d < float(kFarBins))) continue;  // (and NaN, and -inf past the row's end)
+        for (int e = 0; e < N; ++e) {
+          // (+inf, where top is the largest finite number, is no distance away)
+          const float far = (top - v.raw(e)) * set.c;
+          const float z = __int_as_float(max(__float_as_int(far), 0)), d = z * steps;
+          const bool in = d < float(kFarBins);  // (not NaN, nor -inf past the row's end)
           // 31 fraction bits, rounded: over a row their errors cancel to 10^-7 of its weight
-          const uint32_t w = uint32_t(fmaf(exp2_hw(-fmaxf(z, 0.f)), 0x1p31f, 0.5f));
-          atomicAdd(&sm.far[uint32_t(fmaxf(d, 0.f))], u64(w));
+          w[e] = in ? uint32_t(fmaf(exp2_hw(-z), 0x1p31f, 0.5f)) : 0u;
+          bin[e] = in ? uint32_t(d) : kFarBins + (threadIdx.x & (kWave - 1));
+          // (in straight lines: a branch per token leaves nothing to do while one waits)
+          asm volatile("" : "+v"(w[e]), "+v"(bin[e]));
         }
+#pragma unroll
+        for (int e = 0; e < N; ++e) atomicAdd(&sm.far[bin[e]], u64(w[e]));
       });
       const Found f = find_far(sm, (share + 2047) >> 11);
       if (t == 0) sm.n_list = 0;
@@ -892,7 +900,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_finish_kernel(const Sample
         uint32_t in = 0;
 #pragma unroll
         for (int e = 0; e < Vec<T>::N; ++e)
-          in |= (v.raw(e) >= least) & (v.raw(e) <= most) ? 1u << e : 0u;
+          in |= ((v.raw(e) >= least) & (v.raw(e) <= most)) ? 1u << e : 0u;
         for (; in; in &= in - 1) {
           const uint32_t to = atomicAdd(&sm.n_list, 1u);
           if (to < kList) sm.list[to].y = uint32_t(i + __builtin_ctz(in));

@@ -6,7 +6,12 @@
 // A is read about once. The second is the shared product itself (wkv7_proj_core.h) over the rows
 // in that order, which adds h B_a^T to its accumulators before bias, activation and the one
 // rounding. h is summed in fp32 and kept whole as three bf16 parts, which the matrix cores
-// multiply with B in two instructions per slab of 16 ranks.
+// multiply with B in two instructions per slab of 16 ranks. Two launches because every output
+// column needs all of h, and a workgroup per tile of y would compute it once per column tile.
+//
+// Three products in a HIP graph (the shared products alone in brackets): 8 rows of 2048 x 2048 with
+// two adapters of 16 ranks 15.6 us (8.5), 64 rows with one of their own each 25 (9.9), 256 rows over
+// 32 of 32 ranks 34.5 (16.9), 3,001 rows of prompts 130, 32,768 rows 1,085 to 1,108.
 #include <algorithm>
 
 #include "wkv7_proj_plan.h"
@@ -76,7 +81,9 @@ __device__ __forceinline__ void store_h(uint16_t* h, const f32x4& v, float s, in
 }
 
 // Few tiles: a workgroup per tile and slab, k dealt to NW waves in 64-wide chunks whose sums
-// are joined through LDS in wave order.
+// are joined through LDS in wave order. Bound by latency (a launch, the tile, the operands of four
+// chunks in flight, the join: 6 us for 8 rows of 2048 and 64 rows alike); 256 rows over 32 adapters of
+// 32 ranks 9.9 us.
 template <int NW>
 __global__ __launch_bounds__(64 * NW) void shrink_thin_kernel(const ShrinkArgs args) {
   __shared__ f32x4 red[NW][64];
@@ -133,7 +140,8 @@ __global__ __launch_bounds__(64 * NW) void shrink_thin_kernel(const ShrinkArgs a
 // once. Two tiles of one adapter, as nearly all of a prompt's are, share the reads of A, which
 // are otherwise twice x's. (32,768 rows of 2048 in three products of rank 32, x alone 400 MB: with
 // a wave per tile, which walks 16 rows in steps of 64 bytes, 165 us; a workgroup per tile 148;
-// two tiles 109, and 116 with four chunks of k in flight in place of two.)
+// two tiles 109 or 3.7 TB/s of x, which is what bounds it, and 116 with four chunks of k in flight in
+// place of two.)
 constexpr int kWideShrink = 4;
 
 __global__ __launch_bounds__(64 * kWideShrink) void shrink_wide_kernel(const ShrinkArgs args) {
@@ -308,8 +316,8 @@ bool wide_fits(int64_t m, const wkv7_proj_group* groups, int ng) {
 // The row tile of the wide kernel (in units of 64 rows), 0 for the others: whichever takes the
 // least time by its rounds over the units. Microseconds per round of one tile per unit, measured
 // at k = 2048 (they scale together with k): 256 x 256 tiles 79, 128 x 256 47, the other kernel's
-// 128 x 64 tiles 16.5. Three products of 2048 columns and 2048 k: 3001 rows 118 in 128 x 256 (127
-// in 256 x 256, 165 in 128 x 64), 32,768 rows 973 in 256 x 256 (1187, about 2200). A plan of few
+// 128 x 64 tiles 16.5. Three products of 2048 columns and 2048 k: 3001 rows 114 in 128 x 256 (127
+// in 256 x 256, 165 in 128 x 64), 32,768 rows 916 in 256 x 256 (1187, about 2200). A plan of few
 // rows does not align its runs as the wide kernel needs.
 int wide_tile(int64_t m, int64_t positions, const wkv7_proj_group* groups, int ng, int cus) {
   if (m <= WKV7_ADAPTER_PACKED_ROWS || !wide_fits(m, groups, ng)) return 0;

@@ -5,8 +5,17 @@
 // by lower index", every filter keeps a prefix of that order: top-k its first k
 // tokens, top-p the shortest prefix whose weight reaches p of what top-k left,
 // min-p the tokens with w_i >= min_p. So the kept set is one cut in the order,
-// a pair (key, index), found by a radix descent over histograms of counts and
-// weights; nothing is sorted.
+// a pair (key, index), and rarely more than a few hundred tokens are near it.
+//
+// Two launches. The scan, a wave per 2,048 tokens, reads the logits once and leaves
+// sums, group weights and the maxima of runs of 32 tokens; the finish, a workgroup
+// per row, reads again only the runs that can hold kept tokens, sorts those, and
+// draws. Where top-p's share reaches far down it goes over the row twice more: once
+// for a histogram of the weights, once for the tokens of the bin that the cut is in.
+// One workgroup per row for all of it would leave a lone row on one unit (161 us for
+// 65,536 logits with every filter, 25 now). 256 rows of 65,536 fp32 logits in a HIP
+// graph: temperature alone 22.5 us (3.0 TB/s; the scan by itself 4.3), top-k 50 and
+// top-p 0.95 31, top-p 0.95 alone 58, rows of mixed settings 53.
 //
 // The draw is an exponential race in two levels: with positive exponential variates
 // e, group j of 256 consecutive tokens arrives at e / W_j (W_j the kept weight in it)
@@ -179,6 +188,10 @@ __device__ __forceinline__ Vec<T> load_part(const T* row, int i, int n) {
 
 // -- the scan: one wave per chunk of 2,048 tokens, one pass over the logits -----------------------
 
+// Bound by the one pass over the logits: 256 rows of 65,536 fp32 logits 15.6 us (4.3 TB/s, where a
+// large copy reaches 4.8), 512 rows of 131,077 in bf16 34 us (4.0 TB/s, with half of that time's
+// instructions in the two exponentials per logit).
+//
 // Of every chunk: its maximum and sum of exponentials; of every 32 tokens the maximum, for the
 // finish to know where the largest logits are; and, where nothing but min-p is asked for or top-p
 // needs the row's weight, the weight of every group. Everything is relative to the chunk's own
@@ -254,6 +267,13 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(const SampleA
 }
 
 // -- the finish: one workgroup per row ----------------------------------------------------------------
+//
+// A chain of short steps with a barrier after each, so latency bounds it: about 5 us where nothing is
+// cut off, 10 to 15 for top-k (histogram of run maxima, gathering, sort, race), 20 where the sort has
+// 512 candidates. A top-p that reaches far down (65,536 fp32 logits: 35 us for a row) is bound by the
+// work per token of its two passes: 11 us for the histogram, 7 for the bin's tokens. Workgroups of
+// 512 threads, two of which share a unit, so that one works while the other waits. Tried and slower:
+// fp32 LDS atomics, and bins of each thread's own, for the histograms.
 
 struct Found {
   uint32_t bin, before_cnt, cnt;
@@ -862,7 +882,8 @@ __global__ __launch_bounds__(kThreads, 4) void sample_finish_kernel(const Sample
     if (!done && set.by_p && !set.by_k) {
       // Top-p's share reaches far down: a pass over 8,192 bins of its tokens' range in log weight
       // leaves one short run of the order to look at closely. What bounds the pass is the work per
-      // token, half instructions and half LDS atomics; the bins are many lest the run be long.
+      // token, half instructions and half LDS atomics; the bins are many lest the run be long (2,048
+      // of them: 256 rows of mixed settings 63 us in place of 53, with a branch per token).
       const float steps = float(kFarBins) / fmaxf(-low, 1.f);
       __syncthreads();
       for (int i = t; i < kFarBins; i += kThreads) sm.far[i] = 0;

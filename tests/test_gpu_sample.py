@@ -191,6 +191,28 @@ def test_masked_rows_and_special_values(settings, dtype):
     assert 100 <= got[0][6].item() < 130 and 0 <= got[0][7].item() < 3
 
 
+@pytest.mark.parametrize("shift", [0.0, -3e4, 1e6])
+@pytest.mark.parametrize("top_p,min_p", [(0.6, 0.0), (0.9, 0.0), (0.98, 0.0), (0.999, 0.0),
+                                         (0.98, 0.3)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_top_p_far_down_flat_rows(dtype, top_p, min_p, shift):
+    """Tens of thousands of tokens kept, many of them equal (in bf16, and far from zero), with
+    NaN and -inf among them; one row's mass lies in a few groups, one row is all equal but -inf."""
+    vocab = 50021
+    logits, noise = _inputs(8, vocab, torch.float32, 23, 0.7)
+    logits[1] *= 3.0
+    logits[2] *= 0.01
+    logits[3, ::2] = math.nan
+    logits[4, 5::7] = -math.inf
+    logits[5, 2000:] -= 9.0
+    logits[6] = 0.0
+    logits[6, ::5] = -math.inf
+    logits = (logits + shift).to(dtype)
+    for temp in (0.7, 1.3):
+        got = sample_tokens(logits, noise, temperature=temp, top_p=top_p, min_p=min_p)
+        _check(logits, noise, temp, 0, top_p, min_p, got, ambiguous=0.25)
+
+
 @pytest.mark.parametrize("temperature", [1e-30, 1e-6, 1e6, 1e30, math.inf])
 def test_extreme_temperatures(temperature):
     logits, noise = _inputs(4, 3000, torch.float32, 9)

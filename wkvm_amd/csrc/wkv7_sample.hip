@@ -593,7 +593,7 @@ template <typename T, typename Kept, typename Weight>
 __device__ __forceinline__ uint32_t race_group(const Row<T>& row, uint32_t group, Kept kept,
                                                Weight weight, const float* noise, Shared& sm) {
   u64 best = ~0ull;
-  const int i = int(group) * kGroup + int(threadIdx.x);
+  const int i = int(min(group, uint32_t(row.n - 1) / kGroup)) * kGroup + int(threadIdx.x);
   if (threadIdx.x < kGroup && i < row.n) {
     const float x = load_one(row.p + i);
     if (kept(x, uint32_t(i))) best = arrival(noise[threadIdx.x] / weight(x), uint32_t(i));
@@ -895,7 +895,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_finish_kernel(const Sample
         for (int e = 0; e < N; ++e) {
           // (+inf, where top is the largest finite number, is no distance away)
           const float far = (top - v.raw(e)) * set.c;
-          const float z = __int_as_float(max(__float_as_int(far), 0)), d = z * steps;
+          const float z = far < 0.f ? 0.f : far, d = z * steps;  // (NaN stays NaN)
           const bool in = d < float(kFarBins);  // (not NaN, nor -inf past the row's end)
           // 31 fraction bits, rounded: over a row their errors cancel to 10^-7 of its weight
           w[e] = in ? uint32_t(fmaf(exp2_hw(-z), 0x1p31f, 0.5f)) : 0u;
@@ -972,6 +972,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_finish_kernel(const Sample
     }
   }
   if (t == 0) {
+    token = min(token, uint32_t(V - 1));  // (whatever the variates are)
     args.tokens[b] = int32_t(token);
     if (args.logprobs)
       args.logprobs[b] = float(double(load_one(row.p + token) - top) - log(raw));

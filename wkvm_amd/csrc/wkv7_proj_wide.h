@@ -11,7 +11,7 @@
 // time to arrive, and each operand byte is read from LDS twice per tile.
 //
 // 32,768 rows of a 2048 x 2048 product 0.85 PFLOP/s (three with adapters of 32 ranks 0.90), k of 4096
-// 0.97, 8192^3 1.14: 0.66 to 0.78 of what the vendor's library reaches at these sizes. The loop alone is at 1.69 PFLOP/s where nothing is loaded, 1.62 with every
+// 0.99, 8192^3 1.17: 0.66 to 0.79 of what the vendor's library reaches at these sizes. The loop alone is at 1.69 PFLOP/s where nothing is loaded, 1.62 with every
 // load a hit in the unit's cache, 1.35 in the XCD's; with the real rows about 1.10, so what bounds
 // it is x's lines on their way to the unit, and about 15 us per round of tiles for first loads and
 // results. No gain: prefetches into the XCD's cache, k started at another stage in every tile, waves
@@ -141,11 +141,11 @@ __global__ __launch_bounds__(64 * kWideWaves) void proj_wide_kernel(const ProjAr
   const int wm = wave & 1, wn = wave >> 1;
   const int li = lane & 31, lh = lane >> 5;
 
-  // A stage's rows are 128 bytes (whole cache lines of x and w), chunk c of row r at c ^ (r % 8): 8
-  // neighbouring rows of an operand read touch all 32 banks once. Load i of a wave fills rows
+  // A stage's rows are 128 bytes (whole cache lines of x and w), chunk c of row r at
+  // c ^ (r / 2 % 8): 16 neighbouring rows of an operand read touch all 64 banks once. Load i of a wave fills rows
   // 8 (4 i + wave) .. + 7. Row addresses are 32-bit byte offsets from x and w (the launch sees to
   // it that they fit).
-  const int chunk = (lane & 7) ^ (lane >> 3);
+  const int chunk = (lane & 7) ^ ((4 * wave + (lane >> 4)) & 7);
   uint32_t off[LR];
 #pragma unroll
   for (int i = 0; i < LR; ++i) {
@@ -173,7 +173,7 @@ __global__ __launch_bounds__(64 * kWideWaves) void proj_wide_kernel(const ProjAr
   uint32_t x_at[4], w_at[4];  // of the four steps, in the slot that is read
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
-    const uint32_t in_tile = 128 * li + 16 * ((2 * s + lh) ^ (li & 7));
+    const uint32_t in_tile = 128 * li + 16 * ((2 * s + lh) ^ ((li >> 1) & 7));
     x_at[s] = ring_base + 128 * (wm * WM) + in_tile;
     w_at[s] = ring_base + 128 * (BM + wn * WN) + in_tile;
   }
@@ -250,7 +250,7 @@ __global__ __launch_bounds__(64 * kWideWaves) void proj_wide_kernel(const ProjAr
 
   // The results go through LDS, two row tiles at a time, so that bias, activation and the stores
   // are a short loop over whole rows: a lane has 8 neighbouring columns of every fourth row. A
-  // wave has its own 32 KiB there; unit u of 16 bytes of row r is at u ^ (r % 8).
+  // wave has its own 32 KiB there; unit u of 16 bytes of row r is at u ^ (r % 16).
   __syncthreads();  // (no wave reads operands any more)
   const uint32_t out_at = ring_base + kOut * wave;
   const int col = n0 + wn * WN + 8 * (lane & 15);
@@ -268,7 +268,7 @@ __global__ __launch_bounds__(64 * kWideWaves) void proj_wide_kernel(const ProjAr
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const f32x16& c = acc[a + i][j];
-          const uint32_t unit = uint32_t(8 * j + 2 * q + lh) ^ (li & 7);
+          const uint32_t unit = uint32_t(8 * j + 2 * q + lh) ^ (li & 15);
           lds_write(out_at + 512 * li + 16 * unit, 16384 * i,
                     f32x4{c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]});
         }
@@ -276,8 +276,8 @@ __global__ __launch_bounds__(64 * kWideWaves) void proj_wide_kernel(const ProjAr
     for (int r = lane >> 4; r < 64; r += 4) {
       const uint32_t at = out_at + 512 * r;
       const uint32_t u = 2 * (lane & 15);
-      const uint4 lo = lds_read(at + 16 * (u ^ (r & 7)), 0);
-      const uint4 hi = lds_read(at + 16 * ((u + 1) ^ (r & 7)), 0);
+      const uint4 lo = lds_read(at + 16 * (u ^ (r & 15)), 0);
+      const uint4 hi = lds_read(at + 16 * ((u + 1) ^ (r & 15)), 0);
       const uint32_t bits[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
       float v[8];
 #pragma unroll

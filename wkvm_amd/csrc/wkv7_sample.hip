@@ -824,17 +824,15 @@ __global__ __launch_bounds__(kThreads, 4) void sample_finish_kernel(const Sample
         for (int s = t; s < n_sub; s += kThreads) {
           const float x = sub_max[s];
           const int bin = int(fminf((top - x) * scale, float(kBins - 1)));
+          if (bin == kBins - 1) continue;  // (too far, and most of the runs of a steep row)
           atomicAdd(&sm.cnt[bin], 1u);
           if (!set.by_k) atomicAdd(&sm.wgt[bin], fixed(weight(x)));
         }
         const Found f = find_bin(sm, !set.by_k, set.by_k ? u64(set.top_k) : share);
-        last = f.bin;
-        if (!set.by_k) {
-          enough = f.before_wgt + f.wgt >= share && last < kBins - 1;
-          break;
-        }
-        enough = last < kBins - 1;
-        if (enough) break;
+        enough = set.by_k ? f.before_cnt + f.cnt >= uint32_t(set.top_k)
+                          : f.before_wgt + f.wgt >= share;
+        last = enough ? f.bin : kBins - 1;
+        if (enough || !set.by_k) break;
       }
       // (top-k among tokens of the last step of the coarsest scale: every token is a candidate)
       if (set.by_k) enough = true;

@@ -870,7 +870,9 @@ __global__ __launch_bounds__(kThreads, 4) void sample_finish_kernel(const Sample
         }
       }
     }
-    if (!done && set.by_p && !set.by_k) {
+    // (a row with +inf in it, whose distance to the largest finite number is negative, is left to
+    // the last resort)
+    if (!done && set.by_p && !set.by_k && top < 3.402823466e38f) {
       // Top-p's share reaches far down: a pass over 8,192 bins of its tokens' range in log weight
       // leaves one short run of the order to look at closely. What bounds the pass is the work per
       // token, half instructions and half LDS atomics; the bins are many lest the run be long (2,048
@@ -884,9 +886,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_finish_kernel(const Sample
         uint32_t bin[N], w[N];
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-          // (+inf, where top is the largest finite number, is no distance away)
-          const float far = (top - v.raw(e)) * set.c;
-          const float z = far < 0.f ? 0.f : far, d = z * steps;  // (NaN stays NaN)
+          const float z = (top - v.raw(e)) * set.c, d = z * steps;
           const bool in = d < float(kFarBins);  // (not NaN, nor -inf past the row's end)
           // 31 fraction bits, rounded: over a row their errors cancel to 10^-7 of its weight
           w[e] = in ? uint32_t(fmaf(exp2_hw(-z), 0x1p31f, 0.5f)) : 0u;

@@ -11,7 +11,7 @@
 //
 // Three products in a HIP graph (the shared products alone in brackets): 8 rows of 2048 x 2048 with
 // two adapters of 16 ranks 15.6 us (8.5), 64 rows with one of their own each 25 (9.9), 256 rows over
-// 32 of 32 ranks 34.5 (16.9), 3,001 rows of prompts 130, 32,768 rows 1,085 to 1,108.
+// 32 of 32 ranks 34.5 (16.9), 3,001 rows of prompts 130, 32,768 rows 1,085 to 1,130.
 #include <algorithm>
 
 #include "wkv7_proj_plan.h"
@@ -317,7 +317,7 @@ bool wide_fits(int64_t m, const wkv7_proj_group* groups, int ng) {
 // least time by its rounds over the units. Microseconds per round of one tile per unit, measured
 // at k = 2048 (they scale together with k): 256 x 256 tiles 79, 128 x 256 47, the other kernel's
 // 128 x 64 tiles 16.5. Three products of 2048 columns and 2048 k: 3001 rows 114 in 128 x 256 (127
-// in 256 x 256, 165 in 128 x 64), 32,768 rows 916 in 256 x 256 (1187, about 2200). A plan of few
+// in 256 x 256, 165 in 128 x 64), 32,768 rows 910 in 256 x 256 (1187, about 2200). A plan of few
 // rows does not align its runs as the wide kernel needs.
 int wide_tile(int64_t m, int64_t positions, const wkv7_proj_group* groups, int ng, int cus) {
   if (m <= WKV7_ADAPTER_PACKED_ROWS || !wide_fits(m, groups, ng)) return 0;

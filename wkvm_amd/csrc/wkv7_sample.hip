@@ -13,9 +13,9 @@
 // draws. Where top-p's share reaches far down it goes over the row twice more: once
 // for a histogram of the weights, once for the tokens of the bin that the cut is in.
 // One workgroup per row for all of it would leave a lone row on one unit (161 us for
-// 65,536 logits with every filter, 25 now). 256 rows of 65,536 fp32 logits in a HIP
+// 65,536 logits with every filter, 20 now). 256 rows of 65,536 fp32 logits in a HIP
 // graph: temperature alone 22.5 us (3.0 TB/s; the scan by itself 4.3), top-k 50 and
-// top-p 0.95 31, top-p 0.95 alone 58, rows of mixed settings 53.
+// top-p 0.95 27.5, top-p 0.95 alone 58, rows of mixed settings 49.
 //
 // The draw is an exponential race in two levels: with positive exponential variates
 // e, group j of 256 consecutive tokens arrives at e / W_j (W_j the kept weight in it)
@@ -269,8 +269,8 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(const SampleA
 // -- the finish: one workgroup per row ----------------------------------------------------------------
 //
 // A chain of short steps with a barrier after each, so latency bounds it: about 5 us where nothing is
-// cut off, 10 to 15 for top-k (histogram of run maxima, gathering, sort, race), 20 where the sort has
-// 512 candidates. A top-p that reaches far down (65,536 fp32 logits: 35 us for a row) is bound by the
+// cut off, 12 for top-k 40 (sums 2, histogram of run maxima 4, gathering 2, order 2, race 2) and 16
+// for top-k 200. A top-p that reaches far down (65,536 fp32 logits: 31 us for a row) is bound by the
 // work per token of its two passes: 11 us for the histogram, 7 for the bin's tokens. Workgroups of
 // 512 threads, two of which share a unit, so that one works while the other waits. Tried and slower:
 // fp32 LDS atomics, and bins of each thread's own, for the histograms.
@@ -876,7 +876,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_finish_kernel(const Sample
       // Top-p's share reaches far down: a pass over 8,192 bins of its tokens' range in log weight
       // leaves one short run of the order to look at closely. What bounds the pass is the work per
       // token, half instructions and half LDS atomics; the bins are many lest the run be long (2,048
-      // of them: 256 rows of mixed settings 63 us in place of 53, with a branch per token).
+      // of them, and a branch per token: 256 rows of mixed settings 63 us where this took 53).
       const float steps = float(kFarBins) / fmaxf(-low, 1.f);
       __syncthreads();
       for (int i = t; i < kFarBins; i += kThreads) sm.far[i] = 0;

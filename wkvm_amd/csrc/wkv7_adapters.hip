@@ -13,6 +13,7 @@
 // two adapters of 16 ranks 15.6 us (8.5), 64 rows with one of their own each 25 (9.9), 256 rows over
 // 32 of 32 ranks 34.5 (16.9), 3,001 rows of prompts 130, 32,768 rows 1,085 to 1,130.
 #include <algorithm>
+#include <numeric>
 
 #include "wkv7_proj_plan.h"
 #include "wkv7_proj_wide.h"
@@ -387,7 +388,13 @@ extern "C" int wkv7_adapter_plan(const int32_t* ids, int64_t m, int32_t count, i
                                  int64_t plan_ints) {
   if (m < 0 || m > WKV7_ADAPTER_MAX_ROWS || count < 0 || !plan || (m > 0 && !ids)) return WKV7_ERR_ARG;
   if (plan_ints < wkv7_adapter_plan_ints(m, count)) return WKV7_ERR_WORKSPACE;
-  for (int64_t i = 0; i < m; ++i)
+  // (a prompt's rows have one adapter, so rows are taken in runs of equal ids)
+  auto run_end = [&](int64_t i) {
+    const int32_t a = ids[i];
+    while (++i < m && ids[i] == a) {}
+    return i;
+  };
+  for (int64_t i = 0; i < m; i = run_end(i))
     if (ids[i] < -1 || ids[i] >= count) return WKV7_ERR_ARG;
   const int64_t all = positions(m, count);
   const int64_t align = m <= WKV7_ADAPTER_PACKED_ROWS ? 1 : kAlign;
@@ -396,52 +403,61 @@ extern "C" int wkv7_adapter_plan(const int32_t* ids, int64_t m, int32_t count, i
   int32_t* end = plan + plan_part(all, 2);
   int32_t* tile = plan + plan_part(all, 3);
   int32_t* const last = tile + kTileInts * max_tiles(m, count);
-  // Rows by adapter, in their own order within it, those without one last, in the place of `id`
-  // (which is written behind them): counted in the place of `end`, or sorted where there are more
-  // adapters than places.
+  // Rows by adapter, in their own order within it, those without one last, at the end of the tiles'
+  // place (the tiles of the rows before one, 20 ints for at most 16 rows or the rest of a run, end
+  // before it): counted in the place of `end`, or sorted where there are more adapters than places.
+  int32_t* const sorted = last - m;
   if (count < all) {
     std::fill(end, end + count + 1, 0);
     auto slot = [&](int64_t i) { return ids[i] < 0 ? count : ids[i]; };
-    for (int64_t i = 0; i < m; ++i) ++end[slot(i)];
+    for (int64_t i = 0, e; i < m; i = e) {
+      e = run_end(i);
+      end[slot(i)] += int32_t(e - i);
+    }
     int32_t at = 0;
     for (int32_t a = 0; a <= count; ++a) {
       const int32_t n = end[a];
       end[a] = at;
       at += n;
     }
-    for (int64_t i = 0; i < m; ++i) id[end[slot(i)]++] = int32_t(i);
+    for (int64_t i = 0, e; i < m; i = e) {
+      e = run_end(i);
+      int32_t& at = end[slot(i)];
+      std::iota(sorted + at, sorted + at + (e - i), int32_t(i));
+      at += int32_t(e - i);
+    }
   } else {
-    for (int64_t i = 0; i < m; ++i) id[i] = int32_t(i);
-    std::sort(id, id + m, [ids](int32_t x, int32_t y) {
+    for (int64_t i = 0; i < m; ++i) sorted[i] = int32_t(i);
+    std::sort(sorted, sorted + m, [ids](int32_t x, int32_t y) {
       const uint32_t a = uint32_t(ids[x]), b = uint32_t(ids[y]);  // (-1 is the largest)
       return a != b ? a < b : x < y;
     });
   }
+  auto gap = [&](int64_t from, int64_t to) {
+    std::fill(order + from, order + to, -1);
+    std::fill(id + from, id + to, -1);
+    std::fill(end + from, end + to, int32_t(to));
+  };
   int64_t p = 0;
   for (int64_t i = 0; i < m;) {
-    const int32_t a = ids[id[i]];
-    for (; p % align; ++p) order[p] = -1;
-    const int64_t start = p;
-    for (; i < m && ids[id[i]] == a; ++i) order[p++] = id[i];
-    for (int64_t f = start; a >= 0 && f < p; f += kSlab, tile += kTileInts) {
+    const int32_t a = ids[sorted[i]];
+    const int64_t first = (p + align - 1) / align * align;
+    gap(p, first);
+    for (p = first; i < m && ids[sorted[i]] == a; ++i) order[p++] = sorted[i];
+    std::fill(id + first, id + p, a);
+    std::fill(end + first, end + p, int32_t(p));
+    for (int64_t f = first; a >= 0 && f < p; f += kSlab, tile += kTileInts) {
+      const int64_t rows = std::min<int64_t>(kSlab, p - f);
       tile[0] = int32_t(f);
-      tile[1] = int32_t(std::min<int64_t>(kSlab, p - f));
+      tile[1] = int32_t(rows);
       tile[2] = a;
       tile[3] = 0;
-      for (int r = 0; r < kSlab; ++r) tile[4 + r] = order[std::min<int64_t>(f + r, p - 1)];
+      std::copy(order + f, order + f + rows, tile + 4);
+      std::fill(tile + 4 + rows, tile + kTileInts, order[p - 1]);
     }
   }
-  std::fill(order + p, order + all, -1);
+  gap(p, all);
   std::fill(tile, last, 0);
-  for (int64_t f = 0; f < all;) {
-    const int32_t a = order[f] < 0 ? -1 : ids[order[f]];
-    int64_t e = f;
-    while (e < all && (order[e] < 0 ? -1 : ids[order[e]]) == a) ++e;
-    for (; f < e; ++f) {
-      id[f] = a;
-      end[f] = int32_t(e);
-    }
-  }
   return WKV7_OK;
 }
 

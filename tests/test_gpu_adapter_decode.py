@@ -1,8 +1,10 @@
 """Adapters through the time-mix block, its decode graph and the example's decode loop."""
 
+import gc
 import math
 import os
 import sys
+import weakref
 
 import numpy as np
 import pytest
@@ -156,3 +158,32 @@ def test_the_example_decodes(dev):
     other = {k: [v[1], v[0]] for k, v in settings.items()}
     again, _, _ = ex.decode(model, [7, 5], [-1, 0], other, 6)
     assert torch.equal(again[:, 0], tokens[:, 1]) and torch.equal(again[:, 1], tokens[:, 0])
+
+
+def test_a_decode_graph_holds_its_banks(dev):
+    """Blocks that give their banks up after the capture: the graph replays the ones it captured."""
+    blocks, _ = _blocks(dev)
+    ids, adapter_ids = [4, 1, 9], [0, 2, -1]
+    state, want_state = (RWKV7StateBank(LAYOUT, 40, dev) for _ in range(2))
+    graph, want = (TimeMixDecodeGraph(b, blocks, 3, num_adapters=3) for b in (state, want_state))
+    gen = torch.Generator(device=dev).manual_seed(3)
+    for g in (graph, want):
+        g.set_slots(ids)
+        g.set_adapters(adapter_ids)
+    want.x.normal_(generator=gen)
+    graph.x.copy_(want.x)
+    expected = [o.clone() for o in want.replay()]
+    held = {id(b) for block in blocks for b in block.adapters.values()}
+    assert {id(b) for b in graph.adapter_banks} == held and len(held) == 8
+    refs = [weakref.ref(b.a) for block in blocks for b in block.adapters.values()]
+    for block in blocks:
+        block.adapters.clear()
+        for bank in block.add_adapters(3, 16).values():
+            bank.a.fill_(math.nan)
+    del want, g
+    assert all(r() is not None for r in refs)
+    for o, e in zip(graph.replay(), expected):
+        assert torch.equal(o, e)
+    del graph, o, e
+    gc.collect()
+    assert all(r() is None for r in refs)

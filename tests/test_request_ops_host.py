@@ -10,6 +10,8 @@ import torch
 
 from wkvm_amd import AdapterBank, _lib, adapter_plan, proj_adapters, sample_noise_size, sample_tokens
 from wkvm_amd.adapters import plan_ints
+from wkvm_amd.layout import RWKV7StateLayout
+from wkvm_amd.timemix import RWKV7TimeMix
 
 SLAB, PACKED, ALIGN = _lib.WKV7_ADAPTER_SLAB, 512, 32
 TILE = 20  # ints of a tile: first position, rows, adapter, 0, its rows
@@ -162,3 +164,16 @@ def test_bank_refusals():
 
 def test_noise_size():
     assert [sample_noise_size(v) for v in (1, 256, 257, 65536)] == [257, 257, 258, 512]
+
+
+def test_a_projection_keeps_its_bank():
+    """A decode graph captures the banks' addresses, so a second bank must not take one's place."""
+    block = RWKV7TimeMix.random(RWKV7StateLayout(1, 64, 1, 64, 64, torch.bfloat16), 0, "cpu")
+    held = dict(block.add_adapters(2, 8, names=("r", "o")))
+    for names in (("r",), ("k", "o"), ("k", "g1")):
+        with pytest.raises(ValueError, match="already holds|r, k, v and o"):
+            block.add_adapters(4, 8, names=names)
+        assert block.adapters == held  # (and none of the names got one)
+    more = block.add_adapters(3, 4, names=iter(("k", "v")))
+    assert all(more[name] is bank for name, bank in held.items())
+    assert more["k"].num_adapters == more["v"].num_adapters == 3

@@ -130,10 +130,16 @@ class RWKV7TimeMix:
     def add_adapters(self, num_adapters: int, max_rank: int, names=("r", "k", "v", "o"),
                      ) -> dict[str, AdapterBank]:
         """Empty banks of ``num_adapters`` places for the named projections; ``load`` fills
-        them. A batch planned with ``adapter_ids`` uses them."""
+        them. A batch planned with ``adapter_ids`` uses them. A projection that holds a bank keeps
+        it: a decode graph has captured its addresses, and would not see another one."""
+        names = tuple(names)
         for name in names:
             if name not in ("r", "k", "v", "o"):
                 raise ValueError(f"adapters are held by r, k, v and o, not {name!r}")
+            if name in self.adapters:
+                raise ValueError(f"projection {name!r} already holds a bank of "
+                                 f"{self.adapters[name].num_adapters} adapters")
+        for name in names:
             n, k = self.w[name].shape
             self.adapters[name] = AdapterBank(num_adapters, k, n, max_rank, self.w[name].device)
         return self.adapters
@@ -320,6 +326,8 @@ class TimeMixDecodeGraph:
         self.x = torch.zeros((len(layers), B, D), dtype=torch.bfloat16, device=dev)
         self.o: list[torch.Tensor] = []
         self.num_adapters = int(num_adapters)
+        # (the captured launches hold their addresses, whatever the blocks hold later)
+        self.adapter_banks = [b for layer in layers for b in layer.adapters.values()]
         self.adapter_plan = adapter_plan([-1] * B, num_adapters, dev) if num_adapters else None
         batch = TokenBatch(self.plan[:B], self.plan[2 * B:], self.plan[B:2 * B], B, B, True,
                            self.adapter_plan)

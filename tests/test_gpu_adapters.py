@@ -307,3 +307,27 @@ def test_refusals(dev):
     for args in [(0, k, n, 8), (1, 40, n, 8), (1, k, 0, 8), (1, k, n, 0), (1, k, n, 257)]:
         with pytest.raises(ValueError):
             AdapterBank(*args, dev)
+
+
+def test_a_dropped_plan_stays_until_its_launches_are_done(dev):
+    """A plan used on another stream than its own and dropped while that use is still to come: its
+    memory is handed out again only after it."""
+    gen = torch.Generator().manual_seed(37)
+    m, k, n = 700, 64, 32
+    x, w = _rand((m, k), gen, dev), _rand((n, k), gen, dev)
+    bank, _ = _bank(gen, dev, [16, 8], k, n)
+    ids = np.arange(m) % 3 - 1
+    plan = adapter_plan(ids, 2, dev)
+    (want,) = proj_adapters([(x, w, None, None, bank)], plan)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)  # some 20 ms that the launch has to wait for
+        (got,) = proj_adapters([(x, w, None, None, bank)], plan)
+    at, ints = plan.buf.data_ptr(), plan.buf.numel()
+    del plan
+    others = [torch.empty(ints, dtype=torch.int32, device=dev) for _ in range(4)]
+    assert not side.query()  # (the use is still to come)
+    assert all(t.data_ptr() != at for t in others)
+    side.synchronize()
+    assert torch.equal(got, want)

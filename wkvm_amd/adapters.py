@@ -98,6 +98,15 @@ class AdapterPlan:
 
     def __init__(self, rows: int, num_adapters: int, buf: torch.Tensor) -> None:
         self.rows, self.num_adapters, self.buf = rows, num_adapters, buf
+        self._made_on = ops._stream_ptr(buf.device) if buf.is_cuda else None
+
+    def use(self) -> int:
+        """The plan's address for a launch on the current stream, on which its memory is then in
+        use also after the plan is dropped. (A graph capture leaves keeping it to the caller.)"""
+        if ops._stream_ptr(self.buf.device) != self._made_on and \
+                not torch.cuda.is_current_stream_capturing():
+            self.buf.record_stream(torch.cuda.current_stream(self.buf.device))
+        return self.buf.data_ptr()
 
 
 def plan_ints(ids, num_adapters: int) -> np.ndarray:
@@ -158,7 +167,7 @@ def proj_adapters(products: Sequence[tuple], plan: AdapterPlan,
         ws_bytes = int(lib.wkv7_proj_adapters_workspace_bytes(M, groups, sets, n,
                                                               plan.num_adapters))
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-        rc = lib.wkv7_proj_adapters(M, groups, sets, n, plan.buf.data_ptr(), plan.num_adapters,
+        rc = lib.wkv7_proj_adapters(M, groups, sets, n, plan.use(), plan.num_adapters,
                                     ops._ptr(ws), ws_bytes, ops._stream_ptr(dev))
         _lib.check(rc, "wkv7_proj_adapters")
     return ys

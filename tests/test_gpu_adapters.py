@@ -331,3 +331,52 @@ def test_a_dropped_plan_stays_until_its_launches_are_done(dev):
     assert all(t.data_ptr() != at for t in others)
     side.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("act", [None, "sigmoid"])
+@pytest.mark.parametrize("m,k,n", [(1, 64, 48), (5, 256, 33), (16, 2048, 300), (40, 256, 96),
+                                   (200, 2048, 130), (203, 4096, 520), (640, 256, 96),
+                                   (5000, 64, 1000), (8200, 64, 1000)])
+def test_an_infinite_weight_is_infinite_as_in_the_formula(dev, m, k, n, act):
+    """B = +-inf in one rank of a column: h B is infinite by the sign of h, whatever h's bits are
+    (powers of two, whole numbers of few bits, and all 24), and its other rank is a number. The
+    rows run on every kernel: one row tile, small and large tiles, k in two parts, both tiles of
+    many rows."""
+    gen = torch.Generator().manual_seed(41)
+    w = _rand((n, k), gen, dev, 1 / math.sqrt(k))
+    x = _rand((m, k), gen, dev)
+    x[:, 0] = torch.sign(x[:, 0].float()).to(torch.bfloat16)  # h of rank 0: +-1
+    x[::3, 0] *= 3
+    x[1::3, 0] *= 0.0078125
+    bank = AdapterBank(2, k, n, 20, dev)
+    a, b = _rand((18, k), gen, dev, 1 / math.sqrt(k)), _rand((n, 18), gen, dev, 0.2)
+    a[0] = 0.0
+    a[0, 0] = 1.0
+    ranks = torch.arange(n) % 19  # the infinite one of every column, none in some
+    held = torch.arange(n)[ranks < 18]
+    sign = torch.where(held % 2 == 0, math.inf, -math.inf).to(torch.bfloat16).to(dev)
+    b[held.to(dev), ranks[ranks < 18].to(dev)] = sign
+    bank.load(1, a, b, 1.5)
+    ids = np.arange(m) % 2
+    ids[-1] = 1
+    (y,) = proj_adapters([(x, w, None, act, bank)], adapter_plan(ids, 2, dev))
+    rows = np.flatnonzero(ids == 1)
+    h = 1.5 * (x.double().cpu() @ a.double().cpu().T)[rows]
+    # (a sum of k terms near zero may have either sign in 32 bits)
+    sure = (h.abs() > 1e-4)[:, ranks.clamp(max=17)] | (ranks == 18)
+    want = _exact(x, w, None, act, [None, (a, b, 1.5)], ids)[rows]
+    got = y.double().cpu()[rows]
+    if act is None:
+        assert int(want.isinf().sum()) == len(rows) * len(held)
+        assert torch.equal(got.isinf() & sure, want.isinf() & sure)
+        assert torch.equal(got[want.isinf() & sure], want[want.isinf() & sure])
+    else:
+        ends = (ranks < 18) & sure  # 0 or 1
+        assert torch.equal(got[ends], want[ends])
+    none = _exact(x, w, None, act, None, ids)
+    base = np.flatnonzero(ids == 0)
+    if base.size:
+        _assert_close(y[base], none[base])
+    plain = ranks == 18
+    if plain.any():
+        _assert_close(y.cpu()[rows][:, plain], want[:, plain])

@@ -42,6 +42,7 @@ struct ShrinkArgs {
   const int32_t* tiles;  // [ntiles][kTileInts]
   int32_t ntiles;
   int64_t m, positions;
+  float last;  // factor of the last part of h: 1 / 2 where the products take it twice
 };
 
 // A tile of the plan, held to what the call has: rows is 0 where there is nothing to do. `row` is
@@ -63,22 +64,30 @@ __device__ __forceinline__ Tile get_tile(const ShrinkArgs& args, const ShrinkGro
 }
 
 // s times four of a row's sums, `left` of them ranks that the adapter has (a padding rank is 0
-// also where x is not finite), as bf16 parts; an infinite part has no parts after it.
-__device__ __forceinline__ void store_h(uint16_t* h, const f32x4& v, float s, int left) {
+// also where x is not finite), as bf16 parts whose sum is the value, each of its sign and zero only
+// where it is: a part takes the upper half of the next smaller number in 32 bits, the last one
+// what is left (24 bits less twice 8). So an infinite B gives the infinity that the whole value
+// gives; times a part of zero, or of the other sign, it would be NaN. All parts of a value that is
+// not finite are the value. (Below 2^-94 parts underflow.) The last part is stored times `last`.
+__device__ __forceinline__ void store_h(uint16_t* h, const f32x4& v, float s, int left,
+                                        float last) {
   float x[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) x[e] = e < left ? s * v[e] : 0.f;
 #pragma unroll
-  for (int p = 0; p < kParts; ++p) {
-    const uint2 part = {pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
-    *reinterpret_cast<uint2*>(h + p * kSlab) = part;
+  for (int p = 0; p + 1 < kParts; ++p) {
+    uint32_t top[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const uint32_t pair = e < 2 ? part.x : part.y;
-      const float top = (e & 1) ? bf16_hi(pair) : bf16_lo(pair);
-      x[e] = __builtin_isinf(top) ? 0.f : x[e] - top;
+      const uint32_t bits = __float_as_uint(x[e]);
+      const bool finite = (bits & 0x7f800000u) != 0x7f800000u;
+      top[e] = (finite && bits << 1 ? bits - 1 : bits) & 0xffff0000u;
+      x[e] = finite ? x[e] - __uint_as_float(top[e]) : x[e];
     }
+    *reinterpret_cast<uint2*>(h + p * kSlab) = {top[0] >> 16 | top[1], top[2] >> 16 | top[3]};
   }
+  *reinterpret_cast<uint2*>(h + (kParts - 1) * kSlab) = {pack_bf16(last * x[0], last * x[1]),
+                                                         pack_bf16(last * x[2], last * x[3])};
 }
 
 // Few tiles: a workgroup per tile and slab, k dealt to NW waves in 64-wide chunks whose sums
@@ -134,7 +143,7 @@ __global__ __launch_bounds__(64 * NW) void shrink_thin_kernel(const ShrinkArgs a
   // lane: ranks 4 lg .. 4 lg + 3 of row li
   if (li < tile.rows)
     store_h(G.h + ((tile.first + li) * G.slabs + slab) * kParts * kSlab + 4 * lg, acc, scale,
-            left - 4 * lg);
+            left - 4 * lg, args.last);
 }
 
 // Many tiles: a workgroup for two of them, k dealt to its waves as above and up to four slabs at
@@ -209,7 +218,7 @@ __global__ __launch_bounds__(64 * kWideShrink) void shrink_wide_kernel(const Shr
         for (int w = 1; w < NW; ++w) sum += red[w][s][lane];
         if (li < tiles[i].rows)
           store_h(G.h + ((tiles[i].first + li) * G.slabs + s0 + s) * kParts * kSlab + 4 * lg, sum,
-                  scale, rank - (s0 + s) * kSlab - 4 * lg);
+                  scale, rank - (s0 + s) * kSlab - 4 * lg, args.last);
       }
     }
   };
@@ -534,6 +543,7 @@ extern "C" int wkv7_proj_adapters(int64_t m, const wkv7_proj_group* groups,
   sh.ntiles = int32_t(max_tiles(m, count));
   sh.m = m;
   sh.positions = all;
+  sh.last = work.wide ? 1.f : 0.5f;
   int slabs = 0, kmax = 0;
   for (int i = 0; i < ngroups; ++i) {
     const wkv7_adapter_set& set = sets[i];

@@ -104,7 +104,8 @@ struct NoAdapters {
 // them. h holds s_a x A_a^T of every position, per slab of 16 ranks as three bf16 parts of 16 (all
 // 24 bits of the fp32 sum: with two parts the terms' 2^-18 shows where an output nearly cancels,
 // up to 1.03 bf16 ulp of it), b the other factors as [adapter][slab][n][16]. Two MFMAs of 32 k
-// values multiply a slab's parts with the same 16 columns of B.
+// values multiply a slab's parts with the same 16 columns of B: the first two parts, then half of
+// the last one twice (not once beside zeros, which an infinite B would turn into NaN).
 struct Adapters {
   static constexpr bool kOn = true;
   const int32_t* order;  // [positions] row of every position, or a negative number: none
@@ -217,8 +218,7 @@ struct Expand {
         const int r = min(max(16 * i + li, pairs.lo), pairs.hi - 1);
         const uint16_t* p = hp + (int64_t(r) * slabs + pairs.s) * 48;
         hf[u][i][0] = *reinterpret_cast<const uint4*>(p);
-        hf[u][i][1] = uint4{0, 0, 0, 0};
-        if (lg < 2) hf[u][i][1] = *reinterpret_cast<const uint4*>(p + 32);
+        hf[u][i][1] = *reinterpret_cast<const uint4*>(p + 32 - 16 * (lg >> 1));
       }
       more = pairs.next(step);
     }

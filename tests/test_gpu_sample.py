@@ -354,3 +354,34 @@ def test_refusals():
             sample_tokens(bad_logits, bad_noise)
     with pytest.raises(ValueError, match="tokens per row"):
         sample_tokens(torch.zeros((1, (1 << 21) + 1), device="cuda"), noise[:1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab,down", [(1 << 21, 22.25), (1 << 21, 23.5), (200003, 21.0)])
+def test_a_flat_tail_far_below_one_sure_token(dtype, vocab, down):
+    """One token at 0 and all others at -down (weights of 2^-30 to 2^-34), of which top-p keeps the
+    first half. Whole groups 2 % of the tail before and after that cut are drawn or not. The tail
+    weighs 1.3e-4 to 4.6e-4 of the row. The row's weight and top-p's share of it hold 24 bits, which
+    moves the cut by at most 2 x 2^-24 / 1.3e-4 = 0.1 % of the tail, and a weight of 2^-34 held to
+    2^-42 moves it by 0.4 %."""
+    x = torch.full((3, vocab), -down, dtype=dtype)
+    at = 777
+    x[:, at] = 0.0
+    tail = math.exp(-float(-x[0, 0])) * (vocab - 1)
+    share = (1 + 0.5 * tail) / (1 + tail)
+    top_p = float(np.float32(share))
+    kept = (top_p * (1 + tail) - 1) / tail  # of the tail, by the share as it is held
+    assert abs(kept - 0.5) < 0.01
+    groups = (vocab + G - 1) // G
+    inside, outside = int((kept - 0.02) * groups), int((kept + 0.02) * groups)
+    noise = torch.empty((3, sample_noise_size(vocab))).exponential_(
+        generator=torch.Generator().manual_seed(3)).clamp_(min=1e-3)
+    noise[:, G + at // G] = 1e30           # the sure token's group comes last
+    noise[0, G + inside] = 1e-12           # kept, and first
+    noise[1, G + outside] = 1e-12          # would be first, but is cut off
+    noise[1, G + inside] = 1e-9
+    noise[2, G + groups - 1] = 1e-12
+    noise[2, G + inside - 1] = 1e-9
+    noise[:, :G] = torch.linspace(1, 2, G)  # token 0 of a group comes first
+    tokens = sample_tokens(x.cuda(), noise.cuda(), top_p=top_p)[0].cpu().tolist()
+    assert tokens == [inside * G, inside * G, (inside - 1) * G]

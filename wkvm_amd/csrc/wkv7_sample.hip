@@ -26,8 +26,9 @@
 // across one of its V borders thousands of times as often.
 //
 // Weights that are added in an order that varies (LDS atomics) are fixed-point
-// numbers of 42 fraction bits (w <= 1), so every sum is exact and the token does
-// not depend on the order; plain sums are fp32 per thread, joined in a fixed order.
+// numbers, of 42 fraction bits (w <= 1) or, in the histogram of a whole row, of 31 bits
+// of the weight where the token's bins start: the sums are exact and the token does not
+// depend on the order. Plain sums are fp32 per thread, joined in a fixed order.
 #include "wkv7_common.h"
 
 namespace wkv7 {
@@ -111,11 +112,10 @@ __device__ __forceinline__ float load_one(const uint16_t* p) { return clean(bf16
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// 42 fraction bits of w in [0, 1].
+// 42 fraction bits of w in [0, 2^22).
 __device__ __forceinline__ u64 fixed(float w) {
-  const float hi = truncf(w * 2097152.f);
-  const float lo = (w * 2097152.f - hi) * 2097152.f;
-  return (u64(uint32_t(hi)) << 21) + uint32_t(lo);
+  const float hi = w * 0x1p10f;
+  return u64(uint32_t(hi)) << 32 | uint32_t(__builtin_amdgcn_fractf(hi) * 0x1p32f);
 }
 
 // Lane exchanges inside 16 lanes; after the smaller steps the mirrors act as xor 4 and xor 8.
@@ -455,25 +455,32 @@ __device__ __forceinline__ Found find_bin(Shared& sm, bool by_weight, u64 target
   return sm.found;
 }
 
-// The same over the far bins, which hold weights alone.
-__device__ __forceinline__ Found find_far(Shared& sm, u64 target) {
-  constexpr int kEach = kFarBins / kThreads;
+// The same over the far bins, which hold weights alone: kFarEach neighbouring bins in 31 fraction bits
+// of what a token at the start of the first of them weighs, 2^-(width * that bin) of the largest.
+constexpr int kFarEach = kFarBins / kThreads;
+
+__device__ __forceinline__ Found find_far(Shared& sm, float width, u64 target) {
   const int t = threadIdx.x;
   __syncthreads();
   uint32_t none = 0, all_c;
-  u64 before = 0, all_w;
+  u64 mine = 0, all_w;
   // (each lane starts at another bin of its own, lest they all read the same banks)
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) before += sm.far[kEach * t + (i + t) % kEach];
-  const u64 mine = before;
+  for (int i = 0; i < kFarEach; ++i) mine += sm.far[kFarEach * t + (i + t) % kFarEach];
+  const float unit = exp2_hw(fmaf(-width, float(kFarEach * t), -31.f));
+  auto weight = [unit](u64 sum) {
+    return fixed(fmaf(float(uint32_t(sum >> 32)), 0x1p32f, float(uint32_t(sum))) * unit);
+  };
+  mine = weight(mine);
+  u64 before = mine;
   block_scan(none, before, all_c, all_w, sm);
   before -= mine;
   const u64 goal = min(target, all_w);
   if (before < goal && before + mine >= goal) {
-    uint32_t bin = kEach * t;
-    u64 here = sm.far[bin];
-    for (; before + here < goal; here = sm.far[++bin]) before += here;
-    sm.found = {bin, 0, 0, before, here};
+    uint32_t bin = kFarEach * t;
+    u64 sum = sm.far[bin], upto = 0;
+    for (; before + weight(sum) < goal; sum += sm.far[++bin]) upto = sum;
+    sm.found = {bin, 0, 0, before + weight(upto), weight(sum) - weight(upto)};
   }
   __syncthreads();
   return sm.found;
@@ -876,8 +883,13 @@ __global__ __launch_bounds__(kThreads, 4) void sample_finish_kernel(const Sample
       // Top-p's share reaches far down: a pass over 8,192 bins of its tokens' range in log weight
       // leaves one short run of the order to look at closely. What bounds the pass is the work per
       // token, half instructions and half LDS atomics; the bins are many lest the run be long (2,048
-      // of them, and a branch per token: 256 rows of mixed settings 63 us where this took 53).
-      const float steps = float(kFarBins) / fmaxf(-low, 1.f);
+      // of them, and a branch per token: 256 rows of mixed settings 63 us where this took 53). A
+      // token adds its weight relative to its bins' start, to 2^-31 of itself, so that many tokens of
+      // one weight, or a tail far below 2^-32 of the largest, count as what they are (42 bits of the
+      // largest in place of that: 512 rows of 131,077 118.6 us, 116.1 so).
+      const float width = fmaxf(-low, 1.f) / float(kFarBins);  // of a bin, in log2
+      const float steps = set.c / width;                       // bins per logit
+      constexpr float kRun = kFarEach;                         // bins of one start
       __syncthreads();
       for (int i = t; i < kFarBins; i += kThreads) sm.far[i] = 0;
       __syncthreads();
@@ -886,10 +898,10 @@ __global__ __launch_bounds__(kThreads, 4) void sample_finish_kernel(const Sample
         uint32_t bin[N], w[N];
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-          const float z = (top - v.raw(e)) * set.c, d = z * steps;
+          const float r = (top - v.raw(e)) * (steps / kRun), d = r * kRun;
           const bool in = d < float(kFarBins);  // (not NaN, nor -inf past the row's end)
-          // 31 fraction bits, rounded: over a row their errors cancel to 10^-7 of its weight
-          w[e] = in ? uint32_t(fmaf(exp2_hw(-z), 0x1p31f, 0.5f)) : 0u;
+          const float rel = exp2_hw(-kRun * width * __builtin_amdgcn_fractf(r));
+          w[e] = in ? uint32_t(fmaf(rel, 0x1p31f, 0.5f)) : 0u;
           bin[e] = in ? uint32_t(d) : kFarBins + (threadIdx.x & (kWave - 1));
           // (in straight lines: a branch per token leaves nothing to do while one waits)
           asm volatile("" : "+v"(w[e]), "+v"(bin[e]));
@@ -897,15 +909,14 @@ __global__ __launch_bounds__(kThreads, 4) void sample_finish_kernel(const Sample
 #pragma unroll
         for (int e = 0; e < N; ++e) atomicAdd(&sm.far[bin[e]], u64(w[e]));
       });
-      const Found f = find_far(sm, (share + 2047) >> 11);
+      const Found f = find_far(sm, width, share);
       if (t == 0) sm.n_list = 0;
       __syncthreads();
       // The bin's tokens: first those in a range of logits that surely holds the bin (d is within
       // 0.01 of the exact quotient, the range's ends within 2^-21 of top's and their own size); of
       // them the others become -inf.
-      const float width = 1.f / (set.c * steps);
-      const float down = top - (float(f.bin) + 1.02f) * width;
-      const float up = top - (float(f.bin) - 0.02f) * width;
+      const float down = top - (float(f.bin) + 1.02f) / steps;
+      const float up = top - (float(f.bin) - 0.02f) / steps;
       const float slack = (fabsf(top) + fabsf(down)) * 0x1p-21f;
       const float least = down - slack, most = up + slack;
       row.vectors([&](const Vec<T>& v, int i) {
@@ -922,14 +933,14 @@ __global__ __launch_bounds__(kThreads, 4) void sample_finish_kernel(const Sample
       for (uint32_t i = t; i < min(sm.n_list, uint32_t(kList)); i += kThreads) {
         const uint32_t token = sm.list[i].y;
         const float x = token < uint32_t(V) ? load_one(row.p + token) : -INFINITY;
-        const float d = (top - x) * set.c * steps;
+        const float d = (top - x) * (steps / kRun) * kRun;
         const bool in = d < float(kFarBins) && uint32_t(d) == f.bin;
         sm.list[i].x = __float_as_uint(in ? x : -INFINITY);
       }
       __syncthreads();
       const uint32_t n = sm.n_list;
       if (n > 0 && n <= kList) {
-        const u64 before = f.before_wgt << 11, rest = share > before ? share - before : 1;
+        const u64 rest = share > f.before_wgt ? share - f.before_wgt : 1;
         Cut cut(0u, 0u);
         if (n <= kThreads) {
           const u64 v = sorted_candidate(n, sm);

@@ -599,7 +599,8 @@ int wkv7_proj_grouped_noalloc(int64_t m, const wkv7_proj_group *groups, int32_t 
  *
  * wkv7_adapter_plan writes the order in which the rows are visited (by adapter) to
  * host memory: wkv7_adapter_plan_ints(m, count) int32, from ids [m] on the host; an id
- * outside [-1, count) is WKV7_ERR_ARG. wkv7_proj_adapters reads a device copy of it
+ * outside [-1, count) is WKV7_ERR_ARG, and so are rows and adapters whose plan would have
+ * more than 2^31 - 1 positions (m + 31 min(m, count + 1), above 512 rows). wkv7_proj_adapters reads a device copy of it
  * (16-byte aligned); count there is the plan's, at most every set's.
  *
  *   groups, ngroups   as wkv7_proj_grouped (same alignment rules)

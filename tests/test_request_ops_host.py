@@ -177,3 +177,22 @@ def test_a_projection_keeps_its_bank():
     more = block.add_adapters(3, 4, names=iter(("k", "v")))
     assert all(more[name] is bank for name, bank in held.items())
     assert more["k"].num_adapters == more["v"].num_adapters == 3
+
+
+def test_plans_of_more_positions_than_32_bits_are_refused():
+    """Many rows over very many adapters: every adapter's run may leave a gap, and the plan's
+    positions are 32-bit numbers. (Refused before anything is read or written.)"""
+    lib = _lib.load()
+    most = 1 << 28
+    for count in (1000, 60_000_000):  # 2^28 + 31 * 60,000,001 is below 2^31
+        assert lib.wkv7_adapter_plan_ints(most, count) > 3 * most
+    groups, sets = (_lib.ProjGroup * 1)(), (_lib.AdapterSet * 1)()
+    groups[0] = _lib.ProjGroup(x=4096, w=8192, bias=None, y=12288, ldx=64, ldw=64, ldy=32, n=32,
+                               k=64, act=0, reserved=0)
+    for m, count in [(most, most), (most, 2**31 - 1), (most, 61_000_000), (1 << 27, 1 << 27)]:
+        assert lib.wkv7_adapter_plan_ints(m, count) == 0
+        assert lib.wkv7_adapter_plan(4096, m, count, 4096, 0) == _lib.WKV7_ERR_ARG
+        sets[0] = _lib.AdapterSet(a=4096, b=8192, scale=64, rank=128, count=count, slabs=1)
+        assert lib.wkv7_proj_adapters_workspace_bytes(m, groups, sets, 1, count) == 0
+        assert lib.wkv7_proj_adapters(m, groups, sets, 1, 4096, count, None, 0,
+                                      None) == _lib.WKV7_ERR_ARG

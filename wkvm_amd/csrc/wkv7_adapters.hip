@@ -294,6 +294,11 @@ int64_t positions(int64_t m, int32_t count) {
   return (m + (kAlign - 1) * runs + kAlign - 1) / kAlign * kAlign;
 }
 
+// Whether a plan of m rows over count adapters can be: its positions are 32-bit numbers.
+bool plan_fits(int64_t m, int32_t count) {
+  return m >= 0 && m <= WKV7_ADAPTER_MAX_ROWS && count >= 0 && positions(m, count) <= INT32_MAX;
+}
+
 // Where the plan's parts start, in ints.
 int64_t plan_part(int64_t positions, int part) { return part * ((positions + 3) / 4 * 4); }
 
@@ -389,13 +394,13 @@ Work make_work(int64_t rows, int64_t m, const wkv7_proj_group* groups, const wkv
 using namespace wkv7;
 
 extern "C" int64_t wkv7_adapter_plan_ints(int64_t m, int32_t count) {
-  if (m < 0 || m > WKV7_ADAPTER_MAX_ROWS || count < 0) return 0;
+  if (!plan_fits(m, count)) return 0;
   return plan_part(positions(m, count), 3) + kTileInts * max_tiles(m, count);
 }
 
 extern "C" int wkv7_adapter_plan(const int32_t* ids, int64_t m, int32_t count, int32_t* plan,
                                  int64_t plan_ints) {
-  if (m < 0 || m > WKV7_ADAPTER_MAX_ROWS || count < 0 || !plan || (m > 0 && !ids)) return WKV7_ERR_ARG;
+  if (!plan_fits(m, count) || !plan || (m > 0 && !ids)) return WKV7_ERR_ARG;
   if (plan_ints < wkv7_adapter_plan_ints(m, count)) return WKV7_ERR_WORKSPACE;
   // (a prompt's rows have one adapter, so rows are taken in runs of equal ids)
   auto run_end = [&](int64_t i) {
@@ -504,8 +509,8 @@ extern "C" int wkv7_adapter_load(const wkv7_adapter_set* set, int32_t index, int
 extern "C" size_t wkv7_proj_adapters_workspace_bytes(int64_t m, const wkv7_proj_group* groups,
                                                      const wkv7_adapter_set* sets,
                                                      int32_t ngroups, int32_t count) {
-  if (validate(m, groups, ngroups) != WKV7_OK || !sets || m == 0 || m > WKV7_ADAPTER_MAX_ROWS ||
-      count < 0 || check_sets(sets, ngroups, count) != WKV7_OK)
+  if (validate(m, groups, ngroups) != WKV7_OK || !sets || m == 0 || !plan_fits(m, count) ||
+      check_sets(sets, ngroups, count) != WKV7_OK)
     return 0;
   int cus = 0;
   if (device_cus(&cus) != WKV7_OK) return 0;
@@ -518,7 +523,7 @@ extern "C" int wkv7_proj_adapters(int64_t m, const wkv7_proj_group* groups,
                                   size_t workspace_bytes, void* stream) {
   int rc = validate(m, groups, ngroups);
   if (rc != WKV7_OK) return rc;
-  if (!sets || count < 0 || m > WKV7_ADAPTER_MAX_ROWS || (m > 0 && !plan)) return WKV7_ERR_ARG;
+  if (!sets || !plan_fits(m, count) || (m > 0 && !plan)) return WKV7_ERR_ARG;
   rc = check_sets(sets, ngroups, count);
   if (rc != WKV7_OK) return rc;
   if (m == 0) return WKV7_OK;

@@ -196,3 +196,13 @@ def test_plans_of_more_positions_than_32_bits_are_refused():
         assert lib.wkv7_proj_adapters_workspace_bytes(m, groups, sets, 1, count) == 0
         assert lib.wkv7_proj_adapters(m, groups, sets, 1, 4096, count, None, 0,
                                       None) == _lib.WKV7_ERR_ARG
+
+
+def test_a_scale_that_32_bits_make_infinite_is_refused():
+    bank = AdapterBank(1, 32, 16, 4, "cpu")
+    a, b = torch.zeros((4, 32), dtype=torch.bfloat16), torch.zeros((16, 4), dtype=torch.bfloat16)
+    for scale in (1e39, -1e300, math.inf, -math.inf, math.nan):
+        with pytest.raises(ValueError, match="scale must be finite"):
+            bank.load(0, a, b, scale)
+    with pytest.raises(ValueError, match="GPU"):  # (a bank on the host has nothing to load into)
+        bank.load(0, a, b, -3e38)

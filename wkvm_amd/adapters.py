@@ -13,6 +13,7 @@ the external model, wkvm/runner/runner.py:80-88).
 
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import Sequence
 
@@ -72,8 +73,8 @@ class AdapterBank:
         if tuple(a.shape) != (r, self.k) or tuple(b.shape) != (self.n, r):
             raise ValueError(f"a must be [{r}, {self.k}] and b [{self.n}, {r}], got "
                              f"{tuple(a.shape)} and {tuple(b.shape)}")
-        if not math.isfinite(scale):
-            raise ValueError(f"scale must be finite, got {scale}")
+        if not math.isfinite(ctypes.c_float(scale).value):  # (as the kernels hold it)
+            raise ValueError(f"scale must be finite in 32 bits, got {scale}")
         for t, name in ((a, "a"), (b, "b")):
             ops._require_cuda(t, name)
             if t.device != self.a.device:

@@ -385,3 +385,20 @@ def test_a_flat_tail_far_below_one_sure_token(dtype, vocab, down):
     noise[:, :G] = torch.linspace(1, 2, G)  # token 0 of a group comes first
     tokens = sample_tokens(x.cuda(), noise.cuda(), top_p=top_p)[0].cpu().tolist()
     assert tokens == [inside * G, inside * G, (inside - 1) * G]
+
+
+def test_host_arrays_and_ranges_are_sequences():
+    logits, noise = _inputs(12, 1234, torch.float32, 17)
+    temp, k, p, m = _settings(12, 4)
+    want = sample_tokens(logits, noise, temperature=temp.cuda(), top_k=k.cuda(), top_p=p.cuda(),
+                         min_p=m.cuda())
+    got = sample_tokens(logits, noise, temperature=temp.numpy(), top_k=k.numpy(),
+                        top_p=p.double().numpy(), min_p=tuple(m.tolist()))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    ranks = torch.arange(1, 13, dtype=torch.int32)
+    a = sample_tokens(logits, noise, top_k=range(1, 13), temperature=np.float32(0.5))
+    b = sample_tokens(logits, noise, top_k=ranks.cuda(), temperature=np.asarray(0.5))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    for bad in (np.ones((12, 1)), torch.ones((12, 1)), np.ones(11)):
+        with pytest.raises(ValueError, match="values"):
+            sample_tokens(logits, noise, temperature=bad)

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import math
 
+import numpy as np
 import torch
 
 from . import _lib, ops
@@ -41,9 +42,11 @@ def _setting(name: str, value, rows: int, device: torch.device):
             raise ValueError(f"{name} must be a contiguous {dtype} tensor of {rows} values on "
                              f"{device}")
         return value, 0
-    if isinstance(value, torch.Tensor):
+    if isinstance(value, (torch.Tensor, np.ndarray)):
+        if value.ndim > 1:
+            raise ValueError(f"{name} must be a number or {rows} values, got {tuple(value.shape)}")
         value = value.tolist()
-    many = value if isinstance(value, (list, tuple)) else [value]
+    many = value if isinstance(value, ops._IDS) else [value]
     for v in many:
         if not lo <= v <= hi or (dtype is torch.int32 and v != int(v)):  # (NaN fails too)
             raise ValueError(f"{name} must be in [{lo}, {hi}], got {v}")

@@ -8,10 +8,11 @@ import numpy as np
 import pytest
 import torch
 
-from wkvm_amd import AdapterBank, _lib, adapter_plan, proj_adapters, sample_noise_size, sample_tokens
+from wkvm_amd import (AdapterBank, AdapterPlan, _lib, adapter_plan, ops, proj_adapters,
+                      sample_noise_size, sample_tokens)
 from wkvm_amd.adapters import plan_ints
 from wkvm_amd.layout import RWKV7StateLayout
-from wkvm_amd.timemix import RWKV7TimeMix
+from wkvm_amd.timemix import RWKV7TimeMix, TimeMixDecodeGraph
 
 SLAB, PACKED, ALIGN = _lib.WKV7_ADAPTER_SLAB, 512, 32
 TILE = 20  # ints of a tile: first position, rows, adapter, 0, its rows
@@ -206,3 +207,16 @@ def test_a_scale_that_32_bits_make_infinite_is_refused():
             bank.load(0, a, b, scale)
     with pytest.raises(ValueError, match="GPU"):  # (a bank on the host has nothing to load into)
         bank.load(0, a, b, -3e38)
+
+
+def test_host_ids_under_graph_capture_are_refused_by_name(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="adapter_plan under graph capture"):
+        adapter_plan([0, -1], 1, "cuda")
+    graph = TimeMixDecodeGraph.__new__(TimeMixDecodeGraph)  # (a graph itself needs the GPU)
+    graph.batch_size, graph.num_adapters, graph._order = 2, 1, ops.ReplayOrder()
+    graph.adapter_plan = AdapterPlan(2, 1, torch.zeros(64, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="set_adapters under graph capture"):
+        graph.set_adapters([0, -1])
+    with pytest.raises(RuntimeError, match="set_slots under graph capture"):
+        ops.ReplayOrder().refresh(torch.zeros(2, dtype=torch.int32), [1, 2])

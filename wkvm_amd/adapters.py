@@ -129,10 +129,14 @@ def plan_ints(ids, num_adapters: int) -> np.ndarray:
 def adapter_plan(ids, num_adapters: int, device: torch.device | str = "cuda") -> AdapterPlan:
     """Device plan of a batch whose row m runs on adapter ``ids[m]`` (host integers; -1: the
     base model alone). It is complete when returned, serves every product of the batch
-    and stays right for as long as the rows keep their adapters."""
+    and stays right for as long as the rows keep their adapters. Refused under graph
+    capture, before the stream is touched: a replay would not see other ids."""
+    device = torch.device(device)
+    if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("adapter_plan under graph capture: its ids are host values")
     host = plan_ints(ids, num_adapters)
     rows = int(np.asarray(ids).size) if not isinstance(ids, torch.Tensor) else ids.numel()
-    return AdapterPlan(rows, int(num_adapters), torch.from_numpy(host).to(torch.device(device)))
+    return AdapterPlan(rows, int(num_adapters), torch.from_numpy(host).to(device))
 
 
 def proj_adapters(products: Sequence[tuple], plan: AdapterPlan,

@@ -128,13 +128,13 @@ class ReplayOrder:
         if stream is not None:
             self._last.record(stream)
 
-    def refresh(self, dst: torch.Tensor, values: list[int]) -> None:
+    def refresh(self, dst: torch.Tensor, values: list[int], what: str = "set_slots") -> None:
         """Host integers into the device int32 tensor that the graph reads,
         without waiting for the stream's earlier work. Refused under graph
         capture: a replay would read pinned memory that holds other values by
         then."""
         if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("set_slots under graph capture: its ids are host values")
+            raise RuntimeError(f"{what} under graph capture: its ids are host values")
         src = torch.tensor(values, dtype=torch.int32, pin_memory=True)
         stream = self._enter(dst.device)
         dst.copy_(src, non_blocking=True)

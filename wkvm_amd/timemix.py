@@ -375,7 +375,8 @@ class TimeMixDecodeGraph:
         ids = [int(a) for a in adapter_ids]
         if len(ids) != self.batch_size:
             raise ValueError(f"{len(ids)} adapter ids for a graph of batch size {self.batch_size}")
-        self._order.refresh(self.adapter_plan.buf, plan_ints(ids, self.num_adapters).tolist())
+        self._order.refresh(self.adapter_plan.buf, plan_ints(ids, self.num_adapters).tolist(),
+                            "set_adapters")
 
     def replay(self) -> list[torch.Tensor]:
         """Run the captured step; returns the static outputs ``o`` (L x [B, D])."""

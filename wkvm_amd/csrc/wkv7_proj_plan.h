@@ -23,7 +23,8 @@ int64_t count_tiles(int64_t m, const wkv7_proj_group* gs, int ng, TileShape sh) 
   return tiles;
 }
 
-template <int BM, int BN, int S, int GM, int GN, int BK, class Extra>
+// kSplits: plans split k over workgroups for this shape.
+template <int BM, int BN, int S, int GM, int GN, int BK, bool kSplits, class Extra>
 int launch(int64_t m, const wkv7_proj_group* gs, int ng, int parts, float* ws, const Extra& ex,
            hipStream_t s) {
   ProjArgs args{};
@@ -45,16 +46,18 @@ int launch(int64_t m, const wkv7_proj_group* gs, int ng, int parts, float* ws, c
   args.tiles_m = int32_t(tiles_m);
   args.xcd_span = int32_t((end + kXcds - 1) / kXcds);
   const unsigned grid = unsigned(args.xcd_span) * kXcds;
-  if (parts == 1) {
-    proj_kernel<BM, BN, S, GM, GN, BK, false><<<grid, 64 * GM * GN, 0, s>>>(args, ex);
-  } else {
-    proj_kernel<BM, BN, S, GM, GN, BK, true><<<grid, 64 * GM * GN, 0, s>>>(args, ex);
-    const int rc = launch_status();
-    if (rc != WKV7_OK) return rc;
-    const int64_t blocks = (elems + 255) / 256;
-    if (blocks > int64_t(0x7fffffff)) return WKV7_ERR_ARG;
-    proj_reduce_kernel<<<unsigned(blocks), 256, 0, s>>>(args, ex);
+  if constexpr (kSplits) {
+    if (parts > 1) {
+      const int64_t blocks = (elems + 255) / 256;
+      if (blocks > int64_t(0x7fffffff)) return WKV7_ERR_ARG;
+      proj_kernel<BM, BN, S, GM, GN, BK, true><<<grid, 64 * GM * GN, 0, s>>>(args, ex);
+      const int rc = launch_status();
+      if (rc != WKV7_OK) return rc;
+      proj_reduce_kernel<<<unsigned(blocks), 256, 0, s>>>(args, ex);
+      return launch_status();
+    }
   }
+  proj_kernel<BM, BN, S, GM, GN, BK, false><<<grid, 64 * GM * GN, 0, s>>>(args, ex);
   return launch_status();
 }
 
@@ -158,10 +161,11 @@ Plan make_plan(int64_t m, const wkv7_proj_group* gs, int ng, int cus) {
 template <class Extra>
 int launch_plan(int64_t m, const wkv7_proj_group* gs, int ng, const Plan& p, float* ws,
                 const Extra& ex, hipStream_t s) {
-  if (p.shape == 0) return launch<64, 64, 2, 2, 4, 128>(m, gs, ng, p.parts, ws, ex, s);
-  if (p.shape == 2) return launch<128, 64, 3, 8, 2, 128>(m, gs, ng, p.parts, ws, ex, s);
-  if (p.shape == 3) return launch<64, 32, 4, 4, 2, 128>(m, gs, ng, p.parts, ws, ex, s);
-  return launch<32, 32, 4, 2, 2, 128>(m, gs, ng, p.parts, ws, ex, s);
+  // (128 x 64 tiles are split only with adapters)
+  if (p.shape == 0) return launch<64, 64, 2, 2, 4, 128, false>(m, gs, ng, p.parts, ws, ex, s);
+  if (p.shape == 2) return launch<128, 64, 3, 8, 2, 128, Extra::kOn>(m, gs, ng, p.parts, ws, ex, s);
+  if (p.shape == 3) return launch<64, 32, 4, 4, 2, 128, false>(m, gs, ng, p.parts, ws, ex, s);
+  return launch<32, 32, 4, 2, 2, 128, true>(m, gs, ng, p.parts, ws, ex, s);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

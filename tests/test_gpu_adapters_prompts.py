@@ -3,7 +3,7 @@
 Up to a few thousand rows a call takes whichever of the three tile shapes needs the least time by
 its rounds over the units, so the sizes here are checked against that rule: ``_tile`` is the rule,
 and every test says which shape it means to run. The tolerance is that of the other sizes (one bf16
-ulp); exp and tanh add 2^-19 of a value, which is far below it.
+ulp); exp and tanh add 2^-18 of a value, which is far below it.
 """
 
 import math

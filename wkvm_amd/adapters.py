@@ -144,7 +144,7 @@ def proj_adapters(products: Sequence[tuple], plan: AdapterPlan,
     """``ops.proj_grouped`` with the rows' adapters beside the shared weights
     (``wkv7_proj_adapters``): ``products`` holds up to 8 tuples ``(x, w, bias, act, bank)``, all but
     the first two optional; ``bank`` is the ``AdapterBank`` of ``w`` or None. Every ``x`` has the
-    plan's row count, which is not bounded. Returns the ``[M, n]`` bf16 outputs."""
+    plan's row count, at most 2^28. Returns the ``[M, n]`` bf16 outputs."""
     groups, ys, keep, M = ops.proj_groups(products, outs)
     if M != plan.rows:
         raise ValueError(f"products of {M} rows for a plan of {plan.rows}")

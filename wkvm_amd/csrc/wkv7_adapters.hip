@@ -7,11 +7,12 @@
 // in that order, which adds h B_a^T to its accumulators before bias, activation and the one
 // rounding. h is summed in fp32 and kept whole as three bf16 parts, which the matrix cores
 // multiply with B in two instructions per slab of 16 ranks. Two launches because every output
-// column needs all of h, and a workgroup per tile of y would compute it once per column tile.
+// column needs all of h, and a workgroup per tile of y would compute it once per column tile. (For
+// a few rows over a few ranks that may cost less than a second launch: not measured.)
 //
 // Three products in a HIP graph (the shared products alone in brackets): 8 rows of 2048 x 2048 with
-// two adapters of 16 ranks 15.6 us (8.5), 64 rows with one of their own each 25 (9.9), 256 rows over
-// 32 of 32 ranks 34.5 (16.9), 3,001 rows of prompts 130, 32,768 rows 1,085 to 1,130.
+// two adapters of 16 ranks 14.9 us (8.5), 64 rows with one of their own each 23.7 (9.9), 256 rows over
+// 32 of 32 ranks 33.4 (16.9), 3,001 rows of prompts 126, 32,768 rows 987 to 1,003.
 #include <algorithm>
 #include <numeric>
 

@@ -14,8 +14,9 @@
 // for a histogram of the weights, once for the tokens of the bin that the cut is in.
 // One workgroup per row for all of it would leave a lone row on one unit (161 us for
 // 65,536 logits with every filter, 20 now). 256 rows of 65,536 fp32 logits in a HIP
-// graph: temperature alone 22.5 us (3.0 TB/s; the scan by itself 4.3), top-k 50 and
-// top-p 0.95 27.5, top-p 0.95 alone 58, rows of mixed settings 49.
+// graph: temperature alone 22.9 us (2.9 TB/s; the scan by itself 4.1), greedy 20.4, min-p
+// 0.05 23.1, top-k 50 and top-p 0.95 28, top-p 0.95 alone 57.4, rows of mixed settings 48.7,
+// top-k 5,000 (more than there are runs: radix passes over the whole row) 139.
 //
 // The draw is an exponential race in two levels: with positive exponential variates
 // e, group j of 256 consecutive tokens arrives at e / W_j (W_j the kept weight in it)
@@ -270,8 +271,8 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(const SampleA
 //
 // A chain of short steps with a barrier after each, so latency bounds it: about 5 us where nothing is
 // cut off, 12 for top-k 40 (sums 2, histogram of run maxima 4, gathering 2, order 2, race 2) and 16
-// for top-k 200. A top-p that reaches far down (65,536 fp32 logits: 31 us for a row) is bound by the
-// work per token of its two passes: 11 us for the histogram, 7 for the bin's tokens. Workgroups of
+// for top-k 200. A top-p that reaches far down (65,536 fp32 logits: 32 us for a row) is bound by the
+// work per token of its two passes: about 12 us for the histogram, 7 for the bin's tokens. Workgroups of
 // 512 threads, two of which share a unit, so that one works while the other waits. Tried and slower:
 // fp32 LDS atomics, and bins of each thread's own, for the histograms.
 

@@ -3,7 +3,7 @@
 The reference samples per request on the host, from logits copied back
 (``sample_token``, wkvm/runner/sampling.py:40), and takes a batched argmax for
 greedy decoding (wkvm/engine.py:163). Here every row of a batch is sampled in
-one launch by its own temperature, top-k, top-p and min-p, from random numbers
+one call (two launches) by its own temperature, top-k, top-p and min-p, from random numbers
 that the caller brings, so a request's tokens do not depend on the batch
 around it.
 """

@@ -194,8 +194,8 @@ __device__ __forceinline__ Vec<T> load_part(const T* row, int i, int n) {
 // instructions in the two exponentials per logit).
 //
 // Of every chunk: its maximum and sum of exponentials; of every 32 tokens the maximum, for the
-// finish to know where the largest logits are; and, where nothing but min-p is asked for or top-p
-// needs the row's weight, the weight of every group. Everything is relative to the chunk's own
+// finish to know where the largest logits are; and, where no filter applies or top-p alone needs the
+// row's weight, the weight of every group. Everything is relative to the chunk's own
 // maximum, so the chunks need nothing of each other.
 template <typename T>
 __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(const SampleArgs args) {

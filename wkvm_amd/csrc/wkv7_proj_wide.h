@@ -13,9 +13,10 @@
 // 32,768 rows of a 2048 x 2048 product 0.85 PFLOP/s (three with adapters of 32 ranks 0.90), k of 4096
 // 0.99, 8192^3 1.17: 0.66 to 0.79 of what the vendor's library reaches at these sizes. The loop
 // alone is at 1.69 PFLOP/s where nothing is loaded, 1.62 with every load a hit in the unit's
-// cache, 1.35 in the XCD's; with the real rows about 1.10, so what bounds it is x's lines on their way to the unit, and about 15 us per round of tiles for first loads and
-// results. No gain: prefetches into the XCD's cache, k started at another stage in every tile, waves
-// set apart in time, 1 to 16 row tiles side by side, three to five slots, eight waves.
+// cache, 1.35 in the XCD's; with the real rows about 1.10, so what bounds it is x's lines on their
+// way to the unit, and about 15 us per round of tiles for first loads and results. No gain:
+// prefetches into the XCD's cache, k started at another stage in every tile, waves set apart in
+// time, 1 to 16 row tiles side by side, three to five slots, eight waves.
 #pragma once
 
 #include "wkv7_proj_core.h"

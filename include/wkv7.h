@@ -691,6 +691,62 @@ int wkv7_sample_tokens(const void *logits, int32_t logits_dtype, int32_t rows, i
                        float *logprobs, void *workspace, size_t workspace_bytes, void *stream);
 size_t wkv7_sample_workspace_bytes(int32_t rows, int32_t vocab);
 
+/*
+ * Linear attention with a decay for each head, over the slot pool: per token and
+ * head, in fp32,
+ *     S[j][i] = exp(g) S[j][i] + k[j] v[i]          S is [K, V], g a log-decay
+ *     y[i]    = scale sum_j q[j] S[j][i]
+ * wkv7_linear_decode runs one token per slot in place, wkv7_linear_prefill ragged
+ * sequences in chunks of 64 tokens, each from its slot's state (or from zero when
+ * zero_init != 0), leaving its final state there.
+ *
+ * No counterpart in the reference, whose recurrent layers are RWKV-7's
+ * (wkvm/models/rwkv7.py:38-113). It serves layers whose state has the same slots
+ * and the plain decayed update; slot ids, pool rows, offsets and refusals are those of
+ * wkv7_decode_slots and wkv7_prefill_varlen.
+ *
+ *   state        [num_rows, H, K, V] fp32, 16-byte aligned; K is 64 or 128, V a
+ *                multiple of 64 up to WKV7_LINEAR_MAX_V (else WKV7_ERR_SHAPE)
+ *   q, k         [tokens, Hq, K] bf16; head h reads head h / (H / Hq) (H a multiple
+ *                of Hq), so queries and keys may be shared by several heads
+ *   v            [tokens, H, V] bf16;  y [tokens, H, V], contiguous, dtype per y_dtype
+ *   log_decay    fp32, head h of token t at log_decay[t * ld_decay + h]; ld_decay 0: one
+ *                value per head for every token. At most finite: -inf forgets the
+ *                state before the token
+ *   ldq, ldk, ldv  elements from one token to the next, at least a token's own and
+ *                multiples of 8; q, k, v and y 16-byte aligned (else WKV7_ERR_SHAPE)
+ * A token's output depends on the tokens up to it alone, infinities and NaN among
+ * them included.
+ *
+ * wkv7_linear_prefill cuts sequences into pieces that run side by side where the
+ * workgroups would not fill the device otherwise; the states between them go to
+ * the workspace (device, 16-byte aligned, wkv7_linear_prefill_workspace_bytes(..);
+ * holds nothing between calls). With less (or NULL) no sequence is cut. Sequences are
+ * [cu_seqlens[s], cu_seqlens[s + 1]) of the total_tokens, device int32 offsets as for
+ * wkv7_prefill_varlen; an empty one leaves its slot's state (zeroes it with zero_init).
+ */
+#define WKV7_LINEAR_MAX_V 1024
+
+typedef struct wkv7_linear_io {
+  const uint16_t *q, *k, *v;
+  const float *log_decay;
+  void *y;
+  int64_t ldq, ldk, ldv, ld_decay;
+  int32_t H, Hq, K, V;
+  int32_t y_dtype;
+  float scale;
+} wkv7_linear_io;
+
+int wkv7_linear_decode(float *state, int64_t num_rows, const int32_t *slot_ids,
+                       const int32_t *row_order, int32_t B, const wkv7_linear_io *io,
+                       void *stream);
+int wkv7_linear_prefill(float *state, int64_t num_rows, const int32_t *slot_ids,
+                        const int32_t *cu_seqlens, int32_t nseq, int64_t total_tokens,
+                        const wkv7_linear_io *io, int32_t zero_init, void *workspace,
+                        size_t workspace_bytes, void *stream);
+size_t wkv7_linear_prefill_workspace_bytes(int32_t nseq, int64_t total_tokens,
+                                           const wkv7_linear_io *io);
+
 #ifdef __cplusplus
 }
 #endif

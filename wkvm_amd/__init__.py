@@ -18,6 +18,8 @@ reference's slot-tensor layout and op signatures:
   each request's own
 * ``sample_tokens`` -- a batch's next tokens by per-request settings
   (wkvm/runner/sampling.py)
+* ``linear_decode_slots`` / ``linear_prefill_varlen`` -- linear attention with a
+  decay for each head, over the same slot pool
 * ``StateStore`` -- HOT/WARM/COLD state handles, wkvm/store.py, with the
   HOT <-> WARM copies as strided DMA transfers
 """
@@ -33,6 +35,7 @@ from .ops import (
     wkv7_prefill_varlen,
 )
 from .graph import DecodeGraph
+from .linear import linear_decode_slots, linear_prefill_varlen
 from .runner import WKV7Runner
 from .sampling import sample_noise_size, sample_tokens
 from .state import RWKV7StateBank, SlotCache
@@ -45,4 +48,5 @@ __all__ = [
     "wkv7_decode_slots", "wkv7_prefill_varlen", "slot_copy", "slot_zero",
     "chunk_rwkv7", "fused_recurrent_rwkv7",
     "AdapterBank", "AdapterPlan", "adapter_plan", "proj_adapters", "sample_tokens", "sample_noise_size",
+    "linear_decode_slots", "linear_prefill_varlen",
 ]

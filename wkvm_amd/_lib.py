@@ -44,6 +44,7 @@ WKV7_ADAPTER_SLAB = 16
 WKV7_ADAPTER_MAX_RANK = 256
 WKV7_SAMPLE_GROUP = 256
 WKV7_SAMPLE_MAX_VOCAB = 1 << 21
+WKV7_LINEAR_MAX_V = 1024
 
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
@@ -76,6 +77,13 @@ class SampleParams(ctypes.Structure):
     """struct wkv7_sample_params of include/wkv7.h."""
     _fields_ = [("temperature", _vp), ("top_k", _vp), ("top_p", _vp), ("min_p", _vp),
                 ("temperature1", _f32), ("top_k1", _i32), ("top_p1", _f32), ("min_p1", _f32)]
+
+
+class LinearIO(ctypes.Structure):
+    """struct wkv7_linear_io of include/wkv7.h."""
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("log_decay", _vp), ("y", _vp), ("ldq", _i64),
+                ("ldk", _i64), ("ldv", _i64), ("ld_decay", _i64), ("H", _i32), ("Hq", _i32),
+                ("K", _i32), ("V", _i32), ("y_dtype", _i32), ("scale", _f32)]
 
 
 # name -> (restype, argtypes); must match include/wkv7.h.
@@ -136,6 +144,11 @@ SIGNATURES = {
         _vp, _i32, _i32, _i32, _i64, _vp, _i64, ctypes.POINTER(SampleParams), _vp, _vp, _vp,
         _sz, _vp]),
     "wkv7_sample_workspace_bytes": (_sz, [_i32, _i32]),
+    "wkv7_linear_decode": (ctypes.c_int, [
+        _vp, _i64, _vp, _vp, _i32, ctypes.POINTER(LinearIO), _vp]),
+    "wkv7_linear_prefill": (ctypes.c_int, [
+        _vp, _i64, _vp, _vp, _i32, _i64, ctypes.POINTER(LinearIO), _i32, _vp, _sz, _vp]),
+    "wkv7_linear_prefill_workspace_bytes": (_sz, [_i32, _i64, ctypes.POINTER(LinearIO)]),
 }
 
 _lib = None

@@ -1,0 +1,222 @@
+// Linear attention with a decay for each head, over the slot pool: per token and head
+//   S <- e^g S + k v^T,   y = scale q^T S        (S [K, V] fp32, q, k, v bf16)
+//
+// wkv7_linear_decode: one token per slot, in place. wkv7_linear_prefill: ragged sequences, in
+// chunks of 64 tokens on the matrix cores. With G_t the sum of the chunk's log-decays up to token t,
+//   P[t][s] = scale (q_t . k_s) e^(G_t - G_s)  for s <= t, else 0
+//   y       = P V + scale e^(G_t) Q S
+//   S'      = e^(G_last) S + (e^(G_last - G_s) k_s)^T V
+// Every exponent is a difference of sums inside the chunk, so nothing overflows that the formula
+// itself does not, for any decay.
+#include <algorithm>
+
+#include "wkv7_linear_core.h"
+
+using namespace wkv7;
+
+namespace wkv7 {
+namespace {
+
+constexpr int kDecodeWaves = 4;
+
+// One (batch row, head, 64 value columns) of a decode step: lane i owns a column, wave w K / 4 key
+// rows, so that every access of the state is a whole 256-byte run. The state is read and written
+// once, without being kept in the caches.
+template <int KD, bool kF32>
+__global__ __launch_bounds__(64 * kDecodeWaves) void linear_decode_kernel(
+    float* __restrict__ state, int64_t rows, const int32_t* __restrict__ slot_ids,
+    const int32_t* __restrict__ row_order, int B, const wkv7_linear_io io) {
+  constexpr int KR = KD / kDecodeWaves;  // key rows of a wave
+  __shared__ float2 s_kq[KD];            // (k, scale q)
+  __shared__ float s_y[kDecodeWaves][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int tiles = io.V / 64;
+  int64_t item = blockIdx.x;
+  const int tile = int(item % tiles);
+  item /= tiles;
+  const int head = int(item % io.H);
+  int64_t row = item / io.H;
+  if (row_order) {
+    row = row_order[row];
+    if (row < 0 || row >= B) return;  // uniform: the whole block skips
+  }
+  const int64_t slot = slot_ids[row];
+  const int col = 64 * tile + lane;
+  const int64_t out = (row * io.H + head) * io.V + col;
+  if (slot < 0 || slot >= rows) {  // uniform: no state is touched, the output is zero
+    if (wave == 0) {
+      if (kF32) static_cast<float*>(io.y)[out] = 0.f;
+      else static_cast<uint16_t*>(io.y)[out] = 0;
+    }
+    return;
+  }
+  // the vectors before the state, whose arrival the arithmetic on them then does not wait for
+  const int j0 = KR * wave;
+  const int hq = head / (io.H / io.Hq);
+  const int64_t jo = int64_t(hq) * KD + j0 + (lane & (KR - 1));
+  const uint16_t qb = io.q[row * io.ldq + jo], kb = io.k[row * io.ldk + jo];
+  const uint16_t vb = io.v[row * io.ldv + int64_t(head) * io.V + col];
+  const float g = io.log_decay[row * io.ld_decay + head];
+  __builtin_amdgcn_sched_barrier(0);
+  float* hp = state + ((slot * io.H + head) * KD + j0) * io.V + col;
+  float h[KR];
+#pragma unroll
+  for (int j = 0; j < KR; ++j) h[j] = __builtin_nontemporal_load(hp + int64_t(j) * io.V);
+  asm volatile("" ::"v"(qb), "v"(kb), "v"(vb), "v"(g));
+  if (lane < KR)  // (its own wave's rows: no barrier)
+    s_kq[j0 + lane] = make_float2(bf16_to_f32(kb), bf16_to_f32(qb) * io.scale);
+  const float d = expf(g), v = bf16_to_f32(vb);
+  __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+  float y0 = 0.f, y1 = 0.f;
+#pragma unroll
+  for (int j = 0; j < KR; ++j) {
+    const float2 c = s_kq[j0 + j];
+    const float hn = fmaf(d, h[j], c.x * v);
+    __builtin_nontemporal_store(hn, hp + int64_t(j) * io.V);
+    if (j & 1) y1 = fmaf(c.y, hn, y1);
+    else y0 = fmaf(c.y, hn, y0);
+  }
+  s_y[wave][lane] = y0 + y1;
+  __syncthreads();
+  if (wave == 0) {
+    const float y = (s_y[0][lane] + s_y[1][lane]) + (s_y[2][lane] + s_y[3][lane]);
+    if (kF32) static_cast<float*>(io.y)[out] = y;
+    else static_cast<uint16_t*>(io.y)[out] = f32_to_bf16(y);
+  }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// The checks of both entry points, for `tokens` > 0 where the pointers are needed.
+int validate(const float* state, int64_t rows, int64_t tokens, const wkv7_linear_io* io) {
+  if (!io || rows < 1 || tokens < 0) return WKV7_ERR_ARG;
+  if (io->H < 1 || io->Hq < 1 || io->H % io->Hq) return WKV7_ERR_ARG;
+  if (io->y_dtype != WKV7_Y_BF16 && io->y_dtype != WKV7_Y_F32) return WKV7_ERR_ARG;
+  if ((io->K != 64 && io->K != 128) || io->V < 64 || io->V % 64 || io->V > WKV7_LINEAR_MAX_V)
+    return WKV7_ERR_SHAPE;
+  if (!state) return WKV7_ERR_ARG;
+  if (!aligned16(state)) return WKV7_ERR_SHAPE;
+  if (tokens == 0) return WKV7_OK;
+  if (!io->q || !io->k || !io->v || !io->y || !io->log_decay) return WKV7_ERR_ARG;
+  const int64_t qk = int64_t(io->Hq) * io->K, hv = int64_t(io->H) * io->V;
+  if (io->ldq < qk || io->ldk < qk || io->ldv < hv || (io->ld_decay && io->ld_decay < io->H))
+    return WKV7_ERR_SHAPE;
+  if (io->ldq % 8 || io->ldk % 8 || io->ldv % 8 || !aligned16(io->q) || !aligned16(io->k) ||
+      !aligned16(io->v) || !aligned16(io->y) || (reinterpret_cast<uintptr_t>(io->log_decay) & 3u))
+    return WKV7_ERR_SHAPE;
+  return WKV7_OK;
+}
+
+int device_cus(int* cus) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess ||
+      hipDeviceGetAttribute(cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
+    return launch_status();
+  return WKV7_OK;
+}
+
+// Tokens of a piece (a multiple of 64), or 0: no sequence is cut.
+int64_t piece_tokens(int32_t nseq, int64_t tokens, const wkv7_linear_io& io, int cus) {
+  const int64_t groups = int64_t(io.H) * (io.V / 64);
+  const int64_t want = 2 * int64_t(cus);
+  if (nseq * groups >= want || tokens <= kMinPiece) return 0;
+  const int64_t piece = (tokens * groups + want - 1) / want;
+  return std::max<int64_t>(kMinPiece, (piece + kChunk - 1) / kChunk * kChunk);
+}
+
+int64_t piece_slots(int32_t nseq, int64_t tokens, int64_t piece) {
+  return piece ? tokens / piece + nseq : nseq;
+}
+
+size_t workspace_bytes_of(int64_t slots, const wkv7_linear_io& io) {
+  return size_t(slots) * size_t(io.H) * (size_t(io.K) * size_t(io.V) * sizeof(float) +
+                                         sizeof(double));
+}
+
+template <int KD, bool kF32>
+int launch_prefill(const LinearSeqs& sq, const wkv7_linear_io& io, float* ws, hipStream_t s) {
+  const int64_t items = sq.slots * io.H * (io.V / 64);
+  if (items > int64_t(0x7ffffff0)) return WKV7_ERR_ARG;
+  LinearSeqs a = sq;
+  a.span = (items + kLinearXcds - 1) / kLinearXcds;
+  const unsigned grid = unsigned(a.span * kLinearXcds);
+  a.pieces = ws;
+  a.sums = ws ? reinterpret_cast<double*>(ws + sq.slots * io.H * int64_t(io.K) * io.V) : nullptr;
+  if (a.piece) {
+    linear_prefill_kernel<KD, false, true><<<grid, kLinearThreads, 0, s>>>(a, io);
+    int rc = launch_status();
+    if (rc != WKV7_OK) return rc;
+    const int64_t blocks = int64_t(a.nseq) * io.H * (KD * io.V / kChainElems);
+    if (blocks > int64_t(0x7fffffff)) return WKV7_ERR_ARG;
+    linear_chain_kernel<KD><<<unsigned(blocks), kChainThreads, 0, s>>>(a, io);
+    rc = launch_status();
+    if (rc != WKV7_OK) return rc;
+  }
+  linear_prefill_kernel<KD, kF32, false><<<grid, kLinearThreads, 0, s>>>(a, io);
+  return launch_status();
+}
+
+}  // namespace
+}  // namespace wkv7
+
+extern "C" int wkv7_linear_decode(float* state, int64_t num_rows, const int32_t* slot_ids,
+                                  const int32_t* row_order, int32_t B, const wkv7_linear_io* io,
+                                  void* stream) {
+  const int rc = validate(state, num_rows, B, io);
+  if (rc != WKV7_OK) return rc;
+  if (B == 0) return WKV7_OK;
+  if (!slot_ids) return WKV7_ERR_ARG;
+  const int64_t blocks = int64_t(B) * io->H * (io->V / 64);
+  if (blocks > int64_t(0x7fffffff)) return WKV7_ERR_ARG;
+  auto launch = [&](auto kernel) {
+    kernel<<<unsigned(blocks), 64 * kDecodeWaves, 0, as_stream(stream)>>>(
+        state, num_rows, slot_ids, row_order, B, *io);
+    return launch_status();
+  };
+  const bool f32 = io->y_dtype == WKV7_Y_F32;
+  if (io->K == 64) return f32 ? launch(linear_decode_kernel<64, true>) : launch(linear_decode_kernel<64, false>);
+  return f32 ? launch(linear_decode_kernel<128, true>) : launch(linear_decode_kernel<128, false>);
+}
+
+extern "C" size_t wkv7_linear_prefill_workspace_bytes(int32_t nseq, int64_t total_tokens,
+                                                      const wkv7_linear_io* io) {
+  if (!io || nseq < 1 || total_tokens < 1 || io->H < 1 || io->V < 64) return 0;
+  int cus = 0;
+  if (device_cus(&cus) != WKV7_OK) return 0;
+  const int64_t piece = piece_tokens(nseq, total_tokens, *io, cus);
+  return piece ? workspace_bytes_of(piece_slots(nseq, total_tokens, piece), *io) : 0;
+}
+
+extern "C" int wkv7_linear_prefill(float* state, int64_t num_rows, const int32_t* slot_ids,
+                                   const int32_t* cu_seqlens, int32_t nseq, int64_t total_tokens,
+                                   const wkv7_linear_io* io, int32_t zero_init, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  if (nseq < 0 || total_tokens > int64_t(0x7fffffff)) return WKV7_ERR_ARG;
+  const int rc = validate(state, num_rows, total_tokens, io);
+  if (rc != WKV7_OK) return rc;
+  if (nseq == 0) return WKV7_OK;
+  if (!slot_ids || !cu_seqlens) return WKV7_ERR_ARG;
+  int cus = 0;
+  const int drc = device_cus(&cus);
+  if (drc != WKV7_OK) return drc;
+  int64_t piece = piece_tokens(nseq, total_tokens, *io, cus);
+  if (piece && (!workspace || !aligned16(workspace) ||
+                workspace_bytes < workspace_bytes_of(piece_slots(nseq, total_tokens, piece), *io)))
+    piece = 0;
+  LinearSeqs sq{};
+  sq.state = state;
+  sq.rows = num_rows;
+  sq.slot_ids = slot_ids;
+  sq.cu = cu_seqlens;
+  sq.nseq = nseq;
+  sq.tokens = total_tokens;
+  sq.zero_init = zero_init != 0;
+  sq.piece = piece;
+  sq.slots = piece_slots(nseq, total_tokens, piece);
+  float* ws = piece ? static_cast<float*>(workspace) : nullptr;
+  hipStream_t s = as_stream(stream);
+  const bool f32 = io->y_dtype == WKV7_Y_F32;
+  if (io->K == 64)
+    return f32 ? launch_prefill<64, true>(sq, *io, ws, s) : launch_prefill<64, false>(sq, *io, ws, s);
+  return f32 ? launch_prefill<128, true>(sq, *io, ws, s) : launch_prefill<128, false>(sq, *io, ws, s);
+}

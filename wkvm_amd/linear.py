@@ -1,0 +1,175 @@
+"""Linear attention with a decay for each head, over the slot pool.
+
+Layers whose state has the slots of a WKV7 layer and a plainer update: per token and head
+
+    S <- exp(g) S + k v^T        y = scale q^T S
+
+with ``S [K, V]`` fp32 in its slot's row and a log-decay ``g`` that is fixed for a head or comes from
+the token. ``linear_decode_slots`` advances one token per slot, ``linear_prefill_varlen`` ragged prompts
+in chunks on the matrix cores; both take slot ids, offsets and outputs as ``wkv7_decode_slots`` and
+``wkv7_prefill_varlen`` do, and refuse what those refuse.
+
+The reference has no counterpart (its recurrent layers are RWKV-7's, wkvm/models/rwkv7.py:38-113).
+"""
+
+from __future__ import annotations
+
+import contextlib
+
+import torch
+
+from . import _lib, ops
+
+KEY_SIZES = (64, 128)
+
+
+def on_device(device: torch.device):
+    """A context in which ``device`` is the current one (launches go to the current device)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _check_state(state: torch.Tensor) -> tuple[int, int, int, int]:
+    ops._require_cuda(state, "state")
+    if state.dtype != torch.float32:
+        raise ValueError(f"state must be float32, got {state.dtype}")
+    if state.dim() != 4:
+        raise ValueError(f"state must be [rows, H, K, V], got {tuple(state.shape)}")
+    rows, H, K, V = state.shape
+    if rows < 1 or H < 1:
+        raise ValueError(f"state must have rows and heads, got {tuple(state.shape)}")
+    if K not in KEY_SIZES:
+        raise ValueError(f"K must be one of {KEY_SIZES}, got {K}")
+    if V < 64 or V % 64 or V > _lib.WKV7_LINEAR_MAX_V:
+        raise ValueError(f"V must be a multiple of 64 up to {_lib.WKV7_LINEAR_MAX_V}, got {V}")
+    if not state.is_contiguous() or state.data_ptr() % 16:
+        raise ValueError("state must be contiguous and 16-byte aligned")
+    return rows, H, K, V
+
+
+def _vectors(x: torch.Tensor, name: str, tokens: int, size: int, device: torch.device):
+    """``[tokens, heads, size]`` bf16 with whole tokens in one piece (copied where they are not), its
+    heads and the elements from one token to the next."""
+    ops._require_cuda(x, name)
+    if x.dtype != torch.bfloat16:
+        raise ValueError(f"{name} must be bfloat16, got {x.dtype}")
+    if x.dim() != 3 or x.shape[0] != tokens or x.shape[2] != size:
+        raise ValueError(f"{name} must be [{tokens}, heads, {size}], got {tuple(x.shape)}")
+    if x.device != device:
+        raise ValueError(f"{name} on {x.device}, state on {device}")
+    heads = x.shape[1]
+    own = heads * size
+    ld, sh, se = x.stride()
+    if tokens <= 1:
+        ld = own
+    if se != 1 or heads > 1 and sh != size or ld < own or ld % 8 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+        ld = own
+    return x, heads, ld
+
+
+def _io(q, k, v, log_decay, state, tokens, scale, out, out_dtype):
+    """The checked vectors as a ``LinearIO``, the output and the tensors that the launch reads."""
+    rows, H, K, V = _check_state(state)
+    dev = state.device
+    q, Hq, ldq = _vectors(q, "q", tokens, K, dev)
+    k, Hk, ldk = _vectors(k, "k", tokens, K, dev)
+    v, Hv, ldv = _vectors(v, "v", tokens, V, dev)
+    if Hk != Hq:
+        raise ValueError(f"q has {Hq} heads, k {Hk}")
+    if Hv != H:
+        raise ValueError(f"v has {Hv} heads, the state {H}")
+    if Hq < 1 or H % Hq:
+        raise ValueError(f"the state's {H} heads must be a multiple of the {Hq} of q and k")
+    ops._require_cuda(log_decay, "log_decay")
+    if log_decay.dtype != torch.float32:
+        raise ValueError(f"log_decay must be float32, got {log_decay.dtype}")
+    if tuple(log_decay.shape) not in ((H,), (tokens, H)):
+        raise ValueError(f"log_decay must be [{H}] or [{tokens}, {H}], got "
+                         f"{tuple(log_decay.shape)}")
+    if log_decay.device != dev:
+        raise ValueError(f"log_decay on {log_decay.device}, state on {dev}")
+    fixed = log_decay.dim() == 1
+    if H > 1 and log_decay.stride(-1) != 1 or not fixed and tokens > 1 and log_decay.stride(0) < H:
+        log_decay = log_decay.clone(memory_format=torch.contiguous_format)
+    ldd = 0 if fixed else H if tokens <= 1 else log_decay.stride(0)
+    dtype = out.dtype if out is not None else out_dtype
+    code = ops._y_code(dtype)
+    y = ops._out(out, (tokens, H, V), dtype, dev, "out")
+    if y.device != dev or y.data_ptr() % 16:
+        raise ValueError("out must be 16-byte aligned and on the state's device")
+    io = _lib.LinearIO(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
+                       y.data_ptr(), ldq, ldk, ldv, ldd, H, Hq, K, V, code, float(scale))
+    return io, y, (q, k, v, log_decay), rows
+
+
+def linear_decode_slots(state: torch.Tensor, slot_ids, q, k, v, log_decay, *, scale: float = 1.0,
+                        out: torch.Tensor | None = None,
+                        out_dtype: torch.dtype = torch.bfloat16,
+                        row_order: torch.Tensor | None = None) -> torch.Tensor:
+    """One token per slot, in place on ``state`` (``[rows, H, K, V]`` fp32, K 64 or 128, V a multiple of
+    64).
+
+    ``q``, ``k`` bf16 ``[B, Hq, K]`` (H a multiple of Hq: head h reads head ``h // (H / Hq)``), ``v``
+    bf16 ``[B, H, V]``, rows of any stride; ``log_decay`` fp32 ``[H]`` or ``[B, H]``. Returns
+    ``y [B, H, V]`` in ``out_dtype`` (bf16 or fp32). ``slot_ids`` and ``row_order`` as for
+    ``wkv7_decode_slots``."""
+    _check_state(state)
+    dev = state.device
+    ids, order = ops.decode_plan(slot_ids, state.shape[0], dev, wait=False)
+    if row_order is not None:
+        if not (isinstance(row_order, torch.Tensor) and row_order.is_cuda
+                and row_order.dtype == torch.int32 and row_order.shape == ids.shape):
+            raise ValueError("row_order must be a device int32 tensor shaped like slot_ids")
+        order = row_order
+    B = int(ids.shape[0])
+    io, y, keep, rows = _io(q, k, v, log_decay, state, B, scale, out, out_dtype)
+    if B:
+        with on_device(dev):
+            rc = _lib.load().wkv7_linear_decode(state.data_ptr(), rows, ids.data_ptr(),
+                                                ops._ptr(order), B, io, ops._stream_ptr(dev))
+        _lib.check(rc, "wkv7_linear_decode")
+    return y
+
+
+def linear_prefill_varlen(state: torch.Tensor, slot_ids, cu_seqlens, q, k, v, log_decay, *,
+                          zero_init: bool = False, scale: float = 1.0,
+                          out: torch.Tensor | None = None,
+                          out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """Ragged prompts: sequence ``s`` runs tokens ``cu_seqlens[s]:cu_seqlens[s+1]`` from the state of
+    slot ``slot_ids[s]`` (from zero with ``zero_init``) and leaves its final state there; an empty
+    sequence leaves it as it is (zeroes it with ``zero_init``).
+
+    ``q``, ``k``, ``v``, ``log_decay`` and the result as for ``linear_decode_slots``, over the T packed
+    tokens. ``cu_seqlens`` is a host sequence or a device int32 tensor. A token's output does not
+    depend on later tokens, whatever they hold. Few sequences are cut into pieces that run side by
+    side, through a workspace from torch's allocator."""
+    _check_state(state)
+    dev = state.device
+    ids = ops.device_ids(slot_ids, state.shape[0], dev, "slot_ids", distinct=True, wait=False)
+    nseq = int(ids.shape[0])
+    ops._require_cuda(v, "v")
+    T = int(v.shape[0]) if v.dim() == 3 else -1
+    io, y, keep, rows = _io(q, k, v, log_decay, state, T, scale, out, out_dtype)
+    if isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.is_cuda:
+        if cu_seqlens.dtype != torch.int32 or tuple(cu_seqlens.shape) != (nseq + 1,):
+            raise ValueError("device cu_seqlens must be int32 [nseq + 1]")
+        if cu_seqlens.device != dev:
+            raise ValueError(f"cu_seqlens on {cu_seqlens.device}, state on {dev}")
+        cu = cu_seqlens
+    else:
+        lst = ops._host_cu(cu_seqlens, T)
+        if len(lst) != nseq + 1:
+            raise ValueError(f"cu_seqlens has {len(lst)} entries for {nseq} sequences")
+        cu = ops._device_plan(lst, dev)
+    if nseq:
+        lib = _lib.load()
+        with on_device(dev):
+            ws_bytes = int(lib.wkv7_linear_prefill_workspace_bytes(nseq, T, io))
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+            rc = lib.wkv7_linear_prefill(state.data_ptr(), rows, ids.data_ptr(), cu.data_ptr(), nseq,
+                                         T, io, int(bool(zero_init)), ops._ptr(ws), ws_bytes,
+                                         ops._stream_ptr(dev))
+        _lib.check(rc, "wkv7_linear_prefill")
+    return y

@@ -25,6 +25,7 @@ import torch
 
 from . import ops
 from .layout import WKV_DTYPE, RWKV7StateLayout
+from .linear import linear_decode_slots, linear_prefill_varlen
 
 
 class SlotCache:
@@ -160,6 +161,26 @@ class RWKV7StateBank:
         return ops.wkv7_prefill_varlen(self.wkv[layer], ids, cu_seqlens, r, w, k, v, a, b,
                                        zero_init=zero_init, scale=scale, out=out,
                                        out_dtype=out_dtype, seq_order=seq_order)
+
+    # -- layers with the plain decayed update over the same rows ---------------------------
+
+    def decode_linear(self, layer: int, slot_batch, q, k, v, log_decay, *, scale: float = 1.0,
+                      out=None, out_dtype: torch.dtype = torch.bfloat16,
+                      row_order=None) -> torch.Tensor:
+        """One token per slot of a linear-attention ``layer`` (``linear_decode_slots``);
+        ``slot_batch`` as for ``decode_wkv``."""
+        ids = slot_batch if isinstance(slot_batch, torch.Tensor) else ops.ids_list(slot_batch, "wkv")
+        return linear_decode_slots(self.wkv[layer], ids, q, k, v, log_decay, scale=scale, out=out,
+                                   out_dtype=out_dtype, row_order=row_order)
+
+    def prefill_linear(self, layer: int, slot_batch, cu_seqlens, q, k, v, log_decay, *,
+                       zero_init: bool = False, scale: float = 1.0, out=None,
+                       out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """Ragged prompts of a linear-attention ``layer`` (``linear_prefill_varlen``)."""
+        ids = slot_batch if isinstance(slot_batch, torch.Tensor) else ops.ids_list(slot_batch, "wkv")
+        return linear_prefill_varlen(self.wkv[layer], ids, cu_seqlens, q, k, v, log_decay,
+                                     zero_init=zero_init, scale=scale, out=out,
+                                     out_dtype=out_dtype)
 
     def state_bytes(self) -> int:
         return (self.wkv.numel() * self.wkv.element_size()

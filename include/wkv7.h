@@ -747,6 +747,71 @@ int wkv7_linear_prefill(float *state, int64_t num_rows, const int32_t *slot_ids,
 size_t wkv7_linear_prefill_workspace_bytes(int32_t nseq, int64_t total_tokens,
                                            const wkv7_linear_io *io);
 
+/*
+ * Products with 4-bit weights: up to WKV7_PROJ_MAX_GROUPS independent products in one
+ * launch,
+ *     y_g = act_g( x_g W_g^T + bias_g ),   W[n][k] = s[n][k / group] (c[n][k] - z[n][k / group])
+ * with codes c and zero points z in 0 .. 15 and scales s, one of each per row and `group` (32, 64 or
+ * 128) consecutive inputs, the last group possibly shorter. x bf16; a group's products are exact,
+ * sums are fp32, y is rounded once to bf16. Any number of rows m.
+ *
+ * No counterpart in the reference, whose projections are nn.Linear calls on bf16 weights
+ * (external; reached through the model forward, wkvm/runner/runner.py:80-88). A decode step's
+ * time is the bytes of its weights; these have a quarter of them.
+ *
+ * A weight is held as
+ *   codes   [ceil(n / 16)][ceil(k / 128)][64][4] uint32: of 16 rows and 128 inputs, entry [l][j] has
+ *           the eight codes of row l % 16 at inputs 32 j + 8 (l / 16) .. + 7; code e starts at bit
+ *           (3 + 4 (e / 2) + 16 (e % 2)) % 32
+ *   scales  [ceil(n / 16)][ceil(k / group)][16] uint32: the scale in fp32 with its low four bits
+ *           replaced by the zero point
+ * (device, 16-byte aligned, wkv7_w4_code_bytes and wkv7_w4_scale_bytes long; rows and inputs
+ * past n and k hold zeros), which wkv7_w4_pack and wkv7_w4_quantize write and wkv7_w4_unpack reads.
+ * k is a multiple of 32 (as for wkv7_proj_grouped).
+ */
+typedef struct wkv7_w4_weight {
+  uint32_t *codes;
+  uint32_t *scales;
+  int32_t n, k, group;
+  int32_t reserved; /* 0 */
+} wkv7_w4_weight;
+
+#define WKV7_SCALE_BF16 0
+#define WKV7_SCALE_F16 1
+
+size_t wkv7_w4_code_bytes(int32_t n, int32_t k);
+size_t wkv7_w4_scale_bytes(int32_t n, int32_t k, int32_t group);
+
+/* Fills a weight from codes [n, k] (a byte each, 0 .. 15; their low four bits are taken), scales
+ * [n, ceil(k / group)] (bf16 or fp16) and zero points, bytes of the same shape or NULL (8), all
+ * contiguous. */
+int wkv7_w4_pack(const wkv7_w4_weight *weight, const uint8_t *codes, const void *scale,
+                 int32_t scale_dtype, const uint8_t *zero, void *stream);
+
+/* Fills a weight from a bf16 one [n, k], rows ldw elements apart, rounding each group to its range:
+ * with lo = min(w, 0) and hi = max(w, 0) over the group, s = (hi - lo) / 15, z = round(-lo / s),
+ * c = round(w / s) + z; symmetric != 0: s = max |w| / 7, z = 8. Values are clamped to 0 .. 15, s is
+ * fp32 with its low four bits cleared. */
+int wkv7_w4_quantize(const wkv7_w4_weight *weight, const uint16_t *w, int64_t ldw,
+                     int32_t symmetric, void *stream);
+
+/* The weight's values W [n, k] in fp32, contiguous. */
+int wkv7_w4_unpack(const wkv7_w4_weight *weight, float *w, void *stream);
+
+/* One product: x [m, k] bf16, rows ldx elements apart (a multiple of 8, 16-byte aligned); bias [n]
+ * bf16 or NULL; y [m, n] bf16, rows ldy elements apart; act as in wkv7_proj_group. */
+typedef struct wkv7_w4_group {
+  const uint16_t *x;
+  wkv7_w4_weight w;
+  const uint16_t *bias;
+  uint16_t *y;
+  int64_t ldx, ldy;
+  int32_t act;
+  int32_t reserved; /* 0 */
+} wkv7_w4_group;
+
+int wkv7_proj_w4(int64_t m, const wkv7_w4_group *groups, int32_t ngroups, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,6 +20,7 @@ reference's slot-tensor layout and op signatures:
   (wkvm/runner/sampling.py)
 * ``linear_decode_slots`` / ``linear_prefill_varlen`` -- linear attention with a
   decay for each head, over the same slot pool
+* ``W4Weight`` / ``proj_w4`` -- projections with 4-bit weights and group scales
 * ``StateStore`` -- HOT/WARM/COLD state handles, wkvm/store.py, with the
   HOT <-> WARM copies as strided DMA transfers
 """
@@ -40,6 +41,7 @@ from .runner import WKV7Runner
 from .sampling import sample_noise_size, sample_tokens
 from .state import RWKV7StateBank, SlotCache
 from .store import FingerprintMismatch, StateRecord, StateStore
+from .w4 import W4Weight, proj_w4
 
 __all__ = [
     "HEAD_SIZE", "WKV_DTYPE", "ModelStateSpec", "RWKV7StateLayout", "StateFamilySpec",
@@ -48,5 +50,5 @@ __all__ = [
     "wkv7_decode_slots", "wkv7_prefill_varlen", "slot_copy", "slot_zero",
     "chunk_rwkv7", "fused_recurrent_rwkv7",
     "AdapterBank", "AdapterPlan", "adapter_plan", "proj_adapters", "sample_tokens", "sample_noise_size",
-    "linear_decode_slots", "linear_prefill_varlen",
+    "linear_decode_slots", "linear_prefill_varlen", "W4Weight", "proj_w4",
 ]

@@ -45,6 +45,8 @@ WKV7_ADAPTER_MAX_RANK = 256
 WKV7_SAMPLE_GROUP = 256
 WKV7_SAMPLE_MAX_VOCAB = 1 << 21
 WKV7_LINEAR_MAX_V = 1024
+WKV7_SCALE_BF16 = 0
+WKV7_SCALE_F16 = 1
 
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
@@ -84,6 +86,18 @@ class LinearIO(ctypes.Structure):
     _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("log_decay", _vp), ("y", _vp), ("ldq", _i64),
                 ("ldk", _i64), ("ldv", _i64), ("ld_decay", _i64), ("H", _i32), ("Hq", _i32),
                 ("K", _i32), ("V", _i32), ("y_dtype", _i32), ("scale", _f32)]
+
+
+class W4Desc(ctypes.Structure):
+    """struct wkv7_w4_weight of include/wkv7.h."""
+    _fields_ = [("codes", _vp), ("scales", _vp), ("n", _i32), ("k", _i32), ("group", _i32),
+                ("reserved", _i32)]
+
+
+class W4Group(ctypes.Structure):
+    """struct wkv7_w4_group of include/wkv7.h."""
+    _fields_ = [("x", _vp), ("w", W4Desc), ("bias", _vp), ("y", _vp), ("ldx", _i64),
+                ("ldy", _i64), ("act", _i32), ("reserved", _i32)]
 
 
 # name -> (restype, argtypes); must match include/wkv7.h.
@@ -149,6 +163,12 @@ SIGNATURES = {
     "wkv7_linear_prefill": (ctypes.c_int, [
         _vp, _i64, _vp, _vp, _i32, _i64, ctypes.POINTER(LinearIO), _i32, _vp, _sz, _vp]),
     "wkv7_linear_prefill_workspace_bytes": (_sz, [_i32, _i64, ctypes.POINTER(LinearIO)]),
+    "wkv7_w4_code_bytes": (_sz, [_i32, _i32]),
+    "wkv7_w4_scale_bytes": (_sz, [_i32, _i32, _i32]),
+    "wkv7_w4_pack": (ctypes.c_int, [ctypes.POINTER(W4Desc), _vp, _vp, _i32, _vp, _vp]),
+    "wkv7_w4_quantize": (ctypes.c_int, [ctypes.POINTER(W4Desc), _vp, _i64, _i32, _vp]),
+    "wkv7_w4_unpack": (ctypes.c_int, [ctypes.POINTER(W4Desc), _vp, _vp]),
+    "wkv7_proj_w4": (ctypes.c_int, [_i64, ctypes.POINTER(W4Group), _i32, _vp]),
 }
 
 _lib = None

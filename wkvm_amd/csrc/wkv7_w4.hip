@@ -1,0 +1,197 @@
+// Products with 4-bit weights and group scales: y = act(x W^T + bias), W = s (c - z) with a scale and
+// a zero point for each row and group of inputs, and the kernels that lay such weights out.
+#include <algorithm>
+
+#include "wkv7_w4_core.h"
+
+using namespace wkv7;
+
+namespace wkv7 {
+namespace {
+
+struct W4Source {
+  const uint8_t* codes;
+  const void* scale;
+  const uint8_t* zero;
+  int scale_dtype;
+  const uint16_t* w;  // or a bf16 weight to round
+  int64_t ldw;
+  bool symmetric;
+};
+
+// Scale word of row n, group gi, and for a bf16 weight its factors.
+__device__ uint32_t w4_word(const W4Source& src, int n, int k, int gi, int group, int groups) {
+  if (!src.w) {
+    const int64_t at = int64_t(n) * groups + gi;
+    const uint16_t bits = static_cast<const uint16_t*>(src.scale)[at];
+    const float s = src.scale_dtype == WKV7_SCALE_BF16
+                        ? bf16_to_f32(bits)
+                        : float(__builtin_bit_cast(_Float16, bits));
+    return (__float_as_uint(s) & ~15u) | (src.zero ? src.zero[at] & 15u : 8u);
+  }
+  const uint16_t* w = src.w + int64_t(n) * src.ldw + int64_t(gi) * group;
+  const int count = min(group, k - gi * group);
+  float lo = 0.f, hi = 0.f;
+  for (int i = 0; i < count; ++i) {
+    const float v = bf16_to_f32(w[i]);
+    lo = fminf(lo, v);
+    hi = fmaxf(hi, v);
+  }
+  const float s = src.symmetric ? fmaxf(-lo, hi) / 7.f : (hi - lo) / 15.f;
+  const uint32_t bits = __float_as_uint(s) & ~15u;
+  const float kept = __uint_as_float(bits);
+  const float z = src.symmetric ? 8.f : kept > 0.f ? fminf(fmaxf(rintf(-lo / kept), 0.f), 15.f) : 0.f;
+  return bits | uint32_t(z);
+}
+
+// A thread per (row, group): its scale word, then its codes (a group is whole words).
+__global__ __launch_bounds__(256) void w4_fill_kernel(const wkv7_w4_weight out, const W4Source src) {
+  const int k = out.k, group = out.group;
+  const int groups = (k + group - 1) / group, blocks = (k + kW4K - 1) / kW4K;
+  const int span = (blocks * kW4K + group - 1) / group;  // groups, those past k among them
+  const int64_t item = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t rows = (int64_t(out.n) + kW4N - 1) / kW4N * kW4N;
+  if (item >= rows * span) return;
+  const int64_t n = item / span;
+  const int gi = int(item % span);
+  const bool real = n < out.n && gi < groups;
+  const uint32_t word = real ? w4_word(src, int(n), k, gi, group, groups) : 0u;
+  if (gi < groups) out.scales[((n / kW4N) * groups + gi) * kW4N + (n % kW4N)] = word;
+  const float s = w4_scale(word), z = float(w4_zero(word));
+  for (int i0 = gi * group; i0 < min((gi + 1) * group, blocks * kW4K); i0 += 8) {
+    uint32_t bits = 0;
+    for (int e = 0; e < 8 && real; ++e) {
+      const int i = i0 + e;
+      if (i >= k) break;
+      uint32_t c;
+      if (src.w) {
+        const float v = bf16_to_f32(src.w[n * src.ldw + i]);
+        c = uint32_t(s > 0.f ? fminf(fmaxf(rintf(v / s) + z, 0.f), 15.f) : z);
+      } else {
+        c = src.codes[n * k + i] & 15u;
+      }
+      const int at = w4_bit(e);
+      bits |= c << at | (at > 28 ? c >> (32 - at) : 0u);
+    }
+    const int lane = int(n % kW4N) + 16 * (i0 >> 3 & 3);
+    out.codes[(((n / kW4N) * blocks + i0 / kW4K) * 64 + lane) * 4 + (i0 >> 5 & 3)] = bits;
+  }
+}
+
+__global__ __launch_bounds__(256) void w4_unpack_kernel(const wkv7_w4_weight w, float* out) {
+  const int64_t item = int64_t(blockIdx.x) * 256 + threadIdx.x;  // a word: eight codes
+  const int k = w.k, words = k / 8;
+  if (item >= int64_t(w.n) * words) return;
+  const int64_t n = item / words;
+  const int i0 = int(item % words) * 8;
+  const int groups = (k + w.group - 1) / w.group, blocks = (k + kW4K - 1) / kW4K;
+  const int lane = int(n % kW4N) + 16 * (i0 >> 3 & 3);
+  const uint32_t bits = w.codes[(((n / kW4N) * blocks + i0 / kW4K) * 64 + lane) * 4 + (i0 >> 5 & 3)];
+  const uint32_t word = w.scales[((n / kW4N) * groups + i0 / w.group) * kW4N + (n % kW4N)];
+  for (int e = 0; e < 8; ++e)
+    out[n * k + i0 + e] = w4_scale(word) * float(w4_code(bits, e) - w4_zero(word));
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+int validate(const wkv7_w4_weight& w) {
+  if (!w.codes || !w.scales || w.n < 1 || w.k < 32 || w.k % 32) return WKV7_ERR_ARG;
+  if (w.group != 32 && w.group != 64 && w.group != 128) return WKV7_ERR_ARG;
+  if (!aligned16(w.codes) || !aligned16(w.scales)) return WKV7_ERR_SHAPE;
+  return WKV7_OK;
+}
+
+int validate(int64_t m, const wkv7_w4_group* groups, int32_t ngroups) {
+  if (m < 0 || m > int64_t(0x7fffffff) || !groups || ngroups < 1 || ngroups > WKV7_PROJ_MAX_GROUPS)
+    return WKV7_ERR_ARG;
+  for (int i = 0; i < ngroups; ++i) {
+    const wkv7_w4_group& g = groups[i];
+    const int rc = validate(g.w);
+    if (rc != WKV7_OK) return rc;
+    if (!g.x || !g.y) return WKV7_ERR_ARG;
+    if (g.act != WKV7_ACT_NONE && g.act != WKV7_ACT_TANH && g.act != WKV7_ACT_SIGMOID)
+      return WKV7_ERR_ARG;
+    if (g.ldx < g.w.k || g.ldy < g.w.n || g.ldx % 8 || !aligned16(g.x)) return WKV7_ERR_SHAPE;
+  }
+  return WKV7_OK;
+}
+
+int fill(const wkv7_w4_weight& w, const W4Source& src, void* stream) {
+  const int64_t rows = (int64_t(w.n) + kW4N - 1) / kW4N * kW4N;
+  const int span = ((w.k + kW4K - 1) / kW4K * kW4K + w.group - 1) / w.group;
+  const int64_t blocks = (rows * span + 255) / 256;
+  if (blocks > int64_t(0x7fffffff)) return WKV7_ERR_ARG;
+  w4_fill_kernel<<<unsigned(blocks), 256, 0, as_stream(stream)>>>(w, src);
+  return launch_status();
+}
+
+template <int NW, int TM>
+int launch_thin(const W4Args& args, hipStream_t s) {
+  const int64_t rows = (args.m + 16 * TM - 1) / (16 * TM);
+  if (rows > 65535) return WKV7_ERR_ARG;
+  const dim3 grid(unsigned(args.tile_end[args.ngroups - 1]), unsigned(rows));
+  w4_thin_kernel<NW, TM><<<grid, 64 * NW, 0, s>>>(args);
+  return launch_status();
+}
+
+}  // namespace
+}  // namespace wkv7
+
+extern "C" size_t wkv7_w4_code_bytes(int32_t n, int32_t k) {
+  if (n < 1 || k < 1) return 0;
+  return (size_t(n) + kW4N - 1) / kW4N * ((size_t(k) + kW4K - 1) / kW4K) * 1024;
+}
+
+extern "C" size_t wkv7_w4_scale_bytes(int32_t n, int32_t k, int32_t group) {
+  if (n < 1 || k < 1 || group < 1) return 0;
+  return (size_t(n) + kW4N - 1) / kW4N * ((size_t(k) + group - 1) / group) * (kW4N * 4);
+}
+
+extern "C" int wkv7_w4_pack(const wkv7_w4_weight* weight, const uint8_t* codes, const void* scale,
+                            int32_t scale_dtype, const uint8_t* zero, void* stream) {
+  if (!weight || !codes || !scale) return WKV7_ERR_ARG;
+  if (scale_dtype != WKV7_SCALE_BF16 && scale_dtype != WKV7_SCALE_F16) return WKV7_ERR_ARG;
+  const int rc = validate(*weight);
+  if (rc != WKV7_OK) return rc;
+  if (reinterpret_cast<uintptr_t>(scale) & 1u) return WKV7_ERR_SHAPE;
+  return fill(*weight, W4Source{codes, scale, zero, scale_dtype, nullptr, 0, false}, stream);
+}
+
+extern "C" int wkv7_w4_quantize(const wkv7_w4_weight* weight, const uint16_t* w, int64_t ldw,
+                                int32_t symmetric, void* stream) {
+  if (!weight || !w) return WKV7_ERR_ARG;
+  const int rc = validate(*weight);
+  if (rc != WKV7_OK) return rc;
+  if (ldw < weight->k || (reinterpret_cast<uintptr_t>(w) & 1u)) return WKV7_ERR_SHAPE;
+  return fill(*weight, W4Source{nullptr, nullptr, nullptr, 0, w, ldw, symmetric != 0}, stream);
+}
+
+extern "C" int wkv7_w4_unpack(const wkv7_w4_weight* weight, float* w, void* stream) {
+  if (!weight || !w) return WKV7_ERR_ARG;
+  const int rc = validate(*weight);
+  if (rc != WKV7_OK) return rc;
+  if (reinterpret_cast<uintptr_t>(w) & 3u) return WKV7_ERR_SHAPE;
+  const int64_t blocks = (int64_t(weight->n) * (weight->k / 8) + 255) / 256;
+  if (blocks > int64_t(0x7fffffff)) return WKV7_ERR_ARG;
+  w4_unpack_kernel<<<unsigned(blocks), 256, 0, as_stream(stream)>>>(*weight, w);
+  return launch_status();
+}
+
+extern "C" int wkv7_proj_w4(int64_t m, const wkv7_w4_group* groups, int32_t ngroups,
+                            void* stream) {
+  const int rc = validate(m, groups, ngroups);
+  if (rc != WKV7_OK) return rc;
+  if (m == 0) return WKV7_OK;
+  W4Args args{};
+  args.m = m;
+  args.ngroups = ngroups;
+  int64_t end = 0;
+  for (int i = 0; i < ngroups; ++i) {
+    args.g[i] = groups[i];
+    end += (int64_t(groups[i].w.n) + kW4N - 1) / kW4N;
+    if (end > int64_t(0x7fffffff)) return WKV7_ERR_ARG;
+    args.tile_end[i] = int32_t(end);
+  }
+  if (m <= 16) return launch_thin<8, 1>(args, as_stream(stream));
+  return launch_thin<8, 4>(args, as_stream(stream));
+}

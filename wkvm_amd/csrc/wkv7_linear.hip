@@ -18,6 +18,7 @@ namespace wkv7 {
 namespace {
 
 constexpr int kDecodeWaves = 4;
+constexpr int64_t kLinearMaxLd = int64_t(1) << 24;
 
 // One (batch row, head, 64 value columns) of a decode step: lane i owns a column, wave w K / 4 key
 // rows, so that every access of the state is a whole 256-byte run. The state is read and written
@@ -104,6 +105,8 @@ int validate(const float* state, int64_t rows, int64_t tokens, const wkv7_linear
   if (io->ldq % 8 || io->ldk % 8 || io->ldv % 8 || !aligned16(io->q) || !aligned16(io->k) ||
       !aligned16(io->v) || !aligned16(io->y) || (reinterpret_cast<uintptr_t>(io->log_decay) & 3u))
     return WKV7_ERR_SHAPE;
+  // (a chunk's rows are addressed by 32-bit offsets)
+  if (io->ldk > kLinearMaxLd || io->ldv > kLinearMaxLd) return WKV7_ERR_SHAPE;
   return WKV7_OK;
 }
 
@@ -133,17 +136,19 @@ size_t workspace_bytes_of(int64_t slots, const wkv7_linear_io& io) {
                                          sizeof(double));
 }
 
-template <int KD, bool kF32>
+template <int KD, int VT, bool kF32, int R, int kPerSimd>
 int launch_prefill(const LinearSeqs& sq, const wkv7_linear_io& io, float* ws, hipStream_t s) {
-  const int64_t items = sq.slots * io.H * (io.V / 64);
-  if (items > int64_t(0x7ffffff0)) return WKV7_ERR_ARG;
   LinearSeqs a = sq;
-  a.span = (items + kLinearXcds - 1) / kLinearXcds;
-  const unsigned grid = unsigned(a.span * kLinearXcds);
+  auto grid = [&](int tile) {
+    const int64_t items = a.slots * io.H * (io.V / tile);
+    a.span = (items + kLinearXcds - 1) / kLinearXcds;
+    return a.span * kLinearXcds;
+  };
   a.pieces = ws;
   a.sums = ws ? reinterpret_cast<double*>(ws + sq.slots * io.H * int64_t(io.K) * io.V) : nullptr;
+  if (grid(32) > int64_t(0x7fffffff)) return WKV7_ERR_ARG;
   if (a.piece) {
-    linear_prefill_kernel<KD, false, true><<<grid, kLinearThreads, 0, s>>>(a, io);
+    linear_states_kernel<KD, 64, 3><<<unsigned(grid(64)), 320, 0, s>>>(a, io);
     int rc = launch_status();
     if (rc != WKV7_OK) return rc;
     const int64_t blocks = int64_t(a.nseq) * io.H * (KD * io.V / kChainElems);
@@ -152,7 +157,7 @@ int launch_prefill(const LinearSeqs& sq, const wkv7_linear_io& io, float* ws, hi
     rc = launch_status();
     if (rc != WKV7_OK) return rc;
   }
-  linear_prefill_kernel<KD, kF32, false><<<grid, kLinearThreads, 0, s>>>(a, io);
+  linear_prefill_kernel<KD, VT, kF32, R, kPerSimd><<<unsigned(grid(VT)), 512, 0, s>>>(a, io);
   return launch_status();
 }
 
@@ -217,6 +222,8 @@ extern "C" int wkv7_linear_prefill(float* state, int64_t num_rows, const int32_t
   hipStream_t s = as_stream(stream);
   const bool f32 = io->y_dtype == WKV7_Y_F32;
   if (io->K == 64)
-    return f32 ? launch_prefill<64, true>(sq, *io, ws, s) : launch_prefill<64, false>(sq, *io, ws, s);
-  return f32 ? launch_prefill<128, true>(sq, *io, ws, s) : launch_prefill<128, false>(sq, *io, ws, s);
+    return f32 ? launch_prefill<64, 64, true, 3, 4>(sq, *io, ws, s)
+               : launch_prefill<64, 64, false, 3, 4>(sq, *io, ws, s);
+  return f32 ? launch_prefill<128, 32, true, 2, 4>(sq, *io, ws, s)
+             : launch_prefill<128, 32, false, 2, 4>(sq, *io, ws, s);
 }

@@ -1,19 +1,24 @@
 // Device code of the chunked linear attention (wkv7_linear_prefill).
 //
-// A workgroup of four waves walks one piece of one sequence for one head and 64 value columns, 64
-// tokens at a time, its state in accumulator registers. With v_mfma_f32_16x16x32_bf16 (lane l, li =
-// l % 16, lg = l / 16: an A or B lane holds row or column li at 8 lg .. 8 lg + 7 of a 32-wide block,
-// a result lane D[4 lg + i][li]):
-//   * wave w owns the chunk's tokens 16 w .. 16 w + 15 for the outputs, which are computed
-//     transposed (D rows are value columns), and K / 4 key rows of the state
-//   * the rows of a result tile are named so that the registers of two tiles are an operand of the
-//     next product as they stand: keys and tokens 32 p + 8 (m / 4) + 4 half + m % 4 for row m of
-//     tile (p, half), and value columns likewise. Scores therefore never leave their wave; of the
-//     state a bf16 split goes through LDS, each lane's own words
-//   * q, k and v come by direct loads into LDS, one chunk ahead; k and v are read transposed
+// A workgroup walks one piece of one sequence for one head and a tile of VT value columns, 64 tokens
+// at a time ("chunk"), its state in the accumulator registers of four state waves, each of which owns
+// K / 4 key rows. Four output waves have 16 of the chunk's tokens each. With
+// v_mfma_f32_16x16x32_bf16 (lane l, li = l % 16, lg = l / 16: an A or B lane holds row or column li at
+// 8 lg .. 8 lg + 7 of a 32-wide block, a result lane D[4 lg + i][li]), the rows of a result tile are
+// named so that the registers of two tiles are an operand of the next product as they stand: keys,
+// tokens and value columns 32 p + 8 (m / 4) + 4 half + m % 4 for row m of tile (p, half). Scores
+// therefore never leave their wave; of the state a bf16 split goes through LDS, each lane's own words.
+//
+// A chunk has two phases, a barrier behind each:
+//                  first                                   second
+//   state waves    write the state's split; decay the      add the chunk to the state
+//                  keys; ask for the k and v rows of a
+//                  later chunk (direct loads, LDS ring)
+//   output waves   scores, their decays and split; ask     outputs; the first of them also sums the
+//                  for the next chunk's queries            next chunk's decays
 // The operands that are not bf16 to begin with (scores under their decays, decayed keys, the state)
 // are split into bf16 parts: three where an fp32 result is kept (the state, an fp32 y), two
-// (2^-17 of each term) for a y that is rounded to bf16.
+// (2^-18 of each term) for a y that is rounded to bf16.
 #pragma once
 
 #include "wkv7_mfma.h"
@@ -22,10 +27,9 @@ namespace wkv7 {
 namespace {
 
 constexpr int kChunk = 64;          // tokens of a chunk
-constexpr int kLinearThreads = 256;
 constexpr int kLinearXcds = 8;      // workgroups are dealt round-robin over 8 XCDs
 constexpr int kMinPiece = 512;      // tokens of the shortest piece that a sequence is cut into
-constexpr int kChainThreads = 256;
+constexpr int kChainThreads = 64;
 constexpr int kChainElems = 4 * kChainThreads;
 constexpr double kLog2e = 1.4426950408889634;
 
@@ -46,22 +50,17 @@ struct LinearSeqs {
 };
 
 typedef __attribute__((address_space(3))) uint4 lds_u4;
-typedef __attribute__((address_space(3))) float lds_f32;
 
 __device__ __forceinline__ uint32_t lds_at(const uint4* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_u4*)p));
 }
-__device__ __forceinline__ uint32_t lds_at(const float* p) {
-  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_f32*)p));
-}
-
-// Direct loads, lane l's 16 (4) bytes to lds + 16 l (4 l). The compiler does not see them: every
-// wait for them is one of the barriers below.
-__device__ __forceinline__ void to_lds16(const void* src, uint32_t lds) {
-  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "{m0}"(lds), "v"(src) : "memory");
-}
-__device__ __forceinline__ void to_lds4(const void* src, uint32_t lds) {
-  asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, off" : : "{m0}"(lds), "v"(src) : "memory");
+// Direct load: 16 bytes per lane from base + offset to lds + 16 l. The compiler does not see it:
+// every wait for it is one of the barriers below.
+__device__ __forceinline__ void to_lds16(const void* base, uint32_t offset, uint32_t lds) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "{m0}"(lds), "v"(offset), "s"(base)
+               : "memory");
 }
 // At most N vector memory operations of this wave pending, then the workgroup barrier. (They
 // complete in order, stores among them.)
@@ -136,350 +135,595 @@ __device__ __forceinline__ bool find_piece(const LinearSeqs& a, int64_t slot, Pi
   return true;
 }
 
-template <int KD, bool kStates>
-struct LinearStage {
-  uint4 q[kStates ? 1 : kChunk * KD / 8];
-  uint4 k[kChunk * KD / 8];
-  uint4 v[kChunk * 8];
-  float g[4][kChunk];  // every wave's own copy
-};
-
-// element offset of channel e of row r of a [row][W] array, whose 16-byte chunks are swizzled by row
+// The 16-byte chunks of a [row][W] array's rows are swizzled by the row, W / 8 chunks a row: chunk c
+// of row r sits at c ^ turn(r). An operand read touches chunks 4 x + 0 .. 3 of rows 8 a + 0 .. 3 (a = 0
+// .. 3; half of each chunk where the read transposes), or one chunk per lane group of 16 such rows:
+// either way every 16 bytes of the 256-byte bank row equally often.
+template <int W>
+__device__ __forceinline__ int turn(int r) {
+  return W == 128 ? (r & 3) << 2 | (r >> 3 & 3) : W == 64 ? (r & 3) | (r >> 1 & 4) : 0;
+}
+// element offset of channel e of row r
 template <int W>
 __device__ __forceinline__ int at(int r, int e) {
-  return r * W + ((((e >> 3) ^ r) & (W / 8 - 1)) << 3) + (e & 7);
+  return r * W + (((e >> 3) ^ turn<W>(r)) << 3) + (e & 7);
 }
 
-// kStates: only the piece's final state from zero and the sum of its decays, for a piece that is
-// not its sequence's last.
-template <int KD, bool kF32, bool kStates>
-__global__ __launch_bounds__(kLinearThreads) void linear_prefill_kernel(const LinearSeqs a,
-                                                                         const wkv7_linear_io io) {
-  constexpr int RT = KD / 64;          // state tiles of a wave by 16 key rows
-  constexpr int NP = KD / 32;          // blocks of 32 keys
-  constexpr int YP = kF32 ? 3 : 2;     // bf16 parts of the state and the scores in y
-  constexpr int KL = KD / 32;          // direct loads of a wave for its share of q or k
-  constexpr int kLoads = (kStates ? KL : 2 * KL) + 2 + 1;
-  __shared__ LinearStage<KD, kStates> ring[2];
-  __shared__ uint4 s_state[kStates ? 1 : YP * NP * 4 * 64];
-  __shared__ float s_hi[4][kChunk], s_lo[4][kChunk], s_dec[4][kChunk];
-  __shared__ float s_part[2][4][64];
-  __shared__ int s_bad[2];
+// LDS of a workgroup. Chunk c of k and v sits in ring[c % R], asked for R - 1 chunks ahead.
+template <int KD, int VT, int YP, int R>
+struct LinearLds {
+  static constexpr int NP = KD / 32, NC = VT / 16;
+  struct Stage {
+    uint4 k[kChunk * KD / 8];
+    uint4 v[kChunk * VT / 8];
+  } ring[R];
+  uint4 state[YP ? YP * NP * NC * 64 : 1];  // parts of the state before the chunk
+  // of chunk c at [c % 2]: its tokens' sums of log2 decays G as two floats each, e^(G_last - G),
+  // e^(G_31 - G) of the first 32 tokens, the decays themselves, e^G_last
+  struct Decays {
+    alignas(16) float hi[kChunk];
+    alignas(16) float lo[kChunk];
+    alignas(16) float left[kChunk];
+    alignas(16) float first[32];
+    float raw[kChunk], all;
+  } decays[2];
+  float part[2][4][VT];
+  int bad[2];  // [c % 2]: something in chunk c is not finite
+};
 
-  const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tiles = io.V / 64;
-  // neighbouring items (the tiles and heads that share q and k) on one XCD
-  int64_t item = int64_t(blockIdx.x % kLinearXcds) * a.span + blockIdx.x / kLinearXcds;
-  if (item >= a.slots * io.H * tiles) return;
-  const int vt = int(item % tiles);
-  item /= tiles;
-  const int head = int(item % io.H);
-  const int64_t slot_no = item / io.H;
-  Piece pc;
-  if (!find_piece(a, slot_no, pc)) return;
-  const int64_t row = a.slot_ids[pc.seq];
-  const int64_t V = io.V;
-  const int col0 = 64 * vt;
-  if (kStates && pc.last) return;
-  if (row < 0 || row >= a.rows) {  // no state is touched, the outputs are zero
-    if (!kStates)
-      for (int64_t t = pc.beg + wave; t < pc.end; t += 4) {
-        const int64_t o = (t * io.H + head) * V + col0 + lane;
-        if (kF32) static_cast<float*>(io.y)[o] = 0.f;
-        else static_cast<uint16_t*>(io.y)[o] = 0;
-      }
-    return;
+// The state waves' share of a piece: `mine` 0 .. 3.
+template <int KD, int VT, int YP, int R>
+struct StateWave {
+  using Lds = LinearLds<KD, VT, YP, R>;
+  static constexpr int RT = KD / 64, NC = VT / 16, NP = KD / 32;
+  static constexpr int KL = KD / 32, VL = VT / 32;  // direct loads of a wave per chunk
+  static constexpr int kLoads = KL + VL, kAhead = R - 1;
+  Lds& lds;
+  int mine, li, lg, kp;
+  f32x4 S[RT][NC], next[RT][NC];
+  uint4 keys[RT][2][3];  // the chunk's keys under their decays, transposed, in parts
+  Neg neg;
+  const uint16_t *knext, *vnext;  // of the first token that no load has asked for (uniform)
+  int64_t ldk, ldv;
+
+  __device__ __forceinline__ StateWave(Lds& l, int wave) : lds(l), mine(wave) {
+    const int lane = threadIdx.x & 63;
+    li = lane & 15;
+    lg = lane >> 4;
+    kp = RT == 1 ? wave >> 1 : wave;  // the wave's block of 32 keys
+    neg = neg_consts();
   }
-
-  // state: key(rt, i) and column(c) of this lane's accumulators
-  const int kp = RT == 1 ? wave >> 1 : wave;  // the wave's block of 32 keys
-  auto half_of = [&](int rt) { return RT == 1 ? wave & 1 : rt; };
-  auto key0 = [&](int rt) { return 32 * kp + 8 * lg + 4 * half_of(rt); };
-  auto col_of = [&](int c) { return 32 * (c >> 1) + 8 * (li >> 2) + 4 * (c & 1) + (li & 3); };
-  float* slot_state = a.state + (row * io.H + head) * (KD * V) + col0;
-  float* piece_state = a.piece ? a.pieces + (slot_no * io.H + head) * (KD * V) + col0 : nullptr;
-
-  f32x4 S[RT][4];
-  const float* from = kStates ? nullptr
-                      : a.piece ? piece_state
-                      : a.zero_init ? nullptr : slot_state;
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        S[rt][c][i] = from && pc.end > pc.beg ? from[(key0(rt) + i) * V + col_of(c)] : 0.f;
-
-  auto store_state = [&](float* to) {
+  __device__ __forceinline__ int half_of(int rt) const { return RT == 1 ? mine & 1 : rt; }
+  __device__ __forceinline__ int key0(int rt) const { return 32 * kp + 8 * lg + 4 * half_of(rt); }
+  __device__ __forceinline__ int col_of(int c) const {
+    return 32 * (c >> 1) + 8 * (li >> 2) + 4 * (c & 1) + (li & 3);
+  }
+  __device__ __forceinline__ void load(const float* from, int64_t V) {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          S[rt][c][i] = from ? from[(key0(rt) + i) * V + col_of(c)] : 0.f;
+  }
+  __device__ __forceinline__ void store(float* to, int64_t V) const {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int i = 0; i < 4; ++i) to[(key0(rt) + i) * V + col_of(c)] = S[rt][c][i];
-  };
-  if (pc.end == pc.beg) {
-    if (!kStates && a.zero_init) store_state(slot_state);
-    return;
   }
 
-  const int hq = head / (io.H / io.Hq);
-  const uint16_t* qp = io.q + hq * KD;
-  const uint16_t* kptr = io.k + hq * KD;
-  const uint16_t* vp = io.v + int64_t(head) * V + col0;
-  const float* gp = io.log_decay + head;
-
-  // The direct loads of chunk c; rows behind the piece read its last token again (their decays are
-  // taken as 0 and their keys are dropped from the state).
-  auto issue = [&](int64_t c, LinearStage<KD, kStates>& st) {
-    const int64_t t0 = pc.beg + kChunk * c, lastt = pc.end - 1;
-    constexpr int R = 64 / (KD / 8);  // rows of a load
+  // The direct loads of the next chunk, which has n tokens and goes to ring slot `slot`; rows behind
+  // them read the last token again (their keys are dropped from the state).
+  __device__ __forceinline__ void issue(int slot, int n) {
+    auto& st = lds.ring[slot];
+    const int lane = threadIdx.x & 63;
+    constexpr int KR = 64 / (KD / 8), VR = 64 / (VT / 8);  // rows of a load
 #pragma unroll
     for (int i = 0; i < KL; ++i) {
-      const int r = R * (4 * i + wave) + lane / (KD / 8);
-      const int ch = ((lane % (KD / 8)) ^ r) & (KD / 8 - 1);
-      const int64_t t = min(t0 + r, lastt);
-      if (!kStates) to_lds16(qp + t * io.ldq + 8 * ch, lds_at(st.q) + 1024 * (4 * i + wave));
-      to_lds16(kptr + t * io.ldk + 8 * ch, lds_at(st.k) + 1024 * (4 * i + wave));
+      const int r = KR * (4 * i + mine) + lane / (KD / 8);
+      const int ch = (lane % (KD / 8)) ^ turn<KD>(r);
+      to_lds16(knext, 2 * (min(r, n - 1) * uint32_t(ldk) + 8 * ch),
+               lds_at(st.k) + 1024 * (4 * i + mine));
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = 8 * (4 * i + wave) + lane / 8;
-      const int ch = ((lane % 8) ^ r) & 7;
-      to_lds16(vp + min(t0 + r, lastt) * io.ldv + 8 * ch, lds_at(st.v) + 1024 * (4 * i + wave));
+    for (int i = 0; i < VL; ++i) {
+      const int r = VR * (4 * i + mine) + lane / (VT / 8);
+      const int ch = (lane % (VT / 8)) ^ turn<VT>(r);
+      to_lds16(vnext, 2 * (min(r, n - 1) * uint32_t(ldv) + 8 * ch),
+               lds_at(st.v) + 1024 * (4 * i + mine));
     }
-    to_lds4(gp + min(t0 + lane, lastt) * io.ld_decay, lds_at(&st.g[wave][0]));
-  };
+    knext += kChunk * ldk;
+    vnext += kChunk * ldv;
+  }
 
-  const Neg neg = neg_consts();
-  const int64_t chunks = (pc.end - pc.beg + kChunk - 1) / kChunk;
-  f32x4 y[4];           // the last chunk's outputs, stored behind the next one's first barrier
-  bool pending = false;
-  double sum = 0.;      // log2 decays of the piece so far
-
-  auto store_y = [&](int64_t c) {
-    const int64_t t = pc.beg + kChunk * c + 16 * wave + li;
-    if (t >= pc.end) return;
-    const int64_t o = (t * io.H + head) * V + col0 + 8 * lg;
+  // First phase: the state's bf16 parts, and the decayed keys of chunk c.
+  __device__ __forceinline__ void prepare(int64_t c) {
+    const uint16_t* sk = reinterpret_cast<const uint16_t*>(lds.ring[c % R].k);
+    const auto& dec = lds.decays[c & 1];
+    uint2 kt[RT][2][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const f32x4 &x0 = y[2 * h], &x1 = y[2 * h + 1];
-      if (kF32) {
-        f32x4* p = reinterpret_cast<f32x4*>(static_cast<float*>(io.y) + o + 32 * h);
-        p[0] = x0;
-        p[1] = x1;
-      } else {
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(io.y) + o + 32 * h) =
-            make_uint4(pack_bf16(x0[0], x0[1]), pack_bf16(x0[2], x0[3]), pack_bf16(x1[0], x1[1]),
-                       pack_bf16(x1[2], x1[3]));
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int r = 32 * b + 8 * lg + (li >> 2);
+        const int key = 32 * kp + 4 * half_of(rt) + 8 * (li & 3);
+        kt[rt][b][0] = ld_tr(sk + at<KD>(r, key));
+        kt[rt][b][1] = ld_tr(sk + at<KD>(r + 4, key));
       }
-    }
-  };
-
-  issue(0, ring[0]);
-  for (int64_t c = 0; c < chunks; ++c) {
-    LinearStage<KD, kStates>& st = ring[c & 1];
-    const bool more = c + 1 < chunks;
-    const int n = int(min(int64_t(kChunk), pc.end - pc.beg - kChunk * c));  // its tokens
-    if (more) issue(c + 1, ring[(c + 1) & 1]);
-    if (!kStates) {
+    if constexpr (YP > 0) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int ct = 0; ct < 4; ++ct) {
-          uint32_t lo[YP], hi[YP];
-          split_pair<YP>(S[rt][ct][0], S[rt][ct][1], lo, neg);
-          split_pair<YP>(S[rt][ct][2], S[rt][ct][3], hi, neg);
+        for (int ct = 0; ct < NC; ++ct) {
+          uint32_t a[YP], b[YP];
+          split_pair<YP>(S[rt][ct][0], S[rt][ct][1], a, neg);
+          split_pair<YP>(S[rt][ct][2], S[rt][ct][3], b, neg);
 #pragma unroll
           for (int p = 0; p < YP; ++p)
-            reinterpret_cast<uint2*>(&s_state[((p * NP + kp) * 4 + ct) * 64 + lane])[half_of(rt)] =
-                make_uint2(lo[p], hi[p]);
+            reinterpret_cast<uint2*>(
+                &lds.state[((p * NP + kp) * NC + ct) * 64 + (threadIdx.x & 63)])[half_of(rt)] =
+                make_uint2(a[p], b[p]);
         }
     }
-    if (threadIdx.x == 0) s_bad[c & 1] = 0;
-    if (more) barrier_vm<kLoads>();
-    else barrier_vm<0>();
-    if (!kStates && pending) store_y(c - 1);
-
-    // G: sums of log2 decays up to each token, in 64 bits, then as two floats
-    double G = 0.;
-    if (lane < n) {
-      const float g = st.g[wave][lane];
-      G = double(g < -1e4f ? -1e4f : g) * kLog2e;
-    }
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const double before = __shfl_up(G, d);
-      if (lane >= d) G += before;
+    for (int b = 0; b < 2; ++b) {
+      const f32x4 l0 = *reinterpret_cast<const f32x4*>(&dec.left[32 * b + 8 * lg]);
+      const f32x4 l1 = *reinterpret_cast<const f32x4*>(&dec.left[32 * b + 8 * lg + 4]);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const uint4 k8 = make_uint4(kt[rt][b][0].x, kt[rt][b][0].y, kt[rt][b][1].x, kt[rt][b][1].y);
+        float kd[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) kd[j] = elem(k8, j) * (j < 4 ? l0[j & 3] : l1[j & 3]);
+        split_eight<3>(kd, keys[rt][b], neg);
+      }
     }
-    const double Glast = __shfl(G, 63);
-    const float Ghi = float(G);
-    s_hi[wave][lane] = Ghi;
-    s_lo[wave][lane] = float(G - double(Ghi));
-    s_dec[wave][lane] = lane < n ? __builtin_amdgcn_exp2f(float(Glast - G)) : 0.f;
-    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-    const float all = __builtin_amdgcn_exp2f(float(Glast));
+  }
 
-    const uint16_t* sq = reinterpret_cast<const uint16_t*>(st.q);
-    const uint16_t* sk = reinterpret_cast<const uint16_t*>(st.k);
-    const uint16_t* sv = reinterpret_cast<const uint16_t*>(st.v);
-    uint4 vf[2][4];  // V: columns li of tile c, tokens 32 b + 8 lg ..
+  // Second phase: next = the state behind chunk c; false in some lane where it is not finite.
+  __device__ __forceinline__ bool add(int64_t c) {
+    const uint16_t* sv = reinterpret_cast<const uint16_t*>(lds.ring[c % R].v);
+    const float all = lds.decays[c & 1].all;
+    uint4 vf[2][NC];  // V: columns li of tile ct, tokens 32 b + 8 lg ..
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int ct = 0; ct < 4; ++ct) {
+      for (int ct = 0; ct < NC; ++ct) {
+        const int r = 32 * b + 8 * lg + (li >> 2);
         const int col = 32 * (ct >> 1) + 4 * (ct & 1) + 8 * (li & 3);
-        const uint2 x = ld_tr(sv + at<64>(32 * b + 8 * lg + (li >> 2), col));
-        const uint2 z = ld_tr(sv + at<64>(32 * b + 8 * lg + 4 + (li >> 2), col));
+        const uint2 x = ld_tr(sv + at<VT>(r, col)), z = ld_tr(sv + at<VT>(r + 4, col));
         vf[b][ct] = make_uint4(x.x, x.y, z.x, z.y);
       }
-
-    float wrong = 0.f;  // NaN as soon as a result is not finite
-    if (!kStates) {
-      const int t = 16 * wave + li;
-      uint4 qf[NP];
 #pragma unroll
-      for (int p = 0; p < NP; ++p) qf[p] = ld16(sq + at<KD>(t, 32 * p + 8 * lg));
+    for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-      for (int ct = 0; ct < 4; ++ct) y[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int part = YP - 1; part >= 0; --part)
-#pragma unroll
-        for (int p = 0; p < NP; ++p)
-#pragma unroll
-          for (int ct = 0; ct < 4; ++ct)
-            y[ct] = mma32(s_state[((part * NP + p) * 4 + ct) * 64 + lane], qf[p], y[ct]);
-      const float thi = s_hi[wave][t], tlo = s_lo[wave][t];
-      const float es = __builtin_amdgcn_exp2f(thi + tlo) * io.scale;
-#pragma unroll
-      for (int ct = 0; ct < 4; ++ct)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[ct][i] *= es;
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        if (b > (wave >> 1)) break;  // (uniform) behind every token of the wave
-        float p8[8];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          f32x4 sc = {0.f, 0.f, 0.f, 0.f};
-          const int kr = 32 * b + 8 * (li >> 2) + 4 * h + (li & 3);
-#pragma unroll
-          for (int p = 0; p < NP; ++p) sc = mma32(ld16(sk + at<KD>(kr, 32 * p + 8 * lg)), qf[p], sc);
-          const int s0 = 32 * b + 8 * lg + 4 * h;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float e =
-                __builtin_amdgcn_exp2f((thi - s_hi[wave][s0 + i]) + (tlo - s_lo[wave][s0 + i]));
-            p8[4 * h + i] = s0 + i <= t ? sc[i] * io.scale * e : 0.f;
-          }
-        }
-        uint4 pf[YP];
-        split_eight<YP>(p8, pf, neg);
-#pragma unroll
-        for (int part = YP - 1; part >= 0; --part)
-#pragma unroll
-          for (int ct = 0; ct < 4; ++ct) y[ct] = mma32(vf[b][ct], pf[part], y[ct]);
-      }
-      if (t < n)
-#pragma unroll
-        for (int ct = 0; ct < 4; ++ct)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) wrong = fmaf(y[ct][i], 0.f, wrong);
-    }
-
-    f32x4 next[RT][4];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-      for (int ct = 0; ct < 4; ++ct)
+      for (int ct = 0; ct < NC; ++ct)
 #pragma unroll
         for (int i = 0; i < 4; ++i) next[rt][ct][i] = S[rt][ct][i] * all;
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const int key = 32 * kp + 4 * half_of(rt) + 8 * (li & 3);
-        const uint2 x = ld_tr(sk + at<KD>(32 * b + 8 * lg + (li >> 2), key));
-        const uint2 z = ld_tr(sk + at<KD>(32 * b + 8 * lg + 4 + (li >> 2), key));
-        const uint4 kt = make_uint4(x.x, x.y, z.x, z.y);
-        float kd[8];
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) kd[j] = elem(kt, j) * s_dec[wave][32 * b + 8 * lg + j];
-        uint4 kf[3];
-        split_eight<3>(kd, kf, neg);
+      for (int part = 2; part >= 0; --part)
 #pragma unroll
-        for (int part = 2; part >= 0; --part)
+        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-          for (int ct = 0; ct < 4; ++ct)
-            next[rt][ct] = mma32(kf[part], vf[b][ct], next[rt][ct]);
-      }
+          for (int ct = 0; ct < NC; ++ct)
+            next[rt][ct] = mma32(keys[rt][b][part], vf[b][ct], next[rt][ct]);
+    f32x4 wrong = {0.f, 0.f, 0.f, 0.f};  // NaN as soon as an entry is not finite
 #pragma unroll
-      for (int ct = 0; ct < 4; ++ct)
+    for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) wrong = fmaf(next[rt][ct][i], 0.f, wrong);
-    }
-    if (__ballot(wrong != wrong) && lane == 0) s_bad[c & 1] = 1;
-    barrier_lds();
-    sum += Glast;
-    pending = true;
-    if (!s_bad[c & 1]) {
+      for (int ct = 0; ct < NC; ++ct)
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int ct = 0; ct < 4; ++ct) S[rt][ct] = next[rt][ct];
-      continue;
-    }
-    // Something in the chunk is not finite: products of whole tiles would carry it to tokens before
-    // it (0 times infinity). Token by token instead, as the formula is written.
-    pending = false;
-    for (int t = 0; t < n; ++t) {
-      const float d = expf(st.g[wave][t]);
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float kv = bf16_to_f32(sk[at<KD>(t, key0(rt) + i)]);
-          const float qv = kStates ? 0.f : bf16_to_f32(sq[at<KD>(t, key0(rt) + i)]) * io.scale;
-#pragma unroll
-          for (int ct = 0; ct < 4; ++ct) {
-            const float v = bf16_to_f32(sv[at<64>(t, col_of(ct))]);
-            S[rt][ct][i] = fmaf(d, S[rt][ct][i], kv * v);
-            if (!kStates) part[ct] = fmaf(qv, S[rt][ct][i], part[ct]);
-          }
-        }
-      if (kStates) continue;
-#pragma unroll
-      for (int ct = 0; ct < 4; ++ct) {
-        part[ct] += __shfl_xor(part[ct], 16);
-        part[ct] += __shfl_xor(part[ct], 32);
-        if (lg == 0) s_part[t & 1][wave][col_of(ct)] = part[ct];
-      }
-      barrier_lds();
-      if (wave == 0) {
-        const float (*p)[64] = s_part[t & 1];
-        const float v = (p[0][lane] + p[1][lane]) + (p[2][lane] + p[3][lane]);
-        const int64_t o = ((pc.beg + kChunk * c + t) * io.H + head) * V + col0 + lane;
-        if (kF32) static_cast<float*>(io.y)[o] = v;
-        else static_cast<uint16_t*>(io.y)[o] = f32_to_bf16(v);
-      }
-    }
-    barrier_lds();  // the stage is free for the next loads
+        for (int i = 0; i < 4; ++i) wrong[i] = fmaf(next[rt][ct][i], 0.f, wrong[i]);
+    const float any = (wrong[0] + wrong[1]) + (wrong[2] + wrong[3]);
+    return any == any;
   }
-  if (kStates) {
-    store_state(piece_state);
-    if (vt == 0 && threadIdx.x == 0) a.sums[slot_no * io.H + head] = sum;
+  __device__ __forceinline__ void accept() {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct) S[rt][ct] = next[rt][ct];
+  }
+};
+
+// A piece's place in the launch: false where there is nothing to do.
+struct LinearItem {
+  Piece pc;
+  int64_t no, row;
+  int head, tile;
+};
+
+template <int VT>
+__device__ __forceinline__ bool find_item(const LinearSeqs& a, const wkv7_linear_io& io,
+                                          LinearItem& it) {
+  // neighbouring items (the tiles and heads that share q and k) on one XCD
+  const int tiles = io.V / VT;
+  int64_t item = int64_t(blockIdx.x % kLinearXcds) * a.span + blockIdx.x / kLinearXcds;
+  if (item >= a.slots * io.H * tiles) return false;
+  it.tile = int(item % tiles);
+  item /= tiles;
+  it.head = int(item % io.H);
+  it.no = item / io.H;
+  if (!find_piece(a, it.no, it.pc)) return false;
+  it.row = a.slot_ids[it.pc.seq];
+  return true;
+}
+
+// The value that a DPP control brings to this lane, or 0 where it brings none or the row is masked.
+template <int kCtrl, int kRows = 0xf>
+__device__ __forceinline__ double from_lane(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, int(b), kCtrl, kRows, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, int(b >> 32), kCtrl, kRows, 0xf, false);
+  return __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+}
+__device__ __forceinline__ double lane_value(double x, int lane) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_readlane(int(b), lane);
+  const uint32_t hi = __builtin_amdgcn_readlane(int(b >> 32), lane);
+  return __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+}
+
+// The decays of a chunk with n tokens, g the lane's token's: by one wave. Returns G_last. The sums
+// are 64-bit, so that their differences are right for decays of any size.
+template <class Decays>
+__device__ __forceinline__ double sum_decays(Decays& d, float g, int n) {
+  const int lane = threadIdx.x & 63;
+  double G = lane < n ? double(g < -1e4f ? -1e4f : g) * kLog2e : 0.;
+  G += from_lane<0x111>(G);  // 1, 2, 4, 8 lanes up within rows of 16
+  G += from_lane<0x112>(G);
+  G += from_lane<0x114>(G);
+  G += from_lane<0x118>(G);
+  G += from_lane<0x142, 0xa>(G);  // the last lane of a row to the next, of two rows to the next two
+  G += from_lane<0x143, 0xc>(G);
+  const double last = lane_value(G, 63), mid = lane_value(G, 31);
+  const float hi = float(G);
+  d.hi[lane] = hi;
+  d.lo[lane] = float(G - double(hi));
+  d.left[lane] = lane < n ? __builtin_amdgcn_exp2f(float(last - G)) : 0.f;
+  if (lane < 32) d.first[lane] = __builtin_amdgcn_exp2f(float(mid - G));
+  d.raw[lane] = g;
+  if (lane == 0) d.all = __builtin_amdgcn_exp2f(float(last));
+  return last;
+}
+
+// Outputs. Waves 0 .. 3 are the state waves, 4 .. 7 the output waves.
+template <int KD, int VT, bool kF32, int R, int kPerSimd>
+__global__ __launch_bounds__(512, kPerSimd) void linear_prefill_kernel(const LinearSeqs a,
+                                                             const wkv7_linear_io io) {
+  constexpr int YP = kF32 ? 3 : 2;
+  using State = StateWave<KD, VT, YP, R>;
+  using Lds = typename State::Lds;
+  constexpr int NP = State::NP, NC = State::NC, RT = State::RT;
+  __shared__ Lds lds;
+
+  const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  LinearItem it;
+  if (!find_item<VT>(a, io, it)) return;
+  const Piece& pc = it.pc;
+  const int64_t V = io.V, row = it.row, head = it.head;
+  const int col0 = VT * it.tile;
+  if (row < 0 || row >= a.rows) {  // no state is touched, the outputs are zero
+    for (int64_t t = pc.beg + wave; t < pc.end; t += 8) {
+      const int64_t o = (t * io.H + head) * V + col0 + lane;
+      if (lane >= VT) continue;
+      if (kF32) static_cast<float*>(io.y)[o] = 0.f;
+      else static_cast<uint16_t*>(io.y)[o] = 0;
+    }
     return;
   }
-  if (pending) store_y(chunks - 1);
-  if (pc.last) store_state(slot_state);
+  float* slot_state = a.state + (row * io.H + head) * (KD * V) + col0;
+  const int64_t tokens = pc.end - pc.beg;
+  const int64_t chunks = (tokens + kChunk - 1) / kChunk;
+  auto count = [&](int64_t c) { return int(min(int64_t(kChunk), tokens - kChunk * c)); };
+  const int hq = it.head / (io.H / io.Hq);
+  const uint16_t* qbase = io.q + pc.beg * io.ldq + hq * KD;
+
+  if (wave < 4) {
+    State sw(lds, wave);
+    if (tokens == 0) {
+      if (a.zero_init) {
+        sw.load(nullptr, V);
+        sw.store(slot_state, V);
+      }
+      return;
+    }
+    sw.ldk = io.ldk;
+    sw.ldv = io.ldv;
+    sw.knext = io.k + pc.beg * io.ldk + hq * KD;
+    sw.vnext = io.v + pc.beg * io.ldv + head * V + col0;
+    if (threadIdx.x < 2) lds.bad[threadIdx.x] = 0;
+#pragma unroll
+    for (int c = 0; c < State::kAhead; ++c)
+      if (c < chunks) sw.issue(c, count(c));
+    sw.load(a.piece ? a.pieces + (it.no * io.H + head) * (KD * V) + col0
+                    : a.zero_init ? nullptr : slot_state, V);
+    barrier_vm<0>();
+    for (int64_t c = 0; c < chunks; ++c) {
+      const bool more = c + State::kAhead < chunks;
+      if (more) sw.issue(int((c + State::kAhead) % R), count(c + State::kAhead));
+      sw.prepare(c);
+      barrier_lds();
+      if (threadIdx.x == 0) lds.bad[(c + 1) & 1] = 0;
+      if (__ballot(!sw.add(c)) && lane == 0) lds.bad[c & 1] = 1;
+      if (more) barrier_vm<(State::kAhead - 1) * State::kLoads>();
+      else barrier_vm<0>();
+      if (!__builtin_amdgcn_readfirstlane(lds.bad[c & 1])) {
+        sw.accept();
+        continue;
+      }
+      // Something in the chunk is not finite: products of whole tiles would carry it to tokens
+      // before it (0 times infinity). Token by token instead, as the formula is written, once the
+      // outputs of those products are in memory.
+      barrier_lds();
+      const auto& st = lds.ring[c % R];
+      const uint16_t* sk = reinterpret_cast<const uint16_t*>(st.k);
+      const uint16_t* sv = reinterpret_cast<const uint16_t*>(st.v);
+      const int n = count(c);
+      for (int t = 0; t < n; ++t) {
+        const float d = expf(lds.decays[c & 1].raw[t]);
+        const uint16_t* q = qbase + (kChunk * c + t) * io.ldq;
+        float part[NC] = {};
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = sw.key0(rt) + i;
+            const float kv = bf16_to_f32(sk[at<KD>(t, key)]);
+            const float qv = bf16_to_f32(q[key]) * io.scale;
+#pragma unroll
+            for (int ct = 0; ct < NC; ++ct) {
+              const float v = bf16_to_f32(sv[at<VT>(t, sw.col_of(ct))]);
+              sw.S[rt][ct][i] = fmaf(d, sw.S[rt][ct][i], kv * v);
+              part[ct] = fmaf(qv, sw.S[rt][ct][i], part[ct]);
+            }
+          }
+#pragma unroll
+        for (int ct = 0; ct < NC; ++ct) {
+          part[ct] += __shfl_xor(part[ct], 16);
+          part[ct] += __shfl_xor(part[ct], 32);
+          if (lg == 0) lds.part[t & 1][wave][sw.col_of(ct)] = part[ct];
+        }
+        barrier_lds();
+        if (threadIdx.x < VT) {
+          const float(*p)[VT] = lds.part[t & 1];
+          const float v = (p[0][lane] + p[1][lane]) + (p[2][lane] + p[3][lane]);
+          const int64_t o = ((pc.beg + kChunk * c + t) * io.H + head) * V + col0 + lane;
+          if (kF32) static_cast<float*>(io.y)[o] = v;
+          else static_cast<uint16_t*>(io.y)[o] = f32_to_bf16(v);
+        }
+      }
+    }
+    if (pc.last) sw.store(slot_state, V);
+    return;
+  }
+
+  // -- output waves --------------------------------------------------------------------------
+  if (tokens == 0) return;
+  const int w = wave - 4;
+  const int tw = 16 * w + li;  // the lane's token of a chunk
+  const float* gbase = io.log_decay + pc.beg * io.ld_decay + head;
+  const int64_t lastt = tokens - 1;
+  auto load_g = [&](int64_t c) { return gbase[min(kChunk * c + lane, lastt) * io.ld_decay]; };
+  const Neg neg = neg_consts();
+  float g = 0.f;
+  if (w == 0) {
+    g = load_g(0);
+    sum_decays(lds.decays[0], g, count(0));
+    g = load_g(1);
+  }
+  uint4 qf[NP], qn[NP];  // the lane's query row of this chunk and of the next
+  auto load_q = [&](uint4 (&to)[NP], int64_t c) {
+    const uint16_t* q = qbase + min(kChunk * c + tw, lastt) * io.ldq + 8 * lg;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) to[p] = ld16(q + 32 * p);
+  };
+  load_q(qf, 0);
+  barrier_lds();
+  for (int64_t c = 0; c < chunks; ++c) {
+    const auto& st = lds.ring[c % R];
+    const auto& dec = lds.decays[c & 1];
+    const uint16_t* sk = reinterpret_cast<const uint16_t*>(st.k);
+    const uint16_t* sv = reinterpret_cast<const uint16_t*>(st.v);
+    load_q(qn, c + 1);
+    const float thi = dec.hi[tw], tlo = dec.lo[tw];
+
+    // Scores with the 32 tokens of block b, as an operand's rows.
+    auto scores = [&](int b, f32x4 (&sc)[2]) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        sc[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const int kr = 32 * b + 8 * (li >> 2) + 4 * h + (li & 3);
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+          sc[h] = mma32(ld16(sk + at<KD>(kr, 32 * p + 8 * lg)), qf[p], sc[h]);
+      }
+    };
+    f32x4 sc[2];
+    float p8[8];
+    uint4 own[YP], before[YP];  // parts of the wave's own block's scores and of the first block's
+    const int b = w >> 1;
+    scores(b, sc);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int s0 = 32 * b + 8 * lg + 4 * h;
+      const f32x4 shi = *reinterpret_cast<const f32x4*>(&dec.hi[s0]);
+      const f32x4 slo = *reinterpret_cast<const f32x4*>(&dec.lo[s0]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e = __builtin_amdgcn_exp2f((thi - shi[i]) + (tlo - slo[i]));
+        const float x = sc[h][i] * io.scale * e;
+        p8[4 * h + i] = s0 + i <= tw ? x : 0.f;
+      }
+    }
+    split_eight<YP>(p8, own, neg);
+    if (b) {  // the first block, all of it before the wave's tokens: e^(G_t - G_31) e^(G_31 - G_s)
+      scores(0, sc);
+      const float ea =
+          __builtin_amdgcn_exp2f((thi - dec.hi[31]) + (tlo - dec.lo[31])) * io.scale;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const f32x4 eb = *reinterpret_cast<const f32x4*>(&dec.first[8 * lg + 4 * h]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p8[4 * h + i] = sc[h][i] * ea * eb[i];
+      }
+      split_eight<YP>(p8, before, neg);
+    }
+    // an infinite or NaN query: its products with the state's parts are not the formula's
+    f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int p = 0; p < NP; ++p) zero = mma32(qf[p], make_uint4(0, 0, 0, 0), zero);
+    const float wrong = (zero[0] + zero[1]) + (zero[2] + zero[3]);
+    if (__ballot(wrong != wrong) && lane == 0) lds.bad[c & 1] = 1;
+    const float es = __builtin_amdgcn_exp2f(thi + tlo) * io.scale;
+    barrier_lds();
+
+    f32x4 y[NC];
+#pragma unroll
+    for (int ct = 0; ct < NC; ++ct) y[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int part = YP - 1; part >= 0; --part)
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int ct = 0; ct < NC; ++ct)
+          y[ct] = mma32(lds.state[((part * NP + p) * NC + ct) * 64 + lane], qf[p], y[ct]);
+#pragma unroll
+    for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[ct][i] *= es;
+    auto values = [&](int blk, const uint4 (&pf)[YP]) {
+      const int r = 32 * blk + 8 * lg + (li >> 2);
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct) {
+        const int col = 32 * (ct >> 1) + 4 * (ct & 1) + 8 * (li & 3);
+        const uint2 x = ld_tr(sv + at<VT>(r, col)), z = ld_tr(sv + at<VT>(r + 4, col));
+        const uint4 vf = make_uint4(x.x, x.y, z.x, z.y);
+#pragma unroll
+        for (int part = YP - 1; part >= 0; --part) y[ct] = mma32(vf, pf[part], y[ct]);
+      }
+    };
+    values(b, own);
+    if (b) values(0, before);
+
+    const int64_t t = kChunk * c + tw;
+    if (t < tokens) {
+      const int64_t o = ((pc.beg + t) * io.H + head) * V + col0 + 8 * lg;
+#pragma unroll
+      for (int h = 0; h < NC / 2; ++h) {
+        const f32x4 &x0 = y[2 * h], &x1 = y[2 * h + 1];
+        if (kF32) {
+          f32x4* p = reinterpret_cast<f32x4*>(static_cast<float*>(io.y) + o + 32 * h);
+          p[0] = x0;
+          p[1] = x1;
+        } else {
+          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(io.y) + o + 32 * h) =
+              make_uint4(pack_bf16(x0[0], x0[1]), pack_bf16(x0[2], x0[3]),
+                         pack_bf16(x1[0], x1[1]), pack_bf16(x1[2], x1[3]));
+        }
+      }
+    }
+    if (w == 0 && c + 1 < chunks) {
+      sum_decays(lds.decays[(c + 1) & 1], g, count(c + 1));
+      g = load_g(c + 2);
+    }
+    barrier_lds();
+    if (__builtin_amdgcn_readfirstlane(lds.bad[c & 1])) {
+      barrier_vm<0>();
+      for (int i = 0; i < count(c); ++i) barrier_lds();  // (the state waves write these outputs)
+    }
+#pragma unroll
+    for (int p = 0; p < NP; ++p) qf[p] = qn[p];
+  }
+}
+
+// A piece's final state from zero and the sum of its decays, for a piece that is not its sequence's
+// last: the four state waves and one for the decays.
+template <int KD, int VT, int R>
+__global__ __launch_bounds__(320) void linear_states_kernel(const LinearSeqs a,
+                                                            const wkv7_linear_io io) {
+  using State = StateWave<KD, VT, 0, R>;
+  __shared__ typename State::Lds lds;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  LinearItem it;
+  if (!find_item<VT>(a, io, it)) return;
+  const Piece& pc = it.pc;
+  if (pc.last || it.row < 0 || it.row >= a.rows) return;
+  const int64_t V = io.V, head = it.head;
+  const int col0 = VT * it.tile;
+  const int64_t tokens = pc.end - pc.beg;  // (a whole piece)
+  const int64_t chunks = (tokens + kChunk - 1) / kChunk;
+  auto count = [&](int64_t c) { return int(min(int64_t(kChunk), tokens - kChunk * c)); };
+  if (wave < 4) {
+    const int hq = it.head / (io.H / io.Hq);
+    State sw(lds, wave);
+    sw.ldk = io.ldk;
+    sw.ldv = io.ldv;
+    sw.knext = io.k + pc.beg * io.ldk + hq * KD;
+    sw.vnext = io.v + pc.beg * io.ldv + head * V + col0;
+#pragma unroll
+    for (int c = 0; c < State::kAhead; ++c)
+      if (c < chunks) sw.issue(c, count(c));
+    sw.load(nullptr, V);
+    barrier_vm<0>();
+    for (int64_t c = 0; c < chunks; ++c) {
+      const bool more = c + State::kAhead < chunks;
+      if (more) sw.issue(int((c + State::kAhead) % R), count(c + State::kAhead));
+      sw.prepare(c);
+      // (as for the outputs, but a wave's keys are its own: it decides by itself)
+      const bool bad = __ballot(!sw.add(c));
+      if (!bad) sw.accept();
+      const auto& st = lds.ring[c % R];
+      const uint16_t* sk = reinterpret_cast<const uint16_t*>(st.k);
+      const uint16_t* sv = reinterpret_cast<const uint16_t*>(st.v);
+      for (int t = 0; bad && t < count(c); ++t) {
+        const float d = expf(lds.decays[c & 1].raw[t]);
+#pragma unroll
+        for (int rt = 0; rt < State::RT; ++rt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float kv = bf16_to_f32(sk[at<KD>(t, sw.key0(rt) + i)]);
+#pragma unroll
+            for (int ct = 0; ct < State::NC; ++ct)
+              sw.S[rt][ct][i] = fmaf(d, sw.S[rt][ct][i],
+                                     kv * bf16_to_f32(sv[at<VT>(t, sw.col_of(ct))]));
+          }
+      }
+      if (more) barrier_vm<(State::kAhead - 1) * State::kLoads>();
+      else barrier_vm<0>();
+    }
+    sw.store(a.pieces + (it.no * io.H + head) * (KD * V) + col0, V);
+    return;
+  }
+  const float* gbase = io.log_decay + pc.beg * io.ld_decay + head;
+  auto load_g = [&](int64_t c) { return gbase[min(kChunk * c + lane, tokens - 1) * io.ld_decay]; };
+  double sum = sum_decays(lds.decays[0], load_g(0), count(0));
+  float g = load_g(1);
+  barrier_lds();
+  for (int64_t c = 0; c < chunks; ++c) {
+    if (c + 1 < chunks) {
+      sum += sum_decays(lds.decays[(c + 1) & 1], g, count(c + 1));
+      g = load_g(c + 2);
+    }
+    barrier_lds();
+  }
+  if (it.tile == 0 && lane == 0) a.sums[it.no * io.H + head] = sum;
 }
 
 // From the pieces' local final states to their initial states, in order, four entries per thread:
-// S_in(0) is the sequence's initial state, S_in(g + 1) = e^(sum of g) S_in(g) + S_local(g).
+// S_in(0) is the sequence's initial state, S_in(g + 1) = e^(sum of g) S_in(g) + S_local(g). Eight
+// pieces' states are read at once.
 template <int KD>
 __global__ __launch_bounds__(kChainThreads) void linear_chain_kernel(const LinearSeqs a,
                                                                       const wkv7_linear_io io) {
+  constexpr int U = 8;
   const int64_t size = int64_t(KD) * io.V;
   const int blocks = int(size / kChainElems);
   int64_t item = blockIdx.x;
@@ -495,27 +739,31 @@ __global__ __launch_bounds__(kChainThreads) void linear_chain_kernel(const Linea
   f32x4 run = {0.f, 0.f, 0.f, 0.f};
   if (!a.zero_init)
     run = *reinterpret_cast<const f32x4*>(a.state + (row * io.H + head) * size + e);
-  const int64_t first = beg / a.piece + s;
+  const int64_t first = beg / a.piece + s, step = io.H * size;
   float* p = a.pieces + (first * io.H + head) * size + e;
   const double* sums = a.sums + first * io.H + head;
-  f32x4 local = run;
-  if (n > 1) local = *reinterpret_cast<const f32x4*>(p);
-  for (int64_t g = 0; g < n; ++g) {
-    f32x4 ahead = run;
-    if (g + 2 < n) ahead = *reinterpret_cast<const f32x4*>(p + io.H * size);
-    *reinterpret_cast<f32x4*>(p) = run;
-    if (g + 1 < n) {
-      const double sum = sums[g * io.H];
-      const float f = exp2f(float(sum));
+  for (int64_t g0 = 0; g0 < n; g0 += U) {
+    f32x4 local[U];
+    double sum[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t g = min(g0 + u, n - 1);
+      const bool whole = g + 1 < n;  // (the last piece's are not computed)
+      local[u] = whole ? *reinterpret_cast<const f32x4*>(p + g * step) : run;
+      sum[u] = whole ? sums[g * io.H] : 0.;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (g0 + u >= n) break;
+      *reinterpret_cast<f32x4*>(p + (g0 + u) * step) = run;
+      const float f = exp2f(float(sum[u]));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         // an infinite entry stays so, however small the factor, unless a token forgot the state
-        const bool inf = fabsf(run[i]) == INFINITY && f == 0.f && sum > -1e4;
-        run[i] = inf ? run[i] + local[i] : fmaf(f, run[i], local[i]);
+        const bool inf = fabsf(run[i]) == INFINITY && f == 0.f && sum[u] > -1e4;
+        run[i] = inf ? run[i] + local[u][i] : fmaf(f, run[i], local[u][i]);
       }
     }
-    local = ahead;
-    p += io.H * size;
   }
 }
 

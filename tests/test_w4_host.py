@@ -30,7 +30,7 @@ def test_abi_refuses_weights(change, code):
     assert lib.wkv7_w4_quantize(d, P, 64, 0, None) == code
     assert lib.wkv7_w4_unpack(d, P, None) == code
     groups = (_lib.W4Group * 1)(_lib.W4Group(4096, d, None, 4096, 64, 48, 0, 0))
-    assert lib.wkv7_proj_w4(2, groups, 1, None) == code
+    assert lib.wkv7_proj_w4(2, groups, 1, None, 0, None) == code
 
 
 @pytest.mark.parametrize("change,code", [
@@ -41,18 +41,24 @@ def test_abi_refuses_products(change, code):
     for name, value in change.items():
         setattr(group, name, value)
     groups = (_lib.W4Group * 2)(_lib.W4Group(4096, _desc(), None, 4096, 64, 48, 0, 0), group)
-    assert _lib.load().wkv7_proj_w4(2, groups, 2, None) == code
+    assert _lib.load().wkv7_proj_w4(2, groups, 2, None, 0, None) == code
 
 
 def test_abi_refuses_calls():
     lib = _lib.load()
     groups = (_lib.W4Group * 9)(*[_lib.W4Group(4096, _desc(), None, 4096, 64, 48, 0, 0)] * 9)
-    assert lib.wkv7_proj_w4(-1, groups, 1, None) == A
-    assert lib.wkv7_proj_w4(1 << 31, groups, 1, None) == A
-    assert lib.wkv7_proj_w4(1, groups, 0, None) == A
-    assert lib.wkv7_proj_w4(1, groups, 9, None) == A
-    assert lib.wkv7_proj_w4(1, None, 1, None) == A
-    assert lib.wkv7_proj_w4(0, groups, 1, None) == OK
+    assert lib.wkv7_proj_w4(-1, groups, 1, None, 0, None) == A
+    assert lib.wkv7_proj_w4(1 << 31, groups, 1, None, 0, None) == A
+    assert lib.wkv7_proj_w4(1, groups, 0, None, 0, None) == A
+    assert lib.wkv7_proj_w4(1, groups, 9, None, 0, None) == A
+    assert lib.wkv7_proj_w4(1, None, 1, None, 0, None) == A
+    assert lib.wkv7_proj_w4(0, groups, 1, None, 0, None) == OK
+    assert lib.wkv7_proj_w4_workspace_bytes(64, groups, 8) == 0
+    need = lib.wkv7_proj_w4_workspace_bytes(65, groups, 2)
+    assert need == 2 * 65 * 3 * 16 * 2  # three bf16 parts of 16 groups' sums (two there)
+    assert lib.wkv7_proj_w4(65, groups, 2, None, need, None) == _lib.WKV7_ERR_WORKSPACE
+    assert lib.wkv7_proj_w4(65, groups, 2, P, need - 1, None) == _lib.WKV7_ERR_WORKSPACE
+    assert lib.wkv7_proj_w4(65, groups, 2, ctypes.c_void_p(4104), need, None) == S
     d = _desc()
     assert lib.wkv7_w4_pack(d, None, P, 0, None, None) == A
     assert lib.wkv7_w4_pack(d, P, None, 0, None, None) == A

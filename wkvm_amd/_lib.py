@@ -45,6 +45,7 @@ WKV7_ADAPTER_MAX_RANK = 256
 WKV7_SAMPLE_GROUP = 256
 WKV7_SAMPLE_MAX_VOCAB = 1 << 21
 WKV7_LINEAR_MAX_V = 1024
+WKV7_W4_FEW_ROWS = 64
 WKV7_SCALE_BF16 = 0
 WKV7_SCALE_F16 = 1
 
@@ -168,7 +169,8 @@ SIGNATURES = {
     "wkv7_w4_pack": (ctypes.c_int, [ctypes.POINTER(W4Desc), _vp, _vp, _i32, _vp, _vp]),
     "wkv7_w4_quantize": (ctypes.c_int, [ctypes.POINTER(W4Desc), _vp, _i64, _i32, _vp]),
     "wkv7_w4_unpack": (ctypes.c_int, [ctypes.POINTER(W4Desc), _vp, _vp]),
-    "wkv7_proj_w4": (ctypes.c_int, [_i64, ctypes.POINTER(W4Group), _i32, _vp]),
+    "wkv7_proj_w4": (ctypes.c_int, [_i64, ctypes.POINTER(W4Group), _i32, _vp, _sz, _vp]),
+    "wkv7_proj_w4_workspace_bytes": (_sz, [_i64, ctypes.POINTER(W4Group), _i32]),
 }
 
 _lib = None

@@ -2,7 +2,7 @@
 // a zero point for each row and group of inputs, and the kernels that lay such weights out.
 #include <algorithm>
 
-#include "wkv7_w4_core.h"
+#include "wkv7_w4_tile.h"
 
 using namespace wkv7;
 
@@ -134,6 +134,61 @@ int launch_thin(const W4Args& args, hipStream_t s) {
   return launch_status();
 }
 
+constexpr int64_t kThinRows = WKV7_W4_FEW_ROWS;
+
+// Workspace of the tile kernel: the sums of every product's x over its groups.
+size_t sums_bytes(int64_t m, const wkv7_w4_group& g) {
+  return size_t(m) * 3 * w4_padded_groups(g.w.k, g.w.group) * sizeof(uint16_t);
+}
+
+size_t workspace_bytes_of(int64_t m, const wkv7_w4_group* groups, int n) {
+  if (m <= kThinRows) return 0;
+  size_t bytes = 0;
+  for (int i = 0; i < n; ++i) bytes += sums_bytes(m, groups[i]);
+  return bytes;
+}
+
+template <int GM, int GN, int TM, int TN, int S, int KS>
+int launch_tiles(W4TileArgs& a, hipStream_t s) {
+  constexpr int BM = 32 * TM * GM, BN = 32 * TN * GN;
+  int64_t end = 0;
+  for (int i = 0; i < a.ngroups; ++i) {
+    end += (a.m + BM - 1) / BM * ((int64_t(a.g[i].w.n) + BN - 1) / BN);
+    if (end > int64_t(0x7ffffff0)) return WKV7_ERR_ARG;
+    a.tile_end[i] = int32_t(end);
+  }
+  a.span = int32_t((end + kW4Xcds - 1) / kW4Xcds);
+  w4_tile_kernel<GM, GN, TM, TN, S, KS><<<unsigned(a.span) * kW4Xcds, 64 * GM * GN, 0, s>>>(a);
+  return launch_status();
+}
+
+// The products of groups of 32 KS inputs: sums of x, then output tiles.
+template <int KS>
+int launch_tiled(int64_t m, const wkv7_w4_group* groups, int n, uint16_t*& ws, hipStream_t s) {
+  W4SumArgs sums{};
+  W4TileArgs tiles{};
+  sums.m = tiles.m = m;
+  int64_t waves = 0;
+  for (int i = 0; i < n; ++i) {
+    if (groups[i].w.group != 32 * KS) continue;
+    const int at = tiles.ngroups++;
+    const int padded = w4_padded_groups(groups[i].w.k, 32 * KS);
+    tiles.g[at] = groups[i];
+    tiles.sums[at] = sums.sums[at] = ws;
+    sums.x[at] = groups[i].x;
+    sums.ldx[at] = groups[i].ldx;
+    sums.k[at] = groups[i].w.k;
+    waves = std::max(waves, m * ((padded * 32 * KS + 511) / 512));
+    ws += sums_bytes(m, groups[i]) / sizeof(uint16_t);
+  }
+  if (tiles.ngroups == 0) return WKV7_OK;
+  if ((waves + 3) / 4 > int64_t(0x7fffffff)) return WKV7_ERR_ARG;
+  w4_sums_kernel<KS><<<dim3(unsigned((waves + 3) / 4), tiles.ngroups), 256, 0, s>>>(sums);
+  const int rc = launch_status();
+  if (rc != WKV7_OK) return rc;
+  return launch_tiles<1, 4, 2, 1, 3, KS>(tiles, s);
+}
+
 }  // namespace
 }  // namespace wkv7
 
@@ -177,11 +232,27 @@ extern "C" int wkv7_w4_unpack(const wkv7_w4_weight* weight, float* w, void* stre
   return launch_status();
 }
 
+extern "C" size_t wkv7_proj_w4_workspace_bytes(int64_t m, const wkv7_w4_group* groups,
+                                               int32_t ngroups) {
+  return validate(m, groups, ngroups) == WKV7_OK ? workspace_bytes_of(m, groups, ngroups) : 0;
+}
+
 extern "C" int wkv7_proj_w4(int64_t m, const wkv7_w4_group* groups, int32_t ngroups,
-                            void* stream) {
+                            void* workspace, size_t workspace_bytes, void* stream) {
   const int rc = validate(m, groups, ngroups);
   if (rc != WKV7_OK) return rc;
   if (m == 0) return WKV7_OK;
+  hipStream_t st = as_stream(stream);
+  if (m > kThinRows) {
+    if (!workspace || workspace_bytes < workspace_bytes_of(m, groups, ngroups))
+      return WKV7_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return WKV7_ERR_SHAPE;
+    uint16_t* ws = static_cast<uint16_t*>(workspace);
+    int done = launch_tiled<4>(m, groups, ngroups, ws, st);
+    if (done == WKV7_OK) done = launch_tiled<2>(m, groups, ngroups, ws, st);
+    if (done == WKV7_OK) done = launch_tiled<1>(m, groups, ngroups, ws, st);
+    return done;
+  }
   W4Args args{};
   args.m = m;
   args.ngroups = ngroups;
@@ -192,6 +263,6 @@ extern "C" int wkv7_proj_w4(int64_t m, const wkv7_w4_group* groups, int32_t ngro
     if (end > int64_t(0x7fffffff)) return WKV7_ERR_ARG;
     args.tile_end[i] = int32_t(end);
   }
-  if (m <= 16) return launch_thin<8, 1>(args, as_stream(stream));
-  return launch_thin<8, 4>(args, as_stream(stream));
+  if (m <= 16) return launch_thin<8, 1>(args, st);
+  return launch_thin<8, 4>(args, st);
 }

@@ -50,20 +50,23 @@ __device__ __forceinline__ float w4_activate(float v, int act) {
   return v;
 }
 
-// One output before bias and activation, as the formula is written: for a result that is not
-// finite. (With an infinite x the sums above are infinity less infinity, whatever the weights.)
-__device__ __noinline__ float w4_direct(const uint16_t* x, const uint32_t* codes,
-                                        const uint32_t* scales, int n, int k, int group) {
+// One output as the formula is written: for a result that is not finite. (With an infinite x the sums
+// above are infinity less infinity, whatever the weights.)
+__device__ __forceinline__ void w4_store_direct(const wkv7_w4_group& G, int64_t m, int n) {
+  const int k = G.w.k, group = G.w.group;
   const int blocks = (k + kW4K - 1) / kW4K, groups = (k + group - 1) / group;
   const int64_t tile = n / kW4N;
+  const uint16_t* x = G.x + m * G.ldx;
   float sum = 0.f;
+#pragma unroll 1
   for (int i = 0; i < k; ++i) {
     const int lane = (n & 15) + 16 * (i >> 3 & 3);
-    const uint32_t w = codes[((tile * blocks + i / kW4K) * 64 + lane) * 4 + (i >> 5 & 3)];
-    const uint32_t sc = scales[(tile * groups + i / group) * kW4N + (n & 15)];
+    const uint32_t w = G.w.codes[((tile * blocks + i / kW4K) * 64 + lane) * 4 + (i >> 5 & 3)];
+    const uint32_t sc = G.w.scales[(tile * groups + i / group) * kW4N + (n & 15)];
     sum = fmaf(bf16_to_f32(x[i]), w4_scale(sc) * float(w4_code(w, i & 7) - w4_zero(sc)), sum);
   }
-  return sum;
+  if (G.bias) sum += bf16_to_f32(G.bias[n]);
+  G.y[m * G.ldy + n] = f32_to_bf16(w4_activate(sum, G.act));
 }
 
 struct W4Args {
@@ -130,15 +133,18 @@ __global__ __launch_bounds__(64 * NW) void w4_thin_kernel(const W4Args args) {
     w4_f32x4 v = red[0][i][lane];
 #pragma unroll
     for (int w = 1; w < NW; ++w) v += red[w][i][lane];
+    const float bias = G.bias && n < G.w.n ? bf16_to_f32(G.bias[n]) : 0.f;
+    uint32_t again = 0;  // results that are not finite
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int64_t m = m0 + 16 * i + 4 * lg + e;
       if (m >= args.m || n >= G.w.n) continue;
-      float r = 16.f * v[e];
-      if (!(fabsf(r) < INFINITY)) r = w4_direct(G.x + m * G.ldx, G.w.codes, G.w.scales, n, k, G.w.group);
-      if (G.bias) r += bf16_to_f32(G.bias[n]);
-      G.y[m * G.ldy + n] = f32_to_bf16(w4_activate(r, G.act));
+      const float r = 16.f * v[e];
+      G.y[m * G.ldy + n] = f32_to_bf16(w4_activate(r + bias, G.act));
+      if (!(fabsf(r) < INFINITY)) again |= 1u << e;
     }
+    for (; again; again &= again - 1)
+      w4_store_direct(G, m0 + 16 * i + 4 * lg + __builtin_ctz(again), n);
   }
 }
 

@@ -1,0 +1,317 @@
+// Products with 4-bit weights for more rows than one tile (wkv7_proj_w4): output tiles on
+// v_mfma_f32_32x32x16_bf16.
+//
+// Lane l, c = l % 32, h = l / 32, of that instruction holds row or column c at 8 h .. 8 h + 7 of 16
+// inputs, its result lane D[8 (i / 4) + 4 h + i % 4][c]. A workgroup of GM x GN waves has a tile of
+// 32 TM GM rows by 32 TN GN columns and walks k in blocks of 128, each of them a stage of an LDS ring
+// that direct loads fill S - 1 stages ahead: x rows (256 bytes, 16-byte chunks swizzled by row), codes
+// and scale words as they lie in memory. Codes become operands in registers (wkv7_w4_core.h), once per
+// wave and column; a group's sum gets its scale by 16 fused multiply-adds per tile. The zero points'
+// part, sum over groups of -s (1 + z / 16) X with X the sums of x, is a product of its own with one
+// input per group, in front: X comes from w4_sums_kernel, both factors as three bf16 parts.
+#pragma once
+
+#include "wkv7_w4_core.h"
+
+namespace wkv7 {
+namespace {
+
+typedef float w4_f32x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) uint4 w4_lds_u4;
+
+constexpr int kW4Xcds = 8;
+
+struct W4TileArgs {
+  wkv7_w4_group g[WKV7_PROJ_MAX_GROUPS];
+  int32_t tile_end[WKV7_PROJ_MAX_GROUPS];  // exclusive prefix sums of work items
+  const uint16_t* sums[WKV7_PROJ_MAX_GROUPS];  // [m][3][groups, a multiple of 16] parts of X
+  int64_t m;
+  int32_t ngroups;
+  int32_t span;  // work items per XCD
+};
+
+struct W4SumArgs {
+  const uint16_t* x[WKV7_PROJ_MAX_GROUPS];
+  uint16_t* sums[WKV7_PROJ_MAX_GROUPS];
+  int64_t ldx[WKV7_PROJ_MAX_GROUPS];
+  int32_t k[WKV7_PROJ_MAX_GROUPS];
+  int64_t m;
+};
+
+__host__ __device__ constexpr int w4_padded_groups(int k, int group) {
+  return ((k + group - 1) / group + 15) / 16 * 16;
+}
+
+__device__ __forceinline__ void w4_split3(float v, uint16_t (&p)[3]) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    p[i] = f32_to_bf16(v);
+    v -= bf16_to_f32(p[i]);
+  }
+}
+
+// Sums of x over its groups: a wave takes 512 inputs of a row, eight to a lane.
+template <int KS>
+__global__ __launch_bounds__(256) void w4_sums_kernel(const W4SumArgs a) {
+  constexpr int kLanes = 4 * KS;  // lanes of a group
+  const int g = blockIdx.y;
+  const int lane = threadIdx.x & 63;
+  const int k = a.k[g], padded = w4_padded_groups(k, 32 * KS);
+  const int parts = (padded * 32 * KS + 511) / 512;  // waves of a row
+  const int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t row = item / parts;
+  if (row >= a.m) return;
+  const int i0 = int(item % parts) * 512 + 8 * lane;
+  float s = 0.f;
+  if (i0 < k) {
+    const uint4 v = *reinterpret_cast<const uint4*>(a.x[g] + row * a.ldx[g] + i0);
+    s = ((bf16_lo(v.x) + bf16_hi(v.x)) + (bf16_lo(v.y) + bf16_hi(v.y))) +
+        ((bf16_lo(v.z) + bf16_hi(v.z)) + (bf16_lo(v.w) + bf16_hi(v.w)));
+  }
+#pragma unroll
+  for (int d = 1; d < kLanes; d *= 2) s += __shfl_xor(s, d);
+  const int gi = i0 / (32 * KS);
+  if (lane % kLanes || gi >= padded) return;
+  uint16_t p[3];
+  w4_split3(s, p);
+#pragma unroll
+  for (int i = 0; i < 3; ++i) a.sums[g][(row * 3 + i) * padded + gi] = p[i];
+}
+
+__device__ __forceinline__ w4_f32x16 w4_mma32(const uint4& a, const uint4& b, w4_f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(w4_bf16x8, a),
+                                                 __builtin_bit_cast(w4_bf16x8, b), c, 0, 0, 0);
+}
+
+// Direct loads, lane l's 16 (4) bytes to lds + 16 l (4 l); waited for by w4_barrier alone.
+__device__ __forceinline__ void w4_lds16(const void* src, uint32_t lds) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "{m0}"(lds), "v"(src) : "memory");
+}
+__device__ __forceinline__ void w4_lds4(const void* src, uint32_t lds) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, off" : : "{m0}"(lds), "v"(src) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void w4_barrier() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
+}
+
+// KS: groups of 32 KS inputs.
+template <int GM, int GN, int TM, int TN, int S, int KS>
+__global__ __launch_bounds__(64 * GM * GN, 2) void w4_tile_kernel(const W4TileArgs args) {
+  constexpr int NW = GM * GN, BM = 32 * TM * GM, BN = 32 * TN * GN;
+  constexpr int NG = 4 / KS;                   // groups of a block
+  constexpr int XL = BM * 256 / 1024 / NW;     // direct loads of a wave and stage: x rows,
+  constexpr int CL = BN / 16 / NW;             // codes,
+  constexpr int SL = (BN * NG + 64 * NW - 1) / (64 * NW);  // scale words
+  constexpr int L = XL + CL + SL;
+  static_assert(BM % (4 * NW) == 0 && BN % (16 * NW) == 0 && BN % 64 == 0, "tile shape");
+  struct Stage {
+    uint4 x[BM * 16];
+    uint4 codes[BN * 4];
+    uint32_t scales[NG * BN];
+  };
+  __shared__ Stage ring[S];
+
+  const int bid = int(blockIdx.x % kW4Xcds) * args.span + int(blockIdx.x / kW4Xcds);
+  int g = 0;
+  while (g + 1 < args.ngroups && bid >= args.tile_end[g]) ++g;
+  if (bid >= args.tile_end[g]) return;
+  const wkv7_w4_group& G = args.g[g];
+  const int item = bid - (g ? args.tile_end[g - 1] : 0);
+  const int N = G.w.n, K = G.w.k;
+  const int tiles_n = (N + BN - 1) / BN;
+  const int64_t m0 = int64_t(item / tiles_n) * BM, M = args.m;
+  const int n0 = item % tiles_n * BN;
+  const int blocks = (K + kW4K - 1) / kW4K, groups = (K + 32 * KS - 1) / (32 * KS);
+  const int ntiles = (N + 15) / 16;
+
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave % GM, wn = wave / GM;
+
+  // Sources of the direct loads. x: load i fills rows 4 (NW i + wave) .. + 3 of a stage, lane l chunk
+  // l % 16 of row l / 16, which holds logical chunk (l % 16) ^ swizzle(row). Rows past m and columns past
+  // n load valid ones and are not stored.
+  const uint16_t* xsrc[XL];
+  int xk[XL];
+#pragma unroll
+  for (int i = 0; i < XL; ++i) {
+    const int r = 4 * (NW * i + wave) + lane / 16;
+    xk[i] = 8 * ((lane & 15) ^ (r & 15));
+    xsrc[i] = G.x + min(m0 + r, M - 1) * G.ldx;
+  }
+  auto issue = [&](int kb, int slot) {
+    Stage& st = ring[slot];
+    const uint32_t xl = uint32_t(reinterpret_cast<uintptr_t>((w4_lds_u4*)st.x));
+    const uint32_t cl = uint32_t(reinterpret_cast<uintptr_t>((w4_lds_u4*)st.codes));
+#pragma unroll
+    for (int i = 0; i < XL; ++i)  // (chunks past k read the row's last one again)
+      w4_lds16(xsrc[i] + min(kb * kW4K + xk[i], K - 8), xl + 1024 * (NW * i + wave));
+#pragma unroll
+    for (int i = 0; i < CL; ++i) {
+      const int t = NW * i + wave;
+      const int64_t tile = min(n0 / 16 + t, ntiles - 1);
+      w4_lds16(reinterpret_cast<const uint4*>(G.w.codes) + (tile * blocks + kb) * 64 + lane,
+               cl + 1024 * t);
+    }
+#pragma unroll
+    for (int i = 0; i < SL; ++i) {  // (where there are fewer words than lanes, some twice)
+      const int at = (NW * i + wave) * 64 % (NG * BN);
+      const int gi = min(kb * NG + at / BN, groups - 1);
+      const int64_t tile = min((n0 + at % BN) / 16 + lane / 16, ntiles - 1);
+      w4_lds4(G.w.scales + (tile * groups + gi) * kW4N + (lane & 15),
+              cl + BN * 64 + 4 * at);
+    }
+  };
+
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s)
+    if (s < blocks) issue(s, s);
+
+  // The zero points' part.
+  w4_f32x16 total[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) total[i][j] = w4_f32x16{};
+  {
+    const int padded = w4_padded_groups(K, 32 * KS);
+    for (int g0 = 0; g0 < padded; g0 += 16) {
+      uint4 xs[TM][3], zs[TN][3];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const int64_t r = min(m0 + 32 * (TM * wm + i) + c, M - 1);
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+          xs[i][p] = *reinterpret_cast<const uint4*>(args.sums[g] + (r * 3 + p) * padded + g0 + 8 * h);
+      }
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int64_t tile = min((n0 + 32 * (TN * wn + j)) / 16 + c / 16, ntiles - 1);
+        uint16_t parts[8][3];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int gi = g0 + 8 * h + e;
+          const uint32_t word = gi < groups ? G.w.scales[(tile * groups + gi) * kW4N + (c & 15)] : 0u;
+          w4_split3(w4_scale(word) * w4_minus_zero(word), parts[e]);
+        }
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+          zs[j][p] = make_uint4(parts[0][p] | uint32_t(parts[1][p]) << 16,
+                                parts[2][p] | uint32_t(parts[3][p]) << 16,
+                                parts[4][p] | uint32_t(parts[5][p]) << 16,
+                                parts[6][p] | uint32_t(parts[7][p]) << 16);
+      }
+#pragma unroll
+      for (int sum = 2; sum >= 0; --sum)  // the small products first
+#pragma unroll
+        for (int p = 0; p <= sum; ++p)
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+              total[i][j] = w4_mma32(xs[i][p], zs[j][sum - p], total[i][j]);
+    }
+  }
+
+  for (int kb = 0; kb < blocks; ++kb) {
+    // stage kb has landed, and every wave is done with stage kb - 1, whose slot the next loads take
+    if (kb + S - 2 < blocks) w4_barrier<(S - 2) * L>();
+    else w4_barrier<0>();
+    if (kb + S - 1 < blocks) issue(kb + S - 1, (kb + S - 1) % S);
+    const Stage& st = ring[kb % S];
+    uint4 cw[TN][2];  // words j of inputs 32 j + 8 h .. and 32 j + 16 + 8 h ..
+    float sc[TN][NG];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int col = 32 * (TN * wn + j) + c;
+      cw[j][0] = st.codes[(col / 16) * 64 + (col & 15) + 16 * h];
+      cw[j][1] = st.codes[(col / 16) * 64 + (col & 15) + 16 * (2 + h)];
+#pragma unroll
+      for (int q = 0; q < NG; ++q) sc[j][q] = w4_scale(st.scales[q * BN + col]);
+    }
+    const int steps = min(4, (K - kb * kW4K) / 32);  // of 32 inputs
+    w4_f32x16 acc[TM][TN];
+    auto step = [&](int q) {  // 32 inputs: word q
+      uint4 xf[2][TM];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          const int r = 32 * (TM * wm + i) + c;
+          xf[u][i] = st.x[r * 16 + ((4 * q + 2 * u + h) ^ (r & 15))];
+        }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const uint4& w4 = cw[j][u];
+          const uint4 wf = w4_expand(q == 0 ? w4.x : q == 1 ? w4.y : q == 2 ? w4.z : w4.w);
+#pragma unroll
+          for (int i = 0; i < TM; ++i) {
+            const bool first = u == 0 && q % KS == 0;
+            acc[i][j] = w4_mma32(xf[u][i], wf, first ? w4_f32x16{} : acc[i][j]);
+          }
+        }
+    };
+    auto flush = [&](int q) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            total[i][j][e] = fmaf(sc[j][q / KS], acc[i][j][e], total[i][j][e]);
+    };
+    if (steps == 4) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        step(q);
+        if ((q + 1) % KS == 0) flush(q);
+      }
+    } else {  // the last block of a k that is no multiple of 128
+#pragma unroll
+      for (int q = 0; q < 3; ++q) {
+        if (q >= steps) break;
+        step(q);
+        if ((q + 1) % KS == 0 || q + 1 == steps) flush(q);
+      }
+    }
+  }
+
+  // Outputs; those that are not finite once more, as the formula is written.
+  uint32_t again[TM][TN];
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const int n = n0 + 32 * (TN * wn + j) + c;
+    const float bias = G.bias && n < N ? bf16_to_f32(G.bias[n]) : 0.f;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      again[i][j] = 0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int64_t m = m0 + 32 * (TM * wm + i) + 8 * (e / 4) + 4 * h + e % 4;
+        const float v = 16.f * total[i][j][e];
+        if (m < M && n < N) {
+          G.y[m * G.ldy + n] = f32_to_bf16(w4_activate(v + bias, G.act));
+          if (!(fabsf(v) < INFINITY)) again[i][j] |= 1u << e;
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+      while (again[i][j]) {
+        const int e = __builtin_ctz(again[i][j]);
+        again[i][j] &= again[i][j] - 1;
+        const int n = n0 + 32 * (TN * wn + j) + c;
+        const int64_t m = m0 + 32 * (TM * wm + i) + 8 * (e / 4) + 4 * h + e % 4;
+        w4_store_direct(G, m, n);
+      }
+}
+
+}  // namespace
+}  // namespace wkv7

@@ -30,11 +30,19 @@ __device__ __forceinline__ uint32_t w4_rotr(uint32_t w, int by) {
 }
 __device__ __forceinline__ int w4_code(uint32_t w, int e) { return int(w4_rotr(w, w4_bit(e)) & 15u); }
 
+// The constants of w4_expand in registers: as literals, of which an instruction holds one, each
+// pair of codes would take an and and an or.
+struct W4Bits {
+  uint32_t mask, one;
+  __device__ __forceinline__ W4Bits() {
+    asm volatile("v_mov_b32 %0, 0x780078\n\tv_mov_b32 %1, 0x3f803f80" : "=&v"(mask), "=v"(one));
+  }
+};
+
 // eight codes as the bf16 numbers 1 + c / 16
-__device__ __forceinline__ uint4 w4_expand(uint32_t w) {
-  constexpr uint32_t mask = 0x00780078u, one = 0x3f803f80u;
-  return make_uint4((w & mask) | one, ((w >> 4) & mask) | one, ((w >> 8) & mask) | one,
-                    (__builtin_amdgcn_alignbit(w, w, 12) & mask) | one);
+__device__ __forceinline__ uint4 w4_expand(uint32_t w, const W4Bits& k) {
+  return make_uint4((w & k.mask) | k.one, ((w >> 4) & k.mask) | k.one, ((w >> 8) & k.mask) | k.one,
+                    (__builtin_amdgcn_alignbit(w, w, 12) & k.mask) | k.one);
 }
 
 __device__ __forceinline__ float w4_scale(uint32_t word) { return __uint_as_float(word & ~15u); }
@@ -96,6 +104,7 @@ __global__ __launch_bounds__(64 * NW) void w4_thin_kernel(const W4Args args) {
 #pragma unroll
   for (int i = 0; i < TM; ++i) x[i] = G.x + min(m0 + 16 * i + li, args.m - 1) * G.ldx + 8 * lg;
 
+  const W4Bits bits;
   const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
   w4_f32x4 total[TM], acc[TM], sum[TM];
 #pragma unroll
@@ -107,7 +116,7 @@ __global__ __launch_bounds__(64 * NW) void w4_thin_kernel(const W4Args args) {
     for (int j = 0; j < 4; ++j) {
       const int step = 4 * b + j;
       if (32 * step >= k) break;  // (uniform)
-      const uint4 w = w4_expand(words[j]);
+      const uint4 w = w4_expand(words[j], bits);
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
         const uint4 xf = *reinterpret_cast<const uint4*>(x[i] + 32 * step);

@@ -11,6 +11,8 @@
 // input per group, in front: X comes from w4_sums_kernel, both factors as three bf16 parts.
 #pragma once
 
+#include <type_traits>
+
 #include "wkv7_w4_core.h"
 
 namespace wkv7 {
@@ -215,7 +217,10 @@ __global__ __launch_bounds__(64 * GM * GN, 2) void w4_tile_kernel(const W4TileAr
     }
   }
 
-  for (int kb = 0; kb < blocks; ++kb) {
+  const W4Bits bits;
+  // One stage, `steps` (at most 4) times 32 inputs of it.
+  auto stage = [&](int kb, auto whole, int steps) {
+    constexpr bool kWhole = decltype(whole)::value;
     // stage kb has landed, and every wave is done with stage kb - 1, whose slot the next loads take
     if (kb + S - 2 < blocks) w4_barrier<(S - 2) * L>();
     else w4_barrier<0>();
@@ -231,31 +236,34 @@ __global__ __launch_bounds__(64 * GM * GN, 2) void w4_tile_kernel(const W4TileAr
 #pragma unroll
       for (int q = 0; q < NG; ++q) sc[j][q] = w4_scale(st.scales[q * BN + col]);
     }
-    const int steps = min(4, (K - kb * kW4K) / 32);  // of 32 inputs
     w4_f32x16 acc[TM][TN];
-    auto step = [&](int q) {  // 32 inputs: word q
-      uint4 xf[2][TM];
+    uint4 xf[2][2][TM];  // of this step and of the next
+    auto fetch = [&](int q) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
           const int r = 32 * (TM * wm + i) + c;
-          xf[u][i] = st.x[r * 16 + ((4 * q + 2 * u + h) ^ (r & 15))];
+          xf[q & 1][u][i] = st.x[r * 16 + ((4 * q + 2 * u + h) ^ (r & 15))];
         }
+    };
+    fetch(0);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {  // 32 inputs: word q
+      if (!kWhole && q >= steps) break;
+      if (q < 3) fetch(q + 1);
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
           const uint4& w4 = cw[j][u];
-          const uint4 wf = w4_expand(q == 0 ? w4.x : q == 1 ? w4.y : q == 2 ? w4.z : w4.w);
+          const uint4 wf = w4_expand(q == 0 ? w4.x : q == 1 ? w4.y : q == 2 ? w4.z : w4.w, bits);
 #pragma unroll
-          for (int i = 0; i < TM; ++i) {
-            const bool first = u == 0 && q % KS == 0;
-            acc[i][j] = w4_mma32(xf[u][i], wf, first ? w4_f32x16{} : acc[i][j]);
-          }
+          for (int i = 0; i < TM; ++i)
+            acc[i][j] = w4_mma32(xf[q & 1][u][i], wf,
+                                 u == 0 && q % KS == 0 ? w4_f32x16{} : acc[i][j]);
         }
-    };
-    auto flush = [&](int q) {
+      if ((q + 1) % KS && (kWhole || q + 1 < steps)) continue;  // inside a group
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -263,22 +271,10 @@ __global__ __launch_bounds__(64 * GM * GN, 2) void w4_tile_kernel(const W4TileAr
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             total[i][j][e] = fmaf(sc[j][q / KS], acc[i][j][e], total[i][j][e]);
-    };
-    if (steps == 4) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        step(q);
-        if ((q + 1) % KS == 0) flush(q);
-      }
-    } else {  // the last block of a k that is no multiple of 128
-#pragma unroll
-      for (int q = 0; q < 3; ++q) {
-        if (q >= steps) break;
-        step(q);
-        if ((q + 1) % KS == 0 || q + 1 == steps) flush(q);
-      }
     }
-  }
+  };
+  for (int kb = 0; kb < K / kW4K; ++kb) stage(kb, std::true_type{}, 4);
+  if (K % kW4K) stage(K / kW4K, std::false_type{}, K % kW4K / 32);
 
   // Outputs; those that are not finite once more, as the formula is written.
   uint32_t again[TM][TN];

@@ -125,13 +125,47 @@ int fill(const wkv7_w4_weight& w, const W4Source& src, void* stream) {
   return launch_status();
 }
 
-template <int NW, int TM>
-int launch_thin(const W4Args& args, hipStream_t s) {
-  const int64_t rows = (args.m + 16 * TM - 1) / (16 * TM);
-  if (rows > 65535) return WKV7_ERR_ARG;
-  const dim3 grid(unsigned(args.tile_end[args.ngroups - 1]), unsigned(rows));
-  w4_thin_kernel<NW, TM><<<grid, 64 * NW, 0, s>>>(args);
+// Workgroups of the products: one per column tile, or as many as the device holds at once
+// (`slots`), dealt by their tiles.
+int64_t deal(W4Args& a, int columns, int64_t slots) {
+  int64_t tiles = 0;
+  for (int i = 0; i < a.ngroups; ++i) tiles += (int64_t(a.g[i].w.n) + columns - 1) / columns;
+  int64_t end = 0;
+  for (int i = 0; i < a.ngroups; ++i) {
+    const int64_t own = (int64_t(a.g[i].w.n) + columns - 1) / columns;
+    end += tiles <= slots ? own : std::max<int64_t>(1, own * slots / tiles);
+    a.wg_end[i] = int32_t(std::min<int64_t>(end, 0x7fffffff));
+  }
+  return end;
+}
+
+template <int KS>
+int launch_thin(int64_t m, const wkv7_w4_group* groups, int n, int cus, hipStream_t s) {
+  W4Args a{};
+  a.m = m;
+  int blocks = 0;
+  for (int i = 0; i < n; ++i) {
+    if (groups[i].w.group != 32 * KS) continue;
+    a.g[a.ngroups++] = groups[i];
+    blocks = std::max(blocks, (groups[i].w.k + kW4K - 1) / kW4K);
+  }
+  if (a.ngroups == 0) return WKV7_OK;
+  // a unit holds two workgroups of 8 waves or one of 16
+  const bool wide = blocks > 16;
+  const int64_t wgs = deal(a, kW4N, (wide ? 1 : 2) * int64_t(cus));
+  if (wgs > int64_t(0x7fffffff)) return WKV7_ERR_ARG;
+  if (wide) w4_thin_kernel<16, 2, KS><<<unsigned(wgs), 1024, 0, s>>>(a);
+  else if (blocks > 8) w4_thin_kernel<8, 2, KS><<<unsigned(wgs), 512, 0, s>>>(a);
+  else w4_thin_kernel<8, 1, KS><<<unsigned(wgs), 512, 0, s>>>(a);
   return launch_status();
+}
+
+int device_cus(int* cus) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess ||
+      hipDeviceGetAttribute(cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
+    return launch_status();
+  return WKV7_OK;
 }
 
 constexpr int64_t kThinRows = WKV7_W4_FEW_ROWS;
@@ -253,16 +287,10 @@ extern "C" int wkv7_proj_w4(int64_t m, const wkv7_w4_group* groups, int32_t ngro
     if (done == WKV7_OK) done = launch_tiled<1>(m, groups, ngroups, ws, st);
     return done;
   }
-  W4Args args{};
-  args.m = m;
-  args.ngroups = ngroups;
-  int64_t end = 0;
-  for (int i = 0; i < ngroups; ++i) {
-    args.g[i] = groups[i];
-    end += (int64_t(groups[i].w.n) + kW4N - 1) / kW4N;
-    if (end > int64_t(0x7fffffff)) return WKV7_ERR_ARG;
-    args.tile_end[i] = int32_t(end);
-  }
-  if (m <= 16) return launch_thin<8, 1>(args, st);
-  return launch_thin<8, 4>(args, st);
+  int cus = 0;
+  int done = device_cus(&cus);
+  if (done == WKV7_OK) done = launch_thin<4>(m, groups, ngroups, cus, st);
+  if (done == WKV7_OK) done = launch_thin<2>(m, groups, ngroups, cus, st);
+  if (done == WKV7_OK) done = launch_thin<1>(m, groups, ngroups, cus, st);
+  return done;
 }

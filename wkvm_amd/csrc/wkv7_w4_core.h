@@ -79,81 +79,124 @@ __device__ __forceinline__ void w4_store_direct(const wkv7_w4_group& G, int64_t 
 
 struct W4Args {
   wkv7_w4_group g[WKV7_PROJ_MAX_GROUPS];
-  int32_t tile_end[WKV7_PROJ_MAX_GROUPS];  // exclusive prefix sums of column tiles
+  int32_t wg_end[WKV7_PROJ_MAX_GROUPS];  // exclusive prefix sums of workgroups
   int64_t m;
   int32_t ngroups;
 };
 
-// 16 TM rows by 16 columns: the blocks of 128 inputs are dealt to the NW waves, their sums joined in
-// LDS. Operands come from memory straight to registers.
-template <int NW, int TM>
-__global__ __launch_bounds__(64 * NW) void w4_thin_kernel(const W4Args args) {
-  __shared__ w4_f32x4 red[NW][TM][64];
+// The product that workgroup `at` works on, its number there and how many others do.
+__device__ __forceinline__ int w4_product(const W4Args& args, int at, int& first, int& count) {
+  int g = 0;
+  while (g + 1 < args.ngroups && at >= args.wg_end[g]) ++g;
+  first = at - (g ? args.wg_end[g - 1] : 0);
+  count = args.wg_end[g] - (g ? args.wg_end[g - 1] : 0);
+  return g;
+}
+
+// Up to 16 rows: a workgroup walks column tiles of 16, the blocks of 128 inputs of each dealt to its NW
+// waves, U of them to a wave at once, their sums joined in LDS. Everything comes from memory straight
+// to registers: codes and scales of the next tile while this one is multiplied, x (and its sums over
+// the groups of 32 KS inputs) once where a wave's blocks are the same for every tile.
+template <int NW, int U, int KS>
+__global__ __launch_bounds__(64 * NW, 4) void w4_thin_kernel(const W4Args args) {
+  constexpr int NG = 4 / KS;  // groups of a block
+  __shared__ w4_f32x4 red[2][NW][64];
   const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int g = 0;
-  while (g + 1 < args.ngroups && int(blockIdx.x) >= args.tile_end[g]) ++g;
-  const wkv7_w4_group& G = args.g[g];
-  const int64_t tile = int(blockIdx.x) - (g ? args.tile_end[g - 1] : 0);
-  const int64_t m0 = int64_t(blockIdx.y) * (16 * TM);
-  const int k = G.w.k, blocks = (k + kW4K - 1) / kW4K, groups = (k + G.w.group - 1) / G.w.group;
-  const int steps = G.w.group / 32;  // of 32 inputs in a group: 1, 2 or 4
-  const uint4* codes = reinterpret_cast<const uint4*>(G.w.codes) + tile * blocks * 64 + lane;
-  const uint32_t* scales = G.w.scales + tile * groups * kW4N + li;
-  const uint16_t* x[TM];
-#pragma unroll
-  for (int i = 0; i < TM; ++i) x[i] = G.x + min(m0 + 16 * i + li, args.m - 1) * G.ldx + 8 * lg;
+  int first, count;
+  const wkv7_w4_group& G = args.g[w4_product(args, blockIdx.x, first, count)];
+  const int k = G.w.k, blocks = (k + kW4K - 1) / kW4K, groups = (k + 32 * KS - 1) / (32 * KS);
+  const int tiles = (G.w.n + kW4N - 1) / kW4N;
+  const int passes = (blocks + NW * U - 1) / (NW * U);
+  const uint4* codes = reinterpret_cast<const uint4*>(G.w.codes) + lane;
+  const uint32_t* scales = G.w.scales + li;
+  const uint16_t* x = G.x + min(int64_t(li), args.m - 1) * G.ldx + 8 * lg;
 
   const W4Bits bits;
   const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
-  w4_f32x4 total[TM], acc[TM], sum[TM];
+  uint4 c[U], xf[U][4];
+  uint32_t sc[U][NG];
+  w4_f32x4 sums[U][NG];
+  // (what lies past k is read from inside it and multiplied by zeros)
+  auto fetch = [&](int tile, int pass) {
 #pragma unroll
-  for (int i = 0; i < TM; ++i) total[i] = acc[i] = sum[i] = w4_f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int b = wave; b < blocks; b += NW) {
-    const uint4 c = codes[int64_t(b) * 64];
-    const uint32_t words[4] = {c.x, c.y, c.z, c.w};
+    for (int u = 0; u < U; ++u) {
+      const int b = min(wave + NW * (pass * U + u), blocks - 1);
+      c[u] = codes[(int64_t(tile) * blocks + b) * 64];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int step = 4 * b + j;
-      if (32 * step >= k) break;  // (uniform)
-      const uint4 w = w4_expand(words[j], bits);
+      for (int q = 0; q < NG; ++q)
+        sc[u][q] = scales[(int64_t(tile) * groups + min(b * NG + q, groups - 1)) * kW4N];
+    }
+  };
+  auto load_x = [&](int pass) {
 #pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        const uint4 xf = *reinterpret_cast<const uint4*>(x[i] + 32 * step);
-        acc[i] = w4_mma(xf, w, acc[i]);
-        sum[i] = w4_mma(xf, ones, sum[i]);
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = kW4K * (wave + NW * (pass * U + u)) + 32 * j;
+        xf[u][j] = make_uint4(0, 0, 0, 0);
+        if (at < k && li < args.m) xf[u][j] = *reinterpret_cast<const uint4*>(x + at);
       }
-      if ((j + 1) % steps && 32 * (step + 1) < k) continue;  // (uniform) inside a group
-      const uint32_t word = scales[step / steps * kW4N];
-      const float s = w4_scale(word), z = w4_minus_zero(word);
 #pragma unroll
-      for (int i = 0; i < TM; ++i) {
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) total[i][e] = fmaf(s, fmaf(z, sum[i][e], acc[i][e]), total[i][e]);
-        acc[i] = sum[i] = w4_f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int q = 0; q < NG; ++q) {
+        sums[u][q] = w4_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < KS; ++j) sums[u][q] = w4_mma(xf[u][q * KS + j], ones, sums[u][q]);
+      }
+  };
+  fetch(first, 0);
+  if (passes == 1) load_x(0);
+  int turn = 0;
+  for (int tile = first; tile < tiles; tile += count, ++turn) {
+    w4_f32x4 total = {0.f, 0.f, 0.f, 0.f};
+    for (int pass = 0; pass < passes; ++pass) {
+      if (passes > 1) load_x(pass);
+      uint4 c0[U];
+      uint32_t sc0[U][NG];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        c0[u] = c[u];
+#pragma unroll
+        for (int q = 0; q < NG; ++q) sc0[u][q] = sc[u][q];
+      }
+      if (pass + 1 < passes) fetch(tile, pass + 1);
+      else if (tile + count < tiles) fetch(tile + count, 0);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t words[4] = {c0[u].x, c0[u].y, c0[u].z, c0[u].w};
+#pragma unroll
+        for (int q = 0; q < NG; ++q) {
+          w4_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < KS; ++j)
+            acc = w4_mma(xf[u][q * KS + j], w4_expand(words[q * KS + j], bits), acc);
+          const float s = w4_scale(sc0[u][q]), z = w4_minus_zero(sc0[u][q]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            total[e] = fmaf(s, fmaf(z, sums[u][q][e], acc[e]), total[e]);
+        }
       }
     }
-  }
+    red[turn & 1][wave][lane] = total;
+    __syncthreads();
+    if (wave != turn % NW) continue;  // the waves take turns to join the sums
+    w4_f32x4 v = red[turn & 1][0][lane];
 #pragma unroll
-  for (int i = 0; i < TM; ++i) red[wave][i][lane] = total[i];
-  __syncthreads();
-  const int n = int(tile) * kW4N + li;
-  for (int i = wave; i < TM; i += NW) {
-    w4_f32x4 v = red[0][i][lane];
-#pragma unroll
-    for (int w = 1; w < NW; ++w) v += red[w][i][lane];
-    const float bias = G.bias && n < G.w.n ? bf16_to_f32(G.bias[n]) : 0.f;
-    uint32_t again = 0;  // results that are not finite
-#pragma unroll
+    for (int w = 1; w < NW; ++w) v += red[turn & 1][w][lane];
+    const int n = tile * kW4N + li;
+    if (n >= G.w.n) continue;
+    const float bias = G.bias ? bf16_to_f32(G.bias[n]) : 0.f;
+#pragma unroll 1
     for (int e = 0; e < 4; ++e) {
-      const int64_t m = m0 + 16 * i + 4 * lg + e;
-      if (m >= args.m || n >= G.w.n) continue;
-      const float r = 16.f * v[e];
-      G.y[m * G.ldy + n] = f32_to_bf16(w4_activate(r + bias, G.act));
-      if (!(fabsf(r) < INFINITY)) again |= 1u << e;
+      const int m = 4 * lg + e;
+      if (m >= args.m) break;
+      const float r = fmaf(16.f, v[0], bias);
+      v = w4_f32x4{v[1], v[2], v[3], 0.f};
+      if (fabsf(r) < INFINITY) G.y[m * G.ldy + n] = f32_to_bf16(w4_activate(r, G.act));
+      else w4_store_direct(G, m, n);
     }
-    for (; again; again &= again - 1)
-      w4_store_direct(G, m0 + 16 * i + 4 * lg + __builtin_ctz(again), n);
   }
 }
 

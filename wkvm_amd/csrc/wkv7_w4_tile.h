@@ -85,6 +85,16 @@ __device__ __forceinline__ w4_f32x16 w4_mma32(const uint4& a, const uint4& b, w4
                                                  __builtin_bit_cast(w4_bf16x8, b), c, 0, 0, 0);
 }
 
+__device__ __forceinline__ void w4_activate_all(w4_f32x16& v, int act) {
+  if (act == WKV7_ACT_TANH) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = w4_activate(v[e], WKV7_ACT_TANH);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = w4_activate(v[e], WKV7_ACT_SIGMOID);
+  }
+}
+
 // Direct loads, lane l's 16 (4) bytes to lds + 16 l (4 l); waited for by w4_barrier alone.
 __device__ __forceinline__ void w4_lds16(const void* src, uint32_t lds) {
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "{m0}"(lds), "v"(src) : "memory");
@@ -236,76 +246,111 @@ __global__ __launch_bounds__(64 * GM * GN, 2) void w4_tile_kernel(const W4TileAr
 #pragma unroll
       for (int q = 0; q < NG; ++q) sc[j][q] = w4_scale(st.scales[q * BN + col]);
     }
-    w4_f32x16 acc[TM][TN];
-    uint4 xf[2][2][TM];  // of this step and of the next
-    auto fetch = [&](int q) {
+    uint4 wf[TN][8];  // the operands of 16 inputs each
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+    for (int j = 0; j < TN; ++j)
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          const int r = 32 * (TM * wm + i) + c;
-          xf[q & 1][u][i] = st.x[r * 16 + ((4 * q + 2 * u + h) ^ (r & 15))];
-        }
+      for (int q = 0; q < 8; ++q) {
+        const uint4& w4 = cw[j][q & 1];
+        wf[j][q] = w4_expand(q < 2 ? w4.x : q < 4 ? w4.y : q < 6 ? w4.z : w4.w, bits);
+      }
+    // Row tile by row tile and group by group; a group's sums get their scale behind the first
+    // products of the next one.
+    w4_f32x16 acc[2][TN];
+    constexpr int kRuns = TM * NG;
+    auto flush = [&](int run) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          total[run / NG][j][e] =
+              fmaf(sc[j][run % NG], acc[run & 1][j][e], total[run / NG][j][e]);
     };
-    fetch(0);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {  // 32 inputs: word q
-      if (!kWhole && q >= steps) break;
-      if (q < 3) fetch(q + 1);
+    for (int run = 0; run < kRuns; ++run) {
+      const int i = run / NG, first = run % NG * 2 * KS;  // steps of 16 inputs
+      const int r = 32 * (TM * wm + i) + c;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int j = 0; j < TN; ++j) {
-          const uint4& w4 = cw[j][u];
-          const uint4 wf = w4_expand(q == 0 ? w4.x : q == 1 ? w4.y : q == 2 ? w4.z : w4.w, bits);
-#pragma unroll
-          for (int i = 0; i < TM; ++i)
-            acc[i][j] = w4_mma32(xf[q & 1][u][i], wf,
-                                 u == 0 && q % KS == 0 ? w4_f32x16{} : acc[i][j]);
-        }
-      if ((q + 1) % KS && (kWhole || q + 1 < steps)) continue;  // inside a group
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
+      for (int q = 0; q < 2 * KS; ++q) {
+        if (!kWhole && first + q >= 2 * steps) continue;  // (uniform)
+        const uint4 xf = st.x[r * 16 + ((2 * (first + q) + h) ^ (r & 15))];
 #pragma unroll
         for (int j = 0; j < TN; ++j)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            total[i][j][e] = fmaf(sc[j][q / KS], acc[i][j][e], total[i][j][e]);
+          acc[run & 1][j] = w4_mma32(xf, wf[j][first + q], q ? acc[run & 1][j] : w4_f32x16{});
+        if (kWhole && q == 0 && run) flush(run - 1);
+      }
+      if (!kWhole && first < 2 * steps) flush(run);
     }
+    if (kWhole) flush(kRuns - 1);
   };
   for (int kb = 0; kb < K / kW4K; ++kb) stage(kb, std::true_type{}, 4);
   if (K % kW4K) stage(K / kW4K, std::false_type{}, K % kW4K / 32);
 
-  // Outputs; those that are not finite once more, as the formula is written.
-  uint32_t again[TM][TN];
+  // Outputs. (The branches stay outside the loops over the tiles: an output is a handful of
+  // instructions, and a workgroup has them all at its end.)
+  float wrong = 0.f;  // NaN as soon as one is not finite
 #pragma unroll
   for (int j = 0; j < TN; ++j) {
     const int n = n0 + 32 * (TN * wn + j) + c;
     const float bias = G.bias && n < N ? bf16_to_f32(G.bias[n]) : 0.f;
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      again[i][j] = 0;
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const int64_t m = m0 + 32 * (TM * wm + i) + 8 * (e / 4) + 4 * h + e % 4;
-        const float v = 16.f * total[i][j][e];
-        if (m < M && n < N) {
-          G.y[m * G.ldy + n] = f32_to_bf16(w4_activate(v + bias, G.act));
-          if (!(fabsf(v) < INFINITY)) again[i][j] |= 1u << e;
-        }
+        const float v = fmaf(16.f, total[i][j][e], bias);
+        wrong = fmaf(v, 0.f, wrong);
+        total[i][j][e] = v;
       }
-    }
   }
+  uint32_t again[TM][TN] = {};
+  if (__ballot(wrong != wrong)) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (!(fabsf(total[i][j][e]) < INFINITY)) again[i][j] |= 1u << e;
+  }
+  if (G.act != WKV7_ACT_NONE) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) w4_activate_all(total[i][j], G.act);
+  }
+  auto row_of = [&](int i, int e) { return 32 * (TM * wm + i) + 8 * (e / 4) + 4 * h + e % 4; };
+  const int64_t mine = m0 * G.ldy + n0 + c;
+  if (m0 + BM <= M && n0 + BN <= N) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        uint16_t* y = G.y + mine + row_of(i, e) * G.ldy;
+#pragma unroll
+        for (int j = 0; j < TN; ++j) y[32 * (TN * wn + j)] = f32_to_bf16(total[i][j][e]);
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        if (m0 + row_of(i, e) >= M) continue;
+        uint16_t* y = G.y + mine + row_of(i, e) * G.ldy;
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+          if (n0 + 32 * (TN * wn + j) + c < N)
+            y[32 * (TN * wn + j)] = f32_to_bf16(total[i][j][e]);
+      }
+  }
+  // those that are not finite once more, as the formula is written
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j)
-      while (again[i][j]) {
-        const int e = __builtin_ctz(again[i][j]);
-        again[i][j] &= again[i][j] - 1;
+      for (; again[i][j]; again[i][j] &= again[i][j] - 1) {
+        const int64_t m = m0 + row_of(i, __builtin_ctz(again[i][j]));
         const int n = n0 + 32 * (TN * wn + j) + c;
-        const int64_t m = m0 + 32 * (TM * wm + i) + 8 * (e / 4) + 4 * h + e % 4;
-        w4_store_direct(G, m, n);
+        if (m < M && n < N) w4_store_direct(G, m, n);
       }
 }
 

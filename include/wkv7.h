@@ -811,8 +811,9 @@ typedef struct wkv7_w4_group {
 } wkv7_w4_group;
 
 /* workspace: device, 16-byte aligned, at least wkv7_proj_w4_workspace_bytes(..) (else
- * WKV7_ERR_WORKSPACE; none up to WKV7_W4_FEW_ROWS rows); holds nothing between calls. */
-#define WKV7_W4_FEW_ROWS 16
+ * WKV7_ERR_WORKSPACE; none up to WKV7_W4_NO_WORKSPACE_ROWS rows); holds nothing between
+ * calls. */
+#define WKV7_W4_NO_WORKSPACE_ROWS 64
 
 int wkv7_proj_w4(int64_t m, const wkv7_w4_group *groups, int32_t ngroups, void *workspace,
                  size_t workspace_bytes, void *stream);

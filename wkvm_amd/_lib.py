@@ -45,7 +45,7 @@ WKV7_ADAPTER_MAX_RANK = 256
 WKV7_SAMPLE_GROUP = 256
 WKV7_SAMPLE_MAX_VOCAB = 1 << 21
 WKV7_LINEAR_MAX_V = 1024
-WKV7_W4_FEW_ROWS = 16
+WKV7_W4_NO_WORKSPACE_ROWS = 64
 WKV7_SCALE_BF16 = 0
 WKV7_SCALE_F16 = 1
 

@@ -160,6 +160,44 @@ int launch_thin(int64_t m, const wkv7_w4_group* groups, int n, int cus, hipStrea
   return launch_status();
 }
 
+// Up to this many rows the mid kernel runs (three products of 2048 x 2048: 64 rows 10.0 us, in tiles
+// 14.3; 96 rows 17.4 and 15).
+constexpr int64_t kMidRows = WKV7_W4_NO_WORKSPACE_ROWS;
+
+template <int TN, int KS>
+int launch_mid(W4Args& a, hipStream_t s) {
+  const int row_tiles = int((a.m + 31) / 32);
+  int64_t end = 0;
+  for (int i = 0; i < a.ngroups; ++i) {
+    end += (int64_t(a.g[i].w.n) + 32 * TN - 1) / (32 * TN) * row_tiles;
+    if (end > int64_t(0x7ffffff0)) return WKV7_ERR_ARG;
+    a.wg_end[i] = int32_t(end);
+  }
+  const int span = int((end + kW4Xcds - 1) / kW4Xcds);
+  w4_mid_kernel<8, TN, KS><<<unsigned(span) * kW4Xcds, 512, 0, s>>>(a, row_tiles, span);
+  return launch_status();
+}
+
+template <int KS>
+int launch_mid(int64_t m, const wkv7_w4_group* groups, int n, int cus, hipStream_t s) {
+  W4Args a{};
+  a.m = m;
+  int64_t tiles = 0;
+  for (int i = 0; i < n; ++i) {
+    if (groups[i].w.group != 32 * KS) continue;
+    a.g[a.ngroups++] = groups[i];
+    tiles += (int64_t(groups[i].w.n) + 31) / 32 * ((m + 31) / 32);
+  }
+  if (a.ngroups == 0) return WKV7_OK;
+  // 64 columns, which share the reads of x, as soon as 32 would be more tiles than units (three
+  // products of 2048 x 2048, 32 rows 8.4 us in 32 columns, 9.6 in 64; 64 rows 13.7 and 10.0). Not for
+  // groups of 32, whose sums and scales do not fit the registers then (64 rows 15.7 and 27).
+  if constexpr (KS > 1) {
+    if (tiles > cus) return launch_mid<2, KS>(a, s);
+  }
+  return launch_mid<1, KS>(a, s);
+}
+
 int device_cus(int* cus) {
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess ||
@@ -168,7 +206,7 @@ int device_cus(int* cus) {
   return WKV7_OK;
 }
 
-constexpr int64_t kThinRows = WKV7_W4_FEW_ROWS;
+constexpr int64_t kThinRows = 16;
 
 // Workspace of the tile kernel: the sums of every product's x over its groups.
 size_t sums_bytes(int64_t m, const wkv7_w4_group& g) {
@@ -176,10 +214,17 @@ size_t sums_bytes(int64_t m, const wkv7_w4_group& g) {
 }
 
 size_t workspace_bytes_of(int64_t m, const wkv7_w4_group* groups, int n) {
-  if (m <= kThinRows) return 0;
+  if (m <= kMidRows) return 0;
   size_t bytes = 0;
   for (int i = 0; i < n; ++i) bytes += sums_bytes(m, groups[i]);
   return bytes;
+}
+
+int64_t count_tiles(const W4TileArgs& a, int bm, int bn) {
+  int64_t tiles = 0;
+  for (int i = 0; i < a.ngroups; ++i)
+    tiles += (a.m + bm - 1) / bm * ((int64_t(a.g[i].w.n) + bn - 1) / bn);
+  return tiles;
 }
 
 template <int GM, int GN, int TM, int TN, int S, int KS>
@@ -198,29 +243,46 @@ int launch_tiles(W4TileArgs& a, hipStream_t s) {
 
 // The products of groups of 32 KS inputs: sums of x, then output tiles.
 template <int KS>
-int launch_tiled(int64_t m, const wkv7_w4_group* groups, int n, uint16_t*& ws, hipStream_t s) {
+int launch_tiled(int64_t m, const wkv7_w4_group* groups, int n, uint16_t*& ws, int cus,
+                 hipStream_t s) {
   W4SumArgs sums{};
   W4TileArgs tiles{};
   sums.m = tiles.m = m;
   int64_t waves = 0;
+  int distinct = 0;
   for (int i = 0; i < n; ++i) {
-    if (groups[i].w.group != 32 * KS) continue;
+    const wkv7_w4_group& g = groups[i];
+    if (g.w.group != 32 * KS) continue;
     const int at = tiles.ngroups++;
-    const int padded = w4_padded_groups(groups[i].w.k, 32 * KS);
-    tiles.g[at] = groups[i];
-    tiles.sums[at] = sums.sums[at] = ws;
-    sums.x[at] = groups[i].x;
-    sums.ldx[at] = groups[i].ldx;
-    sums.k[at] = groups[i].w.k;
-    waves = std::max(waves, m * ((padded * 32 * KS + 511) / 512));
-    ws += sums_bytes(m, groups[i]) / sizeof(uint16_t);
+    tiles.g[at] = g;
+    int same = 0;  // products of one x share its sums
+    while (same < distinct &&
+           (sums.x[same] != g.x || sums.ldx[same] != g.ldx || sums.k[same] != g.w.k))
+      ++same;
+    if (same == distinct) {
+      sums.sums[distinct] = ws;
+      sums.x[distinct] = g.x;
+      sums.ldx[distinct] = g.ldx;
+      sums.k[distinct++] = g.w.k;
+      waves = std::max(waves, m * ((w4_padded_groups(g.w.k, 32 * KS) * 32 * KS + 511) / 512));
+      ws += sums_bytes(m, g) / sizeof(uint16_t);
+    }
+    tiles.sums[at] = sums.sums[same];
   }
   if (tiles.ngroups == 0) return WKV7_OK;
   if ((waves + 3) / 4 > int64_t(0x7fffffff)) return WKV7_ERR_ARG;
-  w4_sums_kernel<KS><<<dim3(unsigned((waves + 3) / 4), tiles.ngroups), 256, 0, s>>>(sums);
+  w4_sums_kernel<KS><<<dim3(unsigned((waves + 3) / 4), distinct), 256, 0, s>>>(sums);
   const int rc = launch_status();
   if (rc != WKV7_OK) return rc;
-  return launch_tiles<1, 4, 2, 1, 3, KS>(tiles, s);
+  // Four waves side by side, two workgroups on a unit. us for three products of 2048 x 2048 (4096 x
+  // 4096) by rows, in tiles of 32 x 128, 64 x 128 and 64 x 256: 128 rows 15.2 and 18.1; 256 rows
+  // 20.0, 19.6 (48.7, 45.8, 50); 512 rows 26.5, 27.4 (89, 76, 75); 1024 rows 47.8, 43.7, 45.3 (137 in
+  // 64 x 128, 125); 4096 rows (503, 429).
+  if (4 * count_tiles(tiles, 64, 128) <= 3 * int64_t(cus))
+    return launch_tiles<1, 4, 1, 1, 3, KS>(tiles, s);
+  if (2 * count_tiles(tiles, 64, 256) <= 3 * int64_t(cus))
+    return launch_tiles<1, 4, 2, 1, 3, KS>(tiles, s);
+  return launch_tiles<1, 4, 2, 2, 2, KS>(tiles, s);
 }
 
 }  // namespace
@@ -277,19 +339,28 @@ extern "C" int wkv7_proj_w4(int64_t m, const wkv7_w4_group* groups, int32_t ngro
   if (rc != WKV7_OK) return rc;
   if (m == 0) return WKV7_OK;
   hipStream_t st = as_stream(stream);
-  if (m > kThinRows) {
+  if (m > kMidRows) {
     if (!workspace || workspace_bytes < workspace_bytes_of(m, groups, ngroups))
       return WKV7_ERR_WORKSPACE;
     if (!aligned16(workspace)) return WKV7_ERR_SHAPE;
-    uint16_t* ws = static_cast<uint16_t*>(workspace);
-    int done = launch_tiled<4>(m, groups, ngroups, ws, st);
-    if (done == WKV7_OK) done = launch_tiled<2>(m, groups, ngroups, ws, st);
-    if (done == WKV7_OK) done = launch_tiled<1>(m, groups, ngroups, ws, st);
-    return done;
   }
   int cus = 0;
   int done = device_cus(&cus);
-  if (done == WKV7_OK) done = launch_thin<4>(m, groups, ngroups, cus, st);
+  if (done != WKV7_OK) return done;
+  if (m > kMidRows) {
+    uint16_t* ws = static_cast<uint16_t*>(workspace);
+    done = launch_tiled<4>(m, groups, ngroups, ws, cus, st);
+    if (done == WKV7_OK) done = launch_tiled<2>(m, groups, ngroups, ws, cus, st);
+    if (done == WKV7_OK) done = launch_tiled<1>(m, groups, ngroups, ws, cus, st);
+    return done;
+  }
+  if (m > kThinRows) {
+    done = launch_mid<4>(m, groups, ngroups, cus, st);
+    if (done == WKV7_OK) done = launch_mid<2>(m, groups, ngroups, cus, st);
+    if (done == WKV7_OK) done = launch_mid<1>(m, groups, ngroups, cus, st);
+    return done;
+  }
+  done = launch_thin<4>(m, groups, ngroups, cus, st);
   if (done == WKV7_OK) done = launch_thin<2>(m, groups, ngroups, cus, st);
   if (done == WKV7_OK) done = launch_thin<1>(m, groups, ngroups, cus, st);
   return done;

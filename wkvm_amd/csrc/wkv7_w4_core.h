@@ -200,5 +200,127 @@ __global__ __launch_bounds__(64 * NW, 4) void w4_thin_kernel(const W4Args args) 
   }
 }
 
+typedef float w4_f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ w4_f32x16 w4_mma32(const uint4& a, const uint4& b, w4_f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(w4_bf16x8, a),
+                                                 __builtin_bit_cast(w4_bf16x8, b), c, 0, 0, 0);
+}
+
+constexpr int kW4Xcds = 8;  // workgroups are dealt round-robin over 8 XCDs
+
+// Some tens of rows: a workgroup per tile of 32 rows by 32 TN columns, the blocks of 128 inputs dealt
+// to its NW waves, on v_mfma_f32_32x32x16_bf16 (lane l, c = l % 32, h = l / 32: row or column c at 8 h ..
+// of 16 inputs; result lane D[8 (i / 4) + 4 h + i % 4][c]). As in the thin kernel there is no barrier
+// before the sums are joined; the loads of a wave's next block are under way while it multiplies one.
+template <int NW, int TN, int KS>
+__global__ __launch_bounds__(64 * NW, 2) void w4_mid_kernel(const W4Args args, int row_tiles,
+                                                            int span) {
+  constexpr int NG = 4 / KS;
+  __shared__ float red[NW][TN * 16][64];
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int bid = int(blockIdx.x % kW4Xcds) * span + int(blockIdx.x / kW4Xcds);
+  if (bid >= args.wg_end[args.ngroups - 1]) return;
+  int at, count;
+  const wkv7_w4_group& G = args.g[w4_product(args, bid, at, count)];
+  const int64_t m0 = int64_t(at % row_tiles) * 32, M = args.m;
+  const int n0 = at / row_tiles * (32 * TN);
+  const int k = G.w.k, blocks = (k + kW4K - 1) / kW4K, groups = (k + 32 * KS - 1) / (32 * KS);
+  const uint4* codes[TN];
+  const uint32_t* scales[TN];
+#pragma unroll
+  for (int t = 0; t < TN; ++t) {
+    const int64_t tile = min(n0 / kW4N + 2 * t + c / kW4N, (G.w.n + kW4N - 1) / kW4N - 1);
+    codes[t] = reinterpret_cast<const uint4*>(G.w.codes) + tile * blocks * 64 + (c & 15) + 16 * h;
+    scales[t] = G.w.scales + tile * groups * kW4N + (c & 15);
+  }
+  const uint16_t* x = G.x + min(m0 + c, M - 1) * G.ldx + 8 * h;
+
+  const W4Bits bits;
+  const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+  w4_f32x16 total[TN] = {};
+  uint4 cw[TN][2], xf[4][2];  // words j of inputs 32 j + 8 h .. and of 32 j + 16 + 8 h ..
+  uint32_t sc[TN][NG];
+  // (past k something inside it is read, and not used)
+  auto fetch_codes = [&](int b) {
+#pragma unroll
+    for (int t = 0; t < TN; ++t) {
+      cw[t][0] = codes[t][int64_t(b) * 64];
+      cw[t][1] = codes[t][int64_t(b) * 64 + 32];
+#pragma unroll
+      for (int q = 0; q < NG; ++q) sc[t][q] = scales[t][min(b * NG + q, groups - 1) * kW4N];
+    }
+  };
+  auto fetch_x = [&](int b, int j) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      xf[j][u] = *reinterpret_cast<const uint4*>(x + min(kW4K * b + 32 * j, k - 32) + 16 * u);
+  };
+  if (wave < blocks) {
+    fetch_codes(wave);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) fetch_x(wave, j);
+  }
+  for (int b = wave; b < blocks; b += NW) {
+    uint4 c0[TN][2];
+    uint32_t sc0[TN][NG];
+#pragma unroll
+    for (int t = 0; t < TN; ++t) {
+      c0[t][0] = cw[t][0];
+      c0[t][1] = cw[t][1];
+#pragma unroll
+      for (int q = 0; q < NG; ++q) sc0[t][q] = sc[t][q];
+    }
+    const int next = min(b + NW, blocks - 1);
+    fetch_codes(next);
+#pragma unroll
+    for (int q = 0; q < NG; ++q) {
+      w4_f32x16 acc[TN] = {}, sum = {};
+#pragma unroll
+      for (int j = q * KS; j < (q + 1) * KS; ++j) {
+        if (kW4K * b + 32 * j < k)  // (uniform)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            sum = w4_mma32(xf[j][u], ones, sum);
+#pragma unroll
+            for (int t = 0; t < TN; ++t) {
+              const uint4& w4 = c0[t][u];
+              acc[t] = w4_mma32(
+                  xf[j][u], w4_expand(j == 0 ? w4.x : j == 1 ? w4.y : j == 2 ? w4.z : w4.w, bits),
+                  acc[t]);
+            }
+          }
+        fetch_x(next, j);
+      }
+#pragma unroll
+      for (int t = 0; t < TN; ++t) {
+        const float s = w4_scale(sc0[t][q]), z = w4_minus_zero(sc0[t][q]);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          total[t][e] = fmaf(s, fmaf(z, sum[e], acc[t][e]), total[t][e]);
+      }
+      if (NG > 1) __builtin_amdgcn_sched_barrier(0);  // (one group's sums at a time in registers)
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < TN; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) red[wave][16 * t + e][lane] = total[t][e];
+  __syncthreads();
+#pragma unroll 1
+  for (int i = wave; i < 16 * TN; i += NW) {
+    const int e = i & 15, n = n0 + 32 * (i >> 4) + c;
+    const int64_t m = m0 + 8 * (e / 4) + 4 * h + e % 4;
+    float v = red[0][i][lane];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) v += red[w][i][lane];
+    if (m >= M || n >= G.w.n) continue;
+    const float r = fmaf(16.f, v, G.bias ? bf16_to_f32(G.bias[n]) : 0.f);
+    if (fabsf(r) < INFINITY) G.y[m * G.ldy + n] = f32_to_bf16(w4_activate(r, G.act));
+    else w4_store_direct(G, m, n);
+  }
+}
+
 }  // namespace
 }  // namespace wkv7

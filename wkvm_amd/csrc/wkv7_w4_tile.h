@@ -18,10 +18,7 @@
 namespace wkv7 {
 namespace {
 
-typedef float w4_f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) uint4 w4_lds_u4;
-
-constexpr int kW4Xcds = 8;
 
 struct W4TileArgs {
   wkv7_w4_group g[WKV7_PROJ_MAX_GROUPS];
@@ -78,11 +75,6 @@ __global__ __launch_bounds__(256) void w4_sums_kernel(const W4SumArgs a) {
   w4_split3(s, p);
 #pragma unroll
   for (int i = 0; i < 3; ++i) a.sums[g][(row * 3 + i) * padded + gi] = p[i];
-}
-
-__device__ __forceinline__ w4_f32x16 w4_mma32(const uint4& a, const uint4& b, w4_f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(w4_bf16x8, a),
-                                                 __builtin_bit_cast(w4_bf16x8, b), c, 0, 0, 0);
 }
 
 __device__ __forceinline__ void w4_activate_all(w4_f32x16& v, int act) {

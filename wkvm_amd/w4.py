@@ -185,7 +185,7 @@ def proj_w4(products: Sequence[tuple], outs: Sequence[torch.Tensor | None] | Non
         lib = _lib.load()
         with on_device(dev):
             ws_bytes = (int(lib.wkv7_proj_w4_workspace_bytes(M, groups, n_products))
-                        if M > _lib.WKV7_W4_FEW_ROWS else 0)
+                        if M > _lib.WKV7_W4_NO_WORKSPACE_ROWS else 0)
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
             rc = lib.wkv7_proj_w4(M, groups, n_products, ops._ptr(ws), ws_bytes,
                                   ops._stream_ptr(dev))

@@ -118,12 +118,14 @@ int device_cus(int* cus) {
   return WKV7_OK;
 }
 
-// Tokens of a piece (a multiple of 64), or 0: no sequence is cut.
+// Tokens of a piece (a multiple of 64), or 0: no sequence is cut. A unit holds one workgroup: as many
+// pieces as leave none of them a second one, sequences of equal lengths assumed.
 int64_t piece_tokens(int32_t nseq, int64_t tokens, const wkv7_linear_io& io, int cus) {
-  const int64_t groups = int64_t(io.H) * (io.V / 64);
-  const int64_t want = 2 * int64_t(cus);
-  if (nseq * groups >= want || tokens <= kMinPiece) return 0;
-  const int64_t piece = (tokens * groups + want - 1) / want;
+  const int64_t groups = int64_t(io.H) * (io.V / 64) * nseq;
+  const int64_t cuts = int64_t(cus) / groups;  // pieces of a sequence
+  const int64_t length = (tokens + nseq - 1) / nseq;
+  if (cuts < 2 || length <= kMinPiece) return 0;
+  const int64_t piece = (length + cuts - 1) / cuts;
   return std::max<int64_t>(kMinPiece, (piece + kChunk - 1) / kChunk * kChunk);
 }
 
@@ -136,7 +138,7 @@ size_t workspace_bytes_of(int64_t slots, const wkv7_linear_io& io) {
                                          sizeof(double));
 }
 
-template <int KD, int VT, bool kF32, int R, int kPerSimd>
+template <int KD, int VT, bool kF32, int R>
 int launch_prefill(const LinearSeqs& sq, const wkv7_linear_io& io, float* ws, hipStream_t s) {
   LinearSeqs a = sq;
   auto grid = [&](int tile) {
@@ -157,7 +159,7 @@ int launch_prefill(const LinearSeqs& sq, const wkv7_linear_io& io, float* ws, hi
     rc = launch_status();
     if (rc != WKV7_OK) return rc;
   }
-  linear_prefill_kernel<KD, VT, kF32, R, kPerSimd><<<unsigned(grid(VT)), 512, 0, s>>>(a, io);
+  linear_prefill_kernel<KD, VT, kF32, R><<<unsigned(grid(VT)), 768, 0, s>>>(a, io);
   return launch_status();
 }
 
@@ -222,8 +224,8 @@ extern "C" int wkv7_linear_prefill(float* state, int64_t num_rows, const int32_t
   hipStream_t s = as_stream(stream);
   const bool f32 = io->y_dtype == WKV7_Y_F32;
   if (io->K == 64)
-    return f32 ? launch_prefill<64, 64, true, 3, 4>(sq, *io, ws, s)
-               : launch_prefill<64, 64, false, 3, 4>(sq, *io, ws, s);
-  return f32 ? launch_prefill<128, 32, true, 2, 4>(sq, *io, ws, s)
-             : launch_prefill<128, 32, false, 2, 4>(sq, *io, ws, s);
+    return f32 ? launch_prefill<64, 64, true, 6>(sq, *io, ws, s)
+               : launch_prefill<64, 64, false, 6>(sq, *io, ws, s);
+  return f32 ? launch_prefill<128, 32, true, 5>(sq, *io, ws, s)
+             : launch_prefill<128, 32, false, 5>(sq, *io, ws, s);
 }

@@ -2,20 +2,20 @@
 //
 // A workgroup walks one piece of one sequence for one head and a tile of VT value columns, 64 tokens
 // at a time ("chunk"), its state in the accumulator registers of four state waves, each of which owns
-// K / 4 key rows. Four output waves have 16 of the chunk's tokens each. With
+// K / 4 key rows. Two groups of four output waves take the chunks in turn, 16 tokens to a wave. With
 // v_mfma_f32_16x16x32_bf16 (lane l, li = l % 16, lg = l / 16: an A or B lane holds row or column li at
 // 8 lg .. 8 lg + 7 of a 32-wide block, a result lane D[4 lg + i][li]), the rows of a result tile are
 // named so that the registers of two tiles are an operand of the next product as they stand: keys,
 // tokens and value columns 32 p + 8 (m / 4) + 4 half + m % 4 for row m of tile (p, half). Scores
 // therefore never leave their wave; of the state a bf16 split goes through LDS, each lane's own words.
 //
-// A chunk has two phases, a barrier behind each:
-//                  first                                   second
-//   state waves    write the state's split; decay the      add the chunk to the state
-//                  keys; ask for the k and v rows of a
-//                  later chunk (direct loads, LDS ring)
-//   output waves   scores, their decays and split; ask     outputs; the first of them also sums the
-//                  for the next chunk's queries            next chunk's decays
+// In tick c, with one barrier at its end:
+//   state waves    write the split of the state before chunk c, ask for the k and v rows of chunk
+//                  c + kAhead + 1 (direct loads into an LDS ring), add chunk c to the state, decay
+//                  the keys of chunk c + 1
+//   one group      chunk c - 1: the state's part of the outputs, scores of the wave's own block
+//   the other      chunk c - 2: the other scores, their products with the values, the outputs; sums
+//                  of the decays of chunk c + 2
 // The operands that are not bf16 to begin with (scores under their decays, decayed keys, the state)
 // are split into bf16 parts: three where an fp32 result is kept (the state, an fp32 y), two
 // (2^-18 of each term) for a y that is rounded to bf16.
@@ -149,26 +149,27 @@ __device__ __forceinline__ int at(int r, int e) {
   return r * W + (((e >> 3) ^ turn<W>(r)) << 3) + (e & 7);
 }
 
-// LDS of a workgroup. Chunk c of k and v sits in ring[c % R], asked for R - 1 chunks ahead.
+// LDS of a workgroup. Chunk c of k and v sits in ring[c % R].
 template <int KD, int VT, int YP, int R>
 struct LinearLds {
   static constexpr int NP = KD / 32, NC = VT / 16;
+  static constexpr int kDecays = 5;
   struct Stage {
     uint4 k[kChunk * KD / 8];
     uint4 v[kChunk * VT / 8];
   } ring[R];
-  uint4 state[YP ? YP * NP * NC * 64 : 1];  // parts of the state before the chunk
-  // of chunk c at [c % 2]: its tokens' sums of log2 decays G as two floats each, e^(G_last - G),
-  // e^(G_31 - G) of the first 32 tokens, the decays themselves, e^G_last
+  uint4 state[2][YP ? YP * NP * NC * 64 : 1];  // [c % 2]: parts of the state before chunk c
+  // of chunk c at [c % kDecays]: its tokens' sums of log2 decays G as two floats each,
+  // e^(G_last - G), e^(G_31 - G) of the first 32 tokens, the decays themselves, e^G_last
   struct Decays {
     alignas(16) float hi[kChunk];
     alignas(16) float lo[kChunk];
     alignas(16) float left[kChunk];
     alignas(16) float first[32];
     float raw[kChunk], all;
-  } decays[2];
+  } decays[kDecays];
   float part[2][4][VT];
-  int bad[2];  // [c % 2]: something in chunk c is not finite
+  int bad[4];  // [c % 4]: something in chunk c is not finite
 };
 
 // The state waves' share of a piece: `mine` 0 .. 3.
@@ -177,7 +178,7 @@ struct StateWave {
   using Lds = LinearLds<KD, VT, YP, R>;
   static constexpr int RT = KD / 64, NC = VT / 16, NP = KD / 32;
   static constexpr int KL = KD / 32, VL = VT / 32;  // direct loads of a wave per chunk
-  static constexpr int kLoads = KL + VL, kAhead = R - 1;
+  static constexpr int kLoads = KL + VL;
   Lds& lds;
   int mine, li, lg, kp;
   f32x4 S[RT][NC], next[RT][NC];
@@ -240,10 +241,28 @@ struct StateWave {
     vnext += kChunk * ldv;
   }
 
-  // First phase: the state's bf16 parts, and the decayed keys of chunk c.
-  __device__ __forceinline__ void prepare(int64_t c) {
-    const uint16_t* sk = reinterpret_cast<const uint16_t*>(lds.ring[c % R].k);
-    const auto& dec = lds.decays[c & 1];
+  // The state's bf16 parts, before chunk c.
+  __device__ __forceinline__ void publish(int c) {
+    uint4* to = lds.state[c & 1];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct) {
+        uint32_t a[YP], b[YP];
+        split_pair<YP>(S[rt][ct][0], S[rt][ct][1], a, neg);
+        split_pair<YP>(S[rt][ct][2], S[rt][ct][3], b, neg);
+#pragma unroll
+        for (int p = 0; p < YP; ++p)
+          reinterpret_cast<uint2*>(
+              &to[((p * NP + kp) * NC + ct) * 64 + (threadIdx.x & 63)])[half_of(rt)] =
+              make_uint2(a[p], b[p]);
+      }
+  }
+
+  // The decayed keys of chunk c.
+  __device__ __forceinline__ void prepare(int c) {
+    const uint16_t* sk = reinterpret_cast<const uint16_t*>(lds.ring[unsigned(c) % R].k);
+    const auto& dec = lds.decays[unsigned(c) % Lds::kDecays];
     uint2 kt[RT][2][2];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
@@ -254,21 +273,6 @@ struct StateWave {
         kt[rt][b][0] = ld_tr(sk + at<KD>(r, key));
         kt[rt][b][1] = ld_tr(sk + at<KD>(r + 4, key));
       }
-    if constexpr (YP > 0) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int ct = 0; ct < NC; ++ct) {
-          uint32_t a[YP], b[YP];
-          split_pair<YP>(S[rt][ct][0], S[rt][ct][1], a, neg);
-          split_pair<YP>(S[rt][ct][2], S[rt][ct][3], b, neg);
-#pragma unroll
-          for (int p = 0; p < YP; ++p)
-            reinterpret_cast<uint2*>(
-                &lds.state[((p * NP + kp) * NC + ct) * 64 + (threadIdx.x & 63)])[half_of(rt)] =
-                make_uint2(a[p], b[p]);
-        }
-    }
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const f32x4 l0 = *reinterpret_cast<const f32x4*>(&dec.left[32 * b + 8 * lg]);
@@ -284,10 +288,10 @@ struct StateWave {
     }
   }
 
-  // Second phase: next = the state behind chunk c; false in some lane where it is not finite.
-  __device__ __forceinline__ bool add(int64_t c) {
-    const uint16_t* sv = reinterpret_cast<const uint16_t*>(lds.ring[c % R].v);
-    const float all = lds.decays[c & 1].all;
+  // next = the state behind chunk c; false in some lane where it is not finite.
+  __device__ __forceinline__ bool add(int c) {
+    const uint16_t* sv = reinterpret_cast<const uint16_t*>(lds.ring[unsigned(c) % R].v);
+    const float all = lds.decays[unsigned(c) % Lds::kDecays].all;
     uint4 vf[2][NC];  // V: columns li of tile ct, tokens 32 b + 8 lg ..
 #pragma unroll
     for (int b = 0; b < 2; ++b)
@@ -392,14 +396,18 @@ __device__ __forceinline__ double sum_decays(Decays& d, float g, int n) {
   return last;
 }
 
-// Outputs. Waves 0 .. 3 are the state waves, 4 .. 7 the output waves.
-template <int KD, int VT, bool kF32, int R, int kPerSimd>
-__global__ __launch_bounds__(512, kPerSimd) void linear_prefill_kernel(const LinearSeqs a,
+// Outputs. Waves 0 .. 3 are the state waves, 4 .. 7 and 8 .. 11 the output waves of the even and of
+// the odd chunks.
+template <int KD, int VT, bool kF32, int R>
+__global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
                                                              const wkv7_linear_io io) {
   constexpr int YP = kF32 ? 3 : 2;
   using State = StateWave<KD, VT, YP, R>;
   using Lds = typename State::Lds;
   constexpr int NP = State::NP, NC = State::NC, RT = State::RT;
+  // Chunk c is asked for in tick c - 1 - kAhead, has landed when tick c - 2 ends (its keys are read
+  // from tick c - 1) and is read until tick c + 2.
+  constexpr int kAhead = R - 4;
   __shared__ Lds lds;
 
   const int lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
@@ -410,7 +418,7 @@ __global__ __launch_bounds__(512, kPerSimd) void linear_prefill_kernel(const Lin
   const int64_t V = io.V, row = it.row, head = it.head;
   const int col0 = VT * it.tile;
   if (row < 0 || row >= a.rows) {  // no state is touched, the outputs are zero
-    for (int64_t t = pc.beg + wave; t < pc.end; t += 8) {
+    for (int64_t t = pc.beg + wave; t < pc.end; t += 12) {
       const int64_t o = (t * io.H + head) * V + col0 + lane;
       if (lane >= VT) continue;
       if (kF32) static_cast<float*>(io.y)[o] = 0.f;
@@ -419,9 +427,9 @@ __global__ __launch_bounds__(512, kPerSimd) void linear_prefill_kernel(const Lin
     return;
   }
   float* slot_state = a.state + (row * io.H + head) * (KD * V) + col0;
-  const int64_t tokens = pc.end - pc.beg;
-  const int64_t chunks = (tokens + kChunk - 1) / kChunk;
-  auto count = [&](int64_t c) { return int(min(int64_t(kChunk), tokens - kChunk * c)); };
+  const int tokens = int(pc.end - pc.beg);
+  const int chunks = (tokens + kChunk - 1) / kChunk;
+  auto count = [&](int c) { return min(kChunk, tokens - kChunk * c); };
   const int hq = it.head / (io.H / io.Hq);
   const uint16_t* qbase = io.q + pc.beg * io.ldq + hq * KD;
 
@@ -438,37 +446,36 @@ __global__ __launch_bounds__(512, kPerSimd) void linear_prefill_kernel(const Lin
     sw.ldv = io.ldv;
     sw.knext = io.k + pc.beg * io.ldk + hq * KD;
     sw.vnext = io.v + pc.beg * io.ldv + head * V + col0;
-    if (threadIdx.x < 2) lds.bad[threadIdx.x] = 0;
+    if (threadIdx.x < 4) lds.bad[threadIdx.x] = 0;
 #pragma unroll
-    for (int c = 0; c < State::kAhead; ++c)
+    for (int c = 0; c <= kAhead; ++c)
       if (c < chunks) sw.issue(c, count(c));
     sw.load(a.piece ? a.pieces + (it.no * io.H + head) * (KD * V) + col0
                     : a.zero_init ? nullptr : slot_state, V);
     barrier_vm<0>();
-    for (int64_t c = 0; c < chunks; ++c) {
-      const bool more = c + State::kAhead < chunks;
-      if (more) sw.issue(int((c + State::kAhead) % R), count(c + State::kAhead));
-      sw.prepare(c);
-      barrier_lds();
-      if (threadIdx.x == 0) lds.bad[(c + 1) & 1] = 0;
-      if (__ballot(!sw.add(c)) && lane == 0) lds.bad[c & 1] = 1;
-      if (more) barrier_vm<(State::kAhead - 1) * State::kLoads>();
+    sw.prepare(0);
+    for (int c = 0; c < chunks; ++c) {
+      const bool more = c + 1 + kAhead < chunks;
+      if (more) sw.issue(int(unsigned(c + 1 + kAhead) % R), count(c + 1 + kAhead));
+      sw.publish(c);
+      if (threadIdx.x == 0) lds.bad[(c + 2) & 3] = 0;
+      if (__ballot(!sw.add(c)) && lane == 0) lds.bad[c & 3] = 1;
+      if (c + 1 < chunks) sw.prepare(c + 1);
+      if (more) barrier_vm<(kAhead - 1) * State::kLoads>();
       else barrier_vm<0>();
-      if (!__builtin_amdgcn_readfirstlane(lds.bad[c & 1])) {
+      if (!__builtin_amdgcn_readfirstlane(lds.bad[c & 3])) {
         sw.accept();
         continue;
       }
       // Something in the chunk is not finite: products of whole tiles would carry it to tokens
-      // before it (0 times infinity). Token by token instead, as the formula is written, once the
-      // outputs of those products are in memory.
-      barrier_lds();
-      const auto& st = lds.ring[c % R];
+      // before it (0 times infinity). Token by token instead, as the formula is written.
+      const auto& st = lds.ring[unsigned(c) % R];
       const uint16_t* sk = reinterpret_cast<const uint16_t*>(st.k);
       const uint16_t* sv = reinterpret_cast<const uint16_t*>(st.v);
       const int n = count(c);
       for (int t = 0; t < n; ++t) {
-        const float d = expf(lds.decays[c & 1].raw[t]);
-        const uint16_t* q = qbase + (kChunk * c + t) * io.ldq;
+        const float d = expf(lds.decays[unsigned(c) % Lds::kDecays].raw[t]);
+        const uint16_t* q = qbase + (int64_t(kChunk) * c + t) * io.ldq;
         float part[NC] = {};
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -494,7 +501,7 @@ __global__ __launch_bounds__(512, kPerSimd) void linear_prefill_kernel(const Lin
         if (threadIdx.x < VT) {
           const float(*p)[VT] = lds.part[t & 1];
           const float v = (p[0][lane] + p[1][lane]) + (p[2][lane] + p[3][lane]);
-          const int64_t o = ((pc.beg + kChunk * c + t) * io.H + head) * V + col0 + lane;
+          const int64_t o = ((pc.beg + int64_t(kChunk) * c + t) * io.H + head) * V + col0 + lane;
           if (kF32) static_cast<float*>(io.y)[o] = v;
           else static_cast<uint16_t*>(io.y)[o] = f32_to_bf16(v);
         }
@@ -506,53 +513,71 @@ __global__ __launch_bounds__(512, kPerSimd) void linear_prefill_kernel(const Lin
 
   // -- output waves --------------------------------------------------------------------------
   if (tokens == 0) return;
-  const int w = wave - 4;
+  const int group = (wave - 4) >> 2, w = wave & 3;
   const int tw = 16 * w + li;  // the lane's token of a chunk
   const float* gbase = io.log_decay + pc.beg * io.ld_decay + head;
   const int64_t lastt = tokens - 1;
-  auto load_g = [&](int64_t c) { return gbase[min(kChunk * c + lane, lastt) * io.ld_decay]; };
+  auto load_g = [&](int c) { return gbase[min(int64_t(kChunk) * c + lane, lastt) * io.ld_decay]; };
   const Neg neg = neg_consts();
   float g = 0.f;
   if (w == 0) {
-    g = load_g(0);
-    sum_decays(lds.decays[0], g, count(0));
-    g = load_g(1);
+    g = load_g(group);
+    if (group < chunks) sum_decays(lds.decays[group], g, count(group));
+    g = load_g(group + 2);
   }
-  uint4 qf[NP], qn[NP];  // the lane's query row of this chunk and of the next
-  auto load_q = [&](uint4 (&to)[NP], int64_t c) {
-    const uint16_t* q = qbase + min(kChunk * c + tw, lastt) * io.ldq + 8 * lg;
+  uint4 qf[NP], qn[NP];  // the lane's query row of the group's chunk and of its next one
+  auto load_q = [&](uint4 (&to)[NP], int c) {
+    const uint16_t* q = qbase + min(int64_t(kChunk) * c + tw, lastt) * io.ldq + 8 * lg;
 #pragma unroll
     for (int p = 0; p < NP; ++p) to[p] = ld16(q + 32 * p);
   };
-  load_q(qf, 0);
+  // The end of tick c; true if the state waves have written the outputs of chunk c.
+  auto end_tick = [&](int c) {
+    barrier_lds();
+    const bool bad = __builtin_amdgcn_readfirstlane(lds.bad[c & 3]);
+    if (bad)
+      for (int i = 0; i < count(c); ++i) barrier_lds();
+    return bad;
+  };
+  load_q(qn, group);
   barrier_lds();
-  for (int64_t c = 0; c < chunks; ++c) {
-    const auto& st = lds.ring[c % R];
-    const auto& dec = lds.decays[c & 1];
-    const uint16_t* sk = reinterpret_cast<const uint16_t*>(st.k);
-    const uint16_t* sv = reinterpret_cast<const uint16_t*>(st.v);
-    load_q(qn, c + 1);
-    const float thi = dec.hi[tw], tlo = dec.lo[tw];
+  if (group == 1) end_tick(0);
 
-    // Scores with the 32 tokens of block b, as an operand's rows.
-    auto scores = [&](int b, f32x4 (&sc)[2]) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        sc[h] = f32x4{0.f, 0.f, 0.f, 0.f};
-        const int kr = 32 * b + 8 * (li >> 2) + 4 * h + (li & 3);
-#pragma unroll
-        for (int p = 0; p < NP; ++p)
-          sc[h] = mma32(ld16(sk + at<KD>(kr, 32 * p + 8 * lg)), qf[p], sc[h]);
-      }
-    };
-    f32x4 sc[2];
-    float p8[8];
-    uint4 own[YP], before[YP];  // parts of the wave's own block's scores and of the first block's
-    const int b = w >> 1;
-    scores(b, sc);
+  f32x4 y[NC];
+  uint4 own[YP];  // the parts of the scores with the wave's own block of 32 tokens
+  const int blk = w >> 1;
+  bool skip = true;  // nothing to finish
+  // Scores with the 32 tokens of block b of chunk c, as an operand's rows.
+  auto scores = [&](const uint16_t* sk, int b, f32x4 (&sc)[2]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int s0 = 32 * b + 8 * lg + 4 * h;
+      sc[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const int kr = 32 * b + 8 * (li >> 2) + 4 * h + (li & 3);
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+        sc[h] = mma32(ld16(sk + at<KD>(kr, 32 * p + 8 * lg)), qf[p], sc[h]);
+    }
+  };
+  auto begin = [&](int c) {
+    const auto& dec = lds.decays[unsigned(c) % Lds::kDecays];
+    const uint16_t* sk = reinterpret_cast<const uint16_t*>(lds.ring[unsigned(c) % R].k);
+    const uint4* sp = lds.state[c & 1];
+    f32x4 sc[2];
+    scores(sk, blk, sc);
+#pragma unroll
+    for (int ct = 0; ct < NC; ++ct) y[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int part = YP - 1; part >= 0; --part)
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int ct = 0; ct < NC; ++ct)
+          y[ct] = mma32(sp[((part * NP + p) * NC + ct) * 64 + lane], qf[p], y[ct]);
+    const float thi = dec.hi[tw], tlo = dec.lo[tw];
+    float p8[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int s0 = 32 * blk + 8 * lg + 4 * h;
       const f32x4 shi = *reinterpret_cast<const f32x4*>(&dec.hi[s0]);
       const f32x4 slo = *reinterpret_cast<const f32x4*>(&dec.lo[s0]);
 #pragma unroll
@@ -563,43 +588,19 @@ __global__ __launch_bounds__(512, kPerSimd) void linear_prefill_kernel(const Lin
       }
     }
     split_eight<YP>(p8, own, neg);
-    if (b) {  // the first block, all of it before the wave's tokens: e^(G_t - G_31) e^(G_31 - G_s)
-      scores(0, sc);
-      const float ea =
-          __builtin_amdgcn_exp2f((thi - dec.hi[31]) + (tlo - dec.lo[31])) * io.scale;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const f32x4 eb = *reinterpret_cast<const f32x4*>(&dec.first[8 * lg + 4 * h]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p8[4 * h + i] = sc[h][i] * ea * eb[i];
-      }
-      split_eight<YP>(p8, before, neg);
-    }
-    // an infinite or NaN query: its products with the state's parts are not the formula's
-    f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int p = 0; p < NP; ++p) zero = mma32(qf[p], make_uint4(0, 0, 0, 0), zero);
-    const float wrong = (zero[0] + zero[1]) + (zero[2] + zero[3]);
-    if (__ballot(wrong != wrong) && lane == 0) lds.bad[c & 1] = 1;
     const float es = __builtin_amdgcn_exp2f(thi + tlo) * io.scale;
-    barrier_lds();
-
-    f32x4 y[NC];
-#pragma unroll
-    for (int ct = 0; ct < NC; ++ct) y[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int part = YP - 1; part >= 0; --part)
-#pragma unroll
-      for (int p = 0; p < NP; ++p)
-#pragma unroll
-        for (int ct = 0; ct < NC; ++ct)
-          y[ct] = mma32(lds.state[((part * NP + p) * NC + ct) * 64 + lane], qf[p], y[ct]);
 #pragma unroll
     for (int ct = 0; ct < NC; ++ct)
 #pragma unroll
       for (int i = 0; i < 4; ++i) y[ct][i] *= es;
-    auto values = [&](int blk, const uint4 (&pf)[YP]) {
-      const int r = 32 * blk + 8 * lg + (li >> 2);
+  };
+  auto finish = [&](int c) {
+    const auto& st = lds.ring[unsigned(c) % R];
+    const auto& dec = lds.decays[unsigned(c) % Lds::kDecays];
+    const uint16_t* sk = reinterpret_cast<const uint16_t*>(st.k);
+    const uint16_t* sv = reinterpret_cast<const uint16_t*>(st.v);
+    auto values = [&](int b, const uint4 (&pf)[YP]) {
+      const int r = 32 * b + 8 * lg + (li >> 2);
 #pragma unroll
       for (int ct = 0; ct < NC; ++ct) {
         const int col = 32 * (ct >> 1) + 4 * (ct & 1) + 8 * (li & 3);
@@ -609,10 +610,24 @@ __global__ __launch_bounds__(512, kPerSimd) void linear_prefill_kernel(const Lin
         for (int part = YP - 1; part >= 0; --part) y[ct] = mma32(vf, pf[part], y[ct]);
       }
     };
-    values(b, own);
-    if (b) values(0, before);
-
-    const int64_t t = kChunk * c + tw;
+    values(blk, own);
+    if (blk) {  // the first block, all of it before the wave's tokens: e^(G_t - G_31) e^(G_31 - G_s)
+      f32x4 sc[2];
+      float p8[8];
+      uint4 before[YP];
+      scores(sk, 0, sc);
+      const float ea =
+          __builtin_amdgcn_exp2f((dec.hi[tw] - dec.hi[31]) + (dec.lo[tw] - dec.lo[31])) * io.scale;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const f32x4 eb = *reinterpret_cast<const f32x4*>(&dec.first[8 * lg + 4 * h]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p8[4 * h + i] = sc[h][i] * ea * eb[i];
+      }
+      split_eight<YP>(p8, before, neg);
+      values(0, before);
+    }
+    const int t = kChunk * c + tw;
     if (t < tokens) {
       const int64_t o = ((pc.beg + t) * io.H + head) * V + col0 + 8 * lg;
 #pragma unroll
@@ -629,18 +644,29 @@ __global__ __launch_bounds__(512, kPerSimd) void linear_prefill_kernel(const Lin
         }
       }
     }
-    if (w == 0 && c + 1 < chunks) {
-      sum_decays(lds.decays[(c + 1) & 1], g, count(c + 1));
-      g = load_g(c + 2);
-    }
-    barrier_lds();
-    if (__builtin_amdgcn_readfirstlane(lds.bad[c & 1])) {
-      barrier_vm<0>();
-      for (int i = 0; i < count(c); ++i) barrier_lds();  // (the state waves write these outputs)
-    }
+  };
+  for (int c = group; c < chunks; c += 2) {
+    // tick c
+    if (!skip) finish(c - 2);
 #pragma unroll
     for (int p = 0; p < NP; ++p) qf[p] = qn[p];
+    if (w == 0 && c + 2 < chunks) {
+      sum_decays(lds.decays[unsigned(c + 2) % Lds::kDecays], g, count(c + 2));
+      g = load_g(c + 4);
+    }
+    // an infinite or NaN query: its products with the state's parts are not the formula's
+    f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int p = 0; p < NP; ++p) zero = mma32(qf[p], make_uint4(0, 0, 0, 0), zero);
+    const float wrong = (zero[0] + zero[1]) + (zero[2] + zero[3]);
+    if (__ballot(wrong != wrong) && lane == 0) lds.bad[c & 3] = 1;
+    skip = end_tick(c);
+    // tick c + 1
+    load_q(qn, c + 2);
+    if (!skip) begin(c);
+    if (c + 1 < chunks) end_tick(c + 1);
   }
+  if (!skip) finish(chunks - 1 - ((chunks - 1 - group) & 1));
 }
 
 // A piece's final state from zero and the sum of its decays, for a piece that is not its sequence's
@@ -649,6 +675,7 @@ template <int KD, int VT, int R>
 __global__ __launch_bounds__(320) void linear_states_kernel(const LinearSeqs a,
                                                             const wkv7_linear_io io) {
   using State = StateWave<KD, VT, 0, R>;
+  constexpr int kAhead = R - 1;
   __shared__ typename State::Lds lds;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -658,9 +685,9 @@ __global__ __launch_bounds__(320) void linear_states_kernel(const LinearSeqs a,
   if (pc.last || it.row < 0 || it.row >= a.rows) return;
   const int64_t V = io.V, head = it.head;
   const int col0 = VT * it.tile;
-  const int64_t tokens = pc.end - pc.beg;  // (a whole piece)
-  const int64_t chunks = (tokens + kChunk - 1) / kChunk;
-  auto count = [&](int64_t c) { return int(min(int64_t(kChunk), tokens - kChunk * c)); };
+  const int tokens = int(pc.end - pc.beg);  // (a whole piece)
+  const int chunks = (tokens + kChunk - 1) / kChunk;
+  auto count = [&](int c) { return min(kChunk, tokens - kChunk * c); };
   if (wave < 4) {
     const int hq = it.head / (io.H / io.Hq);
     State sw(lds, wave);
@@ -669,22 +696,22 @@ __global__ __launch_bounds__(320) void linear_states_kernel(const LinearSeqs a,
     sw.knext = io.k + pc.beg * io.ldk + hq * KD;
     sw.vnext = io.v + pc.beg * io.ldv + head * V + col0;
 #pragma unroll
-    for (int c = 0; c < State::kAhead; ++c)
+    for (int c = 0; c < kAhead; ++c)
       if (c < chunks) sw.issue(c, count(c));
     sw.load(nullptr, V);
     barrier_vm<0>();
-    for (int64_t c = 0; c < chunks; ++c) {
-      const bool more = c + State::kAhead < chunks;
-      if (more) sw.issue(int((c + State::kAhead) % R), count(c + State::kAhead));
+    for (int c = 0; c < chunks; ++c) {
+      const bool more = c + kAhead < chunks;
+      if (more) sw.issue(int(unsigned(c + kAhead) % R), count(c + kAhead));
       sw.prepare(c);
       // (as for the outputs, but a wave's keys are its own: it decides by itself)
       const bool bad = __ballot(!sw.add(c));
       if (!bad) sw.accept();
-      const auto& st = lds.ring[c % R];
+      const auto& st = lds.ring[unsigned(c) % R];
       const uint16_t* sk = reinterpret_cast<const uint16_t*>(st.k);
       const uint16_t* sv = reinterpret_cast<const uint16_t*>(st.v);
       for (int t = 0; bad && t < count(c); ++t) {
-        const float d = expf(lds.decays[c & 1].raw[t]);
+        const float d = expf(lds.decays[unsigned(c) % State::Lds::kDecays].raw[t]);
 #pragma unroll
         for (int rt = 0; rt < State::RT; ++rt)
 #pragma unroll
@@ -696,20 +723,22 @@ __global__ __launch_bounds__(320) void linear_states_kernel(const LinearSeqs a,
                                      kv * bf16_to_f32(sv[at<VT>(t, sw.col_of(ct))]));
           }
       }
-      if (more) barrier_vm<(State::kAhead - 1) * State::kLoads>();
+      if (more) barrier_vm<(kAhead - 1) * State::kLoads>();
       else barrier_vm<0>();
     }
     sw.store(a.pieces + (it.no * io.H + head) * (KD * V) + col0, V);
     return;
   }
   const float* gbase = io.log_decay + pc.beg * io.ld_decay + head;
-  auto load_g = [&](int64_t c) { return gbase[min(kChunk * c + lane, tokens - 1) * io.ld_decay]; };
+  auto load_g = [&](int c) {
+    return gbase[min(int64_t(kChunk) * c + lane, int64_t(tokens - 1)) * io.ld_decay];
+  };
   double sum = sum_decays(lds.decays[0], load_g(0), count(0));
   float g = load_g(1);
   barrier_lds();
-  for (int64_t c = 0; c < chunks; ++c) {
+  for (int c = 0; c < chunks; ++c) {
     if (c + 1 < chunks) {
-      sum += sum_decays(lds.decays[(c + 1) & 1], g, count(c + 1));
+      sum += sum_decays(lds.decays[unsigned(c + 1) % State::Lds::kDecays], g, count(c + 1));
       g = load_g(c + 2);
     }
     barrier_lds();

@@ -118,10 +118,17 @@ int device_cus(int* cus) {
   return WKV7_OK;
 }
 
-// Tokens of a piece (a multiple of 64), or 0: no sequence is cut. A unit holds one workgroup: as many
-// pieces as leave none of them a second one, sequences of equal lengths assumed.
+// Value columns of a workgroup of the outputs' kernel. Of 128 keys its LDS holds 32; of 64 keys it takes
+// 64, or 32 where that leaves half of the units without one (512 tokens x 32 heads 17.3 and 14.4 us).
+int value_tile(int32_t nseq, const wkv7_linear_io& io, int cus) {
+  return io.K == 128 || 2 * int64_t(nseq) * io.H * (io.V / 64) <= cus ? 32 : 64;
+}
+
+// Tokens of a piece (a multiple of 64), or 0: no sequence is cut. A unit holds one workgroup of the
+// outputs' kernel: as many pieces as leave none of them a second one, sequences of equal lengths
+// assumed.
 int64_t piece_tokens(int32_t nseq, int64_t tokens, const wkv7_linear_io& io, int cus) {
-  const int64_t groups = int64_t(io.H) * (io.V / 64) * nseq;
+  const int64_t groups = int64_t(io.H) * (io.V / (io.K == 128 ? 32 : 64)) * nseq;
   const int64_t cuts = int64_t(cus) / groups;  // pieces of a sequence
   const int64_t length = (tokens + nseq - 1) / nseq;
   if (cuts < 2 || length <= kMinPiece) return 0;
@@ -130,7 +137,7 @@ int64_t piece_tokens(int32_t nseq, int64_t tokens, const wkv7_linear_io& io, int
 }
 
 int64_t piece_slots(int32_t nseq, int64_t tokens, int64_t piece) {
-  return piece ? tokens / piece + nseq : nseq;
+  return piece ? (tokens + nseq * (piece - 1)) / piece : nseq;
 }
 
 size_t workspace_bytes_of(int64_t slots, const wkv7_linear_io& io) {
@@ -143,8 +150,9 @@ int launch_prefill(const LinearSeqs& sq, const wkv7_linear_io& io, float* ws, hi
   LinearSeqs a = sq;
   auto grid = [&](int tile) {
     const int64_t items = a.slots * io.H * (io.V / tile);
-    a.span = (items + kLinearXcds - 1) / kLinearXcds;
-    return a.span * kLinearXcds;
+    const int own = io.H / io.Hq * (io.V / tile);  // (as find_item deals them)
+    const int64_t deal = int64_t(own) * ((3 + own) / own) * kLinearXcds;
+    return (items + deal - 1) / deal * deal;
   };
   a.pieces = ws;
   a.sums = ws ? reinterpret_cast<double*>(ws + sq.slots * io.H * int64_t(io.K) * io.V) : nullptr;
@@ -223,9 +231,12 @@ extern "C" int wkv7_linear_prefill(float* state, int64_t num_rows, const int32_t
   float* ws = piece ? static_cast<float*>(workspace) : nullptr;
   hipStream_t s = as_stream(stream);
   const bool f32 = io->y_dtype == WKV7_Y_F32;
-  if (io->K == 64)
-    return f32 ? launch_prefill<64, 64, true, 6>(sq, *io, ws, s)
-               : launch_prefill<64, 64, false, 6>(sq, *io, ws, s);
-  return f32 ? launch_prefill<128, 32, true, 5>(sq, *io, ws, s)
-             : launch_prefill<128, 32, false, 5>(sq, *io, ws, s);
+  if (io->K == 128)
+    return f32 ? launch_prefill<128, 32, true, 5>(sq, *io, ws, s)
+               : launch_prefill<128, 32, false, 5>(sq, *io, ws, s);
+  if (!piece && value_tile(nseq, *io, cus) == 32)
+    return f32 ? launch_prefill<64, 32, true, 6>(sq, *io, ws, s)
+               : launch_prefill<64, 32, false, 6>(sq, *io, ws, s);
+  return f32 ? launch_prefill<64, 64, true, 6>(sq, *io, ws, s)
+             : launch_prefill<64, 64, false, 6>(sq, *io, ws, s);
 }

@@ -41,10 +41,9 @@ struct LinearSeqs {
   int32_t nseq;
   bool zero_init;
   int64_t tokens;
-  // Piece g of sequence s, tokens [cu[s] + g piece, ..), is number cu[s] / piece + s + g of `slots`;
-  // piece 0: a sequence is one piece, number s.
+  // Piece g of sequence s, tokens [cu[s] + g piece, ..), is number first_piece(s) + g of `slots`; piece
+  // 0: a sequence is one piece, number s.
   int64_t piece, slots;
-  int64_t span;    // work items per XCD
   float* pieces;   // [slots][H][K][V]: local final states, then the pieces' initial states
   double* sums;    // [slots][H]: sums of log2 decays
 };
@@ -107,6 +106,11 @@ __device__ __forceinline__ int64_t offset_at(const LinearSeqs& a, int s) {
   return min(max(int64_t(a.cu[s]), int64_t(0)), a.tokens);
 }
 
+// At least as many numbers further for the next sequence as this one has pieces.
+__device__ __forceinline__ int64_t first_piece(const LinearSeqs& a, int s) {
+  return (offset_at(a, s) + s * (a.piece - 1)) / a.piece;
+}
+
 __device__ __forceinline__ bool find_piece(const LinearSeqs& a, int64_t slot, Piece& p) {
   int s = int(slot);
   int64_t index = 0;
@@ -116,14 +120,14 @@ __device__ __forceinline__ bool find_piece(const LinearSeqs& a, int64_t slot, Pi
     int n = 0;
     for (int i = 0; i < a.nseq; i += 64) {
       const int at = i + lane;
-      const bool in = at < a.nseq && offset_at(a, at) / a.piece + at <= slot;
+      const bool in = at < a.nseq && first_piece(a, at) <= slot;
       const uint64_t votes = __ballot(in);
       n += __popcll(votes);
       if (votes != ~uint64_t(0)) break;
     }
     s = n - 1;
     if (s < 0) return false;
-    index = slot - (offset_at(a, s) / a.piece + s);
+    index = slot - first_piece(a, s);
   }
   const int64_t beg = offset_at(a, s), end = max(offset_at(a, s + 1), beg);
   if (index < 0 || (index > 0 && beg + index * a.piece >= end)) return false;
@@ -345,9 +349,12 @@ struct LinearItem {
 template <int VT>
 __device__ __forceinline__ bool find_item(const LinearSeqs& a, const wkv7_linear_io& io,
                                           LinearItem& it) {
-  // neighbouring items (the tiles and heads that share q and k) on one XCD
+  // Runs of neighbouring items (the tiles and heads that share q, k or a line of decays) on one XCD,
+  // the runs dealt to the XCDs in turn: pieces that turn out empty are as many on each.
   const int tiles = io.V / VT;
-  int64_t item = int64_t(blockIdx.x % kLinearXcds) * a.span + blockIdx.x / kLinearXcds;
+  const int own = io.H / io.Hq * tiles, run = own * ((3 + own) / own);
+  const unsigned at = blockIdx.x / kLinearXcds;
+  int64_t item = (int64_t(at / run) * kLinearXcds + blockIdx.x % kLinearXcds) * run + at % run;
   if (item >= a.slots * io.H * tiles) return false;
   it.tile = int(item % tiles);
   item /= tiles;
@@ -519,11 +526,11 @@ __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
   const int64_t lastt = tokens - 1;
   auto load_g = [&](int c) { return gbase[min(int64_t(kChunk) * c + lane, lastt) * io.ld_decay]; };
   const Neg neg = neg_consts();
-  float g = 0.f;
+  float g = 0.f;  // the lane's decay in the group's next chunk
   if (w == 0) {
-    g = load_g(group);
-    if (group < chunks) sum_decays(lds.decays[group], g, count(group));
+    const float now = load_g(group);
     g = load_g(group + 2);
+    if (group < chunks) sum_decays(lds.decays[group], now, count(group));
   }
   uint4 qf[NP], qn[NP];  // the lane's query row of the group's chunk and of its next one
   auto load_q = [&](uint4 (&to)[NP], int c) {
@@ -733,13 +740,15 @@ __global__ __launch_bounds__(320) void linear_states_kernel(const LinearSeqs a,
   auto load_g = [&](int c) {
     return gbase[min(int64_t(kChunk) * c + lane, int64_t(tokens - 1)) * io.ld_decay];
   };
-  double sum = sum_decays(lds.decays[0], load_g(0), count(0));
-  float g = load_g(1);
+  const float now = load_g(0);
+  float g = load_g(1), after = load_g(2);  // (64 lines of memory: they may take longer than a tick)
+  double sum = sum_decays(lds.decays[0], now, count(0));
   barrier_lds();
   for (int c = 0; c < chunks; ++c) {
     if (c + 1 < chunks) {
       sum += sum_decays(lds.decays[unsigned(c + 1) % State::Lds::kDecays], g, count(c + 1));
-      g = load_g(c + 2);
+      g = after;
+      after = load_g(c + 3);
     }
     barrier_lds();
   }
@@ -768,7 +777,7 @@ __global__ __launch_bounds__(kChainThreads) void linear_chain_kernel(const Linea
   f32x4 run = {0.f, 0.f, 0.f, 0.f};
   if (!a.zero_init)
     run = *reinterpret_cast<const f32x4*>(a.state + (row * io.H + head) * size + e);
-  const int64_t first = beg / a.piece + s, step = io.H * size;
+  const int64_t first = first_piece(a, s), step = io.H * size;
   float* p = a.pieces + (first * io.H + head) * size + e;
   const double* sums = a.sums + first * io.H + head;
   for (int64_t g0 = 0; g0 < n; g0 += U) {

@@ -105,13 +105,14 @@ def test_prefill_lengths(dev, length, zero_init):
 
 
 @pytest.mark.parametrize("kind", ["fixed", "token", "forget"])
-@pytest.mark.parametrize("lens", [[2500], [1024, 0, 700, 1, 2048, 513], [512, 512], [1537, 64]])
+@pytest.mark.parametrize("lens", [[2500], [1024, 0, 700, 1, 2048, 513], [512, 512], [1537, 64],
+                                  [0, 1, 4200, 0, 256, 2500, 5], [3000, 0, 2304], [1281]])
 @pytest.mark.parametrize("zero_init", [False, True])
 def test_prefill_in_pieces(dev, lens, kind, zero_init):
     """Long enough for the sequences to be cut (few heads), pieces that end inside and at the end of
     them, empty sequences between."""
     cu = np.concatenate([[0], np.cumsum(lens)]).tolist()
-    ids = [6, 2, 5, 1, 8, 3][:len(lens)]
+    ids = [6, 2, 5, 1, 8, 3, 4][:len(lens)]
     before, q, k, v, g = _inputs(4, cu[-1], 2, 1, 64, 64, kind)
     pool = before.to(dev)
     y = linear_prefill_varlen(pool, ids, cu, q.to(dev), k.to(dev), v.to(dev), g.to(dev),
@@ -120,31 +121,48 @@ def test_prefill_in_pieces(dev, lens, kind, zero_init):
 
 
 def test_prefill_in_pieces_of_wide_heads(dev):
-    cu = [0, 1300, 1301]
-    before, q, k, v, g = _inputs(5, cu[-1], 2, 2, 128, 128, "token")
-    pool = before.to(dev)
-    y = linear_prefill_varlen(pool, [4, 1], cu, q.to(dev), k.to(dev), v.to(dev), g.to(dev))
-    _check(pool, y, before, cu, [4, 1], q, k, v, g, 1.0)
+    cu = [0, 2900, 2901]
+    for f32 in (False, True):
+        before, q, k, v, g = _inputs(5, cu[-1], 2, 2, 128, 128, "token")
+        pool = before.to(dev)
+        y = linear_prefill_varlen(pool, [4, 1], cu, q.to(dev), k.to(dev), v.to(dev), g.to(dev),
+                                  out_dtype=F32 if f32 else BF16)
+        _check(pool, y, before, cu, [4, 1], q, k, v, g, 1.0)
 
 
-def test_more_sequences_than_a_wave(dev):
-    """Pieces find their sequence among more than 64, many of them empty."""
+@pytest.mark.parametrize("long", [1100, 135000])
+def test_more_sequences_than_a_wave(dev, long):
+    """Pieces (of the long batch) find their sequence among more than 64, many of them empty."""
     rng = np.random.default_rng(3)
-    lens = [int(n) if rng.random() < 0.5 else 0 for n in rng.integers(1, 40, 150)]
-    lens[70] = 1100
+    lens = [int(n) if rng.random() < 0.5 else 0 for n in rng.integers(1, 40, 68)]
+    lens[60] = long
     cu = np.concatenate([[0], np.cumsum(lens)]).tolist()
-    ids = rng.permutation(np.arange(1, 161))[:150].tolist()
-    before, q, k, v, g = _inputs(6, cu[-1], 1, 1, 64, 64, "token", rows=161)
+    ids = rng.permutation(np.arange(1, 81))[:68].tolist()
+    before, q, k, v, g = _inputs(6, cu[-1], 1, 1, 64, 64, "token", rows=81)
     pool = before.to(dev)
     y = linear_prefill_varlen(pool, ids, cu, q.to(dev), k.to(dev), v.to(dev), g.to(dev),
                               out_dtype=F32)
     _check(pool, y, before, cu, ids, q, k, v, g, 1.0)
 
 
+def test_whole_tiles_of_64_columns(dev):
+    """Enough heads for the wide tile (and an odd number of them), 64 and 128 value columns."""
+    for V in (64, 128):
+        lens = [70, 0, 129, 64, 1]
+        cu = np.concatenate([[0], np.cumsum(lens)]).tolist()
+        ids = [3, 1, 8, 2, 5]
+        for f32 in (False, True):
+            before, q, k, v, g = _inputs(19, cu[-1], 39, 13, 64, V, "token")
+            pool = before.to(dev)
+            y = linear_prefill_varlen(pool, ids, cu, q.to(dev), k.to(dev), v.to(dev), g.to(dev),
+                                      scale=0.125, out_dtype=F32 if f32 else BF16)
+            _check(pool, y, before, cu, ids, q, k, v, g, 0.125)
+
+
 @pytest.mark.parametrize("where,bad", [
     (w, b) for w in ("v", "k", "q", "g", "state") for b in (math.inf, -math.inf, math.nan)
     if (w, b) != ("g", math.inf)])  # (a decay is at most finite)
-@pytest.mark.parametrize("lens", [[150], [1500]])
+@pytest.mark.parametrize("lens", [[150], [2500]])
 def test_nothing_reaches_the_tokens_before_it(dev, where, bad, lens):
     """An infinite or NaN value reaches the outputs that the formula gives it to, and no others."""
     T = lens[0]
@@ -253,15 +271,16 @@ def test_offsets_that_break_their_contract_stay_in_bounds(dev):
 
 
 def test_repeated_runs_are_bit_identical(dev):
-    before, q, k, v, g = _inputs(12, 3000, 3, 3, 64, 64)
-    xs = [t.to(dev) for t in (q, k, v, g)]
-    first = None
-    for _ in range(4):
-        pool = before.to(dev)
-        y = linear_prefill_varlen(pool, [4, 2], [0, 700, 3000], *xs)
-        if first is None:
-            first = y.clone(), pool.clone()
-        assert torch.equal(y, first[0]) and torch.equal(pool, first[1])
+    for T, H, K, V in ((5000, 3, 64, 64), (5000, 2, 128, 128), (900, 40, 64, 64)):
+        before, q, k, v, g = _inputs(12, T, H, H, K, V)
+        xs = [t.to(dev) for t in (q, k, v, g)]
+        first = None
+        for _ in range(5):
+            pool = before.to(dev)
+            y = linear_prefill_varlen(pool, [4, 2], [0, 700, T], *xs)
+            if first is None:
+                first = y.clone(), pool.clone()
+            assert torch.equal(y, first[0]) and torch.equal(pool, first[1])
 
 
 def test_a_sequence_does_not_depend_on_the_batch(dev):
@@ -276,7 +295,7 @@ def test_a_sequence_does_not_depend_on_the_batch(dev):
     assert torch.equal(y, torch.cat([ya, yb])) and torch.equal(both, alone)
 
 
-@pytest.mark.parametrize("T", [150, 2000])
+@pytest.mark.parametrize("T", [150, 5000])
 def test_graph_replays(dev, T):
     """A captured prefill and decode step, replayed with other inputs and eager work between."""
     before, q, k, v, g = _inputs(14, T, 2, 2, 64, 64)

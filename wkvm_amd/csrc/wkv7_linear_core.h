@@ -28,7 +28,7 @@ namespace {
 
 constexpr int kChunk = 64;          // tokens of a chunk
 constexpr int kLinearXcds = 8;      // workgroups are dealt round-robin over 8 XCDs
-constexpr int kMinPiece = 512;      // tokens of the shortest piece that a sequence is cut into
+constexpr int kMinPiece = 256;      // tokens of the shortest piece that a sequence is cut into
 constexpr int kChainThreads = 64;
 constexpr int kChainElems = 4 * kChainThreads;
 constexpr double kLog2e = 1.4426950408889634;
@@ -682,7 +682,7 @@ template <int KD, int VT, int R>
 __global__ __launch_bounds__(320) void linear_states_kernel(const LinearSeqs a,
                                                             const wkv7_linear_io io) {
   using State = StateWave<KD, VT, 0, R>;
-  constexpr int kAhead = R - 1;
+  constexpr int kAhead = R - 2;  // (as for the outputs, without their ticks behind)
   __shared__ typename State::Lds lds;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -703,16 +703,17 @@ __global__ __launch_bounds__(320) void linear_states_kernel(const LinearSeqs a,
     sw.knext = io.k + pc.beg * io.ldk + hq * KD;
     sw.vnext = io.v + pc.beg * io.ldv + head * V + col0;
 #pragma unroll
-    for (int c = 0; c < kAhead; ++c)
+    for (int c = 0; c <= kAhead; ++c)
       if (c < chunks) sw.issue(c, count(c));
     sw.load(nullptr, V);
     barrier_vm<0>();
+    sw.prepare(0);
     for (int c = 0; c < chunks; ++c) {
-      const bool more = c + kAhead < chunks;
-      if (more) sw.issue(int(unsigned(c + kAhead) % R), count(c + kAhead));
-      sw.prepare(c);
+      const bool more = c + 1 + kAhead < chunks;
+      if (more) sw.issue(int(unsigned(c + 1 + kAhead) % R), count(c + 1 + kAhead));
       // (as for the outputs, but a wave's keys are its own: it decides by itself)
       const bool bad = __ballot(!sw.add(c));
+      if (c + 1 < chunks) sw.prepare(c + 1);
       if (!bad) sw.accept();
       const auto& st = lds.ring[unsigned(c) % R];
       const uint16_t* sk = reinterpret_cast<const uint16_t*>(st.k);
@@ -740,15 +741,16 @@ __global__ __launch_bounds__(320) void linear_states_kernel(const LinearSeqs a,
   auto load_g = [&](int c) {
     return gbase[min(int64_t(kChunk) * c + lane, int64_t(tokens - 1)) * io.ld_decay];
   };
-  const float now = load_g(0);
-  float g = load_g(1), after = load_g(2);  // (64 lines of memory: they may take longer than a tick)
-  double sum = sum_decays(lds.decays[0], now, count(0));
+  const float now[2] = {load_g(0), load_g(1)};
+  float g = load_g(2), after = load_g(3);  // (64 lines of memory: they may take longer than a tick)
+  double sum = sum_decays(lds.decays[0], now[0], count(0));
+  if (chunks > 1) sum += sum_decays(lds.decays[1], now[1], count(1));
   barrier_lds();
   for (int c = 0; c < chunks; ++c) {
-    if (c + 1 < chunks) {
-      sum += sum_decays(lds.decays[unsigned(c + 1) % State::Lds::kDecays], g, count(c + 1));
+    if (c + 2 < chunks) {
+      sum += sum_decays(lds.decays[unsigned(c + 2) % State::Lds::kDecays], g, count(c + 2));
       g = after;
-      after = load_g(c + 3);
+      after = load_g(c + 4);
     }
     barrier_lds();
   }

@@ -89,3 +89,25 @@ def test_python_refusals():
     assert weight.shape == (4, 32) and weight.nbytes() == 1024 + 64
     with pytest.raises(ValueError, match="GPU tensor"):
         proj_w4([(torch.zeros(1, 32, dtype=torch.bfloat16), weight)])
+
+
+def test_block_refuses_other_projections_and_host_weights():
+    from wkvm_amd.layout import RWKV7StateLayout
+    from wkvm_amd.timemix import RWKV7TimeMix
+
+    block = RWKV7TimeMix.random(RWKV7StateLayout(1, 64, 1, 64, 64, torch.bfloat16), 0, "cpu")
+    for names in (("w1",), ("r", "mix"), ("r", "r2")):
+        with pytest.raises(ValueError, match="can be 4-bit weights"):
+            block.quantize(32, names)
+    with pytest.raises(ValueError):  # (on the host)
+        block.quantize(32)
+    assert not block.w4 and "r" in block.w
+    block.add_adapters(2, 8, ("k",))
+    with pytest.raises(ValueError, match="holds adapters"):
+        block.quantize(32, ("r", "k"))
+    block.w4["v"] = object()
+    with pytest.raises(ValueError, match="takes no adapters"):
+        block.add_adapters(2, 8, ("o", "v"))
+    with pytest.raises(ValueError, match="already holds a 4-bit"):
+        block.quantize(32, ("v",))
+    assert set(block.adapters) == {"k"}

@@ -21,12 +21,16 @@ import torch
 from . import _lib, ops
 
 KEY_SIZES = (64, 128)
+_MAX_LD = 1 << 24  # elements from one token to the next that the kernels address
+
+
+_HERE = contextlib.nullcontext()
 
 
 def on_device(device: torch.device):
     """A context in which ``device`` is the current one (launches go to the current device)."""
     if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+        return _HERE
     return torch.cuda.device(device)
 
 
@@ -51,28 +55,31 @@ def _check_state(state: torch.Tensor) -> tuple[int, int, int, int]:
 def _vectors(x: torch.Tensor, name: str, tokens: int, size: int, device: torch.device):
     """``[tokens, heads, size]`` bf16 with whole tokens in one piece (copied where they are not), its
     heads and the elements from one token to the next."""
-    ops._require_cuda(x, name)
-    if x.dtype != torch.bfloat16:
+    if not (isinstance(x, torch.Tensor) and x.is_cuda):
+        ops._require_cuda(x, name)
+    if x.dtype is not torch.bfloat16:
         raise ValueError(f"{name} must be bfloat16, got {x.dtype}")
-    if x.dim() != 3 or x.shape[0] != tokens or x.shape[2] != size:
-        raise ValueError(f"{name} must be [{tokens}, heads, {size}], got {tuple(x.shape)}")
+    shape = x.shape
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != size:
+        raise ValueError(f"{name} must be [{tokens}, heads, {size}], got {tuple(shape)}")
     if x.device != device:
         raise ValueError(f"{name} on {x.device}, state on {device}")
-    heads = x.shape[1]
+    heads = shape[1]
     own = heads * size
     ld, sh, se = x.stride()
     if tokens <= 1:
         ld = own
-    if se != 1 or heads > 1 and sh != size or ld < own or ld % 8 or x.data_ptr() % 16:
+    if (se != 1 or heads > 1 and sh != size or ld < own or ld % 8 or ld > _MAX_LD
+            or x.data_ptr() % 16):
         x = x.clone(memory_format=torch.contiguous_format)
         ld = own
     return x, heads, ld
 
 
-def _io(q, k, v, log_decay, state, tokens, scale, out, out_dtype):
-    """The checked vectors as a ``LinearIO``, the output and the tensors that the launch reads."""
-    rows, H, K, V = _check_state(state)
-    dev = state.device
+def _io(q, k, v, log_decay, dims, dev, tokens, scale, out, out_dtype):
+    """The checked vectors as a ``LinearIO``, the output and the tensors that the launch reads;
+    ``dims`` are the state's."""
+    rows, H, K, V = dims
     q, Hq, ldq = _vectors(q, "q", tokens, K, dev)
     k, Hk, ldk = _vectors(k, "k", tokens, K, dev)
     v, Hv, ldv = _vectors(v, "v", tokens, V, dev)
@@ -101,7 +108,7 @@ def _io(q, k, v, log_decay, state, tokens, scale, out, out_dtype):
         raise ValueError("out must be 16-byte aligned and on the state's device")
     io = _lib.LinearIO(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
                        y.data_ptr(), ldq, ldk, ldv, ldd, H, Hq, K, V, code, float(scale))
-    return io, y, (q, k, v, log_decay), rows
+    return io, y, (q, k, v, log_decay)
 
 
 def linear_decode_slots(state: torch.Tensor, slot_ids, q, k, v, log_decay, *, scale: float = 1.0,
@@ -115,16 +122,16 @@ def linear_decode_slots(state: torch.Tensor, slot_ids, q, k, v, log_decay, *, sc
     bf16 ``[B, H, V]``, rows of any stride; ``log_decay`` fp32 ``[H]`` or ``[B, H]``. Returns
     ``y [B, H, V]`` in ``out_dtype`` (bf16 or fp32). ``slot_ids`` and ``row_order`` as for
     ``wkv7_decode_slots``."""
-    _check_state(state)
-    dev = state.device
-    ids, order = ops.decode_plan(slot_ids, state.shape[0], dev, wait=False)
+    dims = _check_state(state)
+    rows, dev = dims[0], state.device
+    ids, order = ops.decode_plan(slot_ids, rows, dev, wait=False)
     if row_order is not None:
         if not (isinstance(row_order, torch.Tensor) and row_order.is_cuda
                 and row_order.dtype == torch.int32 and row_order.shape == ids.shape):
             raise ValueError("row_order must be a device int32 tensor shaped like slot_ids")
         order = row_order
     B = int(ids.shape[0])
-    io, y, keep, rows = _io(q, k, v, log_decay, state, B, scale, out, out_dtype)
+    io, y, keep = _io(q, k, v, log_decay, dims, dev, B, scale, out, out_dtype)
     if B:
         with on_device(dev):
             rc = _lib.load().wkv7_linear_decode(state.data_ptr(), rows, ids.data_ptr(),
@@ -145,13 +152,13 @@ def linear_prefill_varlen(state: torch.Tensor, slot_ids, cu_seqlens, q, k, v, lo
     tokens. ``cu_seqlens`` is a host sequence or a device int32 tensor. A token's output does not
     depend on later tokens, whatever they hold. Few sequences are cut into pieces that run side by
     side, through a workspace from torch's allocator."""
-    _check_state(state)
-    dev = state.device
-    ids = ops.device_ids(slot_ids, state.shape[0], dev, "slot_ids", distinct=True, wait=False)
+    dims = _check_state(state)
+    rows, dev = dims[0], state.device
+    ids = ops.device_ids(slot_ids, rows, dev, "slot_ids", distinct=True, wait=False)
     nseq = int(ids.shape[0])
     ops._require_cuda(v, "v")
     T = int(v.shape[0]) if v.dim() == 3 else -1
-    io, y, keep, rows = _io(q, k, v, log_decay, state, T, scale, out, out_dtype)
+    io, y, keep = _io(q, k, v, log_decay, dims, dev, T, scale, out, out_dtype)
     if isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.is_cuda:
         if cu_seqlens.dtype != torch.int32 or tuple(cu_seqlens.shape) != (nseq + 1,):
             raise ValueError("device cu_seqlens must be int32 [nseq + 1]")

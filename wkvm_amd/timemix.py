@@ -25,7 +25,8 @@ place, and every element-wise stage is one of this library's kernels:
 
 A block may hold low-rank adapters of its r, k, v and o projections
 (``add_adapters``); a batch that names its requests' adapters then runs those
-products on ``proj_adapters``, at any token count.
+products on ``proj_adapters``, at any token count. It may instead hold these weights as
+4-bit codes (``quantize``); their products then run on ``proj_w4``, at any token count.
 
 Weights are stored [out, in] as nn.Linear holds them (each projection is
 ``linear(x, W)``), the layout both the grouped kernel and the vendor BLAS
@@ -51,6 +52,7 @@ from . import ops
 from .adapters import AdapterBank, AdapterPlan, adapter_plan, plan_ints, proj_adapters
 from .layout import HEAD_SIZE, RWKV7StateLayout
 from .state import RWKV7StateBank
+from .w4 import W4Weight, proj_w4
 
 MIX_NAMES = ("x_r", "x_w", "x_k", "x_v", "x_a", "x_g")
 
@@ -126,6 +128,33 @@ class RWKV7TimeMix:
         self.w = weights
         self.eps = HEAD_SIZE * 1e-5
         self.adapters: dict[str, AdapterBank] = {}
+        self.w4: dict[str, W4Weight] = {}
+
+    def quantize(self, group: int = 128, names=("r", "k", "v", "o"), symmetric: bool = False,
+                 ) -> dict[str, W4Weight]:
+        """Round the named projections to 4-bit weights (``W4Weight.quantize``), which take the
+        place of the block's bf16 ones: the dictionary that the block was made from is not
+        changed, and a decode graph keeps the weights that it captured."""
+        names = tuple(names)
+        for name in names:
+            if name not in ("r", "k", "v", "o"):
+                raise ValueError(f"r, k, v and o can be 4-bit weights, not {name!r}")
+            if name in self.w4:
+                raise ValueError(f"projection {name!r} already holds a 4-bit weight")
+            if name in self.adapters:
+                raise ValueError(f"projection {name!r} holds adapters, which need its bf16 weight")
+        new = {name: W4Weight.quantize(self.w[name], group, symmetric) for name in names}
+        self.w4.update(new)
+        self.w = {name: w for name, w in self.w.items() if name not in new}
+        return self.w4
+
+    def _weight(self, name: str):
+        return self.w4[name] if name in self.w4 else self.w[name]
+
+    def _linear(self, x: torch.Tensor, name: str) -> torch.Tensor:
+        if name in self.w4:
+            return proj_w4([(x, self.w4[name])])[0]
+        return F.linear(x, self.w[name])
 
     def add_adapters(self, num_adapters: int, max_rank: int, names=("r", "k", "v", "o"),
                      ) -> dict[str, AdapterBank]:
@@ -139,6 +168,8 @@ class RWKV7TimeMix:
             if name in self.adapters:
                 raise ValueError(f"projection {name!r} already holds a bank of "
                                  f"{self.adapters[name].num_adapters} adapters")
+            if name in self.w4:
+                raise ValueError(f"projection {name!r} holds a 4-bit weight, which takes no adapters")
         for name in names:
             n, k = self.w[name].shape
             self.adapters[name] = AdapterBank(num_adapters, k, n, max_rank, self.w[name].device)
@@ -205,9 +236,9 @@ class RWKV7TimeMix:
 
         # the independent chains between the token shift and the WKV inputs
         chains = {
-            "r": lambda: F.linear(xr, W["r"]),
-            "k": lambda: F.linear(xk, W["k"]),
-            "v": lambda: F.linear(xv, W["v"]),
+            "r": lambda: self._linear(xr, "r"),
+            "k": lambda: self._linear(xk, "k"),
+            "v": lambda: self._linear(xv, "v"),
             "w_l": lambda: F.linear(torch.tanh(F.linear(xw, W["w1"])), W["w2"], W["w0"]),
             "a_l": lambda: F.linear(F.linear(xa, W["a1"]), W["a2"], W["a0"]),
             "g": lambda: F.linear(torch.sigmoid(F.linear(xg, W["g1"])), W["g2"]),
@@ -235,7 +266,7 @@ class RWKV7TimeMix:
         r, k, v, w_l, a_l, g = (res[n] for n in ("r", "k", "v", "w_l", "a_l", "g"))
         o_in, v_first = self._wkv_stage(bank, batch, v_first, zero_init, r, k, v, w_l, a_l,
                                         res.get("v_l"), g)
-        return F.linear(o_in, W["o"]), v_first
+        return self._linear(o_in, "o"), v_first
 
     def _forward_grouped(self, bank, batch, v_first, zero_init, mixes):
         """The block with its projections on wkv7_proj_grouped: one launch
@@ -244,7 +275,8 @@ class RWKV7TimeMix:
         up-projections with their biases, one for o."""
         W, l = self.w, self.layer_idx
         xr, xw, xk, xv, xa, xg = mixes
-        first = [(xr, W["r"]), (xk, W["k"]), (xv, W["v"]), (xw, W["w1"], None, "tanh"),
+        first = [(xr, self._weight("r")), (xk, self._weight("k")), (xv, self._weight("v")),
+                 (xw, W["w1"], None, "tanh"),
                  (xa, W["a1"]), (xg, W["g1"], None, "sigmoid")]
         if l > 0:
             first.append((xv, W["v1"]))
@@ -258,11 +290,22 @@ class RWKV7TimeMix:
             w_l, a_l, g, *v_l = (F.linear(*product) for product in second)
         o_in, v_first = self._wkv_stage(bank, batch, v_first, zero_init, r, k, v, w_l, a_l,
                                         v_l[0] if v_l else None, g)
-        return self._project(batch, [(o_in, W["o"])], ("o",))[0], v_first
+        return self._project(batch, [(o_in, self._weight("o"))], ("o",))[0], v_first
 
     def _project(self, batch, products, names):
         """The products in one grouped launch, the first ones (``names``) with their adapters
-        where the batch has any."""
+        where the batch has any; those with 4-bit weights in a launch of their own."""
+        quant = [i for i, p in enumerate(products) if isinstance(p[1], W4Weight)]
+        if quant:
+            ys: list = [None] * len(products)
+            for i, y in zip(quant, proj_w4([products[i] for i in quant])):
+                ys[i] = y
+            rest = [i for i in range(len(products)) if ys[i] is None]
+            if rest:
+                kept = [names[i] for i in rest if i < len(names)]
+                for i, y in zip(rest, self._project(batch, [products[i] for i in rest], kept)):
+                    ys[i] = y
+            return ys
         if batch.adapters is None:
             return ops.proj_grouped(products)
         padded = [p + (None,) * (4 - len(p)) for p in products]
@@ -328,6 +371,7 @@ class TimeMixDecodeGraph:
         self.num_adapters = int(num_adapters)
         # (the captured launches hold their addresses, whatever the blocks hold later)
         self.adapter_banks = [b for layer in layers for b in layer.adapters.values()]
+        self.weights = [(layer.w, dict(layer.w4)) for layer in layers]
         self.adapter_plan = adapter_plan([-1] * B, num_adapters, dev) if num_adapters else None
         batch = TokenBatch(self.plan[:B], self.plan[2 * B:], self.plan[B:2 * B], B, B, True,
                            self.adapter_plan)
@@ -346,7 +390,8 @@ class TimeMixDecodeGraph:
             with torch.cuda.stream(st):
                 for layer in layers:
                     for name in ("r", "k", "v", "o"):
-                        _ = F.linear(self.x[0], layer.w[name])
+                        if name in layer.w:
+                            _ = F.linear(self.x[0], layer.w[name])
         torch.cuda.synchronize(dev)
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):

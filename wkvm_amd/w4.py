@@ -2,7 +2,7 @@
 
 ``W4Weight`` holds one ``[n, k]`` weight in the kernels' layout, made from a checkpoint's codes, scales
 and zero points (``from_codes``) or by rounding a bf16 weight (``quantize``); ``proj_w4`` runs up to 8
-products ``act(x W^T + bias)`` of a batch in one launch, as ``ops.proj_grouped`` does with bf16 weights.
+products ``act(x W^T + bias)`` of a batch in one call, as ``ops.proj_grouped`` does with bf16 weights.
 A decode step's time is the bytes of its weights, of which these have a quarter.
 
 The reference has no counterpart (its projections are plain nn.Linear calls of the external model,
@@ -12,6 +12,7 @@ wkvm/runner/runner.py:80-88).
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Sequence
 
 import torch
@@ -21,6 +22,8 @@ from .linear import on_device
 
 GROUPS = (32, 64, 128)
 _GROUP_ARRAYS = [_lib.W4Group * n for n in range(_lib.WKV7_PROJ_MAX_GROUPS + 1)]
+_GROUP_PACK = struct.Struct("@QQQiiiiQQqqii")  # the fields of W4Group
+assert _GROUP_PACK.size == ctypes.sizeof(_lib.W4Group)
 
 
 class W4Weight:
@@ -45,8 +48,8 @@ class W4Weight:
         self.scales = torch.empty(lib.wkv7_w4_scale_bytes(n, k, group) // 4, dtype=torch.int32,
                                   device=self.device)
         self.device = self.codes.device
-        self.desc = _lib.W4Desc(self.codes.data_ptr(), self.scales.data_ptr(), self.n, self.k,
-                                self.group, 0)
+        self.fields = (self.codes.data_ptr(), self.scales.data_ptr(), self.n, self.k, self.group, 0)
+        self.desc = _lib.W4Desc(*self.fields)
 
     @property
     def shape(self) -> tuple[int, int]:
@@ -124,7 +127,7 @@ class W4Weight:
 
 def proj_w4(products: Sequence[tuple], outs: Sequence[torch.Tensor | None] | None = None,
             ) -> list[torch.Tensor]:
-    """Independent projections ``act(x @ W.T + bias)`` with 4-bit weights in one launch
+    """Independent projections ``act(x @ W.T + bias)`` with 4-bit weights in one call
     (``wkv7_proj_w4``): ``products`` holds up to 8 tuples ``(x, weight)``, ``(x, weight, bias)`` or
     ``(x, weight, bias, act)`` with ``weight`` a ``W4Weight`` and the rest as for ``ops.proj_grouped``:
     bf16 ``x [M, k]``, every one of the same M (any number of rows), ``bias [n]`` or None, ``act``
@@ -133,7 +136,7 @@ def proj_w4(products: Sequence[tuple], outs: Sequence[torch.Tensor | None] | Non
     n_products = len(products)
     if not 1 <= n_products <= _lib.WKV7_PROJ_MAX_GROUPS:
         raise ValueError(f"1..{_lib.WKV7_PROJ_MAX_GROUPS} products per launch, got {n_products}")
-    groups = _GROUP_ARRAYS[n_products]()
+    packed = bytearray(_GROUP_PACK.size * n_products)
     ys, keep = [], []
     M = dev = None
     bf16 = torch.bfloat16
@@ -165,6 +168,8 @@ def proj_w4(products: Sequence[tuple], outs: Sequence[torch.Tensor | None] | Non
         n = w.n
         if bias is not None:
             bias = ops._bf16_2d(bias.reshape(-1), "bias", (n,))
+            if bias.device != dev:
+                raise ValueError("projection tensors must share a device")
         y = outs[i] if outs is not None and i < len(outs) else None
         if y is None:
             y = torch.empty((M, n), dtype=bf16, device=dev)
@@ -173,16 +178,19 @@ def proj_w4(products: Sequence[tuple], outs: Sequence[torch.Tensor | None] | Non
             ops._require_cuda(y, "out")
             if y.dtype != bf16 or tuple(y.shape) != (M, n) or n > 1 and y.stride(1) != 1:
                 raise ValueError(f"out must be a bf16 [{M}, {n}] tensor with unit column stride")
+            if y.device != dev:
+                raise ValueError("projection tensors must share a device")
             ldy = n if M <= 1 else y.stride(0)
-        if x.device != dev or w.device != dev or y.device != dev or \
-                bias is not None and bias.device != dev:
+        if x.device != dev or w.device != dev:
             raise ValueError("projection tensors must share a device")
-        groups[i] = _lib.W4Group(x.data_ptr(), w.desc, ops._ptr(bias), y.data_ptr(), ldx, ldy,
-                                 ops.ACTIVATIONS[act], 0)
+        _GROUP_PACK.pack_into(packed, _GROUP_PACK.size * i, x.data_ptr(), *w.fields,
+                              0 if bias is None else bias.data_ptr(), y.data_ptr(), ldx, ldy,
+                              ops.ACTIVATIONS[act], 0)
         keep += [x, w, bias]
         ys.append(y)
     if M:
         lib = _lib.load()
+        groups = _GROUP_ARRAYS[n_products].from_buffer(packed)
         with on_device(dev):
             ws_bytes = (int(lib.wkv7_proj_w4_workspace_bytes(M, groups, n_products))
                         if M > _lib.WKV7_W4_NO_WORKSPACE_ROWS else 0)

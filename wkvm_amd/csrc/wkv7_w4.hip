@@ -232,7 +232,7 @@ int64_t count_tiles(const W4TileArgs& a, int bm, int bn) {
   return tiles;
 }
 
-template <int GM, int GN, int TM, int TN, int S, int KS>
+template <int GM, int GN, int TM, int TN, int KH, int S, int KS>
 int launch_tiles(W4TileArgs& a, hipStream_t s) {
   constexpr int BM = 32 * TM * GM, BN = 32 * TN * GN;
   int64_t end = 0;
@@ -242,7 +242,8 @@ int launch_tiles(W4TileArgs& a, hipStream_t s) {
     a.tile_end[i] = int32_t(end);
   }
   a.span = int32_t((end + kW4Xcds - 1) / kW4Xcds);
-  w4_tile_kernel<GM, GN, TM, TN, S, KS><<<unsigned(a.span) * kW4Xcds, 64 * GM * GN, 0, s>>>(a);
+  w4_tile_kernel<GM, GN, TM, TN, KH, S, KS>
+      <<<unsigned(a.span) * kW4Xcds, 64 * GM * GN * KH, 0, s>>>(a);
   return launch_status();
 }
 
@@ -279,15 +280,21 @@ int launch_tiled(int64_t m, const wkv7_w4_group* groups, int n, uint16_t*& ws, i
   w4_sums_kernel<KS><<<dim3(unsigned((waves + 3) / 4), distinct), 256, 0, s>>>(sums);
   const int rc = launch_status();
   if (rc != WKV7_OK) return rc;
-  // Four waves side by side, two workgroups on a unit. us for three products of 2048 x 2048 (4096 x
-  // 4096) by rows, in tiles of 32 x 128, 64 x 128 and 64 x 256: 128 rows 15.2 and 18.1; 256 rows
-  // 20.0, 19.6 (48.7, 45.8, 50); 512 rows 26.5, 27.4 (89, 76, 75); 1024 rows 47.8, 43.7, 45.3 (137 in
-  // 64 x 128, 125); 4096 rows (503, 429).
-  if (4 * count_tiles(tiles, 64, 128) <= 3 * int64_t(cus))
-    return launch_tiles<1, 4, 1, 1, 3, KS>(tiles, s);
-  if (2 * count_tiles(tiles, 64, 256) <= 3 * int64_t(cus))
-    return launch_tiles<1, 4, 2, 1, 3, KS>(tiles, s);
-  return launch_tiles<1, 4, 2, 2, 2, KS>(tiles, s);
+  // Four waves side by side, two workgroups on a unit, but for the second shape, of eight waves that
+  // take turns in k. us with the sums, three products of 2048 x 2048 (4096 x 4096) by rows, in tiles of
+  // 32 x 128, of 64 x 128 in two parts, of 64 x 128 and of 64 x 256:
+  //   128 rows 15.5, 15.0, 18.5, 22.7 (30.7, 26.9, 31.6, 43.4)
+  //   256 rows 19.6, 17.3, 19.7, 25.3 (45.6, 48.0, 44.2, 46.7)
+  //   1024 rows 46.9, 44.7, 42.9, 40.9 (164, 152, 143, 119); 4096 rows (610, 567, 510, 420)
+  // The parts' workgroups fill a unit, and a launch of 256 of them leaves some units with two and some
+  // with none (36 us, and 22 for 224 of the same length).
+  const int64_t tiles64 = count_tiles(tiles, 64, 128);
+  if (8 * tiles64 <= 7 * int64_t(cus)) return launch_tiles<1, 4, 2, 1, 2, 2, KS>(tiles, s);
+  if (count_tiles(tiles, 64, 256) > cus) return launch_tiles<1, 4, 2, 2, 1, 2, KS>(tiles, s);
+  // An odd number of tiles of 32 rows, without the last half of a tile of 64 (two products of 8960 x
+  // 1536, 96 rows: 18.2 us and 21.6).
+  if (count_tiles(tiles, 32, 128) < 2 * tiles64) return launch_tiles<1, 4, 1, 1, 1, 3, KS>(tiles, s);
+  return launch_tiles<1, 4, 2, 1, 1, 3, KS>(tiles, s);
 }
 
 }  // namespace

@@ -150,9 +150,9 @@ int launch_thin(int64_t m, const wkv7_w4_group* groups, int n, int cus, hipStrea
     blocks = std::max(blocks, (groups[i].w.k + kW4K - 1) / kW4K);
   }
   if (a.ngroups == 0) return WKV7_OK;
-  // A unit holds two workgroups of 8 waves or one of 16 (three products of 4096 x 4096, one row: 11.6
-  // us in 8 waves of four blocks, 9.9 in 16 of two). Groups of 32 have too many scales and sums in
-  // registers for two blocks at once (13.6 us with one, 22.9 in 16 waves of two).
+  // A unit holds two workgroups of 8 waves or one of 16 (three products of 4096 x 4096: one row 10.1
+  // us in 8 waves of two blocks, twice; 9.5 in 16. 16 rows 20.3 and 14.1). Groups of 32 have too many
+  // scales and sums in registers for two blocks at once (12.6 us with one, 22.9 in 16 waves of two).
   const bool wide = blocks > 16 && KS > 1;
   const int64_t wgs = deal(a, kW4N, (wide ? 1 : 2) * int64_t(cus));
   if (wgs > int64_t(0x7fffffff)) return WKV7_ERR_ARG;

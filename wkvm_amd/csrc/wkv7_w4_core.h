@@ -114,18 +114,28 @@ __global__ __launch_bounds__(64 * NW, 4) void w4_thin_kernel(const W4Args args) 
 
   const W4Bits bits;
   const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
-  uint4 c[U], xf[U][4];
-  uint32_t sc[U][NG];
+  uint4 xf[U][4];
   w4_f32x4 sums[U][NG];
-  // (what lies past k is read from inside it and multiplied by zeros)
-  auto fetch = [&](int tile, int pass) {
+  // What lies past k is read from inside it and multiplied by zeros. No load stands behind a branch, and
+  // two passes' registers take turns: else the wait for one pass would be one for the next one's loads
+  // too (65536 x 2048, one row: 17.2 us; 15.3 so, 4.6 TB/s, and 16.3 with three passes).
+  struct Pass {
+    uint4 c[U];
+    uint32_t sc[U][NG];
+  } even, odd;
+  int next_tile = first, next_pass = 0;
+  auto fetch = [&](Pass& p) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int b = min(wave + NW * (pass * U + u), blocks - 1);
-      c[u] = codes[(int64_t(tile) * blocks + b) * 64];
+      const int b = min(wave + NW * (next_pass * U + u), blocks - 1);
+      p.c[u] = codes[(int64_t(next_tile) * blocks + b) * 64];
 #pragma unroll
       for (int q = 0; q < NG; ++q)
-        sc[u][q] = scales[(int64_t(tile) * groups + min(b * NG + q, groups - 1)) * kW4N];
+        p.sc[u][q] = scales[(int64_t(next_tile) * groups + min(b * NG + q, groups - 1)) * kW4N];
+    }
+    if (++next_pass == passes) {  // (behind the last tile it once more, unused)
+      next_pass = 0;
+      if (next_tile + count < tiles) next_tile += count;
     }
   };
   auto load_x = [&](int pass) {
@@ -134,8 +144,8 @@ __global__ __launch_bounds__(64 * NW, 4) void w4_thin_kernel(const W4Args args) 
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int at = kW4K * (wave + NW * (pass * U + u)) + 32 * j;
-        xf[u][j] = make_uint4(0, 0, 0, 0);
-        if (at < k && li < args.m) xf[u][j] = *reinterpret_cast<const uint4*>(x + at);
+        xf[u][j] = *reinterpret_cast<const uint4*>(x + min(at, k - 32));
+        if (at >= k || li >= args.m) xf[u][j] = make_uint4(0, 0, 0, 0);
       }
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -146,47 +156,12 @@ __global__ __launch_bounds__(64 * NW, 4) void w4_thin_kernel(const W4Args args) 
         for (int j = 0; j < KS; ++j) sums[u][q] = w4_mma(xf[u][q * KS + j], ones, sums[u][q]);
       }
   };
-  fetch(first, 0);
-  if (passes == 1) load_x(0);
-  int turn = 0;
-  for (int tile = first; tile < tiles; tile += count, ++turn) {
-    w4_f32x4 total = {0.f, 0.f, 0.f, 0.f};
-    for (int pass = 0; pass < passes; ++pass) {
-      if (passes > 1) load_x(pass);
-      uint4 c0[U];
-      uint32_t sc0[U][NG];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        c0[u] = c[u];
-#pragma unroll
-        for (int q = 0; q < NG; ++q) sc0[u][q] = sc[u][q];
-      }
-      if (pass + 1 < passes) fetch(tile, pass + 1);
-      else if (tile + count < tiles) fetch(tile + count, 0);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const uint32_t words[4] = {c0[u].x, c0[u].y, c0[u].z, c0[u].w};
-#pragma unroll
-        for (int q = 0; q < NG; ++q) {
-          w4_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int j = 0; j < KS; ++j)
-            acc = w4_mma(xf[u][q * KS + j], w4_expand(words[q * KS + j], bits), acc);
-          const float s = w4_scale(sc0[u][q]), z = w4_minus_zero(sc0[u][q]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            total[e] = fmaf(s, fmaf(z, sums[u][q][e], acc[e]), total[e]);
-        }
-      }
-    }
-    red[turn & 1][wave][lane] = total;
-    __syncthreads();
-    if (wave != turn % NW) continue;  // the waves take turns to join the sums
+  auto join = [&](int tile, int turn) {
     w4_f32x4 v = red[turn & 1][0][lane];
 #pragma unroll
     for (int w = 1; w < NW; ++w) v += red[turn & 1][w][lane];
     const int n = tile * kW4N + li;
-    if (n >= G.w.n) continue;
+    if (n >= G.w.n) return;
     const float bias = G.bias ? bf16_to_f32(G.bias[n]) : 0.f;
 #pragma unroll 1
     for (int e = 0; e < 4; ++e) {
@@ -197,6 +172,41 @@ __global__ __launch_bounds__(64 * NW, 4) void w4_thin_kernel(const W4Args args) 
       if (fabsf(r) < INFINITY) G.y[m * G.ldy + n] = f32_to_bf16(w4_activate(r, G.act));
       else w4_store_direct(G, m, n);
     }
+  };
+  int tile = first, pass = 0, turn = 0;
+  w4_f32x4 total = {0.f, 0.f, 0.f, 0.f};
+  // One pass over a tile; false behind the last.
+  auto step = [&](const Pass& now, Pass& ahead) {
+    if (passes > 1) load_x(pass);
+    fetch(ahead);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t words[4] = {now.c[u].x, now.c[u].y, now.c[u].z, now.c[u].w};
+#pragma unroll
+      for (int q = 0; q < NG; ++q) {
+        w4_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < KS; ++j)
+          acc = w4_mma(xf[u][q * KS + j], w4_expand(words[q * KS + j], bits), acc);
+        const float s = w4_scale(now.sc[u][q]), z = w4_minus_zero(now.sc[u][q]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          total[e] = fmaf(s, fmaf(z, sums[u][q][e], acc[e]), total[e]);
+      }
+    }
+    if (++pass < passes) return true;
+    red[turn & 1][wave][lane] = total;
+    __syncthreads();
+    if (wave == turn % NW) join(tile, turn);  // the waves take turns to join the sums
+    total = w4_f32x4{0.f, 0.f, 0.f, 0.f};
+    pass = 0;
+    ++turn;
+    tile += count;
+    return tile < tiles;
+  };
+  fetch(even);
+  if (passes == 1) load_x(0);
+  while (step(even, odd) && step(odd, even)) {
   }
 }
 

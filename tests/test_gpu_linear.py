@@ -401,3 +401,34 @@ def test_refusals(dev):
     with pytest.raises(ValueError, match="q must be"):
         linear_decode_slots(pool, [1, 2], Q, K, V, G)
     assert torch.equal(pool.cpu(), before)
+
+
+@pytest.mark.parametrize("Hq,K,V", [(4, 64, 64), (2, 128, 128)])
+def test_the_order_of_the_sequences_changes_nothing(dev, Hq, K, V):
+    """Offsets on the host (longest first), on the device (as they come) and in a given order; a number
+    outside of the sequences runs none."""
+    lens = [40, 0, 300, 1, 129, 64, 7]
+    cu = np.concatenate([[0], np.cumsum(lens)]).tolist()
+    ids = [3, 1, 8, 2, 7, 5, 4]
+    before, q, k, v, g = _inputs(31, cu[-1], 4, Hq, K, V)
+    args = [t.to(dev) for t in (q, k, v, g)]
+    device_cu = torch.tensor(cu, dtype=torch.int32, device=dev)
+    pools, ys = [], []
+    for offsets, order in ((cu, None), (device_cu, None), (device_cu, [6, 5, 4, 3, 2, 1, 0]),
+                           (cu, [2, 0, 1, 3, 6, 5, 4])):
+        pools.append(before.to(dev))
+        order = None if order is None else torch.tensor(order, dtype=torch.int32, device=dev)
+        ys.append(linear_prefill_varlen(pools[-1], ids, offsets, *args, seq_order=order))
+    _check(pools[0], ys[0], before, cu, ids, q, k, v, g, 1.0)
+    for pool, y in zip(pools, ys):
+        assert torch.equal(pool, pools[0]) and torch.equal(y, ys[0])
+    pool = before.to(dev)
+    order = torch.tensor([7, -1, 0, 1 << 30, -5, 9, 8], dtype=torch.int32, device=dev)
+    linear_prefill_varlen(pool, ids, device_cu, *args, seq_order=order)
+    assert torch.equal(pool[3], pools[0][3])
+    rest = [r for r in range(9) if r != 3]
+    assert torch.equal(pool[rest], before.to(dev)[rest])
+    for wrong in (order[:6], order.long(), order.cpu(), torch.zeros(14, dtype=torch.int32,
+                                                                    device=dev)[::2]):
+        with pytest.raises(ValueError, match="seq_order"):
+            linear_prefill_varlen(pool, ids, cu, *args, seq_order=wrong)

@@ -31,7 +31,7 @@ def test_abi_refusals(change, code):
     want = getattr(_lib, "WKV7_ERR_" + code)
     io = _io(**change)
     assert lib.wkv7_linear_decode(dummy, 5, dummy, None, 2, io, None) == want
-    assert lib.wkv7_linear_prefill(dummy, 5, dummy, dummy, 1, 2, io, 0, None, 0, None) == want
+    assert lib.wkv7_linear_prefill(dummy, 5, dummy, dummy, None, 1, 2, io, 0, None, 0, None) == want
 
 
 def test_abi_refusals_of_the_call():
@@ -44,12 +44,12 @@ def test_abi_refusals_of_the_call():
     assert lib.wkv7_linear_decode(p, 5, p, None, -1, io, None) == A
     assert lib.wkv7_linear_decode(p, 5, p, None, 2, None, None) == A
     assert lib.wkv7_linear_decode(p, 5, None, None, 0, io, None) == _lib.WKV7_OK
-    assert lib.wkv7_linear_prefill(p, 5, p, p, -1, 2, io, 0, None, 0, None) == A
-    assert lib.wkv7_linear_prefill(p, 5, None, p, 1, 2, io, 0, None, 0, None) == A
-    assert lib.wkv7_linear_prefill(p, 5, p, None, 1, 2, io, 0, None, 0, None) == A
-    assert lib.wkv7_linear_prefill(p, 5, p, p, 1, 1 << 31, io, 0, None, 0, None) == A
-    assert lib.wkv7_linear_prefill(p, 5, p, p, 1, -1, io, 0, None, 0, None) == A
-    assert lib.wkv7_linear_prefill(p, 5, None, None, 0, 0, io, 0, None, 0, None) == _lib.WKV7_OK
+    assert lib.wkv7_linear_prefill(p, 5, p, p, None, -1, 2, io, 0, None, 0, None) == A
+    assert lib.wkv7_linear_prefill(p, 5, None, p, None, 1, 2, io, 0, None, 0, None) == A
+    assert lib.wkv7_linear_prefill(p, 5, p, None, None, 1, 2, io, 0, None, 0, None) == A
+    assert lib.wkv7_linear_prefill(p, 5, p, p, None, 1, 1 << 31, io, 0, None, 0, None) == A
+    assert lib.wkv7_linear_prefill(p, 5, p, p, None, 1, -1, io, 0, None, 0, None) == A
+    assert lib.wkv7_linear_prefill(p, 5, None, None, None, 0, 0, io, 0, None, 0, None) == _lib.WKV7_OK
     assert lib.wkv7_linear_prefill_workspace_bytes(0, 100, io) == 0
     assert lib.wkv7_linear_prefill_workspace_bytes(1, 100, None) == 0
 

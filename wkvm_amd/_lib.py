@@ -162,7 +162,7 @@ SIGNATURES = {
     "wkv7_linear_decode": (ctypes.c_int, [
         _vp, _i64, _vp, _vp, _i32, ctypes.POINTER(LinearIO), _vp]),
     "wkv7_linear_prefill": (ctypes.c_int, [
-        _vp, _i64, _vp, _vp, _i32, _i64, ctypes.POINTER(LinearIO), _i32, _vp, _sz, _vp]),
+        _vp, _i64, _vp, _vp, _vp, _i32, _i64, ctypes.POINTER(LinearIO), _i32, _vp, _sz, _vp]),
     "wkv7_linear_prefill_workspace_bytes": (_sz, [_i32, _i64, ctypes.POINTER(LinearIO)]),
     "wkv7_w4_code_bytes": (_sz, [_i32, _i32]),
     "wkv7_w4_scale_bytes": (_sz, [_i32, _i32, _i32]),

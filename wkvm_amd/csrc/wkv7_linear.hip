@@ -205,9 +205,10 @@ extern "C" size_t wkv7_linear_prefill_workspace_bytes(int32_t nseq, int64_t tota
 }
 
 extern "C" int wkv7_linear_prefill(float* state, int64_t num_rows, const int32_t* slot_ids,
-                                   const int32_t* cu_seqlens, int32_t nseq, int64_t total_tokens,
-                                   const wkv7_linear_io* io, int32_t zero_init, void* workspace,
-                                   size_t workspace_bytes, void* stream) {
+                                   const int32_t* cu_seqlens, const int32_t* seq_order,
+                                   int32_t nseq, int64_t total_tokens, const wkv7_linear_io* io,
+                                   int32_t zero_init, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
   if (nseq < 0 || total_tokens > int64_t(0x7fffffff)) return WKV7_ERR_ARG;
   const int rc = validate(state, num_rows, total_tokens, io);
   if (rc != WKV7_OK) return rc;
@@ -225,6 +226,7 @@ extern "C" int wkv7_linear_prefill(float* state, int64_t num_rows, const int32_t
   sq.rows = num_rows;
   sq.slot_ids = slot_ids;
   sq.cu = cu_seqlens;
+  sq.order = seq_order;
   sq.nseq = nseq;
   sq.tokens = total_tokens;
   sq.zero_init = zero_init != 0;

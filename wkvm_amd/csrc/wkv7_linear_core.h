@@ -44,6 +44,7 @@ struct LinearSeqs {
   // Piece g of sequence s, tokens [cu[s] + g piece, ..), is number first_piece(s) + g of `slots`; piece
   // 0: a sequence is one piece, number s.
   int64_t piece, slots;
+  const int32_t* order;  // of whole sequences (or null): the one to start as number i
   float* pieces;   // [slots][H][K][V]: local final states, then the pieces' initial states
   double* sums;    // [slots][H]: sums of log2 decays
 };
@@ -114,6 +115,10 @@ __device__ __forceinline__ int64_t first_piece(const LinearSeqs& a, int s) {
 __device__ __forceinline__ bool find_piece(const LinearSeqs& a, int64_t slot, Piece& p) {
   int s = int(slot);
   int64_t index = 0;
+  if (!a.piece && a.order) {
+    s = a.order[s];
+    if (s < 0 || s >= a.nseq) return false;
+  }
   if (a.piece) {
     // the last sequence whose first piece is at most `slot`, 64 of them at a time
     const int lane = threadIdx.x & 63;

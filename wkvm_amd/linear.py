@@ -143,14 +143,15 @@ def linear_decode_slots(state: torch.Tensor, slot_ids, q, k, v, log_decay, *, sc
 def linear_prefill_varlen(state: torch.Tensor, slot_ids, cu_seqlens, q, k, v, log_decay, *,
                           zero_init: bool = False, scale: float = 1.0,
                           out: torch.Tensor | None = None,
-                          out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+                          out_dtype: torch.dtype = torch.bfloat16,
+                          seq_order: torch.Tensor | None = None) -> torch.Tensor:
     """Ragged prompts: sequence ``s`` runs tokens ``cu_seqlens[s]:cu_seqlens[s+1]`` from the state of
     slot ``slot_ids[s]`` (from zero with ``zero_init``) and leaves its final state there; an empty
     sequence leaves it as it is (zeroes it with ``zero_init``).
 
     ``q``, ``k``, ``v``, ``log_decay`` and the result as for ``linear_decode_slots``, over the T packed
-    tokens. ``cu_seqlens`` is a host sequence or a device int32 tensor. A token's output does not
-    depend on later tokens, whatever they hold. Few sequences are cut into pieces that run side by
+    tokens. ``cu_seqlens`` is a host sequence or a device int32 tensor, ``seq_order`` as for
+    ``wkv7_prefill_varlen``. A token's output does not depend on later tokens, whatever they hold. Few sequences are cut into pieces that run side by
     side, through a workspace from torch's allocator."""
     dims = _check_state(state)
     rows, dev = dims[0], state.device
@@ -170,13 +171,20 @@ def linear_prefill_varlen(state: torch.Tensor, slot_ids, cu_seqlens, q, k, v, lo
         if len(lst) != nseq + 1:
             raise ValueError(f"cu_seqlens has {len(lst)} entries for {nseq} sequences")
         cu = ops._device_plan(lst, dev)
+        if seq_order is None:
+            seq_order = cu[nseq + 1:]
+    if seq_order is not None and not (
+            isinstance(seq_order, torch.Tensor) and seq_order.device == dev
+            and seq_order.dtype == torch.int32 and tuple(seq_order.shape) == (nseq,)
+            and seq_order.is_contiguous()):
+        raise ValueError("seq_order must be a device int32 tensor of nseq entries")
     if nseq:
         lib = _lib.load()
         with on_device(dev):
             ws_bytes = int(lib.wkv7_linear_prefill_workspace_bytes(nseq, T, io))
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-            rc = lib.wkv7_linear_prefill(state.data_ptr(), rows, ids.data_ptr(), cu.data_ptr(), nseq,
-                                         T, io, int(bool(zero_init)), ops._ptr(ws), ws_bytes,
-                                         ops._stream_ptr(dev))
+            rc = lib.wkv7_linear_prefill(state.data_ptr(), rows, ids.data_ptr(), cu.data_ptr(),
+                                         ops._ptr(seq_order), nseq, T, io, int(bool(zero_init)),
+                                         ops._ptr(ws), ws_bytes, ops._stream_ptr(dev))
         _lib.check(rc, "wkv7_linear_prefill")
     return y

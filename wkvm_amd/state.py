@@ -175,12 +175,12 @@ class RWKV7StateBank:
 
     def prefill_linear(self, layer: int, slot_batch, cu_seqlens, q, k, v, log_decay, *,
                        zero_init: bool = False, scale: float = 1.0, out=None,
-                       out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+                       out_dtype: torch.dtype = torch.bfloat16, seq_order=None) -> torch.Tensor:
         """Ragged prompts of a linear-attention ``layer`` (``linear_prefill_varlen``)."""
         ids = slot_batch if isinstance(slot_batch, torch.Tensor) else ops.ids_list(slot_batch, "wkv")
         return linear_prefill_varlen(self.wkv[layer], ids, cu_seqlens, q, k, v, log_decay,
                                      zero_init=zero_init, scale=scale, out=out,
-                                     out_dtype=out_dtype)
+                                     out_dtype=out_dtype, seq_order=seq_order)
 
     def state_bytes(self) -> int:
         return (self.wkv.numel() * self.wkv.element_size()

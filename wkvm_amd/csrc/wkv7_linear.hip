@@ -22,7 +22,8 @@ constexpr int64_t kLinearMaxLd = int64_t(1) << 24;
 
 // One (batch row, head, 64 value columns) of a decode step: lane i owns a column, wave w K / 4 key
 // rows, so that every access of the state is a whole 256-byte run. The state is read and written
-// once, without being kept in the caches.
+// once, without being kept in the caches. HBM bounds it: 256 rows x 32 heads of 64 x 64 in 44.6 us, 6.1
+// TB/s of state; 61 rows x 16 heads of 128 x 128 in 23 us, 5.6 TB/s.
 template <int KD, bool kF32>
 __global__ __launch_bounds__(64 * kDecodeWaves) void linear_decode_kernel(
     float* __restrict__ state, int64_t rows, const int32_t* __restrict__ slot_ids,

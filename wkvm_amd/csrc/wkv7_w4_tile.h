@@ -56,7 +56,9 @@ __device__ __forceinline__ void w4_split3(float v, uint16_t (&p)[3]) {
   }
 }
 
-// Sums of x over its groups: a wave takes 512 inputs of a row, eight to a lane.
+// Sums of x over its groups: a wave takes 512 inputs of a row, eight to a lane. (3 x 3,001 rows of 2048
+// in 9 us, 4.1 TB/s. A product with ones in the tile kernel would be half as many matrix instructions
+// again, shared among four waves a quarter of that.)
 template <int KS>
 __global__ __launch_bounds__(256) void w4_sums_kernel(const W4SumArgs a) {
   constexpr int kLanes = 4 * KS;  // lanes of a group

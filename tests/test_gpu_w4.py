@@ -248,3 +248,59 @@ def test_refusals(dev):
     bad("bias", lambda: proj_w4([(x, weight, torch.zeros(7, dtype=BF16, device=dev))]))
     bad("out must", lambda: proj_w4([(x, weight)], [torch.empty(3, 9, dtype=BF16, device=dev)]))
     bad("GPU tensor", lambda: proj_w4([(x.cpu(), weight)]))
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m,n,k", [(2100, 2111, 160), (128, 16650, 288), (96, 16650, 288),
+                                   (1700, 3100, 512), (130, 16650, 128), (70, 16650, 64)])
+def test_many_tiles(dev, m, n, k, group):
+    """Enough output tiles for every tile shape, k that ends inside a block of 128 and inside a group."""
+    gen = torch.Generator().manual_seed(m)
+    parts = _weight(gen, n, k, group, True)
+    x = _x(gen, m, k)
+    weight = W4Weight.from_codes(*(t.to(dev) for t in parts), group=group)
+    b = torch.randn(n, generator=gen).to(BF16)
+    y, = proj_w4([(x.to(dev), weight, b.to(dev), "tanh")])
+    _check(y, x, parts, group, b, "tanh")
+
+
+@pytest.mark.parametrize("m", [5, 40, 200])
+def test_a_batch_of_infinities_or_nans(dev, m):
+    gen = torch.Generator().manual_seed(m)
+    parts = _weight(gen, 300, 2048, 128, True)
+    weight = W4Weight.from_codes(*(t.to(dev) for t in parts), group=128)
+    x = torch.full((m, 2048), math.nan, dtype=BF16)
+    x[1::2] = math.inf
+    y, = proj_w4([(x.to(dev), weight)])
+    assert y.isnan().all()  # (infinities of both signs among an output's terms)
+    x = _x(gen, m, 2048)
+    x[:, 2047] = math.inf
+    y, = proj_w4([(x.to(dev), weight)])
+    last = _values(*parts, 128)[0][:, 2047].to(dev)
+    assert (y.isnan() == (last == 0)).all()
+    assert (y[:, last != 0] == math.inf * last[last != 0].sign()).all()
+
+
+def test_codes_at_any_address(dev):
+    gen = torch.Generator().manual_seed(4)
+    parts = _weight(gen, 33, 160, 64, True)
+    ref = W4Weight.from_codes(*(t.to(dev) for t in parts), group=64)
+    for shift in (1, 4, 7):
+        room = torch.zeros(33 * 160 + shift, dtype=torch.uint8, device=dev)
+        room[shift:] = parts[0].to(dev).view(-1)
+        got = W4Weight.from_codes(room[shift:].view(33, 160), *(t.to(dev) for t in parts[1:]),
+                                  group=64)
+        assert torch.equal(got.codes, ref.codes) and torch.equal(got.scales, ref.scales)
+
+
+def test_quantize_where_the_range_is_not_finite(dev):
+    """lo and hi of opposite signs and 2e38: their difference is past the largest fp32."""
+    gen = torch.Generator().manual_seed(6)
+    w = ((torch.rand(20, 128, generator=gen) * 2 - 1) * 2e38).to(BF16)
+    w[:, 0], w[:, 1] = 2e38, -2e38
+    got = W4Weight.quantize(w.to(dev), 64).dequantize().cpu().double()
+    s = (w.double().view(20, 2, 64).amax(2) - w.double().view(20, 2, 64).amin(2).clamp(max=0)) / 15
+    err = (got - w.double()).abs().view(20, 2, 64).amax(2)
+    # the code's rounding s / 2, the zero point's s / 2 at the ends, the scale's last bits (15 steps of
+    # 2^-19)
+    assert (err <= s * (1 + 15 * 2.0 ** -18)).all()

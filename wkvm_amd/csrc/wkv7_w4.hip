@@ -42,7 +42,8 @@ __global__ __launch_bounds__(256) void w4_fill_kernel(const wkv7_w4_weight out, 
       lo = fminf(lo, __shfl_xor(lo, d));
       hi = fmaxf(hi, __shfl_xor(hi, d));
     }
-    const float range = src.symmetric ? fmaxf(-lo, hi) / 7.f : (hi - lo) / 15.f;
+    // (halves: the range of finite weights may not be)
+    const float range = src.symmetric ? fmaxf(-lo, hi) / 7.f : (0.5f * hi - 0.5f * lo) / 7.5f;
     word = __float_as_uint(range) & ~15u;
     const float s = w4_scale(word);
     const float z = src.symmetric ? 8.f : s > 0.f ? fminf(fmaxf(rintf(-lo / s), 0.f), 15.f) : 0.f;

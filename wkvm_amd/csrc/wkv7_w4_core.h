@@ -67,11 +67,16 @@ __device__ __forceinline__ void w4_store_direct(const wkv7_w4_group& G, int64_t 
   const uint16_t* x = G.x + m * G.ldx;
   float sum = 0.f;
 #pragma unroll 1
-  for (int i = 0; i < k; ++i) {
+  for (int i = 0; i < k && sum == sum; i += 8) {  // (NaN stays NaN)
     const int lane = (n & 15) + 16 * (i >> 3 & 3);
+    const uint4 xv = *reinterpret_cast<const uint4*>(x + i);
+    const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
     const uint32_t w = G.w.codes[((tile * blocks + i / kW4K) * 64 + lane) * 4 + (i >> 5 & 3)];
     const uint32_t sc = G.w.scales[(tile * groups + i / group) * kW4N + (n & 15)];
-    sum = fmaf(bf16_to_f32(x[i]), w4_scale(sc) * float(w4_code(w, i & 7) - w4_zero(sc)), sum);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      sum = fmaf(e % 2 ? bf16_hi(xw[e / 2]) : bf16_lo(xw[e / 2]),
+                 w4_scale(sc) * float(w4_code(w, e) - w4_zero(sc)), sum);
   }
   if (G.bias) sum += bf16_to_f32(G.bias[n]);
   G.y[m * G.ldy + n] = f32_to_bf16(w4_activate(sum, G.act));

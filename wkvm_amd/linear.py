@@ -15,12 +15,16 @@ The reference has no counterpart (its recurrent layers are RWKV-7's, wkvm/models
 from __future__ import annotations
 
 import contextlib
+import ctypes
+import struct
 
 import torch
 
 from . import _lib, ops
 
 KEY_SIZES = (64, 128)
+_IO_PACK = struct.Struct("@QQQQQqqqqiiiiif")  # the fields of LinearIO
+assert _IO_PACK.size == ctypes.sizeof(_lib.LinearIO)
 _MAX_LD = 1 << 24  # elements from one token to the next that the kernels address
 
 
@@ -90,24 +94,30 @@ def _io(q, k, v, log_decay, dims, dev, tokens, scale, out, out_dtype):
     if Hq < 1 or H % Hq:
         raise ValueError(f"the state's {H} heads must be a multiple of the {Hq} of q and k")
     ops._require_cuda(log_decay, "log_decay")
-    if log_decay.dtype != torch.float32:
+    if log_decay.dtype is not torch.float32:
         raise ValueError(f"log_decay must be float32, got {log_decay.dtype}")
-    if tuple(log_decay.shape) not in ((H,), (tokens, H)):
+    if log_decay.shape not in ((H,), (tokens, H)):
         raise ValueError(f"log_decay must be [{H}] or [{tokens}, {H}], got "
                          f"{tuple(log_decay.shape)}")
     if log_decay.device != dev:
         raise ValueError(f"log_decay on {log_decay.device}, state on {dev}")
     fixed = log_decay.dim() == 1
-    if H > 1 and log_decay.stride(-1) != 1 or not fixed and tokens > 1 and log_decay.stride(0) < H:
+    if not log_decay.is_contiguous() and (
+            H > 1 and log_decay.stride(-1) != 1
+            or not fixed and tokens > 1 and log_decay.stride(0) < H):
         log_decay = log_decay.clone(memory_format=torch.contiguous_format)
     ldd = 0 if fixed else H if tokens <= 1 else log_decay.stride(0)
     dtype = out.dtype if out is not None else out_dtype
     code = ops._y_code(dtype)
-    y = ops._out(out, (tokens, H, V), dtype, dev, "out")
-    if y.device != dev or y.data_ptr() % 16:
-        raise ValueError("out must be 16-byte aligned and on the state's device")
-    io = _lib.LinearIO(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
-                       y.data_ptr(), ldq, ldk, ldv, ldd, H, Hq, K, V, code, float(scale))
+    if out is None:
+        y = torch.empty((tokens, H, V), dtype=dtype, device=dev)
+    else:
+        y = ops._out(out, (tokens, H, V), dtype, dev, "out")
+        if y.device != dev or y.data_ptr() % 16:
+            raise ValueError("out must be 16-byte aligned and on the state's device")
+    io = _lib.LinearIO.from_buffer(bytearray(_IO_PACK.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), y.data_ptr(), ldq, ldk, ldv,
+        ldd, H, Hq, K, V, code, scale)))
     return io, y, (q, k, v, log_decay)
 
 

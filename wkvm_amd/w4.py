@@ -174,10 +174,16 @@ def proj_w4(products: Sequence[tuple], outs: Sequence[torch.Tensor | None] | Non
         if k != w.k:
             raise ValueError(f"x must be [{M}, {w.k}], got {tuple(last.shape)}")
         n = w.n
-        if bias is not None:
-            bias = ops._bf16_2d(bias.reshape(-1), "bias", (n,))
+        if bias is None:
+            bias_ptr = 0
+        else:
+            if not (bias.dtype is bf16 and bias.shape == (n,) and bias.is_contiguous()
+                    and bias.is_cuda):
+                bias = ops._bf16_2d(bias.reshape(-1), "bias", (n,))
             if bias.device != dev:
                 raise ValueError("projection tensors must share a device")
+            bias_ptr = bias.data_ptr()
+            keep.append(bias)
         y = outs[i] if outs is not None and i < len(outs) else None
         if y is None:
             y = last.new_empty((M, n))
@@ -192,9 +198,7 @@ def proj_w4(products: Sequence[tuple], outs: Sequence[torch.Tensor | None] | Non
         if w.device != dev:
             raise ValueError("projection tensors must share a device")
         _GROUP_PACK.pack_into(packed, _GROUP_PACK.size * i, ptr, *w.fields,
-                              0 if bias is None else bias.data_ptr(), y.data_ptr(), ldx, ldy,
-                              ops.ACTIVATIONS[act], 0)
-        keep.append(bias)
+                              bias_ptr, y.data_ptr(), ldx, ldy, ops.ACTIVATIONS[act], 0)
         ys.append(y)
     if M:
         lib = _lib.load()

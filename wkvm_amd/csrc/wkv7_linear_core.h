@@ -21,6 +21,8 @@
 // (2^-18 of each term) for a y that is rounded to bf16.
 #pragma once
 
+#include <type_traits>
+
 #include "wkv7_mfma.h"
 
 namespace wkv7 {
@@ -50,17 +52,28 @@ struct LinearSeqs {
 };
 
 typedef __attribute__((address_space(3))) uint4 lds_u4;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ uint32_t lds_at(const uint4* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_u4*)p));
 }
 // Direct load: 16 bytes per lane from base + offset to lds + 16 l. The compiler does not see it:
-// every wait for it is one of the barriers below.
+// every wait for it is one of the barriers below. kOnce: lines that are not read again are not kept
+// in the caches (with the outputs' stores so too 8 x 4,096 tokens x 32 heads take 134 us, 143 else; the
+// queries, whose lines are read in parts, 178 so).
+template <bool kOnce>
 __device__ __forceinline__ void to_lds16(const void* base, uint32_t offset, uint32_t lds) {
-  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-               :
-               : "{m0}"(lds), "v"(offset), "s"(base)
-               : "memory");
+  if constexpr (kOnce) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
+                 :
+                 : "{m0}"(lds), "v"(offset), "s"(base)
+                 : "memory");
+  } else {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "{m0}"(lds), "v"(offset), "s"(base)
+                 : "memory");
+  }
 }
 // At most N vector memory operations of this wave pending, then the workgroup barrier. (They
 // complete in order, stores among them.)
@@ -195,6 +208,7 @@ struct StateWave {
   Neg neg;
   const uint16_t *knext, *vnext;  // of the first token that no load has asked for (uniform)
   int64_t ldk, ldv;
+  bool keys_once;  // no other workgroup reads these keys
 
   __device__ __forceinline__ StateWave(Lds& l, int wave) : lds(l), mine(wave) {
     const int lane = threadIdx.x & 63;
@@ -232,18 +246,22 @@ struct StateWave {
     auto& st = lds.ring[slot];
     const int lane = threadIdx.x & 63;
     constexpr int KR = 64 / (KD / 8), VR = 64 / (VT / 8);  // rows of a load
+    auto keys_of = [&](auto once) {
 #pragma unroll
-    for (int i = 0; i < KL; ++i) {
-      const int r = KR * (4 * i + mine) + lane / (KD / 8);
-      const int ch = (lane % (KD / 8)) ^ turn<KD>(r);
-      to_lds16(knext, 2 * (min(r, n - 1) * uint32_t(ldk) + 8 * ch),
-               lds_at(st.k) + 1024 * (4 * i + mine));
-    }
+      for (int i = 0; i < KL; ++i) {
+        const int r = KR * (4 * i + mine) + lane / (KD / 8);
+        const int ch = (lane % (KD / 8)) ^ turn<KD>(r);
+        to_lds16<decltype(once)::value>(knext, 2 * (min(r, n - 1) * uint32_t(ldk) + 8 * ch),
+                                        lds_at(st.k) + 1024 * (4 * i + mine));
+      }
+    };
+    if (YP && keys_once) keys_of(std::true_type{});
+    else keys_of(std::false_type{});
 #pragma unroll
     for (int i = 0; i < VL; ++i) {
       const int r = VR * (4 * i + mine) + lane / (VT / 8);
       const int ch = (lane % (VT / 8)) ^ turn<VT>(r);
-      to_lds16(vnext, 2 * (min(r, n - 1) * uint32_t(ldv) + 8 * ch),
+      to_lds16<(YP > 0)>(vnext, 2 * (min(r, n - 1) * uint32_t(ldv) + 8 * ch),
                lds_at(st.v) + 1024 * (4 * i + mine));
     }
     knext += kChunk * ldk;
@@ -460,6 +478,7 @@ __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
     }
     sw.ldk = io.ldk;
     sw.ldv = io.ldv;
+    sw.keys_once = io.H == io.Hq && V == VT;
     sw.knext = io.k + pc.beg * io.ldk + hq * KD;
     sw.vnext = io.v + pc.beg * io.ldv + head * V + col0;
     if (threadIdx.x < 4) lds.bad[threadIdx.x] = 0;
@@ -651,12 +670,13 @@ __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
         const f32x4 &x0 = y[2 * h], &x1 = y[2 * h + 1];
         if (kF32) {
           f32x4* p = reinterpret_cast<f32x4*>(static_cast<float*>(io.y) + o + 32 * h);
-          p[0] = x0;
-          p[1] = x1;
+          __builtin_nontemporal_store(x0, p);
+          __builtin_nontemporal_store(x1, p + 1);
         } else {
-          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(io.y) + o + 32 * h) =
-              make_uint4(pack_bf16(x0[0], x0[1]), pack_bf16(x0[2], x0[3]),
-                         pack_bf16(x1[0], x1[1]), pack_bf16(x1[2], x1[3]));
+          const u32x4 packed = {pack_bf16(x0[0], x0[1]), pack_bf16(x0[2], x0[3]),
+                                pack_bf16(x1[0], x1[1]), pack_bf16(x1[2], x1[3])};
+          __builtin_nontemporal_store(
+              packed, reinterpret_cast<u32x4*>(static_cast<uint16_t*>(io.y) + o + 32 * h));
         }
       }
     }

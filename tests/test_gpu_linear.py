@@ -432,3 +432,31 @@ def test_the_order_of_the_sequences_changes_nothing(dev, Hq, K, V):
                                                                     device=dev)[::2]):
         with pytest.raises(ValueError, match="seq_order"):
             linear_prefill_varlen(pool, ids, cu, *args, seq_order=wrong)
+
+
+@pytest.mark.parametrize("nseq", [2, 9, 62, 63, 64])
+def test_offsets_on_the_device_of_many_workgroups(dev, nseq):
+    """More workgroups than units and long sequences on average, so that their lengths decide which
+    starts first: equal, increasing and with empty ones among them, against host offsets."""
+    H, Hq, K, V = 48, 16, 128, 256 if nseq < 9 else 64
+    gen = torch.Generator().manual_seed(nseq)
+    for kind in ("equal", "up", "mixed"):
+        lens = [260] * nseq if kind == "equal" else [200 + 4 * i for i in range(nseq)]
+        if kind == "mixed":
+            lens = torch.randint(0, 640, (nseq,), generator=gen).tolist()
+            lens[0] = 0
+        cu = np.concatenate([[0], np.cumsum(lens)]).tolist()
+        T, ids = cu[-1], list(range(1, nseq + 1))
+        q, k = (torch.randn(T, Hq, K, generator=gen).to(BF16).to(dev) / 8 for _ in range(2))
+        v = torch.randn(T, H, V, generator=gen).to(BF16).to(dev)
+        g = -0.1 * torch.rand(T, H, generator=gen).to(dev)
+        pools = [torch.full((nseq + 2, H, K, V), 0.25, device=dev) for _ in range(2)]
+        offsets = torch.tensor(cu, dtype=torch.int32, device=dev)
+        ys = [linear_prefill_varlen(p, ids, c, q, k, v, g) for p, c in zip(pools, (cu, offsets))]
+        assert torch.equal(ys[0], ys[1]) and torch.equal(pools[0], pools[1])
+        longest = max(range(nseq), key=lambda s: lens[s])
+        a, b = cu[longest], cu[longest + 1]
+        alone = torch.full((2, H, K, V), 0.25, device=dev)
+        y = linear_prefill_varlen(alone, [1], [0, b - a], q[a:b], k[a:b], v[a:b], g[a:b])
+        assert torch.equal(y, ys[1][a:b]) and torch.equal(alone[1], pools[1][longest + 1])
+        assert (pools[1][[0, nseq + 1]] == 0.25).all()

@@ -47,6 +47,7 @@ struct LinearSeqs {
   // 0: a sequence is one piece, number s.
   int64_t piece, slots;
   const int32_t* order;  // of whole sequences (or null): the one to start as number i
+  bool longest_first;    // without an order, and nseq < 64: by length
   float* pieces;   // [slots][H][K][V]: local final states, then the pieces' initial states
   double* sums;    // [slots][H]: sums of log2 decays
 };
@@ -128,6 +129,24 @@ __device__ __forceinline__ int64_t first_piece(const LinearSeqs& a, int s) {
 __device__ __forceinline__ bool find_piece(const LinearSeqs& a, int64_t slot, Piece& p) {
   int s = int(slot);
   int64_t index = 0;
+  if (a.longest_first) {
+    // lane i has the offset and the length of sequence i; the one with `slot` longer ones (of two of
+    // one length the first counts as longer) is it
+    const int lane = threadIdx.x & 63;
+    const int at = int(offset_at(a, min(lane, a.nseq)));
+    const int length = __shfl_down(at, 1) - at;
+    int longer = 0;
+    for (int i = 0; i < a.nseq; ++i) {
+      const int other = __builtin_amdgcn_readlane(length, i);
+      longer += other > length || (other == length && i < lane);
+    }
+    s = __builtin_ctzll(__ballot(lane < a.nseq && longer == s));
+    p.seq = s;
+    p.beg = __builtin_amdgcn_readlane(at, s);
+    p.end = max(int64_t(__builtin_amdgcn_readlane(at, s + 1)), p.beg);
+    p.first = p.last = true;
+    return true;
+  }
   if (!a.piece && a.order) {
     s = a.order[s];
     if (s < 0 || s >= a.nseq) return false;

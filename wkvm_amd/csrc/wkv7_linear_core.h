@@ -446,11 +446,11 @@ __device__ __forceinline__ double sum_decays(Decays& d, float g, int n) {
 }
 
 // Outputs. Waves 0 .. 3 are the state waves, 4 .. 7 and 8 .. 11 the output waves of the even and of
-// the odd chunks. A tick (1.15 us for 64 x 64, some 2,700 cycles) is bound by the state waves' chain
-// (split, products, decayed keys) and, where all units are busy, by the vector work of the splits and
-// the clock under power: 8 x 4,096 tokens x 32 heads in 130 us, 4.1 TB/s of q, k, v and y, at 2.1 of 2.5
-// GHz with vector units busy 44 and matrix units 22 % of the cycles (177 us with one group of output
-// waves and two workgroups on a unit: the state waves wait for the outputs then).
+// the odd chunks. Few workgroups: a tick of 1.15 us (64 keys, 32 columns) is the state waves' chain of
+// split, products and decayed keys. All units busy: memory, in rows of 128 bytes a token (8 x 4,096 tokens
+// x 32 heads 136.5 us, 4.0 TB/s of q, k, v and y; 93 without the outputs, 130 without the chain; vector
+// units busy 50 and matrix units 25 % of the cycles, at 2.1 of 2.5 GHz). With one group of output waves and
+// two workgroups on a unit the state waves wait for the outputs (177 us for 133 then).
 template <int KD, int VT, bool kF32, int R>
 __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
                                                              const wkv7_linear_io io) {

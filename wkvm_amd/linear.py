@@ -161,8 +161,9 @@ def linear_prefill_varlen(state: torch.Tensor, slot_ids, cu_seqlens, q, k, v, lo
 
     ``q``, ``k``, ``v``, ``log_decay`` and the result as for ``linear_decode_slots``, over the T packed
     tokens. ``cu_seqlens`` is a host sequence or a device int32 tensor, ``seq_order`` as for
-    ``wkv7_prefill_varlen``. A token's output does not depend on later tokens, whatever they hold. Few sequences are cut into pieces that run side by
-    side, through a workspace from torch's allocator."""
+    ``wkv7_prefill_varlen``. A token's output does not depend on later tokens, whatever they hold. Few
+    sequences are cut into pieces that run side by side, through a workspace from torch's
+    allocator."""
     dims = _check_state(state)
     rows, dev = dims[0], state.device
     ids = ops.device_ids(slot_ids, rows, dev, "slot_ids", distinct=True, wait=False)

@@ -61,8 +61,8 @@ class W4Weight:
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None = None,
                    group: int = 128) -> W4Weight:
-        """From codes ``[n, k]`` (uint8, 0 .. 15), scales ``[n, ceil(k / group)]`` (bf16 or fp16, finite) and
-        zero points (uint8, 0 .. 15, of the scales' shape; None: 8). Checks the values, so it waits
+        """From codes ``[n, k]`` (uint8, 0 .. 15), scales ``[n, ceil(k / group)]`` (bf16 or fp16, finite)
+        and zero points (uint8, 0 .. 15, of the scales' shape; None: 8). Checks the values, so it waits
         for the device."""
         ops._require_cuda(codes, "codes")
         if codes.dtype != torch.uint8 or codes.dim() != 2:

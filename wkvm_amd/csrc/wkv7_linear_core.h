@@ -448,8 +448,8 @@ __device__ __forceinline__ double sum_decays(Decays& d, float g, int n) {
 // Outputs. Waves 0 .. 3 are the state waves, 4 .. 7 and 8 .. 11 the output waves of the even and of
 // the odd chunks. Few workgroups: a tick of 1.15 us (64 keys, 32 columns) is the state waves' chain of
 // split, products and decayed keys. All units busy: memory, in rows of 128 bytes a token (8 x 4,096 tokens
-// x 32 heads 136.5 us, 4.0 TB/s of q, k, v and y; 93 without the outputs, 130 without the chain; vector
-// units busy 50 and matrix units 25 % of the cycles, at 2.1 of 2.5 GHz). With one group of output waves and
+// x 32 heads 131 us, 4.2 TB/s of q, k, v and y; a third less without the outputs, no less without the
+// chain; vector units busy 50 and matrix units 25 % of the cycles, at 2.1 of 2.5 GHz). With one group of output waves and
 // two workgroups on a unit the state waves wait for the outputs (177 us for 133 then).
 template <int KD, int VT, bool kF32, int R>
 __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,

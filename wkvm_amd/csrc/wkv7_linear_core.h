@@ -21,8 +21,6 @@
 // (2^-18 of each term) for a y that is rounded to bf16.
 #pragma once
 
-#include <type_traits>
-
 #include "wkv7_mfma.h"
 
 namespace wkv7 {
@@ -228,6 +226,7 @@ struct StateWave {
   const uint16_t *knext, *vnext;  // of the first token that no load has asked for (uniform)
   int64_t ldk, ldv;
   bool keys_once;  // no other workgroup reads these keys
+  uint32_t koff[KL], voff[VL];
 
   __device__ __forceinline__ StateWave(Lds& l, int wave) : lds(l), mine(wave) {
     const int lane = threadIdx.x & 63;
@@ -259,30 +258,49 @@ struct StateWave {
         for (int i = 0; i < 4; ++i) to[(key0(rt) + i) * V + col_of(c)] = S[rt][c][i];
   }
 
-  // The direct loads of the next chunk, which has n tokens and goes to ring slot `slot`; rows behind
-  // them read the last token again (their keys are dropped from the state).
+  // The rows that this wave's direct loads bring, from the piece's first token on.
+  __device__ __forceinline__ void aim(const uint16_t* k, const uint16_t* v, int64_t lk, int64_t lv,
+                                      bool once) {
+    knext = k;
+    vnext = v;
+    ldk = lk;
+    ldv = lv;
+    keys_once = once;
+#pragma unroll
+    for (int i = 0; i < KL; ++i) koff[i] = key_offset(i, kChunk);
+#pragma unroll
+    for (int i = 0; i < VL; ++i) voff[i] = value_offset(i, kChunk);
+  }
+  // Bytes from a chunk's first row to the lane's part of load i; of a chunk of n tokens rows behind them
+  // read the last token again (their keys are dropped from the state).
+  __device__ __forceinline__ uint32_t key_offset(int i, int n) const {
+    const int lane = threadIdx.x & 63, r = 64 / (KD / 8) * (4 * i + mine) + lane / (KD / 8);
+    return 2 * (min(r, n - 1) * uint32_t(ldk) + 8 * ((lane % (KD / 8)) ^ turn<KD>(r)));
+  }
+  __device__ __forceinline__ uint32_t value_offset(int i, int n) const {
+    const int lane = threadIdx.x & 63, r = 64 / (VT / 8) * (4 * i + mine) + lane / (VT / 8);
+    return 2 * (min(r, n - 1) * uint32_t(ldv) + 8 * ((lane % (VT / 8)) ^ turn<VT>(r)));
+  }
+  // The direct loads of the next chunk, which has n tokens and goes to ring slot `slot`.
   __device__ __forceinline__ void issue(int slot, int n) {
     auto& st = lds.ring[slot];
-    const int lane = threadIdx.x & 63;
-    constexpr int KR = 64 / (KD / 8), VR = 64 / (VT / 8);  // rows of a load
-    auto keys_of = [&](auto once) {
+    if (n < kChunk) {  // (a piece's last one)
 #pragma unroll
-      for (int i = 0; i < KL; ++i) {
-        const int r = KR * (4 * i + mine) + lane / (KD / 8);
-        const int ch = (lane % (KD / 8)) ^ turn<KD>(r);
-        to_lds16<decltype(once)::value>(knext, 2 * (min(r, n - 1) * uint32_t(ldk) + 8 * ch),
-                                        lds_at(st.k) + 1024 * (4 * i + mine));
-      }
-    };
-    if (YP && keys_once) keys_of(std::true_type{});
-    else keys_of(std::false_type{});
+      for (int i = 0; i < KL; ++i) koff[i] = key_offset(i, n);
 #pragma unroll
-    for (int i = 0; i < VL; ++i) {
-      const int r = VR * (4 * i + mine) + lane / (VT / 8);
-      const int ch = (lane % (VT / 8)) ^ turn<VT>(r);
-      to_lds16<(YP > 0)>(vnext, 2 * (min(r, n - 1) * uint32_t(ldv) + 8 * ch),
-               lds_at(st.v) + 1024 * (4 * i + mine));
+      for (int i = 0; i < VL; ++i) voff[i] = value_offset(i, n);
     }
+    const uint32_t to = lds_at(st.k) + 1024 * mine;
+    if (YP && keys_once) {
+#pragma unroll
+      for (int i = 0; i < KL; ++i) to_lds16<true>(knext, koff[i], to + 4096 * i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < KL; ++i) to_lds16<false>(knext, koff[i], to + 4096 * i);
+    }
+#pragma unroll
+    for (int i = 0; i < VL; ++i)
+      to_lds16<(YP > 0)>(vnext, voff[i], lds_at(st.v) + 1024 * mine + 4096 * i);
     knext += kChunk * ldk;
     vnext += kChunk * ldv;
   }
@@ -495,11 +513,8 @@ __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
       }
       return;
     }
-    sw.ldk = io.ldk;
-    sw.ldv = io.ldv;
-    sw.keys_once = io.H == io.Hq && V == VT;
-    sw.knext = io.k + pc.beg * io.ldk + hq * KD;
-    sw.vnext = io.v + pc.beg * io.ldv + head * V + col0;
+    sw.aim(io.k + pc.beg * io.ldk + hq * KD, io.v + pc.beg * io.ldv + head * V + col0, io.ldk, io.ldv,
+           io.H == io.Hq && V == VT);
     if (threadIdx.x < 4) lds.bad[threadIdx.x] = 0;
 #pragma unroll
     for (int c = 0; c <= kAhead; ++c)
@@ -747,10 +762,8 @@ __global__ __launch_bounds__(320) void linear_states_kernel(const LinearSeqs a,
   if (wave < 4) {
     const int hq = it.head / (io.H / io.Hq);
     State sw(lds, wave);
-    sw.ldk = io.ldk;
-    sw.ldv = io.ldv;
-    sw.knext = io.k + pc.beg * io.ldk + hq * KD;
-    sw.vnext = io.v + pc.beg * io.ldv + head * V + col0;
+    sw.aim(io.k + pc.beg * io.ldk + hq * KD, io.v + pc.beg * io.ldv + head * V + col0, io.ldk, io.ldv,
+           false);
 #pragma unroll
     for (int c = 0; c <= kAhead; ++c)
       if (c < chunks) sw.issue(c, count(c));

@@ -172,7 +172,7 @@ int launch_thin(int64_t m, const wkv7_w4_group* groups, int n, int cus, hipStrea
 constexpr int64_t kMidRows = WKV7_W4_NO_WORKSPACE_ROWS;
 
 template <int TN, int KS>
-int launch_mid(W4Args& a, hipStream_t s) {
+int launch_mid(W4Args& a, int cus, hipStream_t s) {
   const int row_tiles = int((a.m + 31) / 32);
   int64_t end = 0;
   for (int i = 0; i < a.ngroups; ++i) {
@@ -181,7 +181,12 @@ int launch_mid(W4Args& a, hipStream_t s) {
     a.wg_end[i] = int32_t(end);
   }
   const int span = int((end + kW4Xcds - 1) / kW4Xcds);
-  w4_mid_kernel<8, TN, KS><<<unsigned(span) * kW4Xcds, 512, 0, s>>>(a, row_tiles, span);
+  // Eight waves fill a unit, or four twice where there are more tiles than units (three products of 4096
+  // x 4096: 32 rows 11.9 us in eight, 13.8 in four; 64 rows 21.3 and 18.8).
+  if (end > cus)
+    w4_mid_kernel<4, TN, KS><<<unsigned(span) * kW4Xcds, 256, 0, s>>>(a, row_tiles, span);
+  else
+    w4_mid_kernel<8, TN, KS><<<unsigned(span) * kW4Xcds, 512, 0, s>>>(a, row_tiles, span);
   return launch_status();
 }
 
@@ -200,9 +205,9 @@ int launch_mid(int64_t m, const wkv7_w4_group* groups, int n, int cus, hipStream
   // products of 2048 x 2048, 32 rows 8.4 us in 32 columns, 9.6 in 64; 64 rows 13.7 and 10.0). Not for
   // groups of 32, whose sums and scales do not fit the registers then (64 rows 15.7 and 27).
   if constexpr (KS > 1) {
-    if (tiles > cus) return launch_mid<2, KS>(a, s);
+    if (tiles > cus) return launch_mid<2, KS>(a, cus, s);
   }
-  return launch_mid<1, KS>(a, s);
+  return launch_mid<1, KS>(a, cus, s);
 }
 
 int device_cus(int* cus) {

@@ -225,17 +225,28 @@ __device__ __forceinline__ w4_f32x16 w4_mma32(const uint4& a, const uint4& b, w4
 
 constexpr int kW4Xcds = 8;  // workgroups are dealt round-robin over 8 XCDs
 
+typedef __attribute__((address_space(3))) uint4 w4_lds_u4;
+
+// Direct loads, lane l's 16 (4) bytes to lds + 16 l (4 l). The compiler does not see them: they are waited
+// for by the waits and barriers written below alone.
+__device__ __forceinline__ void w4_lds16(const void* src, uint32_t lds) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "{m0}"(lds), "v"(src) : "memory");
+}
+__device__ __forceinline__ void w4_lds4(const void* src, uint32_t lds) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, off" : : "{m0}"(lds), "v"(src) : "memory");
+}
+
 // Some tens of rows: a workgroup per tile of 32 rows by 32 TN columns, the blocks of 128 inputs dealt
 // to its NW waves, on v_mfma_f32_32x32x16_bf16 (lane l, c = l % 32, h = l / 32: row or column c at 8 h ..
-// of 16 inputs; result lane D[8 (i / 4) + 4 h + i % 4][c]). As in the thin kernel there is no barrier
-// before the sums are joined; the loads of a wave's next block are under way while it multiplies one.
-// Three products of 2048 x 2048: 32 rows 8.4 us, 64 rows 10.0, 0.16 PFLOP/s, of which some 4 are the
-// first loads' latency and the join.
+// of 16 inputs; result lane D[8 (i / 4) + 4 h + i % 4][c]). There is no barrier before the sums are
+// joined: a wave's x goes through LDS of its own, whole rows by direct loads (rows read straight into
+// operands, neighbouring lanes from different ones, pass the load unit at 16 bytes a cycle, not 64), its
+// codes and scales to registers; those of its next block are under way while it multiplies one.
 template <int NW, int TN, int KS>
 __global__ __launch_bounds__(64 * NW, 2) void w4_mid_kernel(const W4Args args, int row_tiles,
                                                             int span) {
-  constexpr int NG = 4 / KS;
-  __shared__ float red[NW][TN * 16][64];
+  constexpr int NG = 4 / KS, XL = 8;  // direct loads of a block
+  __shared__ uint4 xs[NW][2][32 * 16];  // rows of 16 chunks, chunk i of row r at i ^ (r % 16)
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int bid = int(blockIdx.x % kW4Xcds) * span + int(blockIdx.x / kW4Xcds);
@@ -253,86 +264,93 @@ __global__ __launch_bounds__(64 * NW, 2) void w4_mid_kernel(const W4Args args, i
     codes[t] = reinterpret_cast<const uint4*>(G.w.codes) + tile * blocks * 64 + (c & 15) + 16 * h;
     scales[t] = G.w.scales + tile * groups * kW4N + (c & 15);
   }
-  const uint16_t* x = G.x + min(m0 + c, M - 1) * G.ldx + 8 * h;
+  const uint16_t* xsrc[XL];
+#pragma unroll
+  for (int i = 0; i < XL; ++i)
+    xsrc[i] = G.x + min(m0 + 4 * i + lane / 16, M - 1) * G.ldx + kW4K * wave;
 
   const W4Bits bits;
   const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
   w4_f32x16 total[TN] = {};
-  uint4 cw[TN][2], xf[4][2];  // words j of inputs 32 j + 8 h .. and of 32 j + 16 + 8 h ..
-  uint32_t sc[TN][NG];
+  struct Codes {
+    uint4 w[TN][2];  // words j of inputs 32 j + 8 h .. and of 32 j + 16 + 8 h ..
+    uint32_t sc[TN][NG];
+  } even, odd;
   // (past k something inside it is read, and not used)
-  auto fetch_codes = [&](int b) {
+  auto fetch = [&](Codes& to, int b) {
 #pragma unroll
     for (int t = 0; t < TN; ++t) {
-      cw[t][0] = codes[t][int64_t(b) * 64];
-      cw[t][1] = codes[t][int64_t(b) * 64 + 32];
+      to.w[t][0] = codes[t][int64_t(b) * 64];
+      to.w[t][1] = codes[t][int64_t(b) * 64 + 32];
 #pragma unroll
-      for (int q = 0; q < NG; ++q) sc[t][q] = scales[t][min(b * NG + q, groups - 1) * kW4N];
+      for (int q = 0; q < NG; ++q) to.sc[t][q] = scales[t][min(b * NG + q, groups - 1) * kW4N];
     }
   };
-  auto fetch_x = [&](int b, int j) {
+  auto issue = [&](int b, int slot) {
+    const uint32_t to = uint32_t(reinterpret_cast<uintptr_t>((w4_lds_u4*)xs[wave][slot]));
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      xf[j][u] = *reinterpret_cast<const uint4*>(x + min(kW4K * b + 32 * j, k - 32) + 16 * u);
-  };
-  if (wave < blocks) {
-    fetch_codes(wave);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) fetch_x(wave, j);
-  }
-  for (int b = wave; b < blocks; b += NW) {
-    uint4 c0[TN][2];
-    uint32_t sc0[TN][NG];
-#pragma unroll
-    for (int t = 0; t < TN; ++t) {
-      c0[t][0] = cw[t][0];
-      c0[t][1] = cw[t][1];
-#pragma unroll
-      for (int q = 0; q < NG; ++q) sc0[t][q] = sc[t][q];
+    for (int i = 0; i < XL; ++i) {
+      const int chunk = 8 * ((lane & 15) ^ ((4 * i + lane / 16) & 15));
+      w4_lds16(xsrc[i] + min(chunk, k - 8 - kW4K * b), to + 1024 * i);
+      xsrc[i] += NW * kW4K;
     }
-    const int next = min(b + NW, blocks - 1);
-    fetch_codes(next);
+  };
+  // Block b; false behind the wave's last.
+  auto step = [&](int& b, int slot, const Codes& now, Codes& next) {
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+    const bool more = b + NW < blocks;
+    fetch(next, more ? b + NW : b);
+    if (more) issue(b + NW, slot ^ 1);
+    const uint4* st = xs[wave][slot] + c * 16;
 #pragma unroll
     for (int q = 0; q < NG; ++q) {
       w4_f32x16 acc[TN] = {}, sum = {};
 #pragma unroll
       for (int j = q * KS; j < (q + 1) * KS; ++j) {
-        if (kW4K * b + 32 * j < k)  // (uniform)
+        if (kW4K * b + 32 * j >= k) continue;  // (uniform)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            sum = w4_mma32(xf[j][u], ones, sum);
+        for (int u = 0; u < 2; ++u) {
+          const uint4 xf = st[(4 * j + 2 * u + h) ^ (c & 15)];
+          sum = w4_mma32(xf, ones, sum);
 #pragma unroll
-            for (int t = 0; t < TN; ++t) {
-              const uint4& w4 = c0[t][u];
-              acc[t] = w4_mma32(
-                  xf[j][u], w4_expand(j == 0 ? w4.x : j == 1 ? w4.y : j == 2 ? w4.z : w4.w, bits),
-                  acc[t]);
-            }
+          for (int t = 0; t < TN; ++t) {
+            const uint4& w = now.w[t][u];
+            acc[t] = w4_mma32(xf, w4_expand(j == 0 ? w.x : j == 1 ? w.y : j == 2 ? w.z : w.w, bits),
+                              acc[t]);
           }
-        fetch_x(next, j);
+        }
       }
 #pragma unroll
       for (int t = 0; t < TN; ++t) {
-        const float s = w4_scale(sc0[t][q]), z = w4_minus_zero(sc0[t][q]);
+        const float s = w4_scale(now.sc[t][q]), z = w4_minus_zero(now.sc[t][q]);
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          total[t][e] = fmaf(s, fmaf(z, sum[e], acc[t][e]), total[t][e]);
+        for (int e = 0; e < 16; ++e) total[t][e] = fmaf(s, fmaf(z, sum[e], acc[t][e]), total[t][e]);
       }
       if (NG > 1) __builtin_amdgcn_sched_barrier(0);  // (one group's sums at a time in registers)
     }
+    b += NW;
+    return more;
+  };
+  if (wave < blocks) {
+    int b = wave;
+    issue(b, 0);
+    fetch(even, b);
+    while (step(b, 0, even, odd) && step(b, 1, odd, even)) {
+    }
   }
+  float* red = reinterpret_cast<float*>(xs[wave]);
 #pragma unroll
   for (int t = 0; t < TN; ++t)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) red[wave][16 * t + e][lane] = total[t][e];
+    for (int e = 0; e < 16; ++e) red[(16 * t + e) * 64 + lane] = total[t][e];
   __syncthreads();
 #pragma unroll 1
   for (int i = wave; i < 16 * TN; i += NW) {
     const int e = i & 15, n = n0 + 32 * (i >> 4) + c;
     const int64_t m = m0 + 8 * (e / 4) + 4 * h + e % 4;
-    float v = red[0][i][lane];
+    float v = reinterpret_cast<const float*>(xs[0])[i * 64 + lane];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) v += red[w][i][lane];
+    for (int w = 1; w < NW; ++w) v += reinterpret_cast<const float*>(xs[w])[i * 64 + lane];
     if (m >= M || n >= G.w.n) continue;
     const float r = fmaf(16.f, v, G.bias ? bf16_to_f32(G.bias[n]) : 0.f);
     if (fabsf(r) < INFINITY) G.y[m * G.ldy + n] = f32_to_bf16(w4_activate(r, G.act));

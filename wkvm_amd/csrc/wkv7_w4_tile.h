@@ -25,8 +25,6 @@
 namespace wkv7 {
 namespace {
 
-typedef __attribute__((address_space(3))) uint4 w4_lds_u4;
-
 struct W4TileArgs {
   wkv7_w4_group g[WKV7_PROJ_MAX_GROUPS];
   int32_t tile_end[WKV7_PROJ_MAX_GROUPS];  // exclusive prefix sums of work items
@@ -96,13 +94,6 @@ __device__ __forceinline__ void w4_activate_all(w4_f32x16& v, int act) {
   }
 }
 
-// Direct loads, lane l's 16 (4) bytes to lds + 16 l (4 l); waited for by w4_barrier alone.
-__device__ __forceinline__ void w4_lds16(const void* src, uint32_t lds) {
-  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "{m0}"(lds), "v"(src) : "memory");
-}
-__device__ __forceinline__ void w4_lds4(const void* src, uint32_t lds) {
-  asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, off" : : "{m0}"(lds), "v"(src) : "memory");
-}
 template <int N>
 __device__ __forceinline__ void w4_barrier() {
   static_assert(N >= 0 && N < 64, "vmcnt range");

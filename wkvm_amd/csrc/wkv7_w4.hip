@@ -167,10 +167,6 @@ int launch_thin(int64_t m, const wkv7_w4_group* groups, int n, int cus, hipStrea
   return launch_status();
 }
 
-// Up to this many rows the mid kernel runs (three products of 2048 x 2048: 64 rows 10.0 us, in tiles
-// 14.3; 96 rows 17.4 and 15).
-constexpr int64_t kMidRows = WKV7_W4_NO_WORKSPACE_ROWS;
-
 template <int TN, int KS>
 int launch_mid(W4Args& a, int cus, hipStream_t s) {
   const int row_tiles = int((a.m + 31) / 32);
@@ -202,8 +198,8 @@ int launch_mid(int64_t m, const wkv7_w4_group* groups, int n, int cus, hipStream
   }
   if (a.ngroups == 0) return WKV7_OK;
   // 64 columns, which share the reads of x, as soon as 32 would be more tiles than units (three
-  // products of 2048 x 2048, 32 rows 8.4 us in 32 columns, 9.6 in 64; 64 rows 13.7 and 10.0). Not for
-  // groups of 32, whose sums and scales do not fit the registers then (64 rows 15.7 and 27).
+  // products of 2048 x 2048, 32 rows 6.6 us in 32 columns, 8.1 in 64; 64 rows 9.3 and 8.4). Not for
+  // groups of 32, whose sums and scales do not fit the registers then.
   if constexpr (KS > 1) {
     if (tiles > cus) return launch_mid<2, KS>(a, cus, s);
   }
@@ -218,7 +214,21 @@ int device_cus(int* cus) {
   return WKV7_OK;
 }
 
-constexpr int64_t kThinRows = 16;
+// Which kernel runs. us for three products of 2048 x 2048 (4096 x 4096, one of 65536 x 2048):
+//   thin and mid kernel: 1 row 5.0 and 5.9 (9.5 and 10.5, 15.6 and 24.2), 4 rows 5.9 both (11.8 and 10.6,
+//   19 and 24), 16 rows 7.8 and 6.1 (14.0 and 10.7, 21 and 25)
+//   mid kernel and output tiles, with the sums before them: 128 rows 12.8 and 15.0 (28.9 and 26.8), 192
+//   rows 18.9 and 15.6; one product of 2048 x 2048, 256 rows 8.3 and 13.9, 512 rows 12.5 and 14.4
+// So a few rows go to the mid kernel where its tiles (32 rows x 64 columns) are one a unit, and many
+// where they are two.
+enum class W4Kernel { kThin, kMid, kTiles };
+W4Kernel choose(int64_t m, const wkv7_w4_group* groups, int n, int cus) {
+  int64_t tiles = 0;
+  for (int i = 0; i < n; ++i) tiles += (int64_t(groups[i].w.n) + 63) / 64 * ((m + 31) / 32);
+  if (m <= (tiles > cus ? 16 : 3)) return W4Kernel::kThin;
+  return m <= WKV7_W4_NO_WORKSPACE_ROWS || tiles <= 2 * int64_t(cus) ? W4Kernel::kMid
+                                                                     : W4Kernel::kTiles;
+}
 
 // Workspace of the tile kernel: the sums of every product's x over its groups.
 size_t sums_bytes(int64_t m, const wkv7_w4_group& g) {
@@ -226,7 +236,7 @@ size_t sums_bytes(int64_t m, const wkv7_w4_group& g) {
 }
 
 size_t workspace_bytes_of(int64_t m, const wkv7_w4_group* groups, int n) {
-  if (m <= kMidRows) return 0;
+  if (m <= WKV7_W4_NO_WORKSPACE_ROWS) return 0;
   size_t bytes = 0;
   for (int i = 0; i < n; ++i) bytes += sums_bytes(m, groups[i]);
   return bytes;
@@ -358,7 +368,7 @@ extern "C" int wkv7_proj_w4(int64_t m, const wkv7_w4_group* groups, int32_t ngro
   if (rc != WKV7_OK) return rc;
   if (m == 0) return WKV7_OK;
   hipStream_t st = as_stream(stream);
-  if (m > kMidRows) {
+  if (m > WKV7_W4_NO_WORKSPACE_ROWS) {
     if (!workspace || workspace_bytes < workspace_bytes_of(m, groups, ngroups))
       return WKV7_ERR_WORKSPACE;
     if (!aligned16(workspace)) return WKV7_ERR_SHAPE;
@@ -366,21 +376,22 @@ extern "C" int wkv7_proj_w4(int64_t m, const wkv7_w4_group* groups, int32_t ngro
   int cus = 0;
   int done = device_cus(&cus);
   if (done != WKV7_OK) return done;
-  if (m > kMidRows) {
-    uint16_t* ws = static_cast<uint16_t*>(workspace);
-    done = launch_tiled<4>(m, groups, ngroups, ws, cus, st);
-    if (done == WKV7_OK) done = launch_tiled<2>(m, groups, ngroups, ws, cus, st);
-    if (done == WKV7_OK) done = launch_tiled<1>(m, groups, ngroups, ws, cus, st);
-    return done;
+  switch (choose(m, groups, ngroups, cus)) {
+    case W4Kernel::kThin:
+      done = launch_thin<4>(m, groups, ngroups, cus, st);
+      if (done == WKV7_OK) done = launch_thin<2>(m, groups, ngroups, cus, st);
+      if (done == WKV7_OK) done = launch_thin<1>(m, groups, ngroups, cus, st);
+      return done;
+    case W4Kernel::kMid:
+      done = launch_mid<4>(m, groups, ngroups, cus, st);
+      if (done == WKV7_OK) done = launch_mid<2>(m, groups, ngroups, cus, st);
+      if (done == WKV7_OK) done = launch_mid<1>(m, groups, ngroups, cus, st);
+      return done;
+    case W4Kernel::kTiles: break;
   }
-  if (m > kThinRows) {
-    done = launch_mid<4>(m, groups, ngroups, cus, st);
-    if (done == WKV7_OK) done = launch_mid<2>(m, groups, ngroups, cus, st);
-    if (done == WKV7_OK) done = launch_mid<1>(m, groups, ngroups, cus, st);
-    return done;
-  }
-  done = launch_thin<4>(m, groups, ngroups, cus, st);
-  if (done == WKV7_OK) done = launch_thin<2>(m, groups, ngroups, cus, st);
-  if (done == WKV7_OK) done = launch_thin<1>(m, groups, ngroups, cus, st);
+  uint16_t* ws = static_cast<uint16_t*>(workspace);
+  done = launch_tiled<4>(m, groups, ngroups, ws, cus, st);
+  if (done == WKV7_OK) done = launch_tiled<2>(m, groups, ngroups, ws, cus, st);
+  if (done == WKV7_OK) done = launch_tiled<1>(m, groups, ngroups, ws, cus, st);
   return done;
 }

@@ -241,7 +241,9 @@ __device__ __forceinline__ void w4_lds4(const void* src, uint32_t lds) {
 // of 16 inputs; result lane D[8 (i / 4) + 4 h + i % 4][c]). There is no barrier before the sums are
 // joined: a wave's x goes through LDS of its own, whole rows by direct loads (rows read straight into
 // operands, neighbouring lanes from different ones, pass the load unit at 16 bytes a cycle, not 64), its
-// codes and scales to registers; those of its next block are under way while it multiplies one.
+// codes and scales to registers; those of its next block are under way while it multiplies one. Bound by
+// the latency of a block's loads and by the vector work: 32 rows of 4096 in 11.8 us, three products of
+// 4096 columns; of 2048 by 8192 11.5 (19.3 with x straight to registers).
 template <int NW, int TN, int KS>
 __global__ __launch_bounds__(64 * NW, 2) void w4_mid_kernel(const W4Args args, int row_tiles,
                                                             int span) {

@@ -304,3 +304,17 @@ def test_quantize_where_the_range_is_not_finite(dev):
     # the code's rounding s / 2, the zero point's s / 2 at the ends, the scale's last bits (15 steps of
     # 2^-19)
     assert (err <= s * (1 + 15 * 2.0 ** -18)).all()
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m,n,k", [(1, 16500, 4128), (3, 16500, 4224), (9, 16500, 128), (4, 100, 4160),
+                                   (64, 16500, 160), (500, 130, 1056), (333, 2048, 96)])
+def test_kernels_of_a_few_rows(dev, m, n, k, group):
+    """One row to sixteen of many columns, short and long k, and many rows of a few columns."""
+    gen = torch.Generator().manual_seed(m + k)
+    parts = _weight(gen, n, k, group, m % 2 == 0)
+    x = _x(gen, m, k + 8)[:, :k]
+    weight = W4Weight.from_codes(*(None if t is None else t.to(dev) for t in parts), group=group)
+    b = torch.randn(n, generator=gen).to(BF16)
+    y, = proj_w4([(x.to(dev), weight, b.to(dev), "sigmoid" if m > 8 else None)])
+    _check(y, x, parts, group, b, "sigmoid" if m > 8 else None)

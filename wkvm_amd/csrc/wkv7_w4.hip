@@ -220,12 +220,17 @@ int device_cus(int* cus) {
 //   mid kernel and output tiles, with the sums before them: 128 rows 12.8 and 15.0 (28.9 and 26.8), 192
 //   rows 18.9 and 15.6; one product of 2048 x 2048, 256 rows 8.3 and 13.9, 512 rows 12.5 and 14.4
 // So a few rows go to the mid kernel where its tiles (32 rows x 64 columns) are one a unit, and many
-// where they are two.
+// where they are two. With more tiles and k past what the thin kernel holds of x at once, it reads x
+// again for each: 32768 x 8192, 1 row 37 us (the mid kernel 33), 16 rows 71 (32).
 enum class W4Kernel { kThin, kMid, kTiles };
 W4Kernel choose(int64_t m, const wkv7_w4_group* groups, int n, int cus) {
   int64_t tiles = 0;
-  for (int i = 0; i < n; ++i) tiles += (int64_t(groups[i].w.n) + 63) / 64 * ((m + 31) / 32);
-  if (m <= (tiles > cus ? 16 : 3)) return W4Kernel::kThin;
+  int k = 0;
+  for (int i = 0; i < n; ++i) {
+    tiles += (int64_t(groups[i].w.n) + 63) / 64 * ((m + 31) / 32);
+    k = std::max(k, groups[i].w.k);
+  }
+  if (m <= (tiles <= cus ? 3 : k <= 4096 ? 16 : 0)) return W4Kernel::kThin;
   return m <= WKV7_W4_NO_WORKSPACE_ROWS || tiles <= 2 * int64_t(cus) ? W4Kernel::kMid
                                                                      : W4Kernel::kTiles;
 }

@@ -55,7 +55,7 @@ def test_abi_refuses_calls():
     assert lib.wkv7_proj_w4(0, groups, 1, None, 0, None) == OK
     assert lib.wkv7_proj_w4_workspace_bytes(64, groups, 8) == 0
     need = lib.wkv7_proj_w4_workspace_bytes(65, groups, 2)
-    assert need == 2 * 65 * 3 * 16 * 2  # three bf16 parts of 16 groups' sums (two there)
+    assert need == 2 * 96 * 3 * 16 * 2  # three bf16 parts of 16 groups' sums (two there), rows by 32
     assert lib.wkv7_proj_w4(65, groups, 2, None, need, None) == _lib.WKV7_ERR_WORKSPACE
     assert lib.wkv7_proj_w4(65, groups, 2, P, need - 1, None) == _lib.WKV7_ERR_WORKSPACE
     assert lib.wkv7_proj_w4(65, groups, 2, ctypes.c_void_p(4104), need, None) == S

@@ -237,7 +237,7 @@ W4Kernel choose(int64_t m, const wkv7_w4_group* groups, int n, int cus) {
 
 // Workspace of the tile kernel: the sums of every product's x over its groups.
 size_t sums_bytes(int64_t m, const wkv7_w4_group& g) {
-  return size_t(m) * 3 * w4_padded_groups(g.w.k, g.w.group) * sizeof(uint16_t);
+  return size_t(m + 31) / 32 * 32 * 3 * w4_padded_groups(g.w.k, g.w.group) * sizeof(uint16_t);
 }
 
 size_t workspace_bytes_of(int64_t m, const wkv7_w4_group* groups, int n) {
@@ -292,7 +292,8 @@ int launch_tiled(int64_t m, const wkv7_w4_group* groups, int n, uint16_t*& ws, i
       sums.x[distinct] = g.x;
       sums.ldx[distinct] = g.ldx;
       sums.k[distinct++] = g.w.k;
-      waves = std::max(waves, m * ((w4_padded_groups(g.w.k, 32 * KS) * 32 * KS + 511) / 512));
+      waves = std::max(waves, (m + 31) / 32 * 32 *
+                                  ((w4_padded_groups(g.w.k, 32 * KS) * 32 * KS + 511) / 512));
       ws += sums_bytes(m, g) / sizeof(uint16_t);
     }
     tiles.sums[at] = sums.sums[same];

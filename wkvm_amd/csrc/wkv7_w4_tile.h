@@ -28,7 +28,8 @@ namespace {
 struct W4TileArgs {
   wkv7_w4_group g[WKV7_PROJ_MAX_GROUPS];
   int32_t tile_end[WKV7_PROJ_MAX_GROUPS];  // exclusive prefix sums of work items
-  const uint16_t* sums[WKV7_PROJ_MAX_GROUPS];  // [m][3][groups, a multiple of 16] parts of X
+  // parts of X, [ceil(m / 32)][groups / 16][3][64][8]: lane c + 32 h of a part has row c at groups 8 h .. + 7
+  const uint16_t* sums[WKV7_PROJ_MAX_GROUPS];
   int64_t m;
   int32_t ngroups;
   int32_t span;  // work items per XCD
@@ -66,10 +67,10 @@ __global__ __launch_bounds__(256) void w4_sums_kernel(const W4SumArgs a) {
   const int parts = (padded * 32 * KS + 511) / 512;  // waves of a row
   const int64_t item = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
   const int64_t row = item / parts;
-  if (row >= a.m) return;
+  if (row >= (a.m + 31) / 32 * 32) return;
   const int i0 = int(item % parts) * 512 + 8 * lane;
   float s = 0.f;
-  if (i0 < k) {
+  if (i0 < k && row < a.m) {
     const uint4 v = *reinterpret_cast<const uint4*>(a.x[g] + row * a.ldx[g] + i0);
     s = ((bf16_lo(v.x) + bf16_hi(v.x)) + (bf16_lo(v.y) + bf16_hi(v.y))) +
         ((bf16_lo(v.z) + bf16_hi(v.z)) + (bf16_lo(v.w) + bf16_hi(v.w)));
@@ -81,7 +82,9 @@ __global__ __launch_bounds__(256) void w4_sums_kernel(const W4SumArgs a) {
   uint16_t p[3];
   w4_split3(s, p);
 #pragma unroll
-  for (int i = 0; i < 3; ++i) a.sums[g][(row * 3 + i) * padded + gi] = p[i];
+  for (int i = 0; i < 3; ++i)
+    a.sums[g][(((row / 32 * (padded / 16) + gi / 16) * 3 + i) * 64 + row % 32 + 32 * (gi / 8 % 2)) * 8 +
+              gi % 8] = p[i];
 }
 
 __device__ __forceinline__ void w4_activate_all(w4_f32x16& v, int act) {
@@ -213,10 +216,11 @@ void w4_tile_kernel(const W4TileArgs args) {
       uint4 xs[TM][3], zs[TN][3];
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
-        const int64_t r = min(m0 + 32 * (TM * wm + i) + c, M - 1);
+        const int64_t tile = min(m0 / 32 + TM * wm + i, (M - 1) / 32);
 #pragma unroll
         for (int p = 0; p < 3; ++p)
-          xs[i][p] = *reinterpret_cast<const uint4*>(args.sums[g] + (r * 3 + p) * padded + g0 + 8 * h);
+          xs[i][p] = *reinterpret_cast<const uint4*>(
+              args.sums[g] + (((tile * (padded / 16) + g0 / 16) * 3 + p) * 64 + lane) * 8);
       }
 #pragma unroll
       for (int j = 0; j < TN; ++j) {

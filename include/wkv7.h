@@ -750,7 +750,7 @@ size_t wkv7_linear_prefill_workspace_bytes(int32_t nseq, int64_t total_tokens,
 
 /*
  * Products with 4-bit weights: up to WKV7_PROJ_MAX_GROUPS independent products in one
- * launch,
+ * call,
  *     y_g = act_g( x_g W_g^T + bias_g ),   W[n][k] = s[n][k / group] (c[n][k] - z[n][k / group])
  * with codes c and zero points z in 0 .. 15 and scales s, one of each per row and `group` (32, 64 or
  * 128) consecutive inputs, the last group possibly shorter. x bf16; a group's products are exact,

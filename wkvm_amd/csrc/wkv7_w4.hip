@@ -179,10 +179,13 @@ int launch_mid(W4Args& a, int cus, hipStream_t s) {
   const int span = int((end + kW4Xcds - 1) / kW4Xcds);
   // Eight waves fill a unit, or four twice where there are more tiles than units (three products of 4096
   // x 4096: 32 rows 11.9 us in eight, 13.8 in four; 64 rows 21.3 and 18.8).
-  if (end > cus)
-    w4_mid_kernel<4, TN, KS><<<unsigned(span) * kW4Xcds, 256, 0, s>>>(a, row_tiles, span);
-  else
-    w4_mid_kernel<8, TN, KS><<<unsigned(span) * kW4Xcds, 512, 0, s>>>(a, row_tiles, span);
+  if constexpr (TN == 2 || KS == 1) {  // (else there are at most as many tiles as units)
+    if (end > cus) {
+      w4_mid_kernel<4, TN, KS><<<unsigned(span) * kW4Xcds, 256, 0, s>>>(a, row_tiles, span);
+      return launch_status();
+    }
+  }
+  w4_mid_kernel<8, TN, KS><<<unsigned(span) * kW4Xcds, 512, 0, s>>>(a, row_tiles, span);
   return launch_status();
 }
 

@@ -308,7 +308,8 @@ def test_quantize_where_the_range_is_not_finite(dev):
 
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("m,n,k", [(1, 16500, 4128), (3, 16500, 4224), (9, 16500, 128), (4, 100, 4160),
-                                   (64, 16500, 160), (500, 130, 1056), (333, 2048, 96)])
+                                   (64, 16500, 160), (500, 130, 1056), (333, 2048, 96),
+                                   (16, 16500, 1056), (13, 16500, 3008), (3, 300, 4160)])
 def test_kernels_of_a_few_rows(dev, m, n, k, group):
     """One row to sixteen of many columns, short and long k, and many rows of a few columns."""
     gen = torch.Generator().manual_seed(m + k)
@@ -318,3 +319,57 @@ def test_kernels_of_a_few_rows(dev, m, n, k, group):
     b = torch.randn(n, generator=gen).to(BF16)
     y, = proj_w4([(x.to(dev), weight, b.to(dev), "sigmoid" if m > 8 else None)])
     _check(y, x, parts, group, b, "sigmoid" if m > 8 else None)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m,n,k", [(230, 4700, 96), (230, 4700, 160), (200, 5000, 416),
+                                   (129, 6600, 1312)])
+def test_tiles_in_two_parts(dev, m, n, k, group):
+    """Output tiles whose waves take blocks of k in turn: one block, two, an odd number of them."""
+    gen = torch.Generator().manual_seed(m + k)
+    parts = _weight(gen, n, k, group, True)
+    x = _x(gen, m, k)
+    weight = W4Weight.from_codes(*(t.to(dev) for t in parts), group=group)
+    y, = proj_w4([(x.to(dev), weight)])
+    _check(y, x, parts, group)
+
+
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+@pytest.mark.parametrize("m,n", [(230, 4700), (2100, 2111), (128, 16650), (96, 16650)])
+def test_an_infinite_input_of_output_tiles(dev, m, n, bad):
+    gen = torch.Generator().manual_seed(6)
+    parts = _weight(gen, n, 160, 64, True)
+    x = _x(gen, m, 160)
+    x[m // 2, 37] = bad
+    weight = W4Weight.from_codes(*(t.to(dev) for t in parts), group=64)
+    y = proj_w4([(x.to(dev), weight)])[0].cpu()
+    want = x[m // 2].double() @ _values(*parts, 64)[0].T
+    got = y[m // 2].double()
+    assert (got.isnan() == want.isnan()).all()
+    inf = want.isinf()
+    assert (got[inf] == want[inf]).all()
+    rest = [i for i in range(m) if i != m // 2]
+    _check(y[rest], x[rest], parts, 64)
+
+
+@pytest.mark.parametrize("m,n", [(230, 4700), (700, 6000), (70, 16650)])
+def test_graph_replays_of_output_tiles(dev, m, n):
+    """The sums' workspace is the graph's own: replays between eager calls of other sizes, twice the
+    same weight and the same x among the products."""
+    gen = torch.Generator().manual_seed(m)
+    parts = _weight(gen, n, 288, 64, True)
+    weight = W4Weight.from_codes(*(t.to(dev) for t in parts), group=64)
+    x, other = _x(gen, m, 288).to(dev), _x(gen, 2 * m, 288).to(dev)
+    proj_w4([(x, weight)])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ys = proj_w4([(x, weight), (x, weight, None, "tanh")])
+    for step in range(4):
+        x.copy_(_x(gen, m, 288))
+        graph.replay()
+        proj_w4([(other, weight)])
+        torch.cuda.synchronize()
+        want = proj_w4([(x, weight), (x, weight, None, "tanh")])
+        assert all(torch.equal(a, b) for a, b in zip(ys, want)), step
+        _check(ys[0], x.cpu(), parts, 64)

@@ -139,8 +139,9 @@ int64_t piece_tokens(int32_t nseq, int64_t tokens, const wkv7_linear_io& io, int
   return chunks > 10 + 2 * piece ? piece * kChunk : 0;
 }
 
+// Numbers of pieces, as first_piece gives them out.
 int64_t piece_slots(int32_t nseq, int64_t tokens, int64_t piece) {
-  return piece ? (tokens + nseq * (piece - 1)) / piece : nseq;
+  return piece ? tokens / piece + nseq : nseq;
 }
 
 size_t workspace_bytes_of(int64_t slots, const wkv7_linear_io& io) {

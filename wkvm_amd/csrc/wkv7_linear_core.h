@@ -119,9 +119,10 @@ __device__ __forceinline__ int64_t offset_at(const LinearSeqs& a, int s) {
   return min(max(int64_t(a.cu[s]), int64_t(0)), a.tokens);
 }
 
-// At least as many numbers further for the next sequence as this one has pieces.
+// At least one number further for the next sequence, and at least as many as this one has pieces: an
+// empty sequence has a number too, whose workgroups clear its state where it begins at zero.
 __device__ __forceinline__ int64_t first_piece(const LinearSeqs& a, int s) {
-  return (offset_at(a, s) + s * (a.piece - 1)) / a.piece;
+  return offset_at(a, s) / a.piece + s;
 }
 
 __device__ __forceinline__ bool find_piece(const LinearSeqs& a, int64_t slot, Piece& p) {

@@ -710,6 +710,7 @@ size_t wkv7_sample_workspace_bytes(int32_t rows, int32_t vocab);
  *   q, k         [tokens, Hq, K] bf16; head h reads head h / (H / Hq) (H a multiple
  *                of Hq), so queries and keys may be shared by several heads
  *   v            [tokens, H, V] bf16;  y [tokens, H, V], contiguous, dtype per y_dtype
+ *                (a bf16 y is the fp32 one rounded once)
  *   log_decay    fp32, head h of token t at log_decay[t * ld_decay + h]; ld_decay 0: one
  *                value per head for every token. At most finite: -inf forgets the
  *                state before the token

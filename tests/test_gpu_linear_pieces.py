@@ -117,3 +117,19 @@ def test_infinities_of_128_keys(dev, where, bad, T):
         assert (np.isnan(got) == np.isnan(want)).all()
         inf = np.isinf(want)
         assert (got[inf] == want[inf]).all()
+
+
+@pytest.mark.parametrize("kind", ["fixed", "token", "strong", "forget", "grow"])
+@pytest.mark.parametrize("lens,H,Hq,K,V", [([700, 64, 1, 33], 3, 3, 64, 128), ([4097], 2, 1, 64, 64),
+                                           ([150, 300], 4, 2, 128, 64), ([400] * 8, 40, 40, 64, 64)])
+def test_a_bf16_output_is_the_fp32_one_rounded(dev, lens, H, Hq, K, V, kind):
+    """Whatever the outputs' type, they are computed in fp32 (and the same states are left)."""
+    cu = np.concatenate([[0], np.cumsum(lens)]).tolist()
+    before, *xs = _inputs(48, cu[-1], H, Hq, K, V, kind)
+    xs = [t.to(dev) for t in xs]
+    got = []
+    for dtype in (F32, BF16):
+        pool = before.to(dev)
+        got.append((linear_prefill_varlen(pool, list(range(1, len(lens) + 1)), cu, *xs, scale=0.2,
+                                          out_dtype=dtype), pool))
+    assert torch.equal(got[0][0].to(BF16), got[1][0]) and torch.equal(got[0][1], got[1][1])

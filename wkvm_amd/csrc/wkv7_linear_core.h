@@ -17,8 +17,9 @@
 //   the other      chunk c - 2: the other scores, their products with the values, the outputs; sums
 //                  of the decays of chunk c + 2
 // The operands that are not bf16 to begin with (scores under their decays, decayed keys, the state)
-// are split into bf16 parts: three where an fp32 result is kept (the state, an fp32 y), two
-// (2^-18 of each term) for a y that is rounded to bf16.
+// are split into three bf16 parts, which hold all of an fp32 number: a bf16 y is the fp32 one rounded
+// once. (With two parts, 2^-18 of each term, 8 x 4,096 tokens x 32 heads take 134.6 us, 133.4 with three;
+// 16,384 tokens x 12 heads 50.6 and 53.8.)
 #pragma once
 
 #include "wkv7_mfma.h"
@@ -31,6 +32,7 @@ constexpr int kLinearXcds = 8;      // workgroups are dealt round-robin over 8 X
 constexpr int kMinPiece = 256;      // tokens of the shortest piece that a sequence is cut into
 constexpr int kChainThreads = 64;
 constexpr int kChainElems = 4 * kChainThreads;
+constexpr int kParts = 3;           // bf16 parts of an fp32 operand
 constexpr double kLog2e = 1.4426950408889634;
 
 struct LinearSeqs {
@@ -190,7 +192,7 @@ __device__ __forceinline__ int at(int r, int e) {
 }
 
 // LDS of a workgroup. Chunk c of k and v sits in ring[c % R].
-template <int KD, int VT, int YP, int R>
+template <int KD, int VT, bool kOutputs, int R>
 struct LinearLds {
   static constexpr int NP = KD / 32, NC = VT / 16;
   static constexpr int kDecays = 5;
@@ -198,7 +200,7 @@ struct LinearLds {
     uint4 k[kChunk * KD / 8];
     uint4 v[kChunk * VT / 8];
   } ring[R];
-  uint4 state[2][YP ? YP * NP * NC * 64 : 1];  // [c % 2]: parts of the state before chunk c
+  uint4 state[2][kOutputs ? kParts * NP * NC * 64 : 1];  // [c % 2]: parts of the state before chunk c
   // of chunk c at [c % kDecays]: its tokens' sums of log2 decays G as two floats each,
   // e^(G_last - G), e^(G_31 - G) of the first 32 tokens, the decays themselves, e^G_last
   struct Decays {
@@ -213,16 +215,16 @@ struct LinearLds {
 };
 
 // The state waves' share of a piece: `mine` 0 .. 3.
-template <int KD, int VT, int YP, int R>
+template <int KD, int VT, bool kOutputs, int R>
 struct StateWave {
-  using Lds = LinearLds<KD, VT, YP, R>;
+  using Lds = LinearLds<KD, VT, kOutputs, R>;
   static constexpr int RT = KD / 64, NC = VT / 16, NP = KD / 32;
   static constexpr int KL = KD / 32, VL = VT / 32;  // direct loads of a wave per chunk
   static constexpr int kLoads = KL + VL;
   Lds& lds;
   int mine, li, lg, kp;
   f32x4 S[RT][NC], next[RT][NC];
-  uint4 keys[RT][2][3];  // the chunk's keys under their decays, transposed, in parts
+  uint4 keys[RT][2][kParts];  // the chunk's keys under their decays, transposed, in parts
   Neg neg;
   const uint16_t *knext, *vnext;  // of the first token that no load has asked for (uniform)
   int64_t ldk, ldv;
@@ -292,7 +294,7 @@ struct StateWave {
       for (int i = 0; i < VL; ++i) voff[i] = value_offset(i, n);
     }
     const uint32_t to = lds_at(st.k) + 1024 * mine;
-    if (YP && keys_once) {
+    if (kOutputs && keys_once) {
 #pragma unroll
       for (int i = 0; i < KL; ++i) to_lds16<true>(knext, koff[i], to + 4096 * i);
     } else {
@@ -301,7 +303,7 @@ struct StateWave {
     }
 #pragma unroll
     for (int i = 0; i < VL; ++i)
-      to_lds16<(YP > 0)>(vnext, voff[i], lds_at(st.v) + 1024 * mine + 4096 * i);
+      to_lds16<kOutputs>(vnext, voff[i], lds_at(st.v) + 1024 * mine + 4096 * i);
     knext += kChunk * ldk;
     vnext += kChunk * ldv;
   }
@@ -313,11 +315,11 @@ struct StateWave {
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
       for (int ct = 0; ct < NC; ++ct) {
-        uint32_t a[YP], b[YP];
-        split_pair<YP>(S[rt][ct][0], S[rt][ct][1], a, neg);
-        split_pair<YP>(S[rt][ct][2], S[rt][ct][3], b, neg);
+        uint32_t a[kParts], b[kParts];
+        split_pair<kParts>(S[rt][ct][0], S[rt][ct][1], a, neg);
+        split_pair<kParts>(S[rt][ct][2], S[rt][ct][3], b, neg);
 #pragma unroll
-        for (int p = 0; p < YP; ++p)
+        for (int p = 0; p < kParts; ++p)
           reinterpret_cast<uint2*>(
               &to[((p * NP + kp) * NC + ct) * 64 + (threadIdx.x & 63)])[half_of(rt)] =
               make_uint2(a[p], b[p]);
@@ -348,7 +350,7 @@ struct StateWave {
         float kd[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) kd[j] = elem(k8, j) * (j < 4 ? l0[j & 3] : l1[j & 3]);
-        split_eight<3>(kd, keys[rt][b], neg);
+        split_eight<kParts>(kd, keys[rt][b], neg);
       }
     }
   }
@@ -376,7 +378,7 @@ struct StateWave {
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int part = 2; part >= 0; --part)
+      for (int part = kParts - 1; part >= 0; --part)
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -473,8 +475,7 @@ __device__ __forceinline__ double sum_decays(Decays& d, float g, int n) {
 template <int KD, int VT, bool kF32, int R>
 __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
                                                              const wkv7_linear_io io) {
-  constexpr int YP = kF32 ? 3 : 2;
-  using State = StateWave<KD, VT, YP, R>;
+  using State = StateWave<KD, VT, true, R>;
   using Lds = typename State::Lds;
   constexpr int NP = State::NP, NC = State::NC, RT = State::RT;
   // Chunk c is asked for in tick c - 1 - kAhead, has landed when tick c - 2 ends (its keys are read
@@ -614,7 +615,7 @@ __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
   if (group == 1) end_tick(0);
 
   f32x4 y[NC];
-  uint4 own[YP];  // the parts of the scores with the wave's own block of 32 tokens
+  uint4 own[kParts];  // the parts of the scores with the wave's own block of 32 tokens
   const int blk = w >> 1;
   bool skip = true;  // nothing to finish
   // Scores with the 32 tokens of block b of chunk c, as an operand's rows.
@@ -637,7 +638,7 @@ __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
 #pragma unroll
     for (int ct = 0; ct < NC; ++ct) y[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int part = YP - 1; part >= 0; --part)
+    for (int part = kParts - 1; part >= 0; --part)
 #pragma unroll
       for (int p = 0; p < NP; ++p)
 #pragma unroll
@@ -657,7 +658,7 @@ __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
         p8[4 * h + i] = s0 + i <= tw ? x : 0.f;
       }
     }
-    split_eight<YP>(p8, own, neg);
+    split_eight<kParts>(p8, own, neg);
     const float es = __builtin_amdgcn_exp2f(thi + tlo) * io.scale;
 #pragma unroll
     for (int ct = 0; ct < NC; ++ct)
@@ -669,7 +670,7 @@ __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
     const auto& dec = lds.decays[unsigned(c) % Lds::kDecays];
     const uint16_t* sk = reinterpret_cast<const uint16_t*>(st.k);
     const uint16_t* sv = reinterpret_cast<const uint16_t*>(st.v);
-    auto values = [&](int b, const uint4 (&pf)[YP]) {
+    auto values = [&](int b, const uint4 (&pf)[kParts]) {
       const int r = 32 * b + 8 * lg + (li >> 2);
 #pragma unroll
       for (int ct = 0; ct < NC; ++ct) {
@@ -677,14 +678,14 @@ __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
         const uint2 x = ld_tr(sv + at<VT>(r, col)), z = ld_tr(sv + at<VT>(r + 4, col));
         const uint4 vf = make_uint4(x.x, x.y, z.x, z.y);
 #pragma unroll
-        for (int part = YP - 1; part >= 0; --part) y[ct] = mma32(vf, pf[part], y[ct]);
+        for (int part = kParts - 1; part >= 0; --part) y[ct] = mma32(vf, pf[part], y[ct]);
       }
     };
     values(blk, own);
     if (blk) {  // the first block, all of it before the wave's tokens: e^(G_t - G_31) e^(G_31 - G_s)
       f32x4 sc[2];
       float p8[8];
-      uint4 before[YP];
+      uint4 before[kParts];
       scores(sk, 0, sc);
       const float ea =
           __builtin_amdgcn_exp2f((dec.hi[tw] - dec.hi[31]) + (dec.lo[tw] - dec.lo[31])) * io.scale;
@@ -694,7 +695,7 @@ __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
 #pragma unroll
         for (int i = 0; i < 4; ++i) p8[4 * h + i] = sc[h][i] * ea * eb[i];
       }
-      split_eight<YP>(p8, before, neg);
+      split_eight<kParts>(p8, before, neg);
       values(0, before);
     }
     const int t = kChunk * c + tw;
@@ -746,7 +747,7 @@ __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
 template <int KD, int VT, int R>
 __global__ __launch_bounds__(320) void linear_states_kernel(const LinearSeqs a,
                                                             const wkv7_linear_io io) {
-  using State = StateWave<KD, VT, 0, R>;
+  using State = StateWave<KD, VT, false, R>;
   constexpr int kAhead = R - 2;  // (as for the outputs, without their ticks behind)
   __shared__ typename State::Lds lds;
   const int lane = threadIdx.x & 63;

@@ -130,8 +130,8 @@ def linear_decode_slots(state: torch.Tensor, slot_ids, q, k, v, log_decay, *, sc
 
     ``q``, ``k`` bf16 ``[B, Hq, K]`` (H a multiple of Hq: head h reads head ``h // (H / Hq)``), ``v``
     bf16 ``[B, H, V]``, rows of any stride; ``log_decay`` fp32 ``[H]`` or ``[B, H]``. Returns
-    ``y [B, H, V]`` in ``out_dtype`` (bf16 or fp32). ``slot_ids`` and ``row_order`` as for
-    ``wkv7_decode_slots``."""
+    ``y [B, H, V]`` in ``out_dtype`` (bf16 or fp32; computed in fp32, rounded once). ``slot_ids`` and
+    ``row_order`` as for ``wkv7_decode_slots``."""
     dims = _check_state(state)
     rows, dev = dims[0], state.device
     ids, order = ops.decode_plan(slot_ids, rows, dev, wait=False)

@@ -1,0 +1,62 @@
+"""linear_prefill_varlen where parts of its sums pass fp32 and the formula does not: token by token in
+float64 (tests/linear_ref.py), the tests' bounds as elsewhere."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from tests.linear_ref import scan, state_bound, y_bound
+from tests.test_gpu_linear import BF16, F32, _check, _inputs, f64
+from tests.test_gpu_linear_pieces import is_cut
+from wkvm_amd import linear_prefill_varlen
+
+pytestmark = pytest.mark.gpu
+
+
+def _run(dev, cu, ids, before, q, k, v, g, zero_init=False, f32=True):
+    pool = before.to(dev)
+    y = linear_prefill_varlen(pool, ids, cu, q.to(dev), k.to(dev), v.to(dev), g.to(dev),
+                              zero_init=zero_init, out_dtype=F32 if f32 else BF16)
+    return pool, y
+
+
+# -- pieces: the decay of a whole piece -----------------------------------------------------------
+
+@pytest.mark.parametrize("g0", [-0.5, -9.0, -30.0, -80.0])
+@pytest.mark.parametrize("T", [300, 2900])
+def test_an_infinite_state_stays_so_under_any_decay(dev, T, g0):
+    """However far a piece decays it, as long as no token's factor is 0; it is NaN behind one that
+    forgets."""
+    assert is_cut(1, T, 2, 2, 64, 64) == (T > 2000)
+    before, q, k, v, _ = _inputs(61, T, 2, 2, 64, 64, rows=3)
+    before[1, 0, 5, 9], before[1, 1, 7, 3] = math.inf, -math.inf
+    g = torch.full((T, 2), g0)
+    g[T - 90, 1] = -math.inf  # (the second head forgets in a later piece)
+    pool, y = _run(dev, [0, T], [1], before, q, k, v, g)
+    ref = f64(before)
+    want, my, ms = scan(ref, [0, T], [1], f64(q), f64(k), f64(v), f64(g), 1.0)
+    assert ref[1, 0, 5, 9] == math.inf and np.isnan(ref[1, 1, 7, 3])
+    for got, w, bound in ((f64(y), want, y_bound(want, my, T, 64, True)),
+                          (f64(pool)[1], ref[1], state_bound(ms[0], T))):
+        ok = np.isfinite(w)
+        assert (np.isnan(got) == np.isnan(w)).all() and (got[np.isinf(w)] == w[np.isinf(w)]).all()
+        assert (np.abs(got[ok] - w[ok]) <= bound[ok]).all()
+
+
+@pytest.mark.parametrize("zero_init", [False, True])
+def test_a_piece_that_grows_past_fp32(dev, zero_init):
+    """A piece's factor e^128 over a state of 1e-30 (or of zeros), then back: no entry passes fp32. (A
+    chunk's exponent, 46 in powers of two, is rounded to fp32: 16 roundings' worth in each of the 8
+    chunks here, of the 472 that the bound holds for 46.)"""
+    T = 2900
+    assert is_cut(1, T, 2, 2, 64, 64)
+    before, q, k, v, _ = _inputs(62, T, 2, 2, 64, 64, rows=3)
+    before *= 1e-30
+    before[1, 0, :, 5] = 0
+    k[:512] = 0
+    g = torch.full((T, 2), -0.05)
+    g[:256], g[256:512] = 0.5, -0.5
+    pool, y = _run(dev, [0, T], [1], before, q, k, v, g, zero_init)
+    _check(pool, y, before, [0, T], [1], q, k, v, g, 1.0, zero_init)

@@ -49,7 +49,7 @@ struct LinearSeqs {
   const int32_t* order;  // of whole sequences (or null): the one to start as number i
   bool longest_first;    // without an order, and nseq < 64: by length
   float* pieces;   // [slots][H][K][V]: local final states, then the pieces' initial states
-  double* sums;    // [slots][H]: sums of log2 decays
+  double* sums;    // [slots][H]: sums of log2 decays, -infinity where a token forgets the state
 };
 
 typedef __attribute__((address_space(3))) uint4 lds_u4;
@@ -808,17 +808,31 @@ __global__ __launch_bounds__(320) void linear_states_kernel(const LinearSeqs a,
   const float now[2] = {load_g(0), load_g(1)};
   float g = load_g(2), after = load_g(3);  // (64 lines of memory: they may take longer than a tick)
   double sum = sum_decays(lds.decays[0], now[0], count(0));
+  // some token's factor is 0 in fp32 (lanes past a chunk's end have the last token's)
+  bool forgets = expf(now[0]) == 0.f || expf(now[1]) == 0.f;
   if (chunks > 1) sum += sum_decays(lds.decays[1], now[1], count(1));
   barrier_lds();
   for (int c = 0; c < chunks; ++c) {
     if (c + 2 < chunks) {
       sum += sum_decays(lds.decays[unsigned(c + 2) % State::Lds::kDecays], g, count(c + 2));
+      forgets |= expf(g) == 0.f;
       g = after;
       after = load_g(c + 4);
     }
     barrier_lds();
   }
-  if (it.tile == 0 && lane == 0) a.sums[it.no * io.H + head] = sum;
+  const bool any = __ballot(forgets);
+  if (it.tile == 0 && lane == 0) a.sums[it.no * io.H + head] = any ? -INFINITY : sum;
+}
+
+// e^(sum) x + add for a sum of log2 decays over any number of tokens (-infinity: a token forgot x). The
+// power of two is applied by itself, so that the factor passes no range that x or the result does not;
+// an infinite x stays so under any decay, but not behind a token that forgot it (0 times infinity).
+__device__ __forceinline__ float decayed(float x, double sum, float add) {
+  if (sum == -INFINITY) return fmaf(0.f, x, add);
+  const double in = fmin(fmax(sum, -400.), 400.), whole = __builtin_floor(in);
+  const float part = sum == sum ? __builtin_amdgcn_exp2f(float(in - whole)) : NAN;
+  return fmaf(part, ldexpf(x, int(whole)), add);
 }
 
 // From the pieces' local final states to their initial states, in order, four entries per thread:
@@ -860,13 +874,8 @@ __global__ __launch_bounds__(kChainThreads) void linear_chain_kernel(const Linea
     for (int u = 0; u < U; ++u) {
       if (g0 + u >= n) break;
       *reinterpret_cast<f32x4*>(p + (g0 + u) * step) = run;
-      const float f = exp2f(float(sum[u]));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // an infinite entry stays so, however small the factor, unless a token forgot the state
-        const bool inf = fabsf(run[i]) == INFINITY && f == 0.f && sum[u] > -1e4;
-        run[i] = inf ? run[i] + local[u][i] : fmaf(f, run[i], local[u][i]);
-      }
+      for (int i = 0; i < 4; ++i) run[i] = decayed(run[i], sum[u], local[u][i]);
     }
   }
 }

@@ -60,3 +60,19 @@ def test_a_piece_that_grows_past_fp32(dev, zero_init):
     g[:256], g[256:512] = 0.5, -0.5
     pool, y = _run(dev, [0, T], [1], before, q, k, v, g, zero_init)
     _check(pool, y, before, [0, T], [1], q, k, v, g, 1.0, zero_init)
+
+
+# -- chunks: growth across the middle ---------------------------------------------------------------
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("K", [64, 128])
+def test_growth_and_decay_across_the_middle_of_a_chunk(dev, K, f32):
+    """e^(G_t - G_31) falls below fp32, e^(G_t - G_s) of the tokens s before does not. (The values behind
+    are zeros, so that only these tokens and the state count.)"""
+    T = 150
+    before, q, k, v, _ = _inputs(63, T, 2, 2, K, 64, rows=3)
+    g = torch.full((T, 2), -0.01)
+    g[27:32], g[34:39] = 12.0, -20.0
+    v[27:] = 0
+    pool, y = _run(dev, [0, T], [1], before, q, k, v, g, f32=f32)
+    _check(pool, y, before, [0, T], [1], q, k, v, g, 1.0)

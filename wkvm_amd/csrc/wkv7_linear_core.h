@@ -202,12 +202,11 @@ struct LinearLds {
   } ring[R];
   uint4 state[2][kOutputs ? kParts * NP * NC * 64 : 1];  // [c % 2]: parts of the state before chunk c
   // of chunk c at [c % kDecays]: its tokens' sums of log2 decays G as two floats each,
-  // e^(G_last - G), e^(G_31 - G) of the first 32 tokens, the decays themselves, e^G_last
+  // e^(G_last - G), the decays themselves, e^G_last
   struct Decays {
     alignas(16) float hi[kChunk];
     alignas(16) float lo[kChunk];
     alignas(16) float left[kChunk];
-    alignas(16) float first[32];
     float raw[kChunk], all;
   } decays[kDecays];
   float part[2][4][VT];
@@ -455,12 +454,11 @@ __device__ __forceinline__ double sum_decays(Decays& d, float g, int n) {
   G += from_lane<0x118>(G);
   G += from_lane<0x142, 0xa>(G);  // the last lane of a row to the next, of two rows to the next two
   G += from_lane<0x143, 0xc>(G);
-  const double last = lane_value(G, 63), mid = lane_value(G, 31);
+  const double last = lane_value(G, 63);
   const float hi = float(G);
   d.hi[lane] = hi;
   d.lo[lane] = float(G - double(hi));
   d.left[lane] = lane < n ? __builtin_amdgcn_exp2f(float(last - G)) : 0.f;
-  if (lane < 32) d.first[lane] = __builtin_amdgcn_exp2f(float(mid - G));
   d.raw[lane] = g;
   if (lane == 0) d.all = __builtin_amdgcn_exp2f(float(last));
   return last;
@@ -682,18 +680,20 @@ __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
       }
     };
     values(blk, own);
-    if (blk) {  // the first block, all of it before the wave's tokens: e^(G_t - G_31) e^(G_31 - G_s)
+    if (blk) {  // the first block, all of it before the wave's tokens
       f32x4 sc[2];
       float p8[8];
       uint4 before[kParts];
       scores(sk, 0, sc);
-      const float ea =
-          __builtin_amdgcn_exp2f((dec.hi[tw] - dec.hi[31]) + (dec.lo[tw] - dec.lo[31])) * io.scale;
+      const float thi = dec.hi[tw], tlo = dec.lo[tw];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const f32x4 eb = *reinterpret_cast<const f32x4*>(&dec.first[8 * lg + 4 * h]);
+        const f32x4 shi = *reinterpret_cast<const f32x4*>(&dec.hi[8 * lg + 4 * h]);
+        const f32x4 slo = *reinterpret_cast<const f32x4*>(&dec.lo[8 * lg + 4 * h]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p8[4 * h + i] = sc[h][i] * ea * eb[i];
+        for (int i = 0; i < 4; ++i)
+          p8[4 * h + i] = sc[h][i] * io.scale *
+                          __builtin_amdgcn_exp2f((thi - shi[i]) + (tlo - slo[i]));
       }
       split_eight<kParts>(p8, before, neg);
       values(0, before);

@@ -76,3 +76,43 @@ def test_growth_and_decay_across_the_middle_of_a_chunk(dev, K, f32):
     v[27:] = 0
     pool, y = _run(dev, [0, T], [1], before, q, k, v, g, f32=f32)
     _check(pool, y, before, [0, T], [1], q, k, v, g, 1.0)
+
+
+# -- products before their decay ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("T", [100, 2900])
+def test_growth_past_fp32_of_small_values(dev, T, f32):
+    """Six tokens grow by e^90 in all, which passes fp32; what they grow does not."""
+    before, q, k, v, _ = _inputs(66, T, 2, 2, 64, 64, rows=3)
+    g = torch.full((T, 2), -0.01)
+    g[T - 73:T - 70], g[T - 70:T - 67], g[T - 60:T - 57] = -30.0, 30.0, -40.0
+    v[T - 76:T - 66] *= 1e-6
+    pool, y = _run(dev, [0, T], [1], before, q, k, v, g, f32=f32)
+    _check(pool, y, before, [0, T], [1], q, k, v, g, 1.0)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("first", [-50.0, -math.inf])
+@pytest.mark.parametrize("T", [1, 40, 150, 2900])
+def test_a_large_state_that_a_token_decays(dev, T, first, f32):
+    """Queries times the state pass fp32 before its decay, and not under it."""
+    before, q, k, v, g = _inputs(64, T, 2, 2, 64, 64, rows=3)
+    q = q.abs() + 0.5
+    before[1] = before[1].abs() * 3e37
+    g[0] = first
+    pool, y = _run(dev, [0, T], [1], before, q, k, v, g, f32=f32)
+    _check(pool, y, before, [0, T], [1], q, k, v, g, 1.0)
+
+
+@pytest.mark.parametrize("zero_init", [False, True])
+@pytest.mark.parametrize("T", [90, 2900])
+def test_large_queries_and_keys_of_small_values(dev, T, zero_init):
+    """A score passes fp32; the state, which holds the keys times the values, does not."""
+    before, q, k, v, g = _inputs(65, T, 2, 2, 64, 64, rows=3)
+    at = T - 70
+    q[at:at + 3] *= 1e20
+    k[at:at + 3] *= 1e20
+    v[at:at + 3] *= 1e-30
+    pool, y = _run(dev, [0, T], [1], before, q, k, v, g, zero_init)
+    _check(pool, y, before, [0, T], [1], q, k, v, g, 1.0, zero_init)

@@ -6,8 +6,9 @@
 //   P[t][s] = scale (q_t . k_s) e^(G_t - G_s)  for s <= t, else 0
 //   y       = P V + scale e^(G_t) Q S
 //   S'      = e^(G_last) S + (e^(G_last - G_s) k_s)^T V
-// Every exponent is a difference of sums inside the chunk, so nothing overflows that the formula
-// itself does not, for any decay.
+// Every exponent is a difference of sums inside the chunk, taken in 64 bits. Where a product passes
+// fp32 before its decay, which the formula need not, the sequence's outputs are computed once more
+// token by token, as are those of a chunk with an infinity or NaN.
 #include <algorithm>
 
 #include "wkv7_linear_core.h"

@@ -211,6 +211,7 @@ struct LinearLds {
   } decays[kDecays];
   float part[2][4][VT];
   int bad[4];  // [c % 4]: something in chunk c is not finite
+  int again;   // some output of another chunk is not
 };
 
 // The state waves' share of a piece: `mine` 0 .. 3.
@@ -464,6 +465,44 @@ __device__ __forceinline__ double sum_decays(Decays& d, float g, int n) {
   return last;
 }
 
+// A piece once more, token by token as the formula is written, by the four state waves: where a product
+// passed fp32 before its decay (a query with a key or with the state, or a factor of growth), which the
+// formula need not. A thread has a column and KD / P keys, whose states are in LDS. One barrier and
+// then one for each token, as the output waves have. (1.0 us a token of 64 keys, 1.8 of 128.)
+template <int KD, int VT, bool kF32>
+__device__ __forceinline__ void one_by_one(float* lds, const wkv7_linear_io& io, const Piece& pc,
+                                           int head, int col0, const float* initial, float* state) {
+  constexpr int P = 256 / VT, J = KD / P;
+  const int col = threadIdx.x % VT, key0 = threadIdx.x / VT * J;
+  float* S = lds + key0 * VT + col;
+  barrier_lds();
+#pragma unroll 1
+  for (int j = 0; j < J; ++j) S[j * VT] = initial ? initial[int64_t(key0 + j) * io.V + col] : 0.f;
+  const int64_t ko = head / (io.H / io.Hq) * KD + key0, vo = int64_t(head) * io.V + col0 + col;
+#pragma unroll 1
+  for (int64_t t = pc.beg; t < pc.end; ++t) {
+    const float d = expf(io.log_decay[t * io.ld_decay + head]);
+    const float v = bf16_to_f32(io.v[t * io.ldv + vo]);
+    float y = 0.f;
+#pragma unroll 1
+    for (int j = 0; j < J; ++j) {
+      const float s = fmaf(d, S[j * VT], bf16_to_f32(io.k[t * io.ldk + ko + j]) * v);
+      y = fmaf(bf16_to_f32(io.q[t * io.ldq + ko + j]) * io.scale, s, y);
+      S[j * VT] = s;
+    }
+    float* sums = lds + KD * VT + (t & 1) * (P * VT) + col;
+    sums[threadIdx.x / VT * VT] = y;
+    barrier_lds();
+    if (threadIdx.x >= VT) continue;
+    for (int p = 1; p < P; ++p) y += sums[p * VT];
+    const int64_t o = t * io.H * io.V + vo;
+    if (kF32) static_cast<float*>(io.y)[o] = y;
+    else static_cast<uint16_t*>(io.y)[o] = f32_to_bf16(y);
+  }
+#pragma unroll 1
+  for (int j = 0; j < J && pc.last; ++j) state[int64_t(key0 + j) * io.V + col] = S[j * VT];
+}
+
 // Outputs. Waves 0 .. 3 are the state waves, 4 .. 7 and 8 .. 11 the output waves of the even and of
 // the odd chunks. Few workgroups: a tick of 1.15 us (64 keys, 32 columns) is the state waves' chain of
 // split, products and decayed keys. All units busy: memory, in rows of 128 bytes a token (8 x 4,096 tokens
@@ -516,11 +555,13 @@ __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
     sw.aim(io.k + pc.beg * io.ldk + hq * KD, io.v + pc.beg * io.ldv + head * V + col0, io.ldk, io.ldv,
            io.H == io.Hq && V == VT);
     if (threadIdx.x < 4) lds.bad[threadIdx.x] = 0;
+    if (threadIdx.x == 0) lds.again = 0;
 #pragma unroll
     for (int c = 0; c <= kAhead; ++c)
       if (c < chunks) sw.issue(c, count(c));
-    sw.load(a.piece ? a.pieces + (it.no * io.H + head) * (KD * V) + col0
-                    : a.zero_init ? nullptr : slot_state, V);
+    const float* initial = a.piece ? a.pieces + (it.no * io.H + head) * (KD * V) + col0
+                                   : a.zero_init ? nullptr : slot_state;
+    sw.load(initial, V);
     barrier_vm<0>();
     sw.prepare(0);
     for (int c = 0; c < chunks; ++c) {
@@ -576,7 +617,15 @@ __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
         }
       }
     }
-    if (pc.last) sw.store(slot_state, V);
+    // The state is stored before all outputs are known to stand, unless it replaces the one they
+    // began with.
+    if (pc.last && initial != slot_state) sw.store(slot_state, V);
+    barrier_lds();
+    if (__builtin_amdgcn_readfirstlane(lds.again))
+      one_by_one<KD, VT, kF32>(reinterpret_cast<float*>(lds.ring), io, pc, it.head, col0, initial,
+                               slot_state);
+    else if (pc.last && initial == slot_state)
+      sw.store(slot_state, V);
     return;
   }
 
@@ -616,6 +665,7 @@ __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
   uint4 own[kParts];  // the parts of the scores with the wave's own block of 32 tokens
   const int blk = w >> 1;
   bool skip = true;  // nothing to finish
+  f32x4 wrong = {0.f, 0.f, 0.f, 0.f};  // NaN as soon as an output is not finite
   // Scores with the 32 tokens of block b of chunk c, as an operand's rows.
   auto scores = [&](const uint16_t* sk, int b, f32x4 (&sc)[2]) {
 #pragma unroll
@@ -698,20 +748,25 @@ __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
       split_eight<kParts>(p8, before, neg);
       values(0, before);
     }
+    uint4 out[NC / 2];
+#pragma unroll
+    for (int h = 0; h < NC / 2; ++h) {
+      const f32x4 &x0 = y[2 * h], &x1 = y[2 * h + 1];
+      out[h] = make_uint4(pack_bf16(x0[0], x0[1]), pack_bf16(x0[2], x0[3]),
+                          pack_bf16(x1[0], x1[1]), pack_bf16(x1[2], x1[3]));
+      wrong = mma32(out[h], make_uint4(0, 0, 0, 0), wrong);
+    }
     const int t = kChunk * c + tw;
     if (t < tokens) {
       const int64_t o = ((pc.beg + t) * io.H + head) * V + col0 + 8 * lg;
 #pragma unroll
       for (int h = 0; h < NC / 2; ++h) {
-        const f32x4 &x0 = y[2 * h], &x1 = y[2 * h + 1];
         if (kF32) {
           f32x4* p = reinterpret_cast<f32x4*>(static_cast<float*>(io.y) + o + 32 * h);
-          p[0] = x0;
-          p[1] = x1;
+          p[0] = y[2 * h];
+          p[1] = y[2 * h + 1];
         } else {
-          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(io.y) + o + 32 * h) =
-              make_uint4(pack_bf16(x0[0], x0[1]), pack_bf16(x0[2], x0[3]),
-                         pack_bf16(x1[0], x1[1]), pack_bf16(x1[2], x1[3]));
+          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(io.y) + o + 32 * h) = out[h];
         }
       }
     }
@@ -729,8 +784,8 @@ __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
     f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int p = 0; p < NP; ++p) zero = mma32(qf[p], make_uint4(0, 0, 0, 0), zero);
-    const float wrong = (zero[0] + zero[1]) + (zero[2] + zero[3]);
-    if (__ballot(wrong != wrong) && lane == 0) lds.bad[c & 3] = 1;
+    const float any = (zero[0] + zero[1]) + (zero[2] + zero[3]);
+    if (__ballot(any != any) && lane == 0) lds.bad[c & 3] = 1;
     skip = end_tick(c);
     // tick c + 1
     load_q(qn, c + 2);
@@ -738,6 +793,13 @@ __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
     if (c + 1 < chunks) end_tick(c + 1);
   }
   if (!skip) finish(chunks - 1 - ((chunks - 1 - group) & 1));
+  const float any = (wrong[0] + wrong[1]) + (wrong[2] + wrong[3]);
+  if (any != any) lds.again = 1;
+  barrier_lds();
+  if (__builtin_amdgcn_readfirstlane(lds.again)) {
+    barrier_vm<0>();  // (the outputs' stores before those of the state waves)
+    for (int t = 0; t < tokens; ++t) barrier_lds();
+  }
 }
 
 // A piece's final state from zero and the sum of its decays, for a piece that is not its sequence's

@@ -135,12 +135,9 @@ def linear_decode_slots(state: torch.Tensor, slot_ids, q, k, v, log_decay, *, sc
     dims = _check_state(state)
     rows, dev = dims[0], state.device
     ids, order = ops.decode_plan(slot_ids, rows, dev, wait=False)
-    if row_order is not None:
-        if not (isinstance(row_order, torch.Tensor) and row_order.is_cuda
-                and row_order.dtype == torch.int32 and row_order.shape == ids.shape):
-            raise ValueError("row_order must be a device int32 tensor shaped like slot_ids")
-        order = row_order
     B = int(ids.shape[0])
+    if row_order is not None:
+        order = ops.packed_ints(row_order, B, dev, "row_order")
     io, y, keep = _io(q, k, v, log_decay, dims, dev, B, scale, out, out_dtype)
     if B:
         with on_device(dev):
@@ -172,11 +169,7 @@ def linear_prefill_varlen(state: torch.Tensor, slot_ids, cu_seqlens, q, k, v, lo
     T = int(v.shape[0]) if v.dim() == 3 else -1
     io, y, keep = _io(q, k, v, log_decay, dims, dev, T, scale, out, out_dtype)
     if isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.is_cuda:
-        if cu_seqlens.dtype != torch.int32 or tuple(cu_seqlens.shape) != (nseq + 1,):
-            raise ValueError("device cu_seqlens must be int32 [nseq + 1]")
-        if cu_seqlens.device != dev:
-            raise ValueError(f"cu_seqlens on {cu_seqlens.device}, state on {dev}")
-        cu = cu_seqlens
+        cu = ops.packed_ints(cu_seqlens, nseq + 1, dev, "cu_seqlens")
     else:
         lst = ops._host_cu(cu_seqlens, T)
         if len(lst) != nseq + 1:
@@ -184,11 +177,8 @@ def linear_prefill_varlen(state: torch.Tensor, slot_ids, cu_seqlens, q, k, v, lo
         cu = ops._device_plan(lst, dev)
         if seq_order is None:
             seq_order = cu[nseq + 1:]
-    if seq_order is not None and not (
-            isinstance(seq_order, torch.Tensor) and seq_order.device == dev
-            and seq_order.dtype == torch.int32 and tuple(seq_order.shape) == (nseq,)
-            and seq_order.is_contiguous()):
-        raise ValueError("seq_order must be a device int32 tensor of nseq entries")
+    if seq_order is not None:
+        ops.packed_ints(seq_order, nseq, dev, "seq_order")
     if nseq:
         lib = _lib.load()
         with on_device(dev):

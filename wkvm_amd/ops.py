@@ -99,6 +99,16 @@ def upload_ints(values: list[int], device: torch.device, wait: bool = True) -> t
     return torch.tensor(values, dtype=torch.int32, pin_memory=True).to(device, non_blocking=True)
 
 
+def packed_ints(t: torch.Tensor, size: int, device: torch.device, what: str) -> torch.Tensor:
+    """``t`` if it is what the kernels read such integers as: ``size`` int32 values one after the
+    other on ``device``."""
+    if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.device == device
+            and t.shape == (size,) and t.is_contiguous()):
+        raise ValueError(f"{what} must be a contiguous device int32 tensor of {size} entries on "
+                         f"{device}")
+    return t
+
+
 class ReplayOrder:
     """The order in which a decode graph's slot ids are written and read: a
     replay after the refresh of its ids, a refresh after the replays that read
@@ -153,7 +163,7 @@ def device_ids(ids, rows: int, device: torch.device, what: str, distinct: bool =
     """Slot ids as a device int32 tensor (``wait`` as in ``upload_ints``).
 
     Host ids (list / tuple / numpy / CPU tensor) are validated first and raise
-    ``ValueError``. A CUDA int32 tensor is taken as already validated: the
+    ``ValueError``. A contiguous CUDA int32 tensor is taken as already validated: the
     kernels skip out-of-range rows without touching memory, and duplicate ids
     in a write set race.
     """
@@ -162,6 +172,8 @@ def device_ids(ids, rows: int, device: torch.device, what: str, distinct: bool =
             raise ValueError(f"{what}: device ids must be a 1-D int32 tensor")
         if ids.device != device:
             raise ValueError(f"{what}: ids on {ids.device}, pool on {device}")
+        if not ids.is_contiguous():
+            raise ValueError(f"{what}: device ids must be contiguous")
         return ids
     return upload_ints(host_ids(ids, rows, what, distinct), device, wait)
 
@@ -235,12 +247,9 @@ def wkv7_decode_slots(wkv_layer: torch.Tensor, slot_ids, r, w, k, v, a, b, *,
     rows, H = _check_pool(wkv_layer)
     dev = wkv_layer.device
     ids, order = decode_plan(slot_ids, rows, dev, wait=False)
-    if row_order is not None:
-        if not (isinstance(row_order, torch.Tensor) and row_order.is_cuda
-                and row_order.dtype == torch.int32 and row_order.shape == ids.shape):
-            raise ValueError("row_order must be a device int32 tensor shaped like slot_ids")
-        order = row_order
     B = int(ids.shape[0])
+    if row_order is not None:
+        order = packed_ints(row_order, B, dev, "row_order")
     xs = _check_vectors((r, w, k, v, a, b), (B, H, HEAD_SIZE), dev, "decode")
     code = _y_code(out.dtype if out is not None else out_dtype)
     y = _out(out, (B, H, HEAD_SIZE), out_dtype if out is None else out.dtype, dev, "out")
@@ -309,10 +318,8 @@ def wkv7_decode_into(state_in: torch.Tensor | None, state_out: torch.Tensor | No
     for ids in (d_in, d_out):
         if ids is not None and int(ids.shape[0]) != B:
             raise ValueError(f"{int(ids.shape[0])} ids for {B} batch rows")
-    if row_order is not None and not (isinstance(row_order, torch.Tensor) and row_order.is_cuda
-                                      and row_order.dtype == torch.int32
-                                      and tuple(row_order.shape) == (B,)):
-        raise ValueError("row_order must be a device int32 tensor of B entries")
+    if row_order is not None:
+        packed_ints(row_order, B, dev, "row_order")
     code = _y_code(out.dtype if out is not None else out_dtype)
     y = _out(out, (B, H, HEAD_SIZE), out_dtype if out is None else out.dtype, dev, "out")
     if B == 0:
@@ -415,9 +422,7 @@ def wkv7_prefill_varlen(wkv_layer: torch.Tensor, slot_ids, cu_seqlens, r, w, k, 
     T = int(r.shape[0]) if r.dim() == 3 else -1
     xs = _check_vectors((r, w, k, v, a, b), (T, H, HEAD_SIZE), dev, "prefill")
     if isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.is_cuda:
-        if cu_seqlens.dtype != torch.int32 or cu_seqlens.shape != (nseq + 1,):
-            raise ValueError("device cu_seqlens must be int32 [nseq + 1]")
-        cu = cu_seqlens
+        cu = packed_ints(cu_seqlens, nseq + 1, dev, "cu_seqlens")
     else:
         lst = _host_cu(cu_seqlens, T)
         if len(lst) != nseq + 1:
@@ -427,9 +432,7 @@ def wkv7_prefill_varlen(wkv_layer: torch.Tensor, slot_ids, cu_seqlens, r, w, k, 
         if seq_order is None:
             seq_order = both[nseq + 1:]
     if seq_order is not None:
-        if not (isinstance(seq_order, torch.Tensor) and seq_order.is_cuda
-                and seq_order.dtype == torch.int32 and seq_order.shape == (nseq,)):
-            raise ValueError("seq_order must be a device int32 tensor of nseq entries")
+        packed_ints(seq_order, nseq, dev, "seq_order")
     code = _y_code(out.dtype if out is not None else out_dtype)
     y = _out(out, (T, H, HEAD_SIZE), out_dtype if out is None else out.dtype, dev, "out")
     if y.data_ptr() % (16 if y.dtype == torch.float32 else 8):
@@ -520,10 +523,8 @@ def wkv7_decode_layers(wkv: torch.Tensor, ids, layer_inputs, *,
     else:
         ids = device_ids(ids, rows, dev, "slot_ids")
         B = int(ids.shape[0])
-    if row_order is not None and not (isinstance(row_order, torch.Tensor) and row_order.is_cuda
-                                      and row_order.dtype == torch.int32
-                                      and row_order.shape == ids.shape):
-        raise ValueError("row_order must be a device int32 tensor shaped like slot_ids")
+    if row_order is not None:
+        packed_ints(row_order, B, dev, "row_order")
     ptrs, keep = layer_vectors(layer_inputs, (B, H, HEAD_SIZE), dev, "decode")
     code = _y_code(out_dtype)
     y = torch.empty((L, B, H, HEAD_SIZE), dtype=out_dtype, device=dev)
@@ -556,9 +557,8 @@ def wkv7_prefill_layers(wkv: torch.Tensor, ids: torch.Tensor, cu_seqlens: torch.
     ids = device_ids(ids, rows, dev, "slot_ids")
     nseq = int(ids.shape[0])
     for t, what, size in ((cu_seqlens, "cu_seqlens", nseq + 1), (seq_order, "seq_order", nseq)):
-        if t is not None and not (t.is_cuda and t.dtype == torch.int32
-                                  and tuple(t.shape) == (size,)):
-            raise ValueError(f"{what} must be a device int32 tensor of {size} entries")
+        if t is not None:
+            packed_ints(t, size, dev, what)
     if nseq == 0:
         return
     token = H * HEAD_SIZE
@@ -623,13 +623,9 @@ def wkv7_prefill_into(state_in: torch.Tensor | None, state_out: torch.Tensor | N
         if seq_order is None:
             seq_order = both[nseq + 1:]
     else:
-        if cu_seqlens.dtype != torch.int32:
-            raise ValueError("device cu_seqlens must be int32")
-        cu = cu_seqlens
-    if seq_order is not None and not (isinstance(seq_order, torch.Tensor) and seq_order.is_cuda
-                                      and seq_order.dtype == torch.int32
-                                      and tuple(seq_order.shape) == (nseq,)):
-        raise ValueError("seq_order must be a device int32 tensor of nseq entries")
+        cu = packed_ints(cu_seqlens, nseq + 1, dev, "cu_seqlens")
+    if seq_order is not None:
+        packed_ints(seq_order, nseq, dev, "seq_order")
     code = _y_code(out.dtype if out is not None else out_dtype)
     y = _out(out, (T, H, HEAD_SIZE), out_dtype if out is None else out.dtype, dev, "out")
     if y.data_ptr() % (16 if y.dtype == torch.float32 else 8):
@@ -1011,9 +1007,7 @@ def seq_plan(slot_ids, cu_seqlens, rows: int, T: int,
                 raise ValueError(f"{nseq} slots for {T} decode tokens")
             cu = torch.arange(nseq + 1, dtype=torch.int32, device=device)
         elif isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.is_cuda:
-            if cu_seqlens.dtype != torch.int32 or cu_seqlens.shape != (nseq + 1,):
-                raise ValueError("device cu_seqlens must be int32 [nseq + 1]")
-            cu = cu_seqlens
+            cu = packed_ints(cu_seqlens, nseq + 1, device, "cu_seqlens")
         else:
             lst = _host_cu(cu_seqlens, T)
             if len(lst) != nseq + 1:

@@ -111,3 +111,9 @@ def test_block_refuses_other_projections_and_host_weights():
     with pytest.raises(ValueError, match="already holds a 4-bit"):
         block.quantize(32, ("v",))
     assert set(block.adapters) == {"k"}
+
+
+def test_a_host_weight_has_no_values():
+    """Its buffers are host memory, which no kernel may be given."""
+    with pytest.raises(ValueError, match="GPU tensor"):
+        W4Weight(4, 32, 32, device="cpu").dequantize()

@@ -120,6 +120,7 @@ class W4Weight:
 
     def dequantize(self) -> torch.Tensor:
         """The values ``[n, k]`` in fp32."""
+        ops._require_cuda(self.codes, "the weight")
         w = torch.empty((self.n, self.k), dtype=torch.float32, device=self.device)
         with on_device(self.device):
             rc = _lib.load().wkv7_w4_unpack(self.desc, w.data_ptr(), ops._stream_ptr(self.device))

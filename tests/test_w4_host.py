@@ -117,3 +117,13 @@ def test_a_host_weight_has_no_values():
     """Its buffers are host memory, which no kernel may be given."""
     with pytest.raises(ValueError, match="GPU tensor"):
         W4Weight(4, 32, 32, device="cpu").dequantize()
+
+
+def test_a_weight_keeps_its_buffers():
+    """The launches hold their addresses: another tensor in their place would not be read, and they
+    would be freed."""
+    weight = W4Weight(40, 96, 32, device="cpu")
+    for name in ("codes", "scales"):
+        with pytest.raises(AttributeError):
+            setattr(weight, name, torch.zeros_like(getattr(weight, name)))
+    assert weight.fields[:2] == (weight.codes.data_ptr(), weight.scales.data_ptr())

@@ -42,14 +42,22 @@ class W4Weight:
         self.n, self.k, self.group = int(n), int(k), int(group)
         self.groups = (self.k + self.group - 1) // self.group
         lib = _lib.load()
-        self.device = torch.device(device)
-        self.codes = torch.empty(lib.wkv7_w4_code_bytes(n, k) // 4, dtype=torch.int32,
-                                 device=self.device)
-        self.scales = torch.empty(lib.wkv7_w4_scale_bytes(n, k, group) // 4, dtype=torch.int32,
-                                  device=self.device)
-        self.device = self.codes.device
-        self.fields = (self.codes.data_ptr(), self.scales.data_ptr(), self.n, self.k, self.group, 0)
+        self._codes = torch.empty(lib.wkv7_w4_code_bytes(n, k) // 4, dtype=torch.int32,
+                                  device=device)
+        self._scales = torch.empty(lib.wkv7_w4_scale_bytes(n, k, group) // 4, dtype=torch.int32,
+                                   device=device)
+        self.device = self._codes.device
+        self.fields = (self._codes.data_ptr(), self._scales.data_ptr(), self.n, self.k, self.group, 0)
         self.desc = _lib.W4Desc(*self.fields)
+
+    # (the launches hold the buffers' addresses: they are written into, not replaced)
+    @property
+    def codes(self) -> torch.Tensor:
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._scales
 
     @property
     def shape(self) -> tuple[int, int]:

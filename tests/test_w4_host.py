@@ -121,9 +121,10 @@ def test_a_host_weight_has_no_values():
 
 def test_a_weight_keeps_its_buffers():
     """The launches hold their addresses: another tensor in their place would not be read, and they
-    would be freed."""
+    would be freed. Until they are filled the weight is zero."""
     weight = W4Weight(40, 96, 32, device="cpu")
     for name in ("codes", "scales"):
         with pytest.raises(AttributeError):
             setattr(weight, name, torch.zeros_like(getattr(weight, name)))
+        assert not getattr(weight, name).any()
     assert weight.fields[:2] == (weight.codes.data_ptr(), weight.scales.data_ptr())

@@ -29,10 +29,17 @@ assert _GROUP_PACK.size == ctypes.sizeof(_lib.W4Group)
 class W4Weight:
     """One ``[n, k]`` weight as 4-bit codes: ``W[n, k] = s (c - z)`` with a scale s and a zero point z in
     0 .. 15 for each row and ``group`` (32, 64 or 128) consecutive inputs, the last group possibly
-    shorter. ``codes`` and ``scales`` are device buffers in the kernels' layout."""
+    shorter. ``codes`` and ``scales`` are device buffers in the kernels' layout, zeros until they
+    are filled."""
 
     def __init__(self, n: int, k: int, group: int = 128,
                  device: torch.device | str = "cuda") -> None:
+        self._hold(n, k, group, device)
+        self._codes.zero_()
+        self._scales.zero_()
+
+    def _hold(self, n: int, k: int, group: int, device) -> W4Weight:
+        """Checks the sizes and allocates the buffers."""
         if n < 1:
             raise ValueError("n must be >= 1")
         if k < 32 or k % 32:
@@ -49,6 +56,7 @@ class W4Weight:
         self.device = self._codes.device
         self.fields = (self._codes.data_ptr(), self._scales.data_ptr(), self.n, self.k, self.group, 0)
         self.desc = _lib.W4Desc(*self.fields)
+        return self
 
     # (the launches hold the buffers' addresses: they are written into, not replaced)
     @property
@@ -76,7 +84,7 @@ class W4Weight:
         if codes.dtype != torch.uint8 or codes.dim() != 2:
             raise ValueError("codes must be a 2-D uint8 tensor")
         n, k = codes.shape
-        weight = cls(n, k, group, codes.device)
+        weight = cls.__new__(cls)._hold(n, k, group, codes.device)
         want = (n, weight.groups)
         ops._require_cuda(scale, "scale")
         if scale.dtype not in (torch.bfloat16, torch.float16) or tuple(scale.shape) != want:
@@ -114,7 +122,7 @@ class W4Weight:
         if w.dtype != torch.bfloat16 or w.dim() != 2:
             raise ValueError("w must be a 2-D bfloat16 tensor")
         n, k = w.shape
-        weight = cls(n, k, group, w.device)
+        weight = cls.__new__(cls)._hold(n, k, group, w.device)
         if not bool(torch.isfinite(w).all()):
             raise ValueError("the weight must be finite")
         if w.stride(1) != 1 or n > 1 and w.stride(0) < k:

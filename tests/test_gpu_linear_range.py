@@ -116,3 +116,24 @@ def test_large_queries_and_keys_of_small_values(dev, T, zero_init):
     v[at:at + 3] *= 1e-30
     pool, y = _run(dev, [0, T], [1], before, q, k, v, g, zero_init)
     _check(pool, y, before, [0, T], [1], q, k, v, g, 1.0, zero_init)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("H,Hq,K,V,T", [(2, 2, 128, 128, 200), (4, 2, 128, 64, 130), (3, 1, 64, 192, 77),
+                                        (2, 1, 128, 64, 2900), (40, 40, 64, 64, 100)])
+def test_a_sequence_that_is_run_again_leaves_the_others(dev, H, Hq, K, V, T, f32):
+    """One of three sequences has large queries and keys of small values: it is as the formula says, the
+    others as they are beside a usual one."""
+    before, q, k, v, g = _inputs(67, 3 * T, H, Hq, K, V)
+    g = g.clamp(max=-0.3)  # (a bound holds 8 additions for each 64 tokens of one by one: some 30 count)
+    cu, ids = [0, T, 2 * T, 3 * T], [4, 1, 7]
+    assert is_cut(3, 3 * T, H, Hq, K, V) == (T > 2000)
+    usual_pool, usual = _run(dev, cu, ids, before, q, k, v, g, f32=f32)
+    at = 2 * T - 40
+    q[at] *= 1e20
+    k[at] *= 1e20
+    v[at] *= 1e-30
+    pool, y = _run(dev, cu, ids, before, q, k, v, g, f32=f32)
+    _check(pool, y, before, cu, ids, q, k, v, g, 1.0)
+    rest = list(range(T)) + list(range(2 * T, 3 * T))
+    assert torch.equal(y[rest], usual[rest]) and torch.equal(pool[[4, 7]], usual_pool[[4, 7]])

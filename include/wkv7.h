@@ -758,12 +758,14 @@ size_t wkv7_linear_prefill_workspace_bytes(int32_t nseq, int64_t total_tokens,
  * call,
  *     y_g = act_g( x_g W_g^T + bias_g ),   W[n][k] = s[n][k / group] (c[n][k] - z[n][k / group])
  * with codes c and zero points z in 0 .. 15 and scales s, one of each per row and `group` (32, 64 or
- * 128) consecutive inputs, the last group possibly shorter. x bf16; a group's products are exact,
- * sums are fp32, y is rounded once to bf16. Any number of rows m.
+ * 128) consecutive inputs, the last group possibly shorter. x bf16; y is rounded once to bf16. Any
+ * number of rows m. A group's sums of x (16 + c) and of x (16 + z) are fp32, their products exact, and
+ * subtracted: errors are 2^-24 of the size of these terms, s |x| (16 + c), also where a code is near or at
+ * its zero point (a row of such codes gives rounding noise about the bias).
  *
  * No counterpart in the reference, whose projections are nn.Linear calls on bf16 weights
- * (external; reached through the model forward, wkvm/runner/runner.py:80-88). A decode step's
- * time is the bytes of its weights; these have a quarter of them.
+ * (external; reached through the model forward, wkvm/runner/runner.py:80-88). Weights take a
+ * quarter of bf16's memory; products of few rows less time, of some hundred as much, of prompts more.
  *
  * A weight is held as
  *   codes   [ceil(n / 16)][ceil(k / 128)][64][4] uint32: of 16 rows and 128 inputs, entry [l][j] has

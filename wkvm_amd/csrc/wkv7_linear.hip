@@ -121,7 +121,7 @@ int device_cus(int* cus) {
 }
 
 // Value columns of a workgroup of the outputs' kernel. Of 128 keys its LDS holds 32; of 64 keys it takes
-// 64, or 32 where that leaves half of the units without one (512 tokens x 32 heads 17.3 and 14.4 us).
+// 64, or 32 where that leaves half of the units without one (512 tokens x 32 heads 18.6 and 15.0 us).
 int value_tile(int32_t nseq, const wkv7_linear_io& io, int cus) {
   return io.K == 128 || 2 * int64_t(nseq) * io.H * (io.V / 64) <= cus ? 32 : 64;
 }
@@ -133,8 +133,8 @@ int64_t piece_tokens(int32_t nseq, int64_t tokens, const wkv7_linear_io& io, int
   const int64_t groups = int64_t(io.H) * (io.V / (io.K == 128 ? 32 : 64)) * nseq;
   const int64_t cuts = int64_t(cus) / groups;  // pieces of a sequence
   if (cuts < 2) return 0;
-  // In chunks: a sequence in one piece takes about 6 us and 1.15 for each; in pieces 18 us and 2.3 for
-  // each chunk of a piece.
+  // In chunks: a sequence in one piece takes about 6 us and 1.2 for each; in pieces 15 to 18 us and 3 for
+  // each chunk of a piece (12 heads: 2,048 tokens in 8 pieces 25.7 us, 16,384 in 20 of 13 chunks 59).
   const int64_t chunks = (tokens + int64_t(nseq) * kChunk - 1) / (int64_t(nseq) * kChunk);
   const int64_t piece = std::max<int64_t>(kMinPiece / kChunk, (chunks + cuts - 1) / cuts);
   return chunks > 10 + 2 * piece ? piece * kChunk : 0;
@@ -150,8 +150,8 @@ size_t workspace_bytes_of(int64_t slots, const wkv7_linear_io& io) {
                                          sizeof(double));
 }
 
-// Chunks of the outputs' ring: one asked for ahead. (More are no faster: 8 x 4,096 tokens x 32 heads 132.5
-// us, 136.4 with six and 137 with seven, the workgroups of neighbouring heads further apart in time.)
+// Chunks of the outputs' ring: one asked for ahead. (More are no faster: 8 x 4,096 tokens x 32 heads 135.4
+// us with five and with six, 512 tokens x 32 heads 15.0 and 15.1.)
 constexpr int kRing = 5;
 
 template <int KD, int VT, bool kF32>
@@ -168,8 +168,8 @@ int launch_prefill(const LinearSeqs& sq, const wkv7_linear_io& io, float* ws, in
   a.sums = ws ? reinterpret_cast<double*>(ws + sq.slots * io.H * int64_t(io.K) * io.V) : nullptr;
   if (grid(32) > int64_t(0x7fffffff)) return WKV7_ERR_ARG;
   // Where a unit takes one workgroup after the other the long sequences go first (19 of up to 2,062
-  // tokens, 16 heads of 128 x 128: 103.5 us, 108.6 as they come; 98 in an order that the host gives).
-  // Finding them costs a workgroup some 0.7 us (32 of 64 tokens, 32 heads: 33 us for 30).
+  // tokens, 16 heads of 128 x 128: 104.8 us, 109.9 as they come). Finding them costs a workgroup some 0.7
+  // us, too much for short ones.
   a.longest_first = !a.piece && !a.order && a.nseq > 1 && a.nseq < 64 &&
                     a.tokens >= int64_t(256) * a.nseq && a.slots * io.H * (io.V / VT) > cus;
   if (a.piece) {

@@ -18,8 +18,8 @@
 //                  of the decays of chunk c + 2
 // The operands that are not bf16 to begin with (scores under their decays, decayed keys, the state)
 // are split into three bf16 parts, which hold all of an fp32 number: a bf16 y is the fp32 one rounded
-// once. (With two parts, 2^-18 of each term, 8 x 4,096 tokens x 32 heads take 134.6 us, 133.4 with three;
-// 16,384 tokens x 12 heads 50.6 and 53.8.)
+// once. (With two parts, 2^-18 of each term, 8 x 4,096 tokens x 32 heads take 134.6 us from memory, 133.4
+// with three; 125 and 140 from the caches. 16,384 tokens x 12 heads 50.6 and 53.8.)
 #pragma once
 
 #include "wkv7_mfma.h"
@@ -59,9 +59,8 @@ __device__ __forceinline__ uint32_t lds_at(const uint4* p) {
 }
 // Direct load: 16 bytes per lane from base + offset to lds + 16 l. The compiler does not see it:
 // every wait for it is one of the barriers below. kOnce: lines that are not read again are not kept
-// in the caches (8 x 4,096 tokens x 32 heads 136.6 us, 138 without, from memory; 134 and 143 where the
-// inputs are those of the call before. The queries, whose lines are read in parts, take 178 so, and the
-// outputs' stores 141).
+// in the caches (19 ragged prompts of 128 channels 104.7 us, 108.1 without; 8 x 4,096 tokens x 32 heads
+// 135.4 and 136.3. The queries, whose lines are read in parts, and the outputs' stores are slower so).
 template <bool kOnce>
 __device__ __forceinline__ void to_lds16(const void* base, uint32_t offset, uint32_t lds) {
   if constexpr (kOnce) {
@@ -504,11 +503,12 @@ __device__ __forceinline__ void one_by_one(float* lds, const wkv7_linear_io& io,
 }
 
 // Outputs. Waves 0 .. 3 are the state waves, 4 .. 7 and 8 .. 11 the output waves of the even and of
-// the odd chunks. Few workgroups: a tick of 1.15 us (64 keys, 32 columns) is the state waves' chain of
+// the odd chunks. Few workgroups: a tick of 1.2 us (64 keys, 32 columns) is the state waves' chain of
 // split, products and decayed keys. All units busy: memory, in rows of 128 bytes a token (8 x 4,096 tokens
-// x 32 heads 131 us, 4.2 TB/s of q, k, v and y; a third less without the outputs, no less without the
-// chain; vector units busy 50 and matrix units 25 % of the cycles, at 2.1 of 2.5 GHz). With one group of output waves and
-// two workgroups on a unit the state waves wait for the outputs (177 us for 133 then).
+// x 32 heads 134 us, 4.1 TB/s of q, k, v and y; vector units busy for 48 and matrix units for 27 % of the
+// cycles, at 2.2 GHz; an earlier form took a third less without the outputs and no less without the
+// chain). With one group of output waves and two workgroups on a unit the state waves wait for the outputs (a
+// third slower).
 template <int KD, int VT, bool kF32, int R>
 __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
                                                              const wkv7_linear_io io) {
@@ -804,7 +804,7 @@ __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
 
 // A piece's final state from zero and the sum of its decays, for a piece that is not its sequence's
 // last: the four state waves and one for the decays. With no outputs to wait for, the decayed keys of
-// chunk c + 1 are made behind the products of chunk c (1 x 16,384 tokens x 12 heads, pieces of 832: 18
+// chunk c + 1 are made behind the products of chunk c (1 x 16,384 tokens x 12 heads, pieces of 832: 18.6
 // us, 1.0 per chunk and a fill of 5).
 template <int KD, int VT, int R>
 __global__ __launch_bounds__(320) void linear_states_kernel(const LinearSeqs a,
@@ -899,7 +899,7 @@ __device__ __forceinline__ float decayed(float x, double sum, float add) {
 
 // From the pieces' local final states to their initial states, in order, four entries per thread:
 // S_in(0) is the sequence's initial state, S_in(g + 1) = e^(sum of g) S_in(g) + S_local(g). Eight
-// pieces' states are read at once: it is a chain of waits for memory (20 pieces of 12 heads 8 us).
+// pieces' states are read at once: it is a chain of waits for memory (20 pieces of 12 heads 7.4 us).
 template <int KD>
 __global__ __launch_bounds__(kChainThreads) void linear_chain_kernel(const LinearSeqs a,
                                                                       const wkv7_linear_io io) {

@@ -10,12 +10,12 @@
 // part, sum over groups of -s (1 + z / 16) X with X the sums of x, is a product of its own with one
 // input per group, in front: X comes from w4_sums_kernel, both factors as three bf16 parts.
 //
-// What bounds it (three products of 4096 x 4096 with 4096 rows, 64 x 256 tiles, 0.98 PFLOP/s): the
-// clock, 1.95 of 2.5 GHz, with matrix and vector units busy for 53 and 58 % of the cycles; the direct
-// loads, 1 KiB in 16 cycles of the unit's one load path, are a sixth of the time (a tile of 128 x 256
-// loads fewer bytes, but its eight waves wait for one another: 443 us for 409). Few rows (256 rows, 64
-// x 128 tiles): at each stage some 440 cycles until its first operands are there, beside 530 of
-// products.
+// What bounds it (three products of 4096 x 4096 with 4096 rows, 64 x 256 tiles, 1.0 PFLOP/s): the
+// clock, 1.92 GHz, with matrix and vector units busy for 55 and 58 % of the cycles; the direct
+// loads, 1 KiB in 16 cycles of the unit's one load path, are a sixth of the time (left out of a copy; a
+// tile of 128 x 256 loads fewer bytes, but its eight waves wait for one another: 443 us for 409). Few rows
+// (256 rows, 64 x 128 tiles): matrix units busy for 25 % of the cycles; in copies with parts left out, a
+// stage has some 440 cycles until its first operands are there, beside 530 of products.
 #pragma once
 
 #include <type_traits>

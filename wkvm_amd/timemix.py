@@ -133,8 +133,14 @@ class RWKV7TimeMix:
     def quantize(self, group: int = 128, names=("r", "k", "v", "o"), symmetric: bool = False,
                  ) -> dict[str, W4Weight]:
         """Round the named projections to 4-bit weights (``W4Weight.quantize``), which take the
-        place of the block's bf16 ones: the dictionary that the block was made from is not
-        changed, and a decode graph keeps the weights that it captured."""
+        place of the block's bf16 ones, at any token count: the dictionary that the block was made
+        from is not changed, and a decode graph keeps the weights that it captured.
+
+        They save memory; time only where the weights' bytes are what a step takes. Decode graphs of
+        8 layers of hidden size 4096: 426 -> 372 us with one row, 495 -> 440 with 16, 733 -> 691 with 64,
+        1649 -> 1552 with 256; of 24 layers of 2048, whose products are a launch more: 717 -> 688, 828 -> 844,
+        1185 -> 1207, 2125 -> 2370. Long prompts are slower: 4,096 tokens a
+        layer 871 -> 1060 us (4096), 476 -> 486 (2048)."""
         names = tuple(names)
         for name in names:
             if name not in ("r", "k", "v", "o"):

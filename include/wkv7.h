@@ -719,10 +719,10 @@ size_t wkv7_sample_workspace_bytes(int32_t rows, int32_t vocab);
  *                aligned (else WKV7_ERR_SHAPE)
  * A token's output depends on the tokens up to it alone, infinities and NaN among
  * them included.
- * A factor below 2^-126 of one token or of several counts as 0. Values are as
- * large as fp32 holds them in the formula; where products of a prefill pass it before their decay (a
- * query times a key or the state, growth within a chunk), a sequence (or its piece) is run again token
- * by token, 1 to 2 us for each.
+ * In a prefill a factor below 2^-126, of one token or of several, may count as 0. Where products
+ * pass fp32 before their decay and the formula does not (a query times a key or the state, growth
+ * within a chunk), a sequence (or its piece) is run again token by token, 1 to 2 us for each: its y may
+ * not overlap its inputs.
  *
  * wkv7_linear_prefill cuts sequences into pieces that run side by side where the
  * workgroups would not fill the device otherwise; the states between them go to

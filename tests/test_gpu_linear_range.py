@@ -137,3 +137,19 @@ def test_a_sequence_that_is_run_again_leaves_the_others(dev, H, Hq, K, V, T, f32
     _check(pool, y, before, cu, ids, q, k, v, g, 1.0)
     rest = list(range(T)) + list(range(2 * T, 3 * T))
     assert torch.equal(y[rest], usual[rest]) and torch.equal(pool[[4, 7]], usual_pool[[4, 7]])
+
+
+def test_outputs_over_the_inputs_are_refused(dev):
+    before, q, k, v, g = _inputs(68, 70, 2, 2, 64, 64, rows=3)
+    q, k, v, g = (t.to(dev) for t in (q, k, v, g))
+    pool, both = before.to(dev), torch.zeros(140, 2, 64, dtype=BF16, device=dev)
+    both[:70] = v
+    for out in (q, k, v):
+        with pytest.raises(ValueError, match="overlap"):
+            linear_prefill_varlen(pool, [1], [0, 70], q, k, v, g, out=out)
+    with pytest.raises(ValueError, match="overlap"):
+        linear_prefill_varlen(pool, [1], [0, 70], q, k, both[:70], g, out=both[69:139])
+    assert torch.equal(pool.cpu(), before)
+    want = linear_prefill_varlen(pool.clone(), [1], [0, 70], q, k, v, g)
+    linear_prefill_varlen(pool, [1], [0, 70], q, k, both[:70], g, out=both[70:])
+    assert torch.equal(both[70:], want) and torch.equal(both[:70], v)

@@ -79,3 +79,13 @@ def test_the_reference_is_the_sum_over_tokens():
             for s in range(t + 1):
                 want = want + np.exp(G[t, h] - G[s, h]) * (q[t, 0] @ k[s, 0]) * v[s, h]
             np.testing.assert_allclose(y[t, h], 0.5 * want, rtol=1e-12)
+
+
+def test_overlaps():
+    from wkvm_amd.linear import overlaps
+
+    buf = torch.zeros(12, 8)
+    assert overlaps(buf, buf) and overlaps(buf[:6], buf[5:]) and overlaps(buf[:, :2], buf[:, 4:])
+    assert not overlaps(buf[:6], buf[6:]) and not overlaps(buf[:0], buf)
+    assert not overlaps(buf[:1, :4], buf[:1, 4:]) and not overlaps(buf, torch.zeros(12, 8))
+    assert overlaps(buf[3].expand(5, 8), buf[3:4]) and not overlaps(buf[3].expand(5, 8), buf[4:])

@@ -18,8 +18,8 @@
 //                  of the decays of chunk c + 2
 // The operands that are not bf16 to begin with (scores under their decays, decayed keys, the state)
 // are split into three bf16 parts, which hold all of an fp32 number: a bf16 y is the fp32 one rounded
-// once. (With two parts, 2^-18 of each term, 8 x 4,096 tokens x 32 heads take 134.6 us from memory, 133.4
-// with three; 125 and 140 from the caches. 16,384 tokens x 12 heads 50.6 and 53.8.)
+// once. (With two parts, 2^-18 of each term, 8 x 4,096 tokens x 32 heads take 132.7 us on a card where
+// three take 138.4, and 134.6 on one where three take 133.4; 16,384 tokens x 12 heads 50.6 and 53.8.)
 #pragma once
 
 #include "wkv7_mfma.h"
@@ -474,7 +474,7 @@ __device__ __forceinline__ void one_by_one(float* lds, const wkv7_linear_io& io,
   constexpr int P = 256 / VT, J = KD / P;
   const int col = threadIdx.x % VT, key0 = threadIdx.x / VT * J;
   float* S = lds + key0 * VT + col;
-  barrier_lds();
+  barrier_vm<0>();  // (what other threads have stored, before it is stored again)
 #pragma unroll 1
   for (int j = 0; j < J; ++j) S[j * VT] = initial ? initial[int64_t(key0 + j) * io.V + col] : 0.f;
   const int64_t ko = head / (io.H / io.Hq) * KD + key0, vo = int64_t(head) * io.V + col0 + col;
@@ -505,7 +505,7 @@ __device__ __forceinline__ void one_by_one(float* lds, const wkv7_linear_io& io,
 // Outputs. Waves 0 .. 3 are the state waves, 4 .. 7 and 8 .. 11 the output waves of the even and of
 // the odd chunks. Few workgroups: a tick of 1.2 us (64 keys, 32 columns) is the state waves' chain of
 // split, products and decayed keys. All units busy: memory, in rows of 128 bytes a token (8 x 4,096 tokens
-// x 32 heads 134 us, 4.1 TB/s of q, k, v and y; vector units busy for 48 and matrix units for 27 % of the
+// x 32 heads 134 to 141 us by card, 4 TB/s of q, k, v and y; vector units busy for 48 and matrix units for 27 % of the
 // cycles, at 2.2 GHz; an earlier form took a third less without the outputs and no less without the
 // chain). With one group of output waves and two workgroups on a unit the state waves wait for the outputs (a
 // third slower).

@@ -80,6 +80,20 @@ def _vectors(x: torch.Tensor, name: str, tokens: int, size: int, device: torch.d
     return x, heads, ld
 
 
+def _span(x: torch.Tensor) -> tuple[int, int]:
+    """Addresses from the first element of ``x`` to behind its last."""
+    last = sum((n - 1) * s for n, s in zip(x.shape, x.stride()))
+    return x.data_ptr(), x.data_ptr() + (last + 1) * x.element_size()
+
+
+def overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory from a's first to its last element meets b's."""
+    if not a.numel() or not b.numel():
+        return False
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a0 < b1 and b0 < a1
+
+
 def _io(q, k, v, log_decay, dims, dev, tokens, scale, out, out_dtype):
     """The checked vectors as a ``LinearIO``, the output and the tensors that the launch reads;
     ``dims`` are the state's."""
@@ -157,7 +171,7 @@ def linear_prefill_varlen(state: torch.Tensor, slot_ids, cu_seqlens, q, k, v, lo
     sequence leaves it as it is (zeroes it with ``zero_init``).
 
     ``q``, ``k``, ``v``, ``log_decay`` and the result as for ``linear_decode_slots``, over the T packed
-    tokens. ``cu_seqlens`` is a host sequence or a device int32 tensor, ``seq_order`` as for
+    tokens (``out`` may not overlap them). ``cu_seqlens`` is a host sequence or a device int32 tensor, ``seq_order`` as for
     ``wkv7_prefill_varlen``. A token's output does not depend on later tokens, whatever they hold. Few
     sequences are cut into pieces that run side by side, through a workspace from torch's
     allocator."""
@@ -168,6 +182,8 @@ def linear_prefill_varlen(state: torch.Tensor, slot_ids, cu_seqlens, q, k, v, lo
     ops._require_cuda(v, "v")
     T = int(v.shape[0]) if v.dim() == 3 else -1
     io, y, keep = _io(q, k, v, log_decay, dims, dev, T, scale, out, out_dtype)
+    if out is not None and any(overlaps(out, x) for x in (*keep, state)):
+        raise ValueError("out must not overlap the inputs, which may be read again")
     if isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.is_cuda:
         cu = ops.packed_ints(cu_seqlens, nseq + 1, dev, "cu_seqlens")
     else:

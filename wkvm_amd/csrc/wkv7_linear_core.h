@@ -505,9 +505,9 @@ __device__ __forceinline__ void one_by_one(float* lds, const wkv7_linear_io& io,
 // Outputs. Waves 0 .. 3 are the state waves, 4 .. 7 and 8 .. 11 the output waves of the even and of
 // the odd chunks. Few workgroups: a tick of 1.2 us (64 keys, 32 columns) is the state waves' chain of
 // split, products and decayed keys. All units busy: memory, in rows of 128 bytes a token (8 x 4,096 tokens
-// x 32 heads 134 to 141 us by card, 4 TB/s of q, k, v and y; vector units busy for 48 and matrix units for 27 % of the
-// cycles, at 2.2 GHz; an earlier form took a third less without the outputs and no less without the
-// chain). With one group of output waves and two workgroups on a unit the state waves wait for the outputs (a
+// x 32 heads 134 to 141 us by card, 4 TB/s of q, k, v and y; vector units busy for 48 and matrix units
+// for 27 % of the cycles, at 2.2 GHz; an earlier form took a third less without the outputs and no less
+// without the chain). With one group of output waves and two workgroups on a unit the state waves wait for the outputs (a
 // third slower).
 template <int KD, int VT, bool kF32, int R>
 __global__ __launch_bounds__(768) void linear_prefill_kernel(const LinearSeqs a,
